@@ -118,6 +118,56 @@ int pulsar_op_moe_dispatch(const void* x_dev, const int64_t* topk_idx_dev, const
                            int64_t D, void* expert_inputs_dev, void* stream);
 
 /* ==================================================================================
+ * Paged KV cache held in 4 bits (no counterpart in the reference). pages_dev: uint8
+ * [num_pages][Hkv][20 * head_dim * page_size / 16], 16-byte aligned; head_dim 64 or 128,
+ * page_size a power of two of at least 16; slot = page * page_size + place in the page.
+ * Each 32 dims of a key or value store z = bf16(min), s = bf16((max - z) / 15) and 4-bit codes
+ * c = round((x - z) / s), which stand for s c + z; a group with a NaN or an infinity reads back
+ * as NaN. csrc/kv4.cuh gives the order of the bytes.
+ * ================================================================================== */
+
+/* Norm and rotation of queries and keys, then storing keys and values. q [N, Hq, head_dim], k and
+ * v [N, Hkv, head_dim] bf16, 16-byte aligned, with strides_host[6] = element strides of tokens and
+ * heads of q, k, v (multiples of 8; the last stride is 1). q_norm [Hq, head_dim], k_norm [Hkv,
+ * head_dim] f32 or NULL: x -> w x / sqrt(mean x^2 + eps). cos, sin [max_pos, rot / 2] f32 turn the
+ * first rot dims (rot 0: none): pairs (i, i + rot / 2), rot a multiple of 16, or (2i, 2i + 1) when
+ * interleaved, rot even. q_gain [max_pos] f32 or NULL: factor of the queries of a position.
+ * positions [N] i32 (may be NULL without tables); slots [N] i64, distinct. q_out [N, Hq, head_dim]
+ * bf16 contiguous. A token with a slot outside the cache or a position outside the tables is not
+ * stored; in the latter case its query is zero. */
+int pulsar_op_kv4_append(const void* q_dev, const void* k_dev, const void* v_dev, const int64_t* strides_host,
+                         int64_t N, int64_t Hq, int64_t Hkv, int64_t head_dim, const float* q_norm_dev,
+                         const float* k_norm_dev, float eps, const float* cos_dev, const float* sin_dev, int64_t rot,
+                         int64_t max_pos, int interleaved, const float* q_gain_dev, const int32_t* positions_dev,
+                         const int64_t* slots_dev, void* pages_dev, int64_t num_pages, int64_t page_size,
+                         void* q_out_dev, void* stream);
+
+/* What the cache holds for slots [N] i64, as bf16 k_out and v_out [N, Hkv, head_dim]; zeros for a
+ * slot outside the cache. */
+int pulsar_op_kv4_read(const void* pages_dev, int64_t num_pages, int64_t page_size, int64_t Hkv, int64_t head_dim,
+                       const int64_t* slots_dev, int64_t N, void* k_out_dev, void* v_out_dev, void* stream);
+
+/* Bytes of scratch that pulsar_op_kv4_attention needs for these sizes (0: none). */
+int pulsar_op_kv4_attention_workspace(int64_t N, int64_t Hq, int64_t Hkv, int64_t head_dim, int64_t B, int64_t max_q,
+                                      int64_t max_kv, int64_t window, int64_t* bytes);
+
+/* Attention of query rows over the cached keys and values of their sequences: rows cu_q[b] ..
+ * cu_q[b + 1] - 1 of q (at most max_q; cu_q [B + 1] i32, NULL: one row for each sequence) are the
+ * last rows of sequence b, whose kv_lens[b] (i32) keys lie in the pages of block_table [B, width]
+ * (i32); row j of n sees keys up to position kv_lens[b] - n + j, with window > 0 the last `window`
+ * of these. q [N, Hq, head_dim] bf16 with even element strides, Hq a multiple of Hkv. max_kv bounds
+ * kv_lens and only decides how the work is split. out [N, Hq, head_dim] bf16: softmax(scale q k^T) v,
+ * 0 for a row that sees no key; rows of no sequence are not written. Page numbers outside the cache
+ * count as masked. workspace_dev: scratch of at least pulsar_op_kv4_attention_workspace bytes, which
+ * calls on different streams must not share. */
+int pulsar_op_kv4_attention(const void* q_dev, int64_t q_row_stride, int64_t q_head_stride, int64_t N, int64_t Hq,
+                            int64_t head_dim, const void* pages_dev, int64_t num_pages, int64_t page_size,
+                            int64_t Hkv, const int32_t* block_table_dev, int64_t B, int64_t width,
+                            const int32_t* kv_lens_dev, const int32_t* cu_q_dev, int64_t max_q, int64_t max_kv,
+                            float scale, int64_t window, void* workspace_dev, int64_t workspace_bytes, void* out_dev,
+                            void* stream);
+
+/* ==================================================================================
  * Engine: the KV-cache decode path of src/infer.py on the device.
  * ================================================================================== */
 

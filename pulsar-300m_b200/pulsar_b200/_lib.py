@@ -49,6 +49,16 @@ PROTOTYPES = {
                                       c_int64, c_int64, c_void_p, c_void_p]),
     "pulsar_op_moe_dispatch": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64,
                                        c_int64, c_void_p, c_void_p]),
+    "pulsar_op_kv4_append": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p,
+                                     c_void_p, c_float, c_void_p, c_void_p, c_int64, c_int64, c_int, c_void_p, c_void_p,
+                                     c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p]),
+    "pulsar_op_kv4_read": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p,
+                                   c_void_p]),
+    "pulsar_op_kv4_attention_workspace": (c_int, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64,
+                                                  C.POINTER(c_int64)]),
+    "pulsar_op_kv4_attention": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_int64,
+                                        c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64,
+                                        c_int64, c_float, c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
     "pulsar_engine_create": (c_int, [C.POINTER(EngineConfig), C.POINTER(c_void_p)]),
     "pulsar_engine_destroy": (c_int, [c_void_p]),
     "pulsar_engine_set_tensor": (c_int, [c_void_p, c_char_p, c_void_p, c_int64]),
