@@ -3,19 +3,19 @@
 // Row j of the n_b query rows of sequence b has position pos = len_b - n_b + j and sees the keys
 // max(0, pos - window + 1) .. pos (window 0: all of 0 .. pos):
 //   out = sum_k p_k v_k / sum_k p_k,  p_k = exp(scale q.k_k - m)
-// with k = s c + z per group of 32 dims, so q.k = sum_g s_g (q.c)_g + z_g sum(q)_g: the codes enter
-// the matrix instruction as small whole numbers (exact in bf16) and s, z are applied in fp32 to
-// its results. Values: O = sum_k (p_k s_kg) (c - 8) + sum_k p_k (z_kg + 8 s_kg): s goes into the
-// weights, whose bf16 hi and lo halves are both multiplied (|x - hi - lo| <= 2^-16 |x|), and the
-// second sum is a scalar per (row, group).
+// with k = s c + z per group of 32 dims, so q.k = sum_g s_g (q.(16 + c))_g + (z_g - 16 s_g) sum(q)_g:
+// the codes enter the matrix instruction as small whole numbers (exact in bf16) and s, z are applied
+// in fp32 to its results. Values: O = sum_k (p_k s_kg) (c - f) + sum_k p_k (z_kg + f s_kg), f = -16
+// for even and 31 for odd tokens: s goes into the weights, whose bf16 hi and lo halves are both
+// multiplied (|x - hi - lo| <= 2^-16 |x|), and the second sum is a scalar per (row, group).
 //
 // A unit is a (query row, head of the kv head's group). CTA (split and unit tile, kv head,
-// sequence): four warps, each walking every fourth 16-token tile of the split's range through a
-// ring of its own (1-D bulk copies of whole tiles, issued by its lane 0; page ids are prefetched
-// 32 tiles at a time, one a lane). Tokens are the M rows of S^T = K Q^T and units its N columns, so
-// a tile's codes are unpacked once for all units, straight into operand registers; the weights
-// pass through movmatrix into the B operand of O^T = V^T P^T. Up to four units the eight columns
-// hold every unit twice and the copies carry the hi and the lo halves.
+// sequence): four warps, each walking every fourth pair of 16-token tiles of the split's range
+// through a ring of its own (1-D bulk copies of whole tiles, issued by its lane 0; page ids are
+// prefetched 32 pairs at a time, one a lane). Tokens are the M rows of S^T = K Q^T and units its N
+// columns, so a tile's codes are unpacked once for all units, straight into operand registers; the
+// weights pass through movmatrix into the B operand of O^T = V^T P^T. Up to four units the eight
+// columns hold every unit twice and the copies carry the hi and the lo halves.
 //
 // The softmax keeps a running maximum per unit that moves only when a score exceeds it by more
 // than 2^LAZY (l and O use the same maximum, so the result does not depend on when it moves).
@@ -25,6 +25,8 @@
 // Splits write (m, l, O) partials; k_kv4_merge joins them in split order.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+
+#include <type_traits>
 
 #include "capi_util.h"
 #include "common.cuh"
@@ -46,7 +48,7 @@ struct AttnArgs {
     __nv_bfloat16* out;
     float *part_o, *part_ml;
     int64_t q_row, q_head, page_bytes;
-    int rows, hq, hkv, group, num_pages, width, page_shift, max_q, window, nsplit, split_tiles;
+    int rows, hq, hkv, group, num_pages, width, page_shift, max_q, window, nsplit, split_pairs;
     float scale_log2;
 };
 
@@ -60,12 +62,13 @@ __device__ __forceinline__ void rows_of(const AttnArgs& a, int b, int& row0, int
     }
 }
 
-__device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
+// d = a b + c (d and c may be the same registers)
+__device__ __forceinline__ void mma16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, const float* c) {
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
@@ -80,16 +83,16 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// Operand register i of a code word: the bf16 pair 16 + c (the nibble goes to bits 3..6 of each
+// Operand register i of a key word: the bf16 pair 16 + c (the nibble goes to bits 3..6 of each
 // half, where a bf16 in [16, 32) holds its whole part).
-__device__ __forceinline__ uint32_t unpack(uint32_t w, int i) {
+__device__ __forceinline__ uint32_t unpack_k(uint32_t w, int i) {
     return ((i == 0 ? w << 3 : w >> (4 * i - 3)) & 0x00780078u) | 0x41804180u;
 }
-// The same, less 24: c - 8, exact.
-__device__ __forceinline__ uint32_t unpack8(uint32_t w, int i) {
-    const uint32_t u = unpack(w, i);
-    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), __floats2bfloat162_rn(24.f, 24.f));
-    return *reinterpret_cast<const uint32_t*>(&d);
+// Operand register i of a value word: 16 + c for the even token of the pair, c - 31 for the odd one
+// (sign and complemented nibble by the same exclusive or): the offsets cancel in the sums over
+// tokens instead of growing, and what is left of them is in the scalar sums.
+__device__ __forceinline__ uint32_t unpack_v(uint32_t w, int i) {
+    return ((i == 0 ? w << 3 : w >> (4 * i - 3)) & 0x00780078u) ^ 0xC1F84180u;
 }
 
 __device__ __forceinline__ uint32_t pack(float a, float b) {
@@ -99,15 +102,16 @@ __device__ __forceinline__ uint32_t pack(float a, float b) {
 __device__ __forceinline__ float lo_of(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float hi_of(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
+// A stage holds two tiles (32 tokens); bytes in flight per warp: 10 KB.
 template <int HD>
-constexpr int stages() { return HD == 64 ? 8 : 4; }
+constexpr int stages() { return HD == 64 ? 4 : 3; }
 template <int HD>
-constexpr int ring_bytes() { return WARPS * stages<HD>() * Kv4Tile<HD>::BYTES; }
+constexpr int ring_bytes() { return WARPS * stages<HD>() * 2 * Kv4Tile<HD>::BYTES; }
 
 template <int HD, int NT, bool DUP>
 __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
     using T = Kv4Tile<HD>;
-    constexpr int NG = T::NG, NB = HD / 64, S = stages<HD>(), MT = HD / 16;
+    constexpr int NG = T::NG, NB = HD / 64, S = stages<HD>(), MT = HD / 16, TB = T::BYTES;
     constexpr int UT = DUP ? 4 : 8 * NT;
     extern __shared__ __align__(128) unsigned char sm[];
     __shared__ uint64_t bars[WARPS][S];
@@ -124,10 +128,11 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
     const int first = len - nq + u0 / a.group, last = len - nq + ulast / a.group;   // their positions
     auto low = [&](int pos) { return a.window > 0 ? max(0, pos - a.window + 1) : 0; };
     const int kmin = low(first), kmax = last + 1;   // keys that some unit sees: [kmin, kmax)
-    const int tile0 = kmin / KV4_TILE, ntiles = kmax > 0 ? (kmax + KV4_TILE - 1) / KV4_TILE : 0;
-    const int t_begin = tile0 + split * a.split_tiles;
-    const int t_end = split == a.nsplit - 1 ? ntiles : min(ntiles, t_begin + a.split_tiles);
-    const int mine = t_end > t_begin + warp ? (t_end - t_begin - warp + WARPS - 1) / WARPS : 0;
+    // pairs of tiles (32 tokens, aligned): the split's range, of which the warp takes every fourth
+    const int pair0 = kmin / 32, npairs = kmax > 0 ? (kmax + 31) / 32 : 0;
+    const int p_begin = pair0 + split * a.split_pairs + warp;
+    const int p_end = split == a.nsplit - 1 ? npairs : min(npairs, pair0 + (split + 1) * a.split_pairs);
+    const int mine = p_end > p_begin ? (p_end - p_begin + WARPS - 1) / WARPS : 0;
 
     if (lane == 0) {
         for (int i = 0; i < S; ++i) mbar_init(&bars[warp][i], 1);
@@ -135,40 +140,57 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
     }
     __syncwarp();
 
-    // page of the warp's i-th tile: lane i % 32 holds it for the current 32
-    int page_of = -1;
-    auto fetch_pages = [&](int i0) {
-        const int i = i0 + lane;
-        page_of = -1;
-        if (i < mine) {
-            const int tl = t_begin + warp + i * WARPS;
-            page_of = a.table[(int64_t)b * a.width + (tl >> (a.page_shift - 4))];
-            if (page_of < 0 || page_of >= a.num_pages) page_of = -1;
+    // pages of the warp's i-th pair (-1: none): lane i % 32 holds them for the current 32; a page of
+    // 16 tokens holds one tile of the pair only
+    const bool two = a.page_shift == 4;
+    auto page_at = [&](int tile) {
+        const int col = tile >> (a.page_shift - 4);
+        const int p = col < a.width ? a.table[(int64_t)b * a.width + col] : -1;
+        return p >= 0 && p < a.num_pages ? p : -1;
+    };
+    auto fetch_pages = [&](int i0, int& pg, int& pg2) {
+        pg = pg2 = -1;
+        if (i0 + lane < mine) {
+            const int tile = 2 * (p_begin + (i0 + lane) * WARPS);
+            pg = pg2 = page_at(tile);
+            if (two) pg2 = page_at(tile + 1);
         }
     };
-    unsigned char* ring = sm + warp * S * T::BYTES;
-    auto issue = [&](int i, int page) {   // lane 0; a tile of no page completes its phase at once
+    unsigned char* ring = sm + warp * S * 2 * TB;
+    auto issue = [&](int i, int pg, int pg2) {   // lane 0; a pair of no page completes its phase at once
         uint64_t* bar = &bars[warp][i % S];
-        if (page < 0) {
-            mbar_arrive(bar);
-            return;
+        unsigned char* dst = ring + (i % S) * 2 * TB;
+        const int tile = 2 * (p_begin + i * WARPS) & ((1 << (a.page_shift - 4)) - 1);
+        if (!two) {
+            if (pg < 0) {
+                mbar_arrive(bar);
+                return;
+            }
+            mbar_arrive_expect_tx(bar, 2 * TB);
+            tma_load_1d(dst, a.pages + ((int64_t)pg * a.hkv + h) * a.page_bytes + tile * TB, 2 * TB, bar);
+        } else {
+            const uint32_t bytes = (pg >= 0 ? TB : 0) + (pg2 >= 0 ? TB : 0);
+            if (bytes == 0) {
+                mbar_arrive(bar);
+                return;
+            }
+            mbar_arrive_expect_tx(bar, bytes);
+            if (pg >= 0) tma_load_1d(dst, a.pages + ((int64_t)pg * a.hkv + h) * a.page_bytes, TB, bar);
+            if (pg2 >= 0) tma_load_1d(dst + TB, a.pages + ((int64_t)pg2 * a.hkv + h) * a.page_bytes, TB, bar);
         }
-        const int tl = t_begin + warp + i * WARPS;
-        const uint8_t* src = a.pages + ((int64_t)page * a.hkv + h) * a.page_bytes +
-                             (int64_t)(tl & ((1 << (a.page_shift - 4)) - 1)) * T::BYTES;
-        mbar_arrive_expect_tx(bar, T::BYTES);
-        tma_load_1d(ring + (i % S) * T::BYTES, src, T::BYTES, bar);
     };
-    fetch_pages(0);
-    int next_pages = page_of;   // of the 32 tiles that hold the next one to issue
+    int pg, pg2, next, next2;   // of the 32 pairs that hold the current one, and the next one to issue
+    fetch_pages(0, pg, pg2);
+    next = pg;
+    next2 = pg2;
     for (int i = 0; i < min(S, mine); ++i) {
-        const int p = __shfl_sync(0xffffffffu, page_of, i);
-        if (lane == 0) issue(i, p);
+        const int p = __shfl_sync(0xffffffffu, pg, i), p2 = __shfl_sync(0xffffffffu, pg2, i);
+        if (lane == 0) issue(i, p, p2);
     }
 
     // queries: B operand of step j (dims 16 j ..): unit n = lane / 4, dims 2t, 2t + 1 and 8 further
     uint32_t qf[NT][2 * MT];
-    float nsum[NT][NG][2];   // -16 sum of q over the group, for the thread's two columns
+    float qsum[NT][NG][2];   // sum of q over the group, for the thread's two columns
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int u = u0 + (DUP ? (r & 3) : nt * 8 + r);
@@ -184,8 +206,8 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
             for (int i = 0; i < 4; ++i) s += lo_of(qf[nt][4 * g4 + i]) + hi_of(qf[nt][4 * g4 + i]);
             s += __shfl_xor_sync(0xffffffffu, s, 1);
             s += __shfl_xor_sync(0xffffffffu, s, 2);
-            nsum[nt][g4][0] = -16.f * __shfl_sync(0xffffffffu, s, 8 * t);
-            nsum[nt][g4][1] = -16.f * __shfl_sync(0xffffffffu, s, 8 * t + 4);
+            qsum[nt][g4][0] = __shfl_sync(0xffffffffu, s, 8 * t);
+            qsum[nt][g4][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
         }
     }
     int hi[NT][2], lo[NT][2];   // keys that the thread's columns see
@@ -200,7 +222,9 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
         }
     const int all_lo = low(last), all_hi = first + 1;   // keys in [all_lo, all_hi) are seen by every unit
 
-    float o[MT][NT][4], zacc[NT][NG][2], m[NT][2], l[NT][2];
+    // m: running maximum of the unscaled scores; top: the score that moves it; nm = -scale m
+    float o[MT][NT][4], zacc[NT][NG][2], m[NT][2], top[NT][2], nm[NT][2], l[NT][2];
+    const float lazy = LAZY / a.scale_log2;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -208,159 +232,181 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
 #pragma unroll
         for (int g = 0; g < NG; ++g) zacc[nt][g][0] = zacc[nt][g][1] = 0.f;
         m[nt][0] = m[nt][1] = NEG;
+        top[nt][0] = top[nt][1] = NEG + lazy;
+        nm[nt][0] = nm[nt][1] = -NEG * a.scale_log2;
         l[nt][0] = l[nt][1] = 0.f;
     }
-    int failed = -1;   // the tile whose copy did not land within the bound
+    const float off = r & 1 ? 31.f : -16.f;                          // of the thread's tokens r and r + 8
+    const uint32_t cut_lo = t < 2 ? 0x4444u : 0x1044u, cut_hi = t < 2 ? 0x4444u : 0x3244u;
+    int failed = -1;   // the pair whose copy did not land within the bound
 
-    for (int i = 0; i < mine; ++i) {
-        const int st = i % S;
-        if (i > 0 && (i & 31) == 0) page_of = next_pages;
-        const int page = __shfl_sync(0xffffffffu, page_of, i & 31);
-        if (!mbar_wait(&bars[warp][st], (i / S) & 1)) {
-            failed = i;
-            break;
-        }
-        const unsigned char* tp = ring + st * T::BYTES;
-        uint4 kc[NB], vc[NB];
-        uint32_t kp[2][NG], vp[2][NG];
+    // one pair of tiles; EDGE: some of its keys are not seen by some unit, or a page is missing
+    auto pair_step = [&](auto edge_tag, const unsigned char* tp, int k0, bool ok0, bool ok1) {
+        constexpr bool EDGE = decltype(edge_tag)::value;
+        float sc[2][NT][4];
 #pragma unroll
-        for (int x = 0; x < NB; ++x) {
-            kc[x] = *reinterpret_cast<const uint4*>(tp + x * T::BLK + lane * 16);
-            vc[x] = *reinterpret_cast<const uint4*>(tp + T::V + x * T::BLK + lane * 16);
-        }
+        for (int x = 0; x < 2; ++x) {
+            const unsigned char* kt = tp + x * TB;
+            uint32_t kp[2][NG], kc[NB][4];
 #pragma unroll
-        for (int x = 0; x < 2 * NG; x += 4) {
-            *reinterpret_cast<uint4*>(&kp[0][0] + x) = *reinterpret_cast<const uint4*>(tp + T::KP + r * 8 * NG + x * 4);
-            *reinterpret_cast<uint4*>(&vp[0][0] + x) = *reinterpret_cast<const uint4*>(tp + T::VP + r * 8 * NG + x * 4);
-        }
-        __syncwarp();   // every lane has read the stage
-        const int nx = i + S;
-        if (nx < mine) {
-            if ((nx & 31) == 0) {
-                const int keep = page_of;
-                fetch_pages(nx);
-                next_pages = page_of;
-                page_of = keep;
-            }
-            const int p = __shfl_sync(0xffffffffu, (nx >> 5) == (i >> 5) ? page_of : next_pages, nx & 31);
-            if (lane == 0) issue(nx, p);
-        }
-        if (page < 0) continue;
-
-        // scores
-        const int k0 = (t_begin + warp + i * WARPS) * KV4_TILE;
-        float sc[NT][4];
+            for (int y = 0; y < NB; ++y)
+                *reinterpret_cast<uint4*>(kc[y]) = *reinterpret_cast<const uint4*>(kt + y * T::BLK + lane * 16);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+            for (int y = 0; y < 2 * NG; y += 4)
+                *reinterpret_cast<uint4*>(&kp[0][0] + y) = *reinterpret_cast<const uint4*>(kt + T::KP + r * 8 * NG + y * 4);
 #pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            const uint32_t wr = g & 1 ? kc[g >> 1].y : kc[g >> 1].x, w8 = g & 1 ? kc[g >> 1].w : kc[g >> 1].z;
-            uint32_t af[2][4];
+            for (int g = 0; g < NG; ++g) {
+                const uint32_t wr = kc[g >> 1][g & 1], w8 = kc[g >> 1][2 + (g & 1)];
+                const uint32_t a0[4] = {unpack_k(wr, 0), unpack_k(w8, 0), unpack_k(wr, 1), unpack_k(w8, 1)};
+                const uint32_t a1[4] = {unpack_k(wr, 2), unpack_k(w8, 2), unpack_k(wr, 3), unpack_k(w8, 3)};
+                const float s0 = lo_of(kp[0][g]), z0 = hi_of(kp[0][g]), s8 = lo_of(kp[1][g]), z8 = hi_of(kp[1][g]);
+                const float y0 = fmaf(-16.f, s0, z0), y8 = fmaf(-16.f, s8, z8);
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                af[x][0] = unpack(wr, 2 * x);
-                af[x][1] = unpack(w8, 2 * x);
-                af[x][2] = unpack(wr, 2 * x + 1);
-                af[x][3] = unpack(w8, 2 * x + 1);
-            }
-            const float s0 = lo_of(kp[0][g]), z0 = hi_of(kp[0][g]) * -0.0625f;
-            const float s8 = lo_of(kp[1][g]), z8 = hi_of(kp[1][g]) * -0.0625f;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const float n0 = nsum[nt][g][0], n1 = nsum[nt][g][1];
-                float acc[4] = {n0, n1, n0, n1};
-                mma16816(acc, af[0][0], af[0][1], af[0][2], af[0][3], qf[nt][4 * g], qf[nt][4 * g + 1]);
-                mma16816(acc, af[1][0], af[1][1], af[1][2], af[1][3], qf[nt][4 * g + 2], qf[nt][4 * g + 3]);
-                sc[nt][0] = fmaf(s0, acc[0], fmaf(z0, n0, sc[nt][0]));
-                sc[nt][1] = fmaf(s0, acc[1], fmaf(z0, n1, sc[nt][1]));
-                sc[nt][2] = fmaf(s8, acc[2], fmaf(z8, n0, sc[nt][2]));
-                sc[nt][3] = fmaf(s8, acc[3], fmaf(z8, n1, sc[nt][3]));
+                for (int nt = 0; nt < NT; ++nt) {
+                    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                    mma16816(acc, a0, qf[nt][4 * g], qf[nt][4 * g + 1], acc);
+                    mma16816(acc, a1, qf[nt][4 * g + 2], qf[nt][4 * g + 3], acc);
+                    const float q0 = qsum[nt][g][0], q1 = qsum[nt][g][1];
+                    float* c = sc[x][nt];
+                    c[0] = g == 0 ? y0 * q0 : fmaf(y0, q0, c[0]);
+                    c[1] = g == 0 ? y0 * q1 : fmaf(y0, q1, c[1]);
+                    c[2] = g == 0 ? y8 * q0 : fmaf(y8, q0, c[2]);
+                    c[3] = g == 0 ? y8 * q1 : fmaf(y8, q1, c[3]);
+                    c[0] = fmaf(s0, acc[0], c[0]);
+                    c[1] = fmaf(s0, acc[1], c[1]);
+                    c[2] = fmaf(s8, acc[2], c[2]);
+                    c[3] = fmaf(s8, acc[3], c[3]);
+                }
             }
         }
-        const bool edge = k0 < all_lo || k0 + KV4_TILE > all_hi;
-        const int ka = k0 + r, kb = ka + 8;
-        bool up = false;
+        bool see[2][NT][4], up = false;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int c = e & 1, k = e < 2 ? ka : kb;
-                sc[nt][e] *= a.scale_log2;
-                if (edge && (k < lo[nt][c] || k >= hi[nt][c])) sc[nt][e] = -INFINITY;
-                up |= sc[nt][e] > m[nt][c] + LAZY;
-            }
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int c = e & 1;
+                    if (EDGE) {
+                        const int k = k0 + 16 * x + r + (e < 2 ? 0 : 8);
+                        see[x][nt][e] = (x ? ok1 : ok0) && k >= lo[nt][c] && k < hi[nt][c];
+                        if (!see[x][nt][e]) sc[x][nt][e] = -INFINITY;
+                    }
+                    up |= sc[x][nt][e] > top[nt][c];
+                }
         if (__any_sync(0xffffffffu, up)) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    float x = fmaxf(sc[nt][c], sc[nt][c + 2]);
+                    float x = fmaxf(fmaxf(sc[0][nt][c], sc[0][nt][c + 2]), fmaxf(sc[1][nt][c], sc[1][nt][c + 2]));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
                     x = fmaxf(x, m[nt][c]);
-                    const float f = ex2(m[nt][c] - x);
+                    const float f = ex2((m[nt][c] - x) * a.scale_log2);
                     m[nt][c] = x;
+                    top[nt][c] = x + lazy;
+                    nm[nt][c] = -x * a.scale_log2;
                     l[nt][c] *= f;
 #pragma unroll
                     for (int g = 0; g < NG; ++g) zacc[nt][g][c] *= f;
 #pragma unroll
-                    for (int x = 0; x < MT; ++x) {
-                        o[x][nt][c] *= f;
-                        o[x][nt][c + 2] *= f;
+                    for (int y = 0; y < MT; ++y) {
+                        o[y][nt][c] *= f;
+                        o[y][nt][c + 2] *= f;
                     }
                 }
         }
-        bool see[NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int x = 0; x < 2; ++x)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int c = e & 1, k = e < 2 ? ka : kb;
-                see[nt][e] = !edge || (k >= lo[nt][c] && k < hi[nt][c]);
-                sc[nt][e] = ex2(sc[nt][e] - m[nt][c]);
-                l[nt][c] += sc[nt][e];
-            }
-        // values
-#pragma unroll
-        for (int g = 0; g < NG; ++g) {
-            const float s0 = lo_of(vp[0][g]), s8 = lo_of(vp[1][g]);
-            const float z0 = fmaf(8.f, s0, hi_of(vp[0][g])), z8 = fmaf(8.f, s8, hi_of(vp[1][g]));
-            const uint32_t w0 = g & 1 ? vc[g >> 1].z : vc[g >> 1].x, w1 = g & 1 ? vc[g >> 1].w : vc[g >> 1].y;
-            uint32_t af[2][4];
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                af[x][0] = unpack8(w0, 2 * x);
-                af[x][1] = unpack8(w0, 2 * x + 1);
-                af[x][2] = unpack8(w1, 2 * x);
-                af[x][3] = unpack8(w1, 2 * x + 1);
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                float w[4], z[4];
+            for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    w[e] = see[nt][e] ? sc[nt][e] * (e < 2 ? s0 : s8) : 0.f;
-                    z[e] = see[nt][e] ? sc[nt][e] * (e < 2 ? z0 : z8) : 0.f;
+                    const int c = e & 1;
+                    sc[x][nt][e] = ex2(fmaf(sc[x][nt][e], a.scale_log2, nm[nt][c]));
+                    l[nt][c] += sc[x][nt][e];
                 }
-                zacc[nt][g][0] += z[0] + z[2];
-                zacc[nt][g][1] += z[1] + z[3];
-                uint32_t pa = pack(w[0], w[1]), pb = pack(w[2], w[3]);
-                const uint32_t la = pack(w[0] - lo_of(pa), w[1] - hi_of(pa)), lb = pack(w[2] - lo_of(pb), w[3] - hi_of(pb));
-                if (DUP) {
-                    const uint32_t b0 = movmatrix(t < 2 ? pa : la), b1 = movmatrix(t < 2 ? pb : lb);
 #pragma unroll
-                    for (int x = 0; x < 2; ++x)
-                        mma16816(o[2 * g + x][nt], af[x][0], af[x][1], af[x][2], af[x][3], b0, b1);
-                } else {
-                    const uint32_t b0 = movmatrix(pa), b1 = movmatrix(pb), c0 = movmatrix(la), c1 = movmatrix(lb);
+        for (int x = 0; x < 2; ++x) {
+            const unsigned char* vt = tp + x * TB;
+            uint32_t vp[2][NG], vc[NB][4];
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        mma16816(o[2 * g + x][nt], af[x][0], af[x][1], af[x][2], af[x][3], b0, b1);
-                        mma16816(o[2 * g + x][nt], af[x][0], af[x][1], af[x][2], af[x][3], c0, c1);
+            for (int y = 0; y < NB; ++y)
+                *reinterpret_cast<uint4*>(vc[y]) = *reinterpret_cast<const uint4*>(vt + T::V + y * T::BLK + lane * 16);
+#pragma unroll
+            for (int y = 0; y < 2 * NG; y += 4)
+                *reinterpret_cast<uint4*>(&vp[0][0] + y) = *reinterpret_cast<const uint4*>(vt + T::VP + r * 8 * NG + y * 4);
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                const uint32_t w0 = vc[g >> 1][2 * (g & 1)], w1 = vc[g >> 1][2 * (g & 1) + 1];
+                const uint32_t a0[4] = {unpack_v(w0, 0), unpack_v(w0, 1), unpack_v(w1, 0), unpack_v(w1, 1)};
+                const uint32_t a1[4] = {unpack_v(w0, 2), unpack_v(w0, 3), unpack_v(w1, 2), unpack_v(w1, 3)};
+                const float s0 = lo_of(vp[0][g]), s8 = lo_of(vp[1][g]);
+                const float z0 = fmaf(off, s0, hi_of(vp[0][g])), z8 = fmaf(off, s8, hi_of(vp[1][g]));
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const float* p = sc[x][nt];
+                    float w[4] = {p[0] * s0, p[1] * s0, p[2] * s8, p[3] * s8};
+                    float* za = zacc[nt][g];
+                    if (EDGE) {   // what a unit does not see may hold anything: left out, not multiplied by 0
+                        const bool* y = see[x][nt];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            w[e] = y[e] ? w[e] : 0.f;
+                            za[e & 1] += y[e] ? p[e] * (e < 2 ? z0 : z8) : 0.f;
+                        }
+                    } else {
+                        za[0] = fmaf(p[0], z0, fmaf(p[2], z8, za[0]));
+                        za[1] = fmaf(p[1], z0, fmaf(p[3], z8, za[1]));
+                    }
+                    uint32_t pa = pack(w[0], w[1]), pb = pack(w[2], w[3]);
+                    if (DUP) {   // columns 4..7 (t >= 2) carry the lo halves: w less its hi half
+                        pa = pack(w[0] - __uint_as_float(__byte_perm(pa, 0, cut_lo)),
+                                  w[1] - __uint_as_float(__byte_perm(pa, 0, cut_hi)));
+                        pb = pack(w[2] - __uint_as_float(__byte_perm(pb, 0, cut_lo)),
+                                  w[3] - __uint_as_float(__byte_perm(pb, 0, cut_hi)));
+                    }
+                    const uint32_t b0 = movmatrix(pa), b1 = movmatrix(pb);
+                    mma16816(o[2 * g][nt], a0, b0, b1, o[2 * g][nt]);
+                    mma16816(o[2 * g + 1][nt], a1, b0, b1, o[2 * g + 1][nt]);
+                    if (!DUP) {
+                        const uint32_t c0 = movmatrix(pack(w[0] - lo_of(pa), w[1] - hi_of(pa)));
+                        const uint32_t c1 = movmatrix(pack(w[2] - lo_of(pb), w[3] - hi_of(pb)));
+                        mma16816(o[2 * g][nt], a0, c0, c1, o[2 * g][nt]);
+                        mma16816(o[2 * g + 1][nt], a1, c0, c1, o[2 * g + 1][nt]);
                     }
                 }
             }
+        }
+    };
+
+    for (int i = 0; i < mine; ++i) {
+        const int st = i % S;
+        if (i > 0 && (i & 31) == 0) {
+            pg = next;
+            pg2 = next2;
+        }
+        const bool ok0 = __shfl_sync(0xffffffffu, pg, i & 31) >= 0, ok1 = __shfl_sync(0xffffffffu, pg2, i & 31) >= 0;
+        if (!mbar_wait(&bars[warp][st], (i / S) & 1)) {
+            failed = i;
+            break;
+        }
+        const int k0 = (p_begin + i * WARPS) * 32;
+        const unsigned char* tp = ring + st * 2 * TB;
+        if (k0 >= all_lo && k0 + 32 <= all_hi && ok0 && ok1)
+            pair_step(std::false_type{}, tp, k0, true, true);
+        else if (ok0 || ok1)
+            pair_step(std::true_type{}, tp, k0, ok0, ok1);
+        __syncwarp();   // every lane has read the stage
+        const int nx = i + S;
+        if (nx < mine) {
+            if ((nx & 31) == 0) fetch_pages(nx, next, next2);
+            const bool same = (nx >> 5) == (i >> 5);
+            const int p = __shfl_sync(0xffffffffu, same ? pg : next, nx & 31);
+            const int p2 = __shfl_sync(0xffffffffu, same ? pg2 : next2, nx & 31);
+            if (lane == 0) issue(nx, p, p2);
         }
     }
     if (failed >= 0)   // let the copies in flight land (bounded again) and answer NaN
@@ -379,7 +425,7 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
             for (int x = 4; x < 32; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
             if (failed >= 0) s = __int_as_float(0x7fffffff);
             if (r == 0 && (!DUP || t < 2)) {
-                wo[u * (HD + 2) + HD] = m[nt][c];
+                wo[u * (HD + 2) + HD] = m[nt][c] * a.scale_log2;
                 wo[u * (HD + 2) + HD + 1] = s;
             }
 #pragma unroll
@@ -446,12 +492,12 @@ __global__ void __launch_bounds__(HD) k_kv4_merge(const AttnArgs a) {
 }
 
 struct Plan {
-    int nt, dup, utiles, nsplit, split_tiles;
+    int nt, dup, utiles, nsplit, split_pairs;
 };
 
 // How a call is cut. Units: the fewest columns that hold max_q rows of a group (four: both halves
 // of the weights in one operand), at most 32 (heads of 128: 16, for the registers). Splits: until
-// about four CTAs an SM are there, of at least 16 tiles (four a warp) each.
+// about four CTAs an SM are there, of at least 8 pairs (two a warp) each.
 Plan make_plan(int64_t B, int64_t Hkv, int64_t group, int64_t head_dim, int64_t max_q, int64_t max_kv,
                int64_t window) {
     Plan p{};
@@ -463,18 +509,18 @@ Plan make_plan(int64_t B, int64_t Hkv, int64_t group, int64_t head_dim, int64_t 
     int64_t span = max_kv;
     if (window > 0) {
         const int64_t rows = (ut + group - 1) / group + 1;   // rows that a unit tile can touch
-        const int64_t w = window + (rows < max_q ? rows : max_q) + KV4_TILE;
+        const int64_t w = window + (rows < max_q ? rows : max_q) + 32;
         if (w < span) span = w;
     }
-    const int64_t tiles = (span + KV4_TILE - 1) / KV4_TILE;
+    const int64_t pairs = (span + 31) / 32;
     const int64_t ctas = B * Hkv * p.utiles;
     int64_t ns = (148 * 4 + ctas - 1) / ctas;
-    if (ns > tiles / 16) ns = tiles / 16;
+    if (ns > pairs / 8) ns = pairs / 8;
     if (ns > 64) ns = 64;
     if (ns < 1) ns = 1;
-    p.split_tiles = (int)((tiles + ns - 1) / ns);
-    if (p.split_tiles < 1) p.split_tiles = 1;
-    p.nsplit = (int)((tiles + p.split_tiles - 1) / p.split_tiles);
+    p.split_pairs = (int)((pairs + ns - 1) / ns);
+    if (p.split_pairs < 1) p.split_pairs = 1;
+    p.nsplit = (int)((pairs + p.split_pairs - 1) / p.split_pairs);
     if (p.nsplit < 1) p.nsplit = 1;
     return p;
 }
@@ -525,6 +571,7 @@ extern "C" int pulsar_op_kv4_attention(const void* q, int64_t q_row_stride, int6
                      "kv4_attention: page_size must be a power of two of at least 16, got %lld", (long long)page_size);
     PULSAR_CHECK_ARG(num_pages >= 0 && num_pages < (int64_t)1 << 31 && width >= 0 && width * page_size < (int64_t)1 << 30,
                      "kv4_attention: invalid page table");
+    PULSAR_CHECK_ARG(scale > 0.f, "kv4_attention: scale must be positive");
     PULSAR_CHECK_ARG(cu_q || (N == B && max_q == 1), "kv4_attention: without cu_q every sequence has one row");
     if (N == 0 || B == 0) return PULSAR_OK;
     PULSAR_CHECK_ARG(q && pages && kv_lens && out && (block_table || width == 0), "kv4_attention: null pointer");
@@ -541,7 +588,7 @@ extern "C" int pulsar_op_kv4_attention(const void* q, int64_t q_row_stride, int6
                p.nsplit > 1 ? ws + N * Hq * p.nsplit * head_dim : nullptr, q_row_stride, q_head_stride,
                page_size / KV4_TILE * 20 * head_dim, (int)N, (int)Hq, (int)Hkv, (int)(Hq / Hkv), (int)num_pages,
                (int)width, __builtin_ctzll((unsigned long long)page_size), (int)max_q, (int)window, p.nsplit,
-               p.split_tiles, scale * 1.4426950408889634f};
+               p.split_pairs, scale * 1.4426950408889634f};
     cudaStream_t st = (cudaStream_t)stream;
     int rc;
     if (head_dim == 64)

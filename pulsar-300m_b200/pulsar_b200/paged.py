@@ -16,6 +16,7 @@ checked on the host: the kernels hold every access inside the tensors (each func
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 
 import torch
@@ -25,48 +26,63 @@ from . import _lib
 _BF16, _F32, _I32, _I64, _U8 = torch.bfloat16, torch.float32, torch.int32, torch.int64, torch.uint8
 
 
-def _check(cond: bool, msg: str) -> None:
-    if not cond:
-        raise RuntimeError(msg)
-
-
-def _stream(t: torch.Tensor) -> int:
-    return torch.cuda.current_stream(t.device).cuda_stream
+def _refuse(msg: str):
+    raise RuntimeError(msg)
 
 
 def _p(t):
     return None if t is None else t.data_ptr()
 
 
+def _call(name, dev, *args):
+    """The library's entry point on dev's current stream, with dev current."""
+    stream = torch.cuda.current_stream(dev).cuda_stream
+    if torch.cuda.current_device() == dev.index:
+        _lib.call(name, *args, stream)
+    else:
+        with torch.cuda.device(dev):
+            _lib.call(name, *args, stream)
+
+
+# The checks below run before every launch of a few microseconds: conditions first, texts only when
+# they fail.
 def _vector(t, name, dtype, n, dev):
-    _check(t.is_cuda and t.device == dev and t.dtype == dtype and t.dim() == 1 and t.is_contiguous(),
-           f"{name} must be a contiguous 1-D {str(dtype)[6:]} tensor on {dev}")
-    _check(n is None or t.shape[0] == n, f"{name} must have {n} elements, got {t.shape[0]}")
+    if t.dtype != dtype or t.dim() != 1 or t.device != dev or not t.is_contiguous():
+        _refuse(f"{name} must be a contiguous 1-D {str(dtype)[6:]} tensor on {dev}")
+    if n is not None and t.shape[0] != n:
+        _refuse(f"{name} must have {n} elements, got {t.shape[0]}")
+
+
+def _check_page(head_dim, page_size):
+    if head_dim not in (64, 128):
+        _refuse(f"head_dim must be 64 or 128, got {head_dim}")
+    if page_size < 16 or page_size & (page_size - 1) or page_size > 65536:
+        _refuse(f"page_size must be a power of two from 16 to 65536, got {page_size}")
 
 
 def kv4_page_bytes(head_dim: int = 64, page_size: int = 64) -> int:
     """Bytes of one kv head's part of a page: 20 * head_dim for every 16 tokens."""
-    _check(head_dim in (64, 128), f"head_dim must be 64 or 128, got {head_dim}")
-    _check(page_size >= 16 and page_size & (page_size - 1) == 0 and page_size <= 65536,
-           f"page_size must be a power of two from 16 to 65536, got {page_size}")
+    _check_page(head_dim, page_size)
     return 20 * head_dim * page_size // 16
 
 
 def kv4_pages(num_pages: int, num_kv_heads: int, head_dim: int = 64, page_size: int = 64, device="cuda"):
     """An empty cache: uint8 [num_pages, num_kv_heads, kv4_page_bytes(head_dim, page_size)]."""
-    _check(num_pages >= 1 and num_kv_heads >= 1, "a cache needs at least one page and one kv head")
+    if num_pages < 1 or num_kv_heads < 1:
+        _refuse("a cache needs at least one page and one kv head")
     return torch.zeros(num_pages, num_kv_heads, kv4_page_bytes(head_dim, page_size), dtype=_U8, device=device)
 
 
 def _cache(pages, head_dim):
     """(number of pages, kv heads, page size) of a cache tensor."""
-    _check(pages.is_cuda and pages.dtype == _U8 and pages.dim() == 3 and pages.is_contiguous(),
-           "pages must be a contiguous uint8 CUDA tensor [num_pages, kv heads, page bytes]")
+    if pages.dtype != _U8 or pages.dim() != 3 or not pages.is_cuda or not pages.is_contiguous():
+        _refuse("pages must be a contiguous uint8 CUDA tensor [num_pages, kv heads, page bytes]")
     num, hkv, nbytes = pages.shape
-    page_size = nbytes * 16 // (20 * head_dim) if head_dim else 0
-    _check(head_dim in (64, 128), f"head_dim must be 64 or 128, got {head_dim}")
-    _check(page_size >= 16 and page_size & (page_size - 1) == 0 and page_size * 20 * head_dim == nbytes * 16,
-           f"a page of {nbytes} bytes is no power of two of tokens (at least 16) with head_dim {head_dim}")
+    page_size = nbytes * 16 // (20 * head_dim) if head_dim > 0 else 0
+    if head_dim not in (64, 128) or page_size < 16 or page_size & (page_size - 1) or (
+            page_size * 20 * head_dim != nbytes * 16):
+        _refuse(f"pages of {nbytes} bytes a kv head: no cache of head_dim {head_dim} (64 or 128) with a power of two "
+                "of tokens, at least 16, in a page")
     return num, hkv, page_size
 
 
@@ -79,9 +95,12 @@ def rope_tables(max_pos: int, rot_dim: int = 64, theta: float = 10000.0, *, scal
     divides the frequencies that turn fewer than ``beta_slow`` times within ``base_len``, keeps those
     that turn more than ``beta_fast`` times, and blends in between.
     """
-    _check(rot_dim >= 2 and rot_dim % 2 == 0, f"rot_dim must be even, got {rot_dim}")
-    _check(scaling in ("none", "linear", "ntk", "yarn"), f"unknown scaling {scaling!r}")
-    _check(factor >= 1.0 and max_pos >= 1, "factor and max_pos must be at least 1")
+    if rot_dim < 2 or rot_dim % 2:
+        _refuse(f"rot_dim must be even, got {rot_dim}")
+    if scaling not in ("none", "linear", "ntk", "yarn"):
+        _refuse(f"unknown scaling {scaling!r}")
+    if factor < 1.0 or max_pos < 1:
+        _refuse("factor and max_pos must be at least 1")
     i = torch.arange(0, rot_dim, 2, dtype=torch.float64)
     if scaling == "ntk" and rot_dim > 2:
         theta = theta * factor ** (rot_dim / (rot_dim - 2))
@@ -97,12 +116,16 @@ def rope_tables(max_pos: int, rot_dim: int = 64, theta: float = 10000.0, *, scal
 
 
 def _heads(x, name, n, hd, dev):
-    _check(x.is_cuda and x.device == dev and x.dtype == _BF16 and x.dim() == 3,
-           f"{name} must be a bfloat16 tensor [tokens, heads, head_dim] on {dev}")
-    _check(x.shape[0] == n and x.shape[2] == hd, f"{name} must be [{n}, heads, {hd}], got {list(x.shape)}")
-    _check(x.numel() == 0 or (x.stride(2) == 1 and x.stride(0) % 8 == 0 and x.stride(1) % 8 == 0
-                              and x.data_ptr() % 16 == 0),
-           f"{name} needs stride(-1) == 1, other strides a multiple of 8 and 16-byte alignment")
+    """Checks x [tokens, heads, head_dim] and gives (heads, token stride, head stride)."""
+    if x.dtype != _BF16 or x.dim() != 3 or x.device != dev:
+        _refuse(f"{name} must be a bfloat16 tensor [tokens, heads, head_dim] on {dev}")
+    rows, heads, dims = x.shape
+    if rows != n or dims != hd:
+        _refuse(f"{name} must be [{n}, heads, {hd}], got {list(x.shape)}")
+    st, sh, sd = x.stride()
+    if n and heads and (sd != 1 or st % 8 or sh % 8 or x.data_ptr() % 16):
+        _refuse(f"{name} needs stride(-1) == 1, other strides a multiple of 8 and 16-byte alignment")
+    return heads, st, sh
 
 
 def kv4_append(q, k, v, pages, slots, positions=None, cos=None, sin=None, *, q_norm=None, k_norm=None,
@@ -120,47 +143,46 @@ def kv4_append(q, k, v, pages, slots, positions=None, cos=None, sin=None, *, q_n
     weights of the norm w x / sqrt(mean(x^2) + eps), before the rotation; None: no norm. q_gain: fp32
     [max_pos], a factor of the query of each position (the long-context temperature of YaRN layers).
     """
-    _check(k.dim() == 3, "k must be [tokens, heads, head_dim]")
-    n, hkv, hd = k.shape
+    if k.dim() != 3:
+        _refuse("k must be [tokens, heads, head_dim]")
+    n, _, hd = k.shape
     dev = pages.device
     num, cache_heads, page_size = _cache(pages, hd)
-    _check(hkv == cache_heads, f"k has {hkv} heads, the cache {cache_heads}")
-    _heads(k, "k", n, hd, dev)
-    _heads(v, "v", n, hd, dev)
-    _check(v.shape[1] == hkv, f"v has {v.shape[1]} heads, k {hkv}")
-    hq = 0
+    hkv, kt, kh = _heads(k, "k", n, hd, dev)
+    v_heads, vt, vh = _heads(v, "v", n, hd, dev)
+    if hkv != cache_heads or v_heads != hkv:
+        _refuse(f"k has {hkv} heads, v {v_heads}, the cache {cache_heads}")
+    hq = qt = qh = 0
+    out = None
     if q is not None:
-        _heads(q, "q", n, hd, dev)
-        hq = q.shape[1]
+        hq, qt, qh = _heads(q, "q", n, hd, dev)
+        out = torch.empty(n, hq, hd, dtype=_BF16, device=dev)
     _vector(slots, "slots", _I64, n, dev)
     rot = max_pos = 0
     if cos is not None:
-        _check(sin is not None and cos.shape == sin.shape and cos.dim() == 2, "cos and sin must be [max_pos, rot / 2]")
-        for x in (cos, sin):
-            _check(x.is_cuda and x.device == dev and x.dtype == _F32 and x.is_contiguous(),
-                   "cos and sin must be contiguous float32 tensors on the cache's device")
-        max_pos, rot = cos.shape[0], 2 * cos.shape[1]
-        _check(0 < rot <= hd and rot % (2 if interleaved else 16) == 0,
-               f"rotated dims must be a multiple of {2 if interleaved else 16} up to {hd}, got {rot}")
+        if sin is None or cos.dim() != 2 or cos.shape != sin.shape:
+            _refuse("cos and sin must be [max_pos, rot / 2]")
+        if cos.dtype != _F32 or sin.dtype != _F32 or cos.device != dev or sin.device != dev or not (
+                cos.is_contiguous() and sin.is_contiguous()):
+            _refuse(f"cos and sin must be contiguous float32 tensors on {dev}")
+        max_pos, rot = cos.shape
+        rot *= 2
+        if not 0 < rot <= hd or rot % (2 if interleaved else 16):
+            _refuse(f"rotated dims must be a multiple of {2 if interleaved else 16} up to {hd}, got {rot}")
     if q_gain is not None:
-        _vector(q_gain, "q_gain", _F32, None, dev)
-        _check(cos is None or q_gain.shape[0] == max_pos, "q_gain must have a factor for each row of cos")
+        _vector(q_gain, "q_gain", _F32, None if cos is None else max_pos, dev)
         max_pos = q_gain.shape[0]
     if rot or q_gain is not None:
-        _check(positions is not None and max_pos > 0, "rotation and q_gain need positions and non-empty tables")
+        if positions is None or max_pos < 1:
+            _refuse("rotation and q_gain need positions and tables that are not empty")
         _vector(positions, "positions", _I32, n, dev)
     for w, name, heads in ((q_norm, "q_norm", hq), (k_norm, "k_norm", hkv)):
-        _check(w is None or (w.is_cuda and w.device == dev and w.dtype == _F32 and w.is_contiguous()
-                             and w.shape == (heads, hd)),
-               f"{name} must be a contiguous float32 tensor [{heads}, {hd}] on the cache's device")
-    out = torch.empty(n, hq, hd, dtype=_BF16, device=dev) if q is not None else None
+        if w is not None and (w.dtype != _F32 or w.shape != (heads, hd) or w.device != dev or not w.is_contiguous()):
+            _refuse(f"{name} must be a contiguous float32 tensor [{heads}, {hd}] on {dev}")
     if n:
-        st = (C.c_int64 * 6)(*((q.stride(0), q.stride(1)) if hq else (0, 0)), k.stride(0), k.stride(1), v.stride(0),
-                             v.stride(1))
-        with torch.cuda.device(dev):
-            _lib.call("pulsar_op_kv4_append", _p(q), _p(k), _p(v), st, n, hq, hkv, hd, _p(q_norm), _p(k_norm), eps,
-                      _p(cos), _p(sin), rot, max_pos, int(interleaved), _p(q_gain), _p(positions), _p(slots),
-                      _p(pages), num, page_size, _p(out), _stream(pages))
+        _call("pulsar_op_kv4_append", dev, _p(q), k.data_ptr(), v.data_ptr(), (C.c_int64 * 6)(qt, qh, kt, kh, vt, vh),
+              n, hq, hkv, hd, _p(q_norm), _p(k_norm), eps, _p(cos), _p(sin), rot, max_pos, int(interleaved),
+              _p(q_gain), _p(positions), slots.data_ptr(), pages.data_ptr(), num, page_size, _p(out))
     return out
 
 
@@ -172,12 +194,18 @@ def kv4_read(pages, slots, head_dim: int = 64):
     _vector(slots, "slots", _I64, None, dev)
     n = slots.shape[0]
     k = torch.empty(n, hkv, head_dim, dtype=_BF16, device=dev)
-    v = torch.empty_like(k)
+    v = torch.empty(n, hkv, head_dim, dtype=_BF16, device=dev)
     if n:
-        with torch.cuda.device(dev):
-            _lib.call("pulsar_op_kv4_read", _p(pages), num, page_size, hkv, head_dim, _p(slots), n, _p(k), _p(v),
-                      _stream(pages))
+        _call("pulsar_op_kv4_read", dev, pages.data_ptr(), num, page_size, hkv, head_dim, slots.data_ptr(), n,
+              k.data_ptr(), v.data_ptr())
     return k, v
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace(n, hq, hkv, hd, b, max_q, max_kv, window):
+    need = C.c_int64()
+    _lib.call("pulsar_op_kv4_attention_workspace", n, hq, hkv, hd, b, max_q, max_kv, window, C.byref(need))
+    return need.value
 
 
 def kv4_attention(q, pages, block_table, kv_lens, cu_q=None, *, max_q: int = 1, max_kv: int | None = None,
@@ -194,38 +222,41 @@ def kv4_attention(q, pages, block_table, kv_lens, cu_q=None, *, max_q: int = 1, 
     A row that sees no key is zero. Lengths past the table end there; pages numbered outside the cache
     are left out as if masked; rows that no sequence claims are not written.
     """
-    _check(q.is_cuda and q.dtype == _BF16 and q.dim() == 3, "q must be a bfloat16 CUDA tensor [rows, heads, head_dim]")
+    dev = pages.device
+    if q.dtype != _BF16 or q.dim() != 3 or q.device != dev:
+        _refuse(f"q must be a bfloat16 tensor [rows, heads, head_dim] on {dev}")
     n, hq, hd = q.shape
     num, hkv, page_size = _cache(pages, hd)
-    dev = pages.device
-    _check(q.device == dev, f"q is on {q.device}, the cache on {dev}")
-    _check(q.numel() == 0 or (q.stride(2) == 1 and q.stride(0) % 2 == 0 and q.stride(1) % 2 == 0
-                              and q.data_ptr() % 4 == 0),
-           "q needs stride(-1) == 1, even strides and 4-byte alignment")
-    _check(hq >= hkv and hq % hkv == 0, f"{hq} query heads over {hkv} kv heads")
-    _check(block_table.is_cuda and block_table.device == dev and block_table.dtype == _I32 and block_table.dim() == 2
-           and block_table.is_contiguous(), "block_table must be a contiguous int32 tensor [sequences, width]")
+    qt, qh, qd = q.stride()
+    if n and (qd != 1 or qt % 2 or qh % 2 or q.data_ptr() % 4):
+        _refuse("q needs stride(-1) == 1, even strides and 4-byte alignment")
+    if hq < hkv or hq % hkv:
+        _refuse(f"{hq} query heads over {hkv} kv heads")
+    if block_table.dtype != _I32 or block_table.dim() != 2 or block_table.device != dev or (
+            not block_table.is_contiguous()):
+        _refuse(f"block_table must be a contiguous int32 tensor [sequences, width] on {dev}")
     b, width = block_table.shape
     _vector(kv_lens, "kv_lens", _I32, b, dev)
-    if cu_q is None:
-        _check(n == b and max_q == 1, f"without cu_q every sequence has one row (max_q 1): {n} rows of {b} sequences")
-    else:
+    if cu_q is not None:
         _vector(cu_q, "cu_q", _I32, b + 1, dev)
-    _check(max_q >= 1 and window >= 0, "max_q must be at least 1, window at least 0")
+    elif n != b or max_q != 1:
+        _refuse(f"without cu_q every sequence has one row (max_q 1): {n} rows of {b} sequences")
     if max_kv is None:
         max_kv = max(1, width * page_size)
-    _check(max_kv >= 1, "max_kv must be at least 1")
+    if max_q < 1 or window < 0 or max_kv < 1:
+        _refuse("max_q and max_kv must be at least 1, window at least 0")
+    if scale is None:
+        scale = hd ** -0.5
+    elif not scale > 0:
+        _refuse(f"scale must be positive, got {scale}")
     if out is None:
         out = torch.empty(n, hq, hd, dtype=_BF16, device=dev)
-    else:
-        _check(out.is_cuda and out.device == dev and out.dtype == _BF16 and out.shape == q.shape
-               and out.is_contiguous(), "out must be a contiguous bfloat16 tensor of q's shape")
+    elif out.dtype != _BF16 or out.shape != q.shape or out.device != dev or not out.is_contiguous():
+        _refuse("out must be a contiguous bfloat16 tensor of q's shape")
     if n and b:
-        need = C.c_int64()
-        _lib.call("pulsar_op_kv4_attention_workspace", n, hq, hkv, hd, b, max_q, max_kv, window, C.byref(need))
-        ws = torch.empty(need.value, dtype=_U8, device=dev) if need.value else None
-        with torch.cuda.device(dev):
-            _lib.call("pulsar_op_kv4_attention", _p(q), q.stride(0), q.stride(1), n, hq, hd, _p(pages), num, page_size,
-                      hkv, _p(block_table), b, width, _p(kv_lens), _p(cu_q), max_q, max_kv,
-                      hd ** -0.5 if scale is None else scale, window, _p(ws), need.value, _p(out), _stream(pages))
+        need = _workspace(n, hq, hkv, hd, b, max_q, max_kv, window)
+        ws = torch.empty(need, dtype=_U8, device=dev) if need else None
+        _call("pulsar_op_kv4_attention", dev, q.data_ptr(), qt, qh, n, hq, hd, pages.data_ptr(), num, page_size, hkv,
+              block_table.data_ptr(), b, width, kv_lens.data_ptr(), _p(cu_q), max_q, max_kv,
+              scale, window, _p(ws), need, out.data_ptr())
     return out
