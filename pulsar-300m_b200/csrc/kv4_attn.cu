@@ -3,11 +3,11 @@
 // Row j of the n_b query rows of sequence b has position pos = len_b - n_b + j and sees the keys
 // max(0, pos - window + 1) .. pos (window 0: all of 0 .. pos):
 //   out = sum_k p_k v_k / sum_k p_k,  p_k = exp(scale q.k_k - m)
-// with k = s c + z per group of 32 dims, so q.k = sum_g s_g (q.(16 + c))_g + (z_g - 16 s_g) sum(q)_g:
-// the codes enter the matrix instruction as small whole numbers (exact in bf16) and s, z are applied
-// in fp32 to its results. Values: O = sum_k (p_k s_kg) (c - f) + sum_k p_k (z_kg + f s_kg), f = -16
-// for even and 31 for odd tokens: s goes into the weights, whose bf16 hi and lo halves are both
-// multiplied (|x - hi - lo| <= 2^-16 |x|), and the second sum is a scalar per (row, group).
+// with k = s c + z per group of 32 dims, so q.k = sum_g s_g (q.c)_g + z_g sum(q)_g: the codes enter
+// the matrix instruction as they are (exact, see unpack) and s, z are applied in fp32 to its
+// results. Values: O = sum_k (p_k s_kg) c + sum_k p_k z_kg: s goes into the weights, whose bf16 hi
+// and lo halves are both multiplied (|x - hi - lo| <= 2^-16 |x|), and the second sum is a scalar per
+// (row, group).
 //
 // A unit is a (query row, head of the kv head's group). CTA (split and unit tile, kv head,
 // sequence): four warps, each walking every fourth pair of 16-token tiles of the split's range
@@ -17,8 +17,8 @@
 // weights pass through movmatrix into the B operand of O^T = V^T P^T. Up to four units the eight
 // columns hold every unit twice and the copies carry the hi and the lo halves.
 //
-// The softmax keeps a running maximum per unit that moves only when a score exceeds it by more
-// than 2^LAZY (l and O use the same maximum, so the result does not depend on when it moves).
+// The softmax keeps a maximum per unit that moves only when a sum of weights relative to it passes
+// 2^LAZY (l and O use the same maximum, so the result does not depend on when it moves).
 // Keys that a unit does not see get weight 0 by selection, not by multiplication: pages past a
 // sequence's end may hold anything, NaN included. Tiles of a page outside the cache are skipped.
 //
@@ -38,7 +38,7 @@ using namespace pulsar;
 namespace {
 
 constexpr int WARPS = 4;
-constexpr float LAZY = 8.f;
+constexpr int LAZY = 30;
 constexpr float NEG = -1e30f;   // "no key yet": finite, so differences with it are defined
 
 struct AttnArgs {
@@ -83,16 +83,24 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
-// Operand register i of a key word: the bf16 pair 16 + c (the nibble goes to bits 3..6 of each
-// half, where a bf16 in [16, 32) holds its whole part).
-__device__ __forceinline__ uint32_t unpack_k(uint32_t w, int i) {
-    return ((i == 0 ? w << 3 : w >> (4 * i - 3)) & 0x00780078u) | 0x41804180u;
+// Operand registers of a code word: its nibbles 0 and 1 of both halves are bf16 bit patterns as they
+// stand, c 2^-133 and 16 c 2^-133 (bits 0..7 of a bf16 count in steps of 2^-133 across the border of
+// the subnormal numbers, and the matrix instruction takes subnormal operands exactly); nibbles 2 and
+// 3 need one shift for the two. No offset, no conversion.
+__device__ __forceinline__ void unpack(uint32_t w, uint32_t& r0, uint32_t& r1, uint32_t& r2, uint32_t& r3) {
+    const uint32_t v = w >> 8;
+    r0 = w & 0x000f000fu;
+    r1 = w & 0x00f000f0u;
+    r2 = v & 0x000f000fu;
+    r3 = v & 0x00f000f0u;
 }
-// Operand register i of a value word: 16 + c for the even token of the pair, c - 31 for the odd one
-// (sign and complemented nibble by the same exclusive or): the offsets cancel in the sums over
-// tokens instead of growing, and what is left of them is in the scalar sums.
-__device__ __forceinline__ uint32_t unpack_v(uint32_t w, int i) {
-    return ((i == 0 ? w << 3 : w >> (4 * i - 3)) & 0x00780078u) ^ 0xC1F84180u;
+constexpr int CODE_EXP = 133;   // a code c is the operand c 2^-133
+constexpr int LIFT = 60;        // queries and weights are scaled by 2^60, so results are normal numbers
+constexpr float pow2(int e) {   // 2^e (constant expressions only)
+    float x = 1.f;
+    for (; e > 0; --e) x *= 2.f;
+    for (; e < 0; ++e) x *= 0.5f;
+    return x;
 }
 
 __device__ __forceinline__ uint32_t pack(float a, float b) {
@@ -190,7 +198,7 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
 
     // queries: B operand of step j (dims 16 j ..): unit n = lane / 4, dims 2t, 2t + 1 and 8 further
     uint32_t qf[NT][2 * MT];
-    float qsum[NT][NG][2];   // sum of q over the group, for the thread's two columns
+    float qsum[NT][NG][2];   // sum of q over the group (in the units of the scores), for the thread's columns
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int u = u0 + (DUP ? (r & 3) : nt * 8 + r);
@@ -206,8 +214,14 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
             for (int i = 0; i < 4; ++i) s += lo_of(qf[nt][4 * g4 + i]) + hi_of(qf[nt][4 * g4 + i]);
             s += __shfl_xor_sync(0xffffffffu, s, 1);
             s += __shfl_xor_sync(0xffffffffu, s, 2);
+            s *= pow2(LIFT - CODE_EXP);
             qsum[nt][g4][0] = __shfl_sync(0xffffffffu, s, 8 * t);
             qsum[nt][g4][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * MT; ++i) {   // odd registers meet 16 c
+            const float f = i & 1 ? pow2(LIFT - 4) : pow2(LIFT);
+            qf[nt][i] = pack(lo_of(qf[nt][i]) * f, hi_of(qf[nt][i]) * f);
         }
     }
     int hi[NT][2], lo[NT][2];   // keys that the thread's columns see
@@ -222,22 +236,22 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
         }
     const int all_lo = low(last), all_hi = first + 1;   // keys in [all_lo, all_hi) are seen by every unit
 
-    // m: running maximum of the unscaled scores; top: the score that moves it; nm = -scale m
-    float o[MT][NT][4], zacc[NT][NG][2], m[NT][2], top[NT][2], nm[NT][2], l[NT][2];
-    const float lazy = LAZY / a.scale_log2;
+    // Scores come in units of 2^(LIFT - CODE_EXP); m: their running maximum, nm = LIFT - scale m, so
+    // that weights are 2^LIFT exp2(scale (s - m))
+    float o[MT][NT][4], zacc[NT][NG][2], m[NT][2], nm[NT][2], l[NT][2];
+    const float scale = a.scale_log2 * pow2(CODE_EXP - LIFT);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int i = 0; i < MT; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
 #pragma unroll
         for (int g = 0; g < NG; ++g) zacc[nt][g][0] = zacc[nt][g][1] = 0.f;
-        m[nt][0] = m[nt][1] = NEG;
-        top[nt][0] = top[nt][1] = NEG + lazy;
+        m[nt][0] = m[nt][1] = NEG * pow2(LIFT - CODE_EXP);
         nm[nt][0] = nm[nt][1] = -NEG * a.scale_log2;
         l[nt][0] = l[nt][1] = 0.f;
     }
-    const float off = r & 1 ? 31.f : -16.f;                          // of the thread's tokens r and r + 8
-    const uint32_t cut_lo = t < 2 ? 0x4444u : 0x1044u, cut_hi = t < 2 ? 0x4444u : 0x3244u;
+    // columns 4..7 of the doubled units (t >= 2) carry the lo halves: x = w lo_w + hi lo_h
+    const float lo_w = t < 2 ? 0.f : 1.f, lo_h = t < 2 ? 1.f : -1.f;
     int failed = -1;   // the pair whose copy did not land within the bound
 
     // one pair of tiles; EDGE: some of its keys are not seen by some unit, or a page is missing
@@ -256,11 +270,10 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
                 *reinterpret_cast<uint4*>(&kp[0][0] + y) = *reinterpret_cast<const uint4*>(kt + T::KP + r * 8 * NG + y * 4);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                const uint32_t wr = kc[g >> 1][g & 1], w8 = kc[g >> 1][2 + (g & 1)];
-                const uint32_t a0[4] = {unpack_k(wr, 0), unpack_k(w8, 0), unpack_k(wr, 1), unpack_k(w8, 1)};
-                const uint32_t a1[4] = {unpack_k(wr, 2), unpack_k(w8, 2), unpack_k(wr, 3), unpack_k(w8, 3)};
-                const float s0 = lo_of(kp[0][g]), z0 = hi_of(kp[0][g]), s8 = lo_of(kp[1][g]), z8 = hi_of(kp[1][g]);
-                const float y0 = fmaf(-16.f, s0, z0), y8 = fmaf(-16.f, s8, z8);
+                uint32_t a0[4], a1[4];
+                unpack(kc[g >> 1][g & 1], a0[0], a0[2], a1[0], a1[2]);
+                unpack(kc[g >> 1][2 + (g & 1)], a0[1], a0[3], a1[1], a1[3]);
+                const float s0 = lo_of(kp[0][g]), y0 = hi_of(kp[0][g]), s8 = lo_of(kp[1][g]), y8 = hi_of(kp[1][g]);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float acc[4] = {0.f, 0.f, 0.f, 0.f};
@@ -280,21 +293,37 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
             }
         }
         bool see[2][NT][4], up = false;
+        float p[2][NT][4], ls[NT][2];
+        auto weigh = [&]() {
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+            for (int nt = 0; nt < NT; ++nt) {
+                ls[nt][0] = l[nt][0];
+                ls[nt][1] = l[nt][1];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+                for (int x = 0; x < 2; ++x)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int c = e & 1;
-                    if (EDGE) {
+                    for (int e = 0; e < 4; ++e) {
+                        p[x][nt][e] = ex2(fmaf(sc[x][nt][e], scale, nm[nt][e & 1]));
+                        ls[nt][e & 1] += p[x][nt][e];
+                    }
+            }
+        };
+        if (EDGE) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
                         const int k = k0 + 16 * x + r + (e < 2 ? 0 : 8);
-                        see[x][nt][e] = (x ? ok1 : ok0) && k >= lo[nt][c] && k < hi[nt][c];
+                        see[x][nt][e] = (x ? ok1 : ok0) && k >= lo[nt][e & 1] && k < hi[nt][e & 1];
                         if (!see[x][nt][e]) sc[x][nt][e] = -INFINITY;
                     }
-                    up |= sc[x][nt][e] > top[nt][c];
-                }
-        if (__any_sync(0xffffffffu, up)) {
+        }
+        weigh();
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) up |= ls[nt][0] > pow2(LIFT + LAZY) || ls[nt][1] > pow2(LIFT + LAZY);
+        if (__any_sync(0xffffffffu, up)) {   // the sums would soon leave the range: move the maximum, weigh again
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -304,10 +333,9 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
                     x = fmaxf(x, m[nt][c]);
-                    const float f = ex2((m[nt][c] - x) * a.scale_log2);
+                    const float f = ex2((m[nt][c] - x) * scale);
                     m[nt][c] = x;
-                    top[nt][c] = x + lazy;
-                    nm[nt][c] = -x * a.scale_log2;
+                    nm[nt][c] = fmaf(-x, scale, (float)LIFT);
                     l[nt][c] *= f;
 #pragma unroll
                     for (int g = 0; g < NG; ++g) zacc[nt][g][c] *= f;
@@ -317,17 +345,13 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
                         o[y][nt][c + 2] *= f;
                     }
                 }
+            weigh();
         }
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int c = e & 1;
-                    sc[x][nt][e] = ex2(fmaf(sc[x][nt][e], a.scale_log2, nm[nt][c]));
-                    l[nt][c] += sc[x][nt][e];
-                }
+        for (int nt = 0; nt < NT; ++nt) {
+            l[nt][0] = ls[nt][0];
+            l[nt][1] = ls[nt][1];
+        }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             const unsigned char* vt = tp + x * TB;
@@ -340,40 +364,45 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
                 *reinterpret_cast<uint4*>(&vp[0][0] + y) = *reinterpret_cast<const uint4*>(vt + T::VP + r * 8 * NG + y * 4);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                const uint32_t w0 = vc[g >> 1][2 * (g & 1)], w1 = vc[g >> 1][2 * (g & 1) + 1];
-                const uint32_t a0[4] = {unpack_v(w0, 0), unpack_v(w0, 1), unpack_v(w1, 0), unpack_v(w1, 1)};
-                const uint32_t a1[4] = {unpack_v(w0, 2), unpack_v(w0, 3), unpack_v(w1, 2), unpack_v(w1, 3)};
-                const float s0 = lo_of(vp[0][g]), s8 = lo_of(vp[1][g]);
-                const float z0 = fmaf(off, s0, hi_of(vp[0][g])), z8 = fmaf(off, s8, hi_of(vp[1][g]));
+                uint32_t a0[4], a1[4];
+                unpack(vc[g >> 1][2 * (g & 1)], a0[0], a0[1], a1[0], a1[1]);
+                unpack(vc[g >> 1][2 * (g & 1) + 1], a0[2], a0[3], a1[2], a1[3]);
+                const float s0 = lo_of(vp[0][g]), z0 = hi_of(vp[0][g]), s8 = lo_of(vp[1][g]), z8 = hi_of(vp[1][g]);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    const float* p = sc[x][nt];
-                    float w[4] = {p[0] * s0, p[1] * s0, p[2] * s8, p[3] * s8};
+                    const float* pp = p[x][nt];
+                    float w[4] = {pp[0] * s0, pp[1] * s0, pp[2] * s8, pp[3] * s8};
                     float* za = zacc[nt][g];
                     if (EDGE) {   // what a unit does not see may hold anything: left out, not multiplied by 0
                         const bool* y = see[x][nt];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             w[e] = y[e] ? w[e] : 0.f;
-                            za[e & 1] += y[e] ? p[e] * (e < 2 ? z0 : z8) : 0.f;
+                            za[e & 1] += y[e] ? pp[e] * (e < 2 ? z0 : z8) : 0.f;
                         }
                     } else {
-                        za[0] = fmaf(p[0], z0, fmaf(p[2], z8, za[0]));
-                        za[1] = fmaf(p[1], z0, fmaf(p[3], z8, za[1]));
+                        za[0] = fmaf(pp[0], z0, fmaf(pp[2], z8, za[0]));
+                        za[1] = fmaf(pp[1], z0, fmaf(pp[3], z8, za[1]));
                     }
-                    uint32_t pa = pack(w[0], w[1]), pb = pack(w[2], w[3]);
-                    if (DUP) {   // columns 4..7 (t >= 2) carry the lo halves: w less its hi half
-                        pa = pack(w[0] - __uint_as_float(__byte_perm(pa, 0, cut_lo)),
-                                  w[1] - __uint_as_float(__byte_perm(pa, 0, cut_hi)));
-                        pb = pack(w[2] - __uint_as_float(__byte_perm(pb, 0, cut_lo)),
-                                  w[3] - __uint_as_float(__byte_perm(pb, 0, cut_hi)));
+                    float wh[4];   // hi halves, cut
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) wh[e] = hi_of(__float_as_uint(w[e]));
+                    uint32_t pa, pb;
+                    if (DUP) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) w[e] = fmaf(wh[e], lo_h, w[e] * lo_w);
+                        pa = pack(w[0], w[1]);
+                        pb = pack(w[2], w[3]);
+                    } else {
+                        pa = __byte_perm(__float_as_uint(w[0]), __float_as_uint(w[1]), 0x7632);
+                        pb = __byte_perm(__float_as_uint(w[2]), __float_as_uint(w[3]), 0x7632);
                     }
                     const uint32_t b0 = movmatrix(pa), b1 = movmatrix(pb);
                     mma16816(o[2 * g][nt], a0, b0, b1, o[2 * g][nt]);
                     mma16816(o[2 * g + 1][nt], a1, b0, b1, o[2 * g + 1][nt]);
                     if (!DUP) {
-                        const uint32_t c0 = movmatrix(pack(w[0] - lo_of(pa), w[1] - hi_of(pa)));
-                        const uint32_t c1 = movmatrix(pack(w[2] - lo_of(pb), w[3] - hi_of(pb)));
+                        const uint32_t c0 = movmatrix(pack(w[0] - wh[0], w[1] - wh[1]));
+                        const uint32_t c1 = movmatrix(pack(w[2] - wh[2], w[3] - wh[3]));
                         mma16816(o[2 * g][nt], a0, c0, c1, o[2 * g][nt]);
                         mma16816(o[2 * g + 1][nt], a1, c0, c1, o[2 * g + 1][nt]);
                     }
@@ -425,21 +454,24 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
             for (int x = 4; x < 32; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
             if (failed >= 0) s = __int_as_float(0x7fffffff);
             if (r == 0 && (!DUP || t < 2)) {
-                wo[u * (HD + 2) + HD] = m[nt][c] * a.scale_log2;
-                wo[u * (HD + 2) + HD + 1] = s;
+                wo[u * (HD + 2) + HD] = m[nt][c] * scale;
+                wo[u * (HD + 2) + HD + 1] = s * pow2(-LIFT);
             }
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 float z = zacc[nt][g][c];
 #pragma unroll
                 for (int x = 4; x < 32; x <<= 1) z += __shfl_xor_sync(0xffffffffu, z, x);
+                z *= pow2(-LIFT);
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         float v = o[2 * g + x][nt][c + 2 * e];
                         if (DUP) v += __shfl_xor_sync(0xffffffffu, v, 2);
-                        if (!DUP || t < 2) wo[u * (HD + 2) + 32 * g + 16 * x + 8 * e + r] = v + z;
+                        if (!DUP || t < 2)
+                            wo[u * (HD + 2) + 32 * g + 16 * x + 8 * e + r] =
+                                fmaf(v, pow2(CODE_EXP - LIFT - 4 * e), z);
                     }
             }
         }
