@@ -29,7 +29,8 @@ struct AppendArgs {
     const int32_t* pos;
     uint8_t* pages;
     __nv_bfloat16* qo;
-    int64_t n, num_slots, page_bytes;
+    int64_t num_slots, page_bytes;
+    uint32_t n;   // n (hq + 2 hkv) < 2^31
     int hq, hkv, page_shift, rot, max_pos, interleaved;
     float eps;
 };
@@ -42,29 +43,36 @@ __device__ __forceinline__ float lanes_sum(float v) {
     return v;
 }
 
+// x / s, correctly rounded, for s with 1 / s = inv correctly rounded: one step of Markstein's division
+// (IBM J. Res. Dev. 34, 1990). s has a bf16 significand, which is none of the method's exceptions.
+__device__ __forceinline__ float divide(float x, float s, float inv) {
+    const float q = __fmul_rn(x, inv);
+    return __fmaf_rn(__fmaf_rn(-q, s, x), inv, q);
+}
+
+constexpr float WHOLE = 12582912.f;   // 1.5 2^23: adding it rounds to a whole number, ties to even
+
 // Codes, s and z of the group of 32 dims whose 8-dim quarter this lane holds (x: its values).
 // Returns the lane's 8 codes, nibble j = dim j.
 __device__ __forceinline__ uint32_t quantise(const float* x, uint32_t& param) {
-    float mn = x[0], mx = x[0];
-    bool bad = false;
+    float mn = x[0], mx = x[0], bad = __fmul_rn(x[0], 0.f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 1; j < 8; ++j) {
         mn = fminf(mn, x[j]);
         mx = fmaxf(mx, x[j]);
-        bad |= !(fabsf(x[j]) < INFINITY);
+        bad = __fmaf_rn(x[j], 0.f, bad);   // NaN once a value is none or infinite
     }
+    if (!(bad == 0.f)) mx = INFINITY;
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
         mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        bad |= __shfl_xor_sync(0xffffffffu, (int)bad, o) != 0;
     }
     const __nv_bfloat16 zb = __float2bfloat16(mn);
     const float z = __bfloat162float(zb);
-    __nv_bfloat16 sb = __float2bfloat16(__fdiv_rn(__fsub_rn(mx, z), 15.f));
-    float s = __bfloat162float(sb);
-    bad |= !(fabsf(z) < INFINITY) || !(s < INFINITY);
-    if (bad) {   // the whole group reads back as NaN
+    const __nv_bfloat16 sb = __float2bfloat16(__fdiv_rn(__fsub_rn(mx, z), 15.f));
+    const float s = __bfloat162float(sb);
+    if (!(fabsf(z) < INFINITY && s < INFINITY)) {   // the whole group reads back as NaN
         param = 0x7fff7fffu;
         return 0u;
     }
@@ -73,195 +81,371 @@ __device__ __forceinline__ uint32_t quantise(const float* x, uint32_t& param) {
         return 0u;
     }
     param = (uint32_t)__bfloat16_as_ushort(zb) << 16 | __bfloat16_as_ushort(sb);
-    uint32_t p = 0;
+    const float inv = __frcp_rn(s);
+    float c[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float c = rintf(__fdiv_rn(__fsub_rn(x[j], z), s));
-        p |= (uint32_t)fminf(fmaxf(c, 0.f), 15.f) << (4 * j);
-    }
-    return p;
+    for (int j = 0; j < 8; ++j)
+        c[j] = __fsub_rn(__fadd_rn(fminf(fmaxf(divide(__fsub_rn(x[j], z), s, inv), 0.f), 15.f), WHOLE), WHOLE);
+    // four codes at a time as the digits of one whole number
+    uint32_t p[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        p[i] = __float_as_uint(__fmaf_rn(__fmaf_rn(__fmaf_rn(c[4 * i + 3], 16.f, c[4 * i + 2]), 16.f, c[4 * i + 1]),
+                                         16.f, c[4 * i]) + 8388608.f);
+    return __byte_perm(p[0], p[1], 0x5410);
 }
 
 // Transpose among the quad of lanes that holds a group: lane j = 2 b + n comes with the codes of
 // dims 16 b + 8 n + x (nibble x) and leaves with the word of x = 2j, 2j + 1: half e = x % 2, byte
 // b of the half, nibble n of the byte.
 __device__ __forceinline__ uint32_t quad_word(uint32_t p, int lane) {
-    uint32_t w = 0;
-    const int j = lane & 3;
+    uint32_t o[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {   // byte j of the codes of lane (b, n) = (i / 2, i % 2)
-        const uint32_t o = __shfl_sync(0xffffffffu, p, (lane & ~3) | i) >> (8 * j);
-        w |= (o & 0xfu) << (8 * (i >> 1) + 4 * (i & 1)) | ((o >> 4) & 0xfu) << (16 + 8 * (i >> 1) + 4 * (i & 1));
-    }
-    return w;
+    for (int i = 0; i < 4; ++i) o[i] = __shfl_sync(0xffffffffu, p, (lane & ~3) | i);
+    const uint32_t j = lane & 3, sel = j | (4 + j) << 4;   // byte j of each of the four
+    const uint32_t v = __byte_perm(__byte_perm(o[0], o[1], sel), __byte_perm(o[2], o[3], sel), 0x5410);
+    const uint32_t e0 = v & 0x0f0f0f0fu, e1 = (v >> 4) & 0x0f0f0f0fu;
+    return __byte_perm(e0 | e0 >> 4, e1 | e1 >> 4, 0x6420);
 }
 
-// D / 8 lanes a head vector, 8 dims a lane.
+__device__ __forceinline__ void load4(const float* p, float* x) {
+    const float4 v = __ldg(reinterpret_cast<const float4*>(p));
+    x[0] = v.x;
+    x[1] = v.y;
+    x[2] = v.z;
+    x[3] = v.w;
+}
+
+// x: the 8 dims (8 l ..) of a head vector that this lane holds, normed (weights w, or none) and
+// turned. Every lane of the warp takes part.
 template <int HD>
-__global__ void __launch_bounds__(256) k_kv4_append(const AppendArgs a) {
-    using T = Kv4Tile<HD>;
+__device__ __forceinline__ void norm_rotate(const AppendArgs& a, const float* w, int pos, bool pos_ok, int lane,
+                                            float* x) {
     constexpr int L = HD / 8;
-    const int heads = a.hq + 2 * a.hkv;
-    const int lane = threadIdx.x & 31, l = lane % L;
-    const int64_t total = a.n * heads;
-    const int64_t stride = (int64_t)gridDim.x * (blockDim.x / L);
-    const int64_t v0 = ((int64_t)blockIdx.x * blockDim.x + (threadIdx.x & ~31)) / L;   // the warp's first vector
-    for (int64_t vb = v0; vb < total; vb += stride) {
-        const int64_t vi = vb + lane / L;
-        const bool live = vi < total;
-        const int64_t tok = live ? vi / heads : 0;
-        const int h = live ? (int)(vi - tok * heads) : 0;
-        const bool is_q = h < a.hq, is_k = !is_q && h < a.hq + a.hkv;
-        const int hh = is_q ? h : is_k ? h - a.hq : h - a.hq - a.hkv;
-        const __nv_bfloat16* src = is_q ? a.q + tok * a.qs + hh * a.qh
-                                 : is_k ? a.k + tok * a.ks + hh * a.kh : a.v + tok * a.vs + hh * a.vh;
-        float x[8];
-        bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(src) + l), x);
-        const int pos = a.pos ? a.pos[tok] : 0;
-        const bool pos_ok = !a.pos || (pos >= 0 && pos < a.max_pos);
-        if (a.qw || a.kw) {   // (uniform: every lane takes part in the shuffles)
-            const float* w = is_q ? a.qw : is_k ? a.kw : nullptr;
-            float t[8];
+    const int l = lane % L;
+    if (w) {
+        float t[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) t[j] = __fmul_rn(x[j], x[j]);
-            float ss = __fadd_rn(__fadd_rn(__fadd_rn(t[0], t[1]), __fadd_rn(t[2], t[3])),
-                                 __fadd_rn(__fadd_rn(t[4], t[5]), __fadd_rn(t[6], t[7])));
-            ss = lanes_sum<L>(ss);
-            if (w) {
-                const float inv = __frcp_rn(__fsqrt_rn(__fadd_rn(__fmul_rn(ss, 1.f / HD), a.eps)));
+        for (int j = 0; j < 8; ++j) t[j] = __fmul_rn(x[j], x[j]);
+        float ss = __fadd_rn(__fadd_rn(__fadd_rn(t[0], t[1]), __fadd_rn(t[2], t[3])),
+                             __fadd_rn(__fadd_rn(t[4], t[5]), __fadd_rn(t[6], t[7])));
+        ss = lanes_sum<L>(ss);
+        const float inv = __frcp_rn(__fsqrt_rn(__fadd_rn(__fmul_rn(ss, 1.f / HD), a.eps)));
+        float wv[8];
+        load4(w + 8 * l, wv);
+        load4(w + 8 * l + 4, wv + 4);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = __fmul_rn(w[hh * HD + 8 * l + j], __fmul_rn(x[j], inv));
-            }
-        }
-        __syncwarp();
-        if (a.rot > 0) {
-            const int half = a.rot >> 1;
-            const float *cs = a.cs + (int64_t)(pos_ok ? pos : 0) * half, *sn = a.sn + (int64_t)(pos_ok ? pos : 0) * half;
-            const bool turn = (is_q || is_k) && 8 * l < a.rot;
-            if (a.interleaved) {
-                if (turn) {
-#pragma unroll
-                    for (int j = 0; j < 8; j += 2) {
-                        if (8 * l + j < a.rot) {
-                            const float c = cs[4 * l + j / 2], s = sn[4 * l + j / 2];
-                            const float u = x[j], v = x[j + 1];
-                            x[j] = __fsub_rn(__fmul_rn(u, c), __fmul_rn(v, s));
-                            x[j + 1] = __fadd_rn(__fmul_rn(v, c), __fmul_rn(u, s));
-                        }
-                    }
-                }
-            } else {   // rot % 16 == 0: the partner's dims are the same 8 of another lane
-                const int hl = half >> 3;
-                const bool first = l < hl;
-                const int from = (lane - l) + (turn ? (first ? l + hl : l - hl) : l);
-                float o[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) o[j] = __shfl_sync(0xffffffffu, x[j], from);
-                if (turn) {
-                    const int b = 8 * (first ? l : l - hl);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float c = cs[b + j], s = sn[b + j];
-                        x[j] = first ? __fsub_rn(__fmul_rn(x[j], c), __fmul_rn(o[j], s))
-                                     : __fadd_rn(__fmul_rn(x[j], c), __fmul_rn(o[j], s));
-                    }
-                }
-            }
-        }
-        __syncwarp();
-        uint32_t param;
-        const uint32_t codes = quantise(x, param);
-        const uint32_t word = quad_word(codes, lane);
-        if (!live) continue;
-        if (is_q) {
-            if (a.gain) {
-                const float g = pos_ok ? a.gain[pos] : 0.f;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = __fmul_rn(x[j], g);
-            }
-            if (!pos_ok) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[j] = 0.f;
-            }
-            reinterpret_cast<uint4*>(a.qo + (tok * a.hq + hh) * HD)[l] = f32_to_bf16x8(x);
-            continue;
-        }
-        const int64_t slot = a.slots[tok];
-        if (slot < 0 || slot >= a.num_slots || !pos_ok) continue;
-        const int64_t page = slot >> a.page_shift;
-        const int off = (int)(slot & ((1 << a.page_shift) - 1));
-        uint8_t* tile = a.pages + (page * a.hkv + hh) * a.page_bytes + (int64_t)(off >> 4) * T::BYTES;
-        const int t = off & 15, r = t & 7, hf = t >> 3, g = l >> 2, j = l & 3;
-        if (is_k) {
-            *reinterpret_cast<uint32_t*>(tile + (g >> 1) * T::BLK + (4 * r + j) * 16 + hf * 8 + (g & 1) * 4) = word;
+        for (int j = 0; j < 8; ++j) x[j] = __fmul_rn(wv[j], __fmul_rn(x[j], inv));
+    }
+    if (a.rot == 0) return;
+    const int half = a.rot >> 1;
+    const int64_t row = (int64_t)(pos_ok ? pos : 0) * half;
+    const float *cs = a.cs + row, *sn = a.sn + row;
+    const bool turn = 8 * l < a.rot;
+    float c[8], s[8];
+    if (a.interleaved) {
+        if (!turn) return;
+        if ((a.rot & 7) == 0) {   // rows of the tables are multiples of 16 bytes
+            load4(cs + 4 * l, c);
+            load4(sn + 4 * l, s);
         } else {
-            uint8_t* p = tile + T::V + (g >> 1) * T::BLK + (8 * j + (r >> 1)) * 16 + (g & 1) * 8 + hf * 4 + (r & 1) * 2;
-            *reinterpret_cast<uint16_t*>(p) = (uint16_t)word;
-            *reinterpret_cast<uint16_t*>(p + 64) = (uint16_t)(word >> 16);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const bool in = 8 * l + 2 * j < a.rot;
+                c[j] = in ? cs[4 * l + j] : 1.f;
+                s[j] = in ? sn[4 * l + j] : 0.f;
+            }
         }
-        if (j == 0)
-            *reinterpret_cast<uint32_t*>(tile + (is_k ? T::KP : T::VP) + ((2 * r + hf) * T::NG + g) * 4) = param;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (8 * l + 2 * j < a.rot) {
+                const float u = x[2 * j], v = x[2 * j + 1];
+                x[2 * j] = __fsub_rn(__fmul_rn(u, c[j]), __fmul_rn(v, s[j]));
+                x[2 * j + 1] = __fadd_rn(__fmul_rn(v, c[j]), __fmul_rn(u, s[j]));
+            }
+        }
+    } else {   // rot % 16 == 0: the partner's dims are the same 8 of another lane, rows multiples of 32 bytes
+        const int hl = half >> 3;
+        const bool first = l < hl;
+        const int from = (lane - l) + (turn ? (first ? l + hl : l - hl) : l);
+        float o[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o[j] = __shfl_sync(0xffffffffu, x[j], from);
+        if (turn) {
+            const int b = 8 * (first ? l : l - hl);
+            load4(cs + b, c);
+            load4(cs + b + 4, c + 4);
+            load4(sn + b, s);
+            load4(sn + b + 4, s + 4);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                x[j] = first ? __fsub_rn(__fmul_rn(x[j], c[j]), __fmul_rn(o[j], s[j]))
+                             : __fadd_rn(__fmul_rn(x[j], c[j]), __fmul_rn(o[j], s[j]));
+        }
     }
 }
 
-// The inverse of quantise and quad_word: bf16(s c + z) of the positions asked for.
+// The warp's 256 / HD query vectors from vb on (of the call's n hq).
 template <int HD>
-__global__ void __launch_bounds__(256) k_kv4_read(const uint8_t* __restrict__ pages, const int64_t* __restrict__ slots,
-                                                  int64_t n, int hkv, int page_shift, int64_t page_bytes,
-                                                  int64_t num_slots, __nv_bfloat16* __restrict__ ko,
-                                                  __nv_bfloat16* __restrict__ vo) {
+__device__ __forceinline__ void append_queries(const AppendArgs& a, uint32_t vb, int lane) {
+    constexpr int L = HD / 8;
+    const int l = lane % L;
+    const uint32_t vi = vb + lane / L;
+    const bool live = vi < a.n * (uint32_t)a.hq;
+    const uint32_t tk = live ? vi / (uint32_t)a.hq : 0u;
+    const int64_t tok = tk;
+    const int h = live ? (int)(vi - tk * a.hq) : 0;
+    float x[8];
+    bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(a.q + tok * a.qs + h * a.qh) + l), x);
+    const int pos = a.pos ? a.pos[tok] : 0;
+    const bool ok = !a.pos || (pos >= 0 && pos < a.max_pos);
+    norm_rotate<HD>(a, a.qw ? a.qw + h * HD : nullptr, pos, ok, lane, x);
+    if (a.gain) {
+        const float g = ok ? a.gain[pos] : 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = __fmul_rn(x[j], g);
+    }
+    if (live)
+        reinterpret_cast<uint4*>(a.qo + (tok * a.hq + h) * HD)[l] = ok ? f32_to_bf16x8(x) : make_uint4(0, 0, 0, 0);
+}
+
+// One (token, kv head) vector for each group of HD / 8 lanes: its codes and parameters, to those of
+// the token's tile (in global or shared memory); t: the token's place in the tile.
+template <int HD>
+__device__ __forceinline__ void store_vector(const float* x, bool is_k, int t, bool put, uint8_t* codes, uint8_t* params,
+                                             int lane) {
+    using T = Kv4Tile<HD>;
+    const int l = lane % (HD / 8), r = t & 7, hf = t >> 3, g = l >> 2, j = l & 3;
+    uint32_t param;
+    const uint32_t word = quad_word(quantise(x, param), lane);
+    if (!put) return;
+    if (is_k) {
+        *reinterpret_cast<uint32_t*>(codes + (g >> 1) * T::BLK + (4 * r + j) * 16 + hf * 8 + (g & 1) * 4) = word;
+    } else {
+        uint8_t* p = codes + (g >> 1) * T::BLK + (8 * j + (r >> 1)) * 16 + (g & 1) * 8 + hf * 4 + (r & 1) * 2;
+        *reinterpret_cast<uint16_t*>(p) = (uint16_t)word;
+        *reinterpret_cast<uint16_t*>(p + 64) = (uint16_t)(word >> 16);
+    }
+    if (j == 0) *reinterpret_cast<uint32_t*>(params + ((2 * r + hf) * T::NG + g) * 4) = param;
+}
+
+// The tile of a slot (0 .. num_slots - 1) and kv head.
+template <int HD>
+__device__ __forceinline__ int64_t tile_at(int64_t slot, int h, int hkv, int page_shift, int64_t page_bytes) {
+    return ((slot >> page_shift) * hkv + h) * page_bytes +
+           (int64_t)((slot & ((1 << page_shift) - 1)) >> 4) * Kv4Tile<HD>::BYTES;
+}
+
+// A head vector of k or v, normed and turned for keys; put: whether it is stored, at slot.
+template <int HD>
+__device__ __forceinline__ bool load_kv(const AppendArgs& a, bool is_k, int64_t tok, int h, int lane, float* x,
+                                        int64_t& slot) {
+    const int l = lane % (HD / 8);
+    const __nv_bfloat16* src = is_k ? a.k + tok * a.ks + h * a.kh : a.v + tok * a.vs + h * a.vh;
+    bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(src) + l), x);
+    const int pos = a.pos ? a.pos[tok] : 0;
+    const bool ok = !a.pos || (pos >= 0 && pos < a.max_pos);
+    slot = a.slots[tok];
+    if (is_k) norm_rotate<HD>(a, a.kw ? a.kw + h * HD : nullptr, pos, ok, lane, x);
+    return ok && slot >= 0 && slot < a.num_slots;
+}
+
+// Few tokens: a warp per 32 / L head vectors of one kind (queries, keys or values), so that no warp
+// quantises what it does not store.
+template <int HD>
+__global__ void __launch_bounds__(128) k_kv4_append(const AppendArgs a) {
+    using T = Kv4Tile<HD>;
+    constexpr int VW = 256 / HD;   // vectors a warp
+    const int lane = threadIdx.x & 31;
+    const uint32_t nq = (a.n * (uint32_t)a.hq + VW - 1) / VW, nk = (a.n * (uint32_t)a.hkv + VW - 1) / VW;
+    const uint32_t w = blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (w < nq) {
+        append_queries<HD>(a, w * VW, lane);
+    } else if (w < nq + 2 * nk) {
+        const bool is_k = w < nq + nk;
+        const uint32_t vi = (w - nq - (is_k ? 0 : nk)) * VW + lane / (HD / 8);
+        const bool live = vi < a.n * (uint32_t)a.hkv;
+        const uint32_t tok = live ? vi / (uint32_t)a.hkv : 0u;
+        const int h = live ? (int)(vi - tok * a.hkv) : 0;
+        float x[8];
+        int64_t slot;
+        const bool put = load_kv<HD>(a, is_k, tok, h, lane, x, slot) && live;
+        uint8_t* tile = a.pages + (put ? tile_at<HD>(slot, h, a.hkv, a.page_shift, a.page_bytes) : 0);
+        store_vector<HD>(x, is_k, (int)(slot & 15), put, tile + (is_k ? 0 : T::V), tile + (is_k ? T::KP : T::VP), lane);
+    }
+}
+
+// Many tokens: a warp per 16 tokens of one kv head's keys or values. Where they fill one tile of the
+// cache, its codes and parameters are put together in shared memory and written in 16-byte pieces
+// (value codes of a token are 2-byte pieces 64 bytes apart); others are written one by one. Groups
+// of 16 start so that the first token's page lines up with them. Queries: 16 vectors a warp.
+constexpr int BULK_WARPS = 8;
+template <int HD>
+__global__ void __launch_bounds__(BULK_WARPS * 32) k_kv4_append_bulk(const AppendArgs a) {
+    using T = Kv4Tile<HD>;
+    constexpr int VW = 256 / HD, L = HD / 8;
+    __shared__ __align__(16) uint8_t images[BULK_WARPS][10 * HD];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lead = (int)(a.slots[0] & 15);   // tokens of the first group that lie before token 0
+    const uint32_t groups = (a.n + lead + 15) / 16, nkv = groups * 2 * a.hkv;
+    const uint32_t nq = (a.n * (uint32_t)a.hq + 15) / 16, w = blockIdx.x * BULK_WARPS + warp;
+    if (w >= nkv) {
+#pragma unroll 2
+        for (int i = 0; i < 16; i += VW)
+            if (w < nkv + nq && (w - nkv) * 16 + i < a.n * (uint32_t)a.hq) append_queries<HD>(a, (w - nkv) * 16 + i, lane);
+    } else {
+        const uint32_t grp = w / (2u * a.hkv);
+        const int kh = (int)(w - grp * 2 * a.hkv);
+        const bool is_k = kh < a.hkv;
+        const int h = is_k ? kh : kh - a.hkv;
+        const int64_t tok0 = (int64_t)grp * 16 - lead;
+        // a whole tile: 16 tokens in the 16 consecutive slots of one, all of them stored
+        bool fits = true;
+        int64_t s0 = -1;
+        {
+            const int64_t tk = tok0 + (lane & 15);
+            const bool in = tk >= 0 && tk < a.n;
+            const int64_t s = in ? a.slots[tk] : -1;
+            const int pos = in && a.pos ? a.pos[tk] : 0;
+            s0 = __shfl_sync(0xffffffffu, s, 0);
+            fits = in && s == s0 + (lane & 15) && s0 >= 0 && (s0 & 15) == 0 && s < a.num_slots &&
+                   (!a.pos || (pos >= 0 && pos < a.max_pos));
+        }
+        const bool whole = __all_sync(0xffffffffu, fits);
+        uint8_t* dst = a.pages + (whole ? tile_at<HD>(s0, h, a.hkv, a.page_shift, a.page_bytes) : 0);
+        for (int i = 0; i < 16; i += VW) {
+            const int64_t tk = tok0 + i + lane / L;
+            const bool live = tk >= 0 && tk < a.n;
+            float x[8];
+            int64_t slot;
+            const bool put = load_kv<HD>(a, is_k, live ? tk : 0, h, lane, x, slot) && live;
+            uint8_t *codes = images[warp], *params = images[warp] + 8 * HD;
+            if (!whole) {
+                codes = a.pages + (put ? tile_at<HD>(slot, h, a.hkv, a.page_shift, a.page_bytes) : 0);
+                params = codes + (is_k ? T::KP : T::VP);
+                codes += is_k ? 0 : T::V;
+            }
+            store_vector<HD>(x, is_k, (int)(slot & 15), put, codes, params, lane);
+        }
+        if (whole) {
+            __syncwarp();
+            const uint4* src = reinterpret_cast<const uint4*>(images[warp]);
+            uint4* codes = reinterpret_cast<uint4*>(dst + (is_k ? 0 : T::V));
+            uint4* par = reinterpret_cast<uint4*>(dst + (is_k ? T::KP : T::VP));
+#pragma unroll
+            for (int i = lane; i < HD / 2; i += 32) codes[i] = src[i];
+            if (lane < HD / 8) par[lane] = src[HD / 2 + lane];
+        }
+    }
+}
+
+// The inverse of quantise and quad_word: bf16(s c + z) of the lane's 8 dims of each group of lanes'
+// head vector, from the codes and parameters of its tile (ok false: zeros).
+template <int HD>
+__device__ __forceinline__ uint4 fetch_vector(const uint8_t* codes, const uint8_t* params, bool is_k, int t, bool ok,
+                                              int lane) {
+    using T = Kv4Tile<HD>;
+    const int l = lane % (HD / 8), g = l >> 2, j = l & 3, r = t & 7, hf = t >> 3;
+    uint32_t word = 0, par = 0;
+    if (ok) {
+        if (is_k) {
+            word = *reinterpret_cast<const uint32_t*>(codes + (g >> 1) * T::BLK + (4 * r + j) * 16 + hf * 8 + (g & 1) * 4);
+        } else {
+            const uint8_t* p = codes + (g >> 1) * T::BLK + (8 * j + (r >> 1)) * 16 + (g & 1) * 8 + hf * 4 + (r & 1) * 2;
+            word = *reinterpret_cast<const uint16_t*>(p) | (uint32_t)*reinterpret_cast<const uint16_t*>(p + 64) << 16;
+        }
+        par = *reinterpret_cast<const uint32_t*>(params + ((2 * r + hf) * T::NG + g) * 4);
+    }
+    const float s = __uint_as_float(par << 16), z = __uint_as_float(par & 0xffff0000u);
+    float x[8];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {   // dims 32 g + 8 j + 2 q, + 1: nibble (j / 2, j % 2) of quad lane q's word
+        const uint32_t o = __shfl_sync(0xffffffffu, word, (lane & ~3) | q) >> (4 * j);
+        // a code under the exponent of 2^23 is 2^23 + c; s c is exact, so the sum is rounded once
+        x[2 * q] = fmaf(__uint_as_float((o & 15u) | 0x4b000000u) - 8388608.f, s, z);
+        x[2 * q + 1] = fmaf(__uint_as_float(((o >> 16) & 15u) | 0x4b000000u) - 8388608.f, s, z);
+    }
+    return f32_to_bf16x8(x);
+}
+
+struct ReadArgs {
+    const uint8_t* pages;
+    const int64_t* slots;
+    __nv_bfloat16 *k, *v;
+    int64_t page_bytes, num_slots;
+    uint32_t n;   // 2 n hkv < 2^31
+    int hkv, page_shift;
+};
+
+// Few positions: a warp per 32 / L head vectors.
+template <int HD>
+__global__ void __launch_bounds__(128) k_kv4_read(const ReadArgs a) {
     using T = Kv4Tile<HD>;
     constexpr int L = HD / 8;
-    const int lane = threadIdx.x & 31, l = lane % L, g = l >> 2, j = l & 3;
-    const int64_t total = n * 2 * hkv;
-    const int64_t stride = (int64_t)gridDim.x * (blockDim.x / L);
-    const int64_t v0 = ((int64_t)blockIdx.x * blockDim.x + (threadIdx.x & ~31)) / L;
-    for (int64_t vb = v0; vb < total; vb += stride) {
-        const int64_t vi = vb + lane / L;
-        const bool live = vi < total;
-        const int64_t tok = live ? vi / (2 * hkv) : 0;
-        const int h = live ? (int)(vi - tok * 2 * hkv) : 0;
-        const bool is_k = h < hkv;
-        const int hh = is_k ? h : h - hkv;
-        const int64_t slot = slots[tok];
-        const bool ok = slot >= 0 && slot < num_slots;
-        const int64_t page = ok ? slot >> page_shift : 0;
-        const int off = ok ? (int)(slot & ((1 << page_shift) - 1)) : 0;
-        const uint8_t* tile = pages + (page * hkv + hh) * page_bytes + (int64_t)(off >> 4) * T::BYTES;
-        const int t = off & 15, r = t & 7, hf = t >> 3;
-        uint32_t word = 0, par = 0;
-        if (ok) {
-            if (is_k) {
-                word = *reinterpret_cast<const uint32_t*>(tile + (g >> 1) * T::BLK + (4 * r + j) * 16 + hf * 8 +
-                                                          (g & 1) * 4);
-            } else {
-                const uint8_t* p = tile + T::V + (g >> 1) * T::BLK + (8 * j + (r >> 1)) * 16 + (g & 1) * 8 + hf * 4 +
-                                   (r & 1) * 2;
-                word = *reinterpret_cast<const uint16_t*>(p) |
-                       (uint32_t)*reinterpret_cast<const uint16_t*>(p + 64) << 16;
-            }
-            par = *reinterpret_cast<const uint32_t*>(tile + (is_k ? T::KP : T::VP) + ((2 * r + hf) * T::NG + g) * 4);
-        }
-        const float s = __uint_as_float(par << 16), z = __uint_as_float(par & 0xffff0000u);
-        float x[8];
-        const int b = j >> 1, nb = j & 1;   // this lane's dims are 32 g + 16 b + 8 nb + x
+    const int lane = threadIdx.x & 31;
+    const uint32_t vi = (blockIdx.x * 128 + threadIdx.x) / L;
+    const bool live = vi < a.n * 2 * a.hkv;
+    const uint32_t tok = live ? vi / (2u * a.hkv) : 0u;
+    const int kh = live ? (int)(vi - tok * 2 * a.hkv) : 0;
+    const bool is_k = kh < a.hkv;
+    const int h = is_k ? kh : kh - a.hkv;
+    const int64_t slot = a.slots[tok];
+    const bool ok = slot >= 0 && slot < a.num_slots;
+    const uint8_t* tile = a.pages + (ok ? tile_at<HD>(slot, h, a.hkv, a.page_shift, a.page_bytes) : 0);
+    const uint4 x = fetch_vector<HD>(tile + (is_k ? 0 : T::V), tile + (is_k ? T::KP : T::VP), is_k, (int)(slot & 15), ok,
+                                     lane);
+    if (live) reinterpret_cast<uint4*>((is_k ? a.k : a.v) + ((int64_t)tok * a.hkv + h) * HD)[lane % L] = x;
+}
+
+// Many positions: a warp per 16 of one kv head's keys or values; where they are one whole tile, its
+// bytes come through shared memory in 16-byte pieces. Groups of 16 start so that the first
+// position's tile lines up with them.
+template <int HD>
+__global__ void __launch_bounds__(BULK_WARPS * 32) k_kv4_read_bulk(const ReadArgs a) {
+    using T = Kv4Tile<HD>;
+    constexpr int VW = 256 / HD, L = HD / 8;
+    __shared__ __align__(16) uint8_t images[BULK_WARPS][10 * HD];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int lead = (int)(a.slots[0] & 15);
+    const uint32_t w = blockIdx.x * BULK_WARPS + warp;
+    if (w >= (a.n + lead + 15) / 16 * 2 * a.hkv) return;
+    const uint32_t grp = w / (2u * a.hkv);
+    const int kh = (int)(w - grp * 2 * a.hkv);
+    const bool is_k = kh < a.hkv;
+    const int h = is_k ? kh : kh - a.hkv;
+    const int64_t tok0 = (int64_t)grp * 16 - lead, mine = tok0 + (lane & 15);
+    const int64_t s = mine >= 0 && mine < a.n ? a.slots[mine] : -1;
+    const int64_t s0 = __shfl_sync(0xffffffffu, s, 0);
+    const bool whole = __all_sync(0xffffffffu, s0 >= 0 && (s0 & 15) == 0 && s == s0 + (lane & 15) && s < a.num_slots);
+    if (whole) {
+        const uint8_t* src = a.pages + tile_at<HD>(s0, h, a.hkv, a.page_shift, a.page_bytes);
+        const uint4* codes = reinterpret_cast<const uint4*>(src + (is_k ? 0 : T::V));
+        const uint4* par = reinterpret_cast<const uint4*>(src + (is_k ? T::KP : T::VP));
+        uint4* img = reinterpret_cast<uint4*>(images[warp]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {       // dims x = 2i, 2i + 1: word of quad lane i
-            const uint32_t o = __shfl_sync(0xffffffffu, word, (lane & ~3) | i) >> (8 * b + 4 * nb);
-            x[2 * i] = __fadd_rn(__fmul_rn((float)(o & 15u), s), z);
-            x[2 * i + 1] = __fadd_rn(__fmul_rn((float)((o >> 16) & 15u), s), z);
+        for (int i = lane; i < HD / 2; i += 32) img[i] = __ldg(codes + i);
+        if (lane < HD / 8) img[HD / 2 + lane] = __ldg(par + lane);
+        __syncwarp();
+    }
+#pragma unroll 4
+    for (int i = 0; i < 16; i += VW) {
+        const int64_t slot = __shfl_sync(0xffffffffu, s, i + lane / L), tk = tok0 + i + lane / L;
+        const bool ok = slot >= 0 && slot < a.num_slots;
+        const uint8_t *codes = images[warp], *params = images[warp] + 8 * HD;
+        if (!whole) {
+            codes = a.pages + (ok ? tile_at<HD>(slot, h, a.hkv, a.page_shift, a.page_bytes) : 0);
+            params = codes + (is_k ? T::KP : T::VP);
+            codes += is_k ? 0 : T::V;
         }
-        if (live)
-            reinterpret_cast<uint4*>((is_k ? ko : vo) + (tok * hkv + hh) * HD)[l] = f32_to_bf16x8(x);
+        const uint4 x = fetch_vector<HD>(codes, params, is_k, (int)(slot & 15), ok, lane);
+        if (tk >= 0 && tk < a.n) reinterpret_cast<uint4*>((is_k ? a.k : a.v) + (tk * a.hkv + h) * HD)[lane % L] = x;
     }
 }
 
-// Blocks of 256 threads for `vectors` head vectors of L lanes: at most eight resident blocks per
-// SM's worth, the rest by the grid-stride loop.
-int blocks_for(int64_t vectors, int lanes) {
-    const int64_t g = (vectors * lanes + 255) / 256;
-    return (int)(g < 148 * 8 ? g : 148 * 8);
-}
+// From this many tokens on a warp takes 16 of them.
+constexpr int64_t BULK_TOKENS = 1024;
+
+int bulk_grid(int64_t warps) { return (int)((warps + BULK_WARPS - 1) / BULK_WARPS); }
 
 int page_geometry(const char* what, int64_t head_dim, int64_t page_size, int64_t num_pages, int64_t hkv,
                   const void* pages, int* shift, int64_t* page_bytes) {
@@ -285,7 +469,8 @@ extern "C" int pulsar_op_kv4_append(const void* q, const void* k, const void* v,
                                     int64_t max_pos, int interleaved, const float* q_gain, const int32_t* positions,
                                     const int64_t* slots, void* pages, int64_t num_pages, int64_t page_size,
                                     void* q_out, void* stream) {
-    PULSAR_CHECK_ARG(N >= 0 && Hq >= 0 && Hq <= 65536, "kv4_append: invalid shape");
+    PULSAR_CHECK_ARG(N >= 0 && Hq >= 0 && Hq <= 65536 && Hkv >= 1 && Hkv <= 1024 && N <= INT32_MAX / (Hq + 2 * Hkv) - 64,
+                     "kv4_append: invalid shape (%lld tokens)", (long long)N);
     int shift;
     int64_t pb;
     PULSAR_TRY(page_geometry("kv4_append", head_dim, page_size, num_pages, Hkv, pages, &shift, &pb));
@@ -299,17 +484,29 @@ extern "C" int pulsar_op_kv4_append(const void* q, const void* k, const void* v,
                      "kv4_append: tables need positions and at least one row");
     for (int i = 0; i < 6; ++i)
         PULSAR_CHECK_ARG(strides[i] % 8 == 0, "kv4_append: token and head strides must be multiples of 8 elements");
-    for (const void* p : {q, k, v, (const void*)q_out})
-        PULSAR_CHECK_ARG((reinterpret_cast<uintptr_t>(p) & 15) == 0, "kv4_append: q, k, v must be 16-byte aligned");
+    for (const void* p : {q, k, v, (const void*)q_out, (const void*)q_norm, (const void*)k_norm, (const void*)cos,
+                          (const void*)sin})
+        PULSAR_CHECK_ARG((reinterpret_cast<uintptr_t>(p) & 15) == 0,
+                         "kv4_append: q, k, v, norm weights and tables must be 16-byte aligned");
     AppendArgs a{(const __nv_bfloat16*)q, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, strides[0], strides[2],
                  strides[4], strides[1], strides[3], strides[5], q_norm, k_norm, cos, sin, q_gain, slots,
-                 (rot > 0 || q_gain) ? positions : nullptr, (uint8_t*)pages, (__nv_bfloat16*)q_out, N,
-                 num_pages * page_size, pb, (int)Hq, (int)Hkv, shift, (int)rot, (int)max_pos, interleaved, eps};
-    const int grid = blocks_for(N * (Hq + 2 * Hkv), (int)head_dim / 8);
-    if (head_dim == 64)
-        k_kv4_append<64><<<grid, 256, 0, (cudaStream_t)stream>>>(a);
-    else
-        k_kv4_append<128><<<grid, 256, 0, (cudaStream_t)stream>>>(a);
+                 (rot > 0 || q_gain) ? positions : nullptr, (uint8_t*)pages, (__nv_bfloat16*)q_out,
+                 num_pages * page_size, pb, (uint32_t)N, (int)Hq, (int)Hkv, shift, (int)rot, (int)max_pos, interleaved, eps};
+    cudaStream_t st = (cudaStream_t)stream;
+    if (N >= BULK_TOKENS) {
+        const int grid = bulk_grid((N + 30) / 16 * 2 * Hkv + (N * Hq + 15) / 16);
+        if (head_dim == 64)
+            k_kv4_append_bulk<64><<<grid, BULK_WARPS * 32, 0, st>>>(a);
+        else
+            k_kv4_append_bulk<128><<<grid, BULK_WARPS * 32, 0, st>>>(a);
+    } else {
+        const int64_t vw = 256 / head_dim, warps = (N * Hq + vw - 1) / vw + 2 * ((N * Hkv + vw - 1) / vw);
+        const int grid = (int)((warps + 3) / 4);
+        if (head_dim == 64)
+            k_kv4_append<64><<<grid, 128, 0, st>>>(a);
+        else
+            k_kv4_append<128><<<grid, 128, 0, st>>>(a);
+    }
     PULSAR_LAUNCH_CHECK("k_kv4_append");
     return PULSAR_OK;
 }
@@ -325,15 +522,23 @@ extern "C" int pulsar_op_kv4_read(const void* pages, int64_t num_pages, int64_t 
     PULSAR_CHECK_ARG(slots && k_out && v_out, "kv4_read: null pointer");
     for (const void* p : {(const void*)k_out, (const void*)v_out})
         PULSAR_CHECK_ARG((reinterpret_cast<uintptr_t>(p) & 15) == 0, "kv4_read: outputs must be 16-byte aligned");
-    const int grid = blocks_for(N * 2 * Hkv, (int)head_dim / 8);
-    if (head_dim == 64)
-        k_kv4_read<64><<<grid, 256, 0, (cudaStream_t)stream>>>((const uint8_t*)pages, slots, N, (int)Hkv, shift, pb,
-                                                               num_pages * page_size, (__nv_bfloat16*)k_out,
-                                                               (__nv_bfloat16*)v_out);
-    else
-        k_kv4_read<128><<<grid, 256, 0, (cudaStream_t)stream>>>((const uint8_t*)pages, slots, N, (int)Hkv, shift, pb,
-                                                                num_pages * page_size, (__nv_bfloat16*)k_out,
-                                                                (__nv_bfloat16*)v_out);
+    PULSAR_CHECK_ARG(N <= INT32_MAX / (2 * Hkv) - 64, "kv4_read: invalid shape (%lld positions)", (long long)N);
+    const ReadArgs a{(const uint8_t*)pages, slots, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, pb,
+                     num_pages * page_size, (uint32_t)N, (int)Hkv, shift};
+    cudaStream_t st = (cudaStream_t)stream;
+    if (N >= BULK_TOKENS) {
+        const int grid = bulk_grid((N + 30) / 16 * 2 * Hkv);
+        if (head_dim == 64)
+            k_kv4_read_bulk<64><<<grid, BULK_WARPS * 32, 0, st>>>(a);
+        else
+            k_kv4_read_bulk<128><<<grid, BULK_WARPS * 32, 0, st>>>(a);
+    } else {
+        const int grid = (int)((N * 2 * Hkv * (head_dim / 8) + 127) / 128);
+        if (head_dim == 64)
+            k_kv4_read<64><<<grid, 128, 0, st>>>(a);
+        else
+            k_kv4_read<128><<<grid, 128, 0, st>>>(a);
+    }
     PULSAR_LAUNCH_CHECK("k_kv4_read");
     return PULSAR_OK;
 }

@@ -192,6 +192,38 @@ def test_stored_codes_follow_the_definition(paged):
     assert torch.equal(ref.nan_to_num(7.0), hv.nan_to_num(7.0)) and torch.equal(hk.nan_to_num(7.0), hv.nan_to_num(7.0))
 
 
+@pytest.mark.parametrize("d,page,start,shuffle", [(64, 64, 0, False), (64, 16, 5, False), (128, 32, 0, False),
+                                                  (128, 64, 15, False), (64, 64, 0, True)])
+def test_many_tokens_match_few(paged, d, page, start, shuffle):
+    """A call of many tokens (whole tiles, a first tile begun elsewhere, scattered slots, some without a
+    slot) stores and reads the same bits as calls of few."""
+    n, hq, hkv = 2100, 6, 2
+    q, k, v = (_randn(i, n, h, d).bfloat16().cuda() for i, h in ((1, hq), (2, hkv), (3, hkv)))
+    pages = paged.kv4_pages(n // page + 3, hkv, d, page)
+    order = torch.randperm(pages.shape[0], generator=torch.Generator().manual_seed(1))
+    at = torch.arange(n) + start
+    if shuffle:
+        at = at[torch.randperm(n, generator=torch.Generator().manual_seed(2))]
+    slots = (order[at // page] * page + at % page).cuda()
+    slots[[7, 600, 601, 2050]] = torch.tensor([-1, 1 << 40, -7, pages.shape[0] * page]).cuda()
+    pos = torch.arange(n).int().cuda()
+    pos[[40, 1111]] = torch.tensor([-1, n]).int().cuda()
+    cos, sin = paged.rope_tables(n, d // 2)
+    w = 1 + 0.1 * _randn(5, hkv, d).cuda()
+    few = pages.clone()
+    out = paged.kv4_append(q, k, v, pages, slots, pos, cos, sin, k_norm=w)
+    parts = []
+    for a in range(0, n, 700):
+        b = slice(a, a + 700)
+        parts.append(paged.kv4_append(q[b], k[b], v[b], few, slots[b], pos[b], cos, sin, k_norm=w))
+    assert torch.equal(out, torch.cat(parts)) and torch.equal(pages, few)
+    many = paged.kv4_read(pages, slots, d)
+    few = [paged.kv4_read(pages, slots[a:a + 700], d) for a in range(0, n, 700)]
+    for i in (0, 1):
+        assert torch.equal(many[i], torch.cat([x[i] for x in few]))
+    assert (out[[40, 1111]] == 0).all() and (many[0][[7, 600, 601, 2050]] == 0).all()
+
+
 def test_append_empty_and_no_queries(paged):
     pages = paged.kv4_pages(2, 2)
     e = torch.empty(0, 2, 64, dtype=torch.bfloat16, device="cuda")
