@@ -1,4 +1,5 @@
-// Attention over the paged 4-bit KV cache (layout: kv4.cuh): pulsar_op_kv4_attention.
+// Attention over the paged 4-bit KV cache (layout: kv4.cuh): pulsar_op_kv4_attention, and its kernel for
+// up to 32 units a sequence and kv head (decoding, verify blocks); more: kv4_prefill.cu.
 //
 // Row j of the n_b query rows of sequence b has position pos = len_b - n_b + j and sees the keys
 // max(0, pos - window + 1) .. pos (window 0: all of 0 .. pos):
@@ -30,7 +31,7 @@
 
 #include "capi_util.h"
 #include "common.cuh"
-#include "kv4.cuh"
+#include "kv4_attn.cuh"
 #include "mega_ptx.cuh"
 
 using namespace pulsar;
@@ -39,28 +40,7 @@ namespace {
 
 constexpr int WARPS = 4;
 constexpr int LAZY = 30;
-constexpr float NEG = -1e30f;   // "no key yet": finite, so differences with it are defined
-
-struct AttnArgs {
-    const __nv_bfloat16* q;
-    const uint8_t* pages;
-    const int32_t *table, *kv_lens, *cu_q;
-    __nv_bfloat16* out;
-    float *part_o, *part_ml;
-    int64_t q_row, q_head, page_bytes;
-    int rows, hq, hkv, group, num_pages, width, page_shift, max_q, window, nsplit, split_pairs;
-    float scale_log2;
-};
-
-// The rows of sequence b, held inside q whatever cu_q says.
-__device__ __forceinline__ void rows_of(const AttnArgs& a, int b, int& row0, int& nq) {
-    row0 = b;
-    nq = 1;
-    if (a.cu_q) {
-        row0 = min(max(a.cu_q[b], 0), a.rows);
-        nq = min(max(a.cu_q[b + 1] - row0, 0), min(a.max_q, a.rows - row0));
-    }
-}
+constexpr float NEG = KV4_NEG;
 
 // d = a b + c (d and c may be the same registers)
 __device__ __forceinline__ void mma16816(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, const float* c) {
@@ -74,12 +54,6 @@ __device__ __forceinline__ void mma16816(float* d, const uint32_t* a, uint32_t b
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
-    return y;
-}
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
 
@@ -117,7 +91,7 @@ template <int HD>
 constexpr int ring_bytes() { return WARPS * stages<HD>() * 2 * Kv4Tile<HD>::BYTES; }
 
 template <int HD, int NT, bool DUP>
-__global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
+__global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const Kv4AttnArgs a) {
     using T = Kv4Tile<HD>;
     constexpr int NG = T::NG, NB = HD / 64, S = stages<HD>(), MT = HD / 16, TB = T::BYTES;
     constexpr int UT = DUP ? 4 : 8 * NT;
@@ -128,7 +102,7 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
     const int h = blockIdx.y, b = blockIdx.z;
 
     int row0, nq;
-    rows_of(a, b, row0, nq);
+    kv4_rows(a, b, row0, nq);
     const int units = nq * a.group;
     if (u0 >= units) return;
     const int len = min(max(a.kv_lens[b], 0), a.width << a.page_shift);
@@ -138,8 +112,8 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
     const int kmin = low(first), kmax = last + 1;   // keys that some unit sees: [kmin, kmax)
     // pairs of tiles (32 tokens, aligned): the split's range, of which the warp takes every fourth
     const int pair0 = kmin / 32, npairs = kmax > 0 ? (kmax + 31) / 32 : 0;
-    const int p_begin = pair0 + split * a.split_pairs + warp;
-    const int p_end = split == a.nsplit - 1 ? npairs : min(npairs, pair0 + (split + 1) * a.split_pairs);
+    const int p_begin = pair0 + split * a.split_len + warp;
+    const int p_end = split == a.nsplit - 1 ? npairs : min(npairs, pair0 + (split + 1) * a.split_len);
     const int mine = p_end > p_begin ? (p_end - p_begin + WARPS - 1) / WARPS : 0;
 
     if (lane == 0) {
@@ -151,17 +125,12 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
     // pages of the warp's i-th pair (-1: none): lane i % 32 holds them for the current 32; a page of
     // 16 tokens holds one tile of the pair only
     const bool two = a.page_shift == 4;
-    auto page_at = [&](int tile) {
-        const int col = tile >> (a.page_shift - 4);
-        const int p = col < a.width ? a.table[(int64_t)b * a.width + col] : -1;
-        return p >= 0 && p < a.num_pages ? p : -1;
-    };
     auto fetch_pages = [&](int i0, int& pg, int& pg2) {
         pg = pg2 = -1;
         if (i0 + lane < mine) {
             const int tile = 2 * (p_begin + (i0 + lane) * WARPS);
-            pg = pg2 = page_at(tile);
-            if (two) pg2 = page_at(tile + 1);
+            pg = pg2 = kv4_page(a, b, tile);
+            if (two) pg2 = kv4_page(a, b, tile + 1);
         }
     };
     unsigned char* ring = sm + warp * S * 2 * TB;
@@ -273,7 +242,7 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
                 uint32_t a0[4], a1[4];
                 unpack(kc[g >> 1][g & 1], a0[0], a0[2], a1[0], a1[2]);
                 unpack(kc[g >> 1][2 + (g & 1)], a0[1], a0[3], a1[1], a1[3]);
-                const float s0 = lo_of(kp[0][g]), y0 = hi_of(kp[0][g]), s8 = lo_of(kp[1][g]), y8 = hi_of(kp[1][g]);
+                const float s0 = kv4_s(kp[0][g]), y0 = kv4_z(kp[0][g]), s8 = kv4_s(kp[1][g]), y8 = kv4_z(kp[1][g]);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float acc[4] = {0.f, 0.f, 0.f, 0.f};
@@ -303,7 +272,7 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
                 for (int x = 0; x < 2; ++x)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        p[x][nt][e] = ex2(fmaf(sc[x][nt][e], scale, nm[nt][e & 1]));
+                        p[x][nt][e] = kv4_ex2(fmaf(sc[x][nt][e], scale, nm[nt][e & 1]));
                         ls[nt][e & 1] += p[x][nt][e];
                     }
             }
@@ -333,7 +302,7 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
                     x = fmaxf(x, m[nt][c]);
-                    const float f = ex2((m[nt][c] - x) * scale);
+                    const float f = kv4_ex2((m[nt][c] - x) * scale);
                     m[nt][c] = x;
                     nm[nt][c] = fmaf(-x, scale, (float)LIFT);
                     l[nt][c] *= f;
@@ -367,7 +336,7 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
                 uint32_t a0[4], a1[4];
                 unpack(vc[g >> 1][2 * (g & 1)], a0[0], a0[1], a1[0], a1[1]);
                 unpack(vc[g >> 1][2 * (g & 1) + 1], a0[2], a0[3], a1[2], a1[3]);
-                const float s0 = lo_of(vp[0][g]), z0 = hi_of(vp[0][g]), s8 = lo_of(vp[1][g]), z8 = hi_of(vp[1][g]);
+                const float s0 = kv4_s(vp[0][g]), z0 = kv4_z(vp[0][g]), s8 = kv4_s(vp[1][g]), z8 = kv4_z(vp[1][g]);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     const float* pp = p[x][nt];
@@ -485,7 +454,7 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
             const float* p = all + (w * UT + u) * (HD + 2);
-            const float f = ex2(p[HD] - mm);
+            const float f = kv4_ex2(p[HD] - mm);
             ll = fmaf(f, p[HD + 1], ll);
             oo = fmaf(f, p[d], oo);
         }
@@ -505,10 +474,10 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const AttnArgs a) {
 
 // out of one (sequence row, head) from its splits' partials, in split order: a block of HD threads.
 template <int HD>
-__global__ void __launch_bounds__(HD) k_kv4_merge(const AttnArgs a) {
+__global__ void __launch_bounds__(HD) k_kv4_merge(const Kv4AttnArgs a) {
     const int j = blockIdx.x / a.hq, b = blockIdx.y;
     int row0, nq;
-    rows_of(a, b, row0, nq);
+    kv4_rows(a, b, row0, nq);
     if (j >= nq) return;
     const int64_t at = (int64_t)(row0 + j) * a.hq + blockIdx.x % a.hq;
     const float* ml = a.part_ml + at * a.nsplit * 2;
@@ -516,7 +485,7 @@ __global__ void __launch_bounds__(HD) k_kv4_merge(const AttnArgs a) {
     for (int s = 0; s < a.nsplit; ++s) mm = fmaxf(mm, ml[2 * s]);
     float ll = 0.f, oo = 0.f;
     for (int s = 0; s < a.nsplit; ++s) {
-        const float f = ex2(ml[2 * s] - mm);
+        const float f = kv4_ex2(ml[2 * s] - mm);
         ll = fmaf(f, ml[2 * s + 1], ll);
         oo = fmaf(f, a.part_o[(at * a.nsplit + s) * HD + threadIdx.x], oo);
     }
@@ -524,41 +493,46 @@ __global__ void __launch_bounds__(HD) k_kv4_merge(const AttnArgs a) {
 }
 
 struct Plan {
-    int nt, dup, utiles, nsplit, split_pairs;
+    bool many;   // k_kv4_prefill
+    int nt, dup, utiles, nsplit, split_len;
 };
 
-// How a call is cut. Units: the fewest columns that hold max_q rows of a group (four: both halves
-// of the weights in one operand), at most 32 (heads of 128: 16, for the registers). Splits: until
-// about four CTAs an SM are there, of at least 8 pairs (two a warp) each.
+// How a call is cut. More than MANY units of a sequence's rows go to k_kv4_prefill in tiles of 256.
+// Others: the fewest columns that hold max_q rows of a group (four: both halves of the weights in
+// one operand), at most 32 (heads of 128: 16, for the registers). Splits of the keys: until about
+// four CTAs an SM are there (k_kv4_prefill: one), of at least 8 pairs of tiles (two a warp; 4 chunks).
+constexpr int64_t MANY = 32;
 Plan make_plan(int64_t B, int64_t Hkv, int64_t group, int64_t head_dim, int64_t max_q, int64_t max_kv,
                int64_t window) {
     Plan p{};
     const int64_t units = max_q * group, cap = head_dim == 64 ? 4 : 2;
+    p.many = units > MANY;
     p.dup = units <= 4;
     p.nt = (int)(units > 8 * cap ? cap : (units + 7) / 8);
-    const int64_t ut = p.dup ? 4 : 8 * p.nt;
+    const int64_t ut = p.many ? KV4_PF_UNITS : p.dup ? 4 : 8 * p.nt;
+    const int64_t step = p.many ? kv4_pf_chunk((int)head_dim) : 32, least = p.many ? 4 : 8, full = p.many ? 148 : 148 * 4;
     p.utiles = (int)((units + ut - 1) / ut);
     int64_t span = max_kv;
     if (window > 0) {
         const int64_t rows = (ut + group - 1) / group + 1;   // rows that a unit tile can touch
-        const int64_t w = window + (rows < max_q ? rows : max_q) + 32;
+        const int64_t w = window + (rows < max_q ? rows : max_q) + step;
         if (w < span) span = w;
     }
-    const int64_t pairs = (span + 31) / 32;
+    const int64_t steps = (span + step - 1) / step;
     const int64_t ctas = B * Hkv * p.utiles;
-    int64_t ns = (148 * 4 + ctas - 1) / ctas;
-    if (ns > pairs / 8) ns = pairs / 8;
+    int64_t ns = p.many ? full / ctas : (full + ctas - 1) / ctas;
+    if (ns > steps / least) ns = steps / least;
     if (ns > 64) ns = 64;
     if (ns < 1) ns = 1;
-    p.split_pairs = (int)((pairs + ns - 1) / ns);
-    if (p.split_pairs < 1) p.split_pairs = 1;
-    p.nsplit = (int)((pairs + p.split_pairs - 1) / p.split_pairs);
+    p.split_len = (int)((steps + ns - 1) / ns);
+    if (p.split_len < 1) p.split_len = 1;
+    p.nsplit = (int)((steps + p.split_len - 1) / p.split_len);
     if (p.nsplit < 1) p.nsplit = 1;
     return p;
 }
 
 template <int HD, int NT, bool DUP>
-int launch(const AttnArgs& a, const Plan& p, int64_t B, cudaStream_t st) {
+int launch(const Kv4AttnArgs& a, const Plan& p, int64_t B, cudaStream_t st) {
     constexpr int merge = WARPS * (DUP ? 4 : 8 * NT) * (HD + 2) * 4;
     constexpr int bytes = ring_bytes<HD>() > merge ? ring_bytes<HD>() : merge;
     PULSAR_TRY(ensure_smem_attr((const void*)k_kv4_attn<HD, NT, DUP>, bytes, "k_kv4_attn shared memory"));
@@ -609,21 +583,25 @@ extern "C" int pulsar_op_kv4_attention(const void* q, int64_t q_row_stride, int6
     PULSAR_CHECK_ARG(q && pages && kv_lens && out && (block_table || width == 0), "kv4_attention: null pointer");
     PULSAR_CHECK_ARG((reinterpret_cast<uintptr_t>(q) & 3) == 0 && q_row_stride % 2 == 0 && q_head_stride % 2 == 0,
                      "kv4_attention: q must be 4-byte aligned with even strides");
-    PULSAR_CHECK_ARG((reinterpret_cast<uintptr_t>(pages) & 15) == 0, "kv4_attention: pages must be 16-byte aligned");
+    PULSAR_CHECK_ARG(((reinterpret_cast<uintptr_t>(pages) | reinterpret_cast<uintptr_t>(out) |
+                       reinterpret_cast<uintptr_t>(workspace)) & 15) == 0,
+                     "kv4_attention: pages, out and the workspace must be 16-byte aligned");
     const Plan p = make_plan(B, Hkv, Hq / Hkv, head_dim, max_q, max_kv, window);
     const int64_t need = p.nsplit > 1 ? N * Hq * p.nsplit * (head_dim + 2) * 4 : 0;
     PULSAR_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need),
                      "kv4_attention: workspace of %lld bytes needed, got %lld", (long long)need,
                      (long long)workspace_bytes);
     float* ws = (float*)workspace;
-    AttnArgs a{(const __nv_bfloat16*)q, (const uint8_t*)pages, block_table, kv_lens, cu_q, (__nv_bfloat16*)out, ws,
+    Kv4AttnArgs a{(const __nv_bfloat16*)q, (const uint8_t*)pages, block_table, kv_lens, cu_q, (__nv_bfloat16*)out, ws,
                p.nsplit > 1 ? ws + N * Hq * p.nsplit * head_dim : nullptr, q_row_stride, q_head_stride,
                page_size / KV4_TILE * 20 * head_dim, (int)N, (int)Hq, (int)Hkv, (int)(Hq / Hkv), (int)num_pages,
                (int)width, __builtin_ctzll((unsigned long long)page_size), (int)max_q, (int)window, p.nsplit,
-               p.split_pairs, scale * 1.4426950408889634f};
+               p.split_len, scale * 1.4426950408889634f};
     cudaStream_t st = (cudaStream_t)stream;
     int rc;
-    if (head_dim == 64)
+    if (p.many)
+        rc = kv4_prefill_launch(a, (int)head_dim, B, p.utiles, st);
+    else if (head_dim == 64)
         rc = p.dup ? launch<64, 1, true>(a, p, B, st) : p.nt == 1 ? launch<64, 1, false>(a, p, B, st)
            : p.nt == 2 ? launch<64, 2, false>(a, p, B, st) : p.nt == 3 ? launch<64, 3, false>(a, p, B, st)
            : launch<64, 4, false>(a, p, B, st);

@@ -1,0 +1,669 @@
+// Attention of many query rows over the paged 4-bit KV cache (layout: kv4.cuh), the tensor-core
+// half of pulsar_op_kv4_attention: prompts and chunks of prompts.
+//
+// CTA: 256 units (query rows x heads of one kv head's group) of a sequence as two tiles of 128, one
+// TMEM lane a unit, over a range of its keys in chunks of CK (128, for heads of 128: 64). Per chunk
+//   copy      the packed tiles into a ring, 1-D bulk copies of whole pages' parts (warp 12)
+//   unpack    K^ [CK keys][HD] and V^T^ [HD][CK keys] in fp16, K-major SWIZZLE_128B (warps 8-11): the
+//             cache keeps codes so that a word's halves are neighbours in the operand's rows
+//   S = Q K^  tcgen05.mma kind::f16, M 128, N CK, fp32 in TMEM (one lane of warp 13 issues every MMA)
+//   softmax   a thread per unit (warps 0-3: tile 0, 4-7: tile 1): weights in fp16 back to TMEM
+//   O += P V^ with P read from TMEM as the A operand, O in TMEM
+// The two tiles take turns: while one tile's weights are computed, the other's MMAs run.
+//
+// Exactness. fp16 has the significand for it (values s c + z of 8-bit s, z and 4-bit c are rounded
+// at 2^-12, weights too) but not the range, so powers of two move out: queries by their row, keys and
+// values by their chunk (2^eK, 2^eV from the largest |value| that s and z allow, over the keys that
+// some unit sees). Score and weight: x = 2^eK 2^eq scale log2(e) S + eV - m, P = 2^x; P V^ = 2^(s - m) V
+// and l = sum 2^-eV P. The reference m of a unit moves when a chunk's sum of weights passes 2^14
+// (then the row of O is rescaled and the chunk's weights taken again), so P stays inside fp16 and no
+// maximum is looked for in other chunks.
+//
+// Keys that a unit does not see get weight 0 by selection. V^ is 0 for keys that no unit sees (pages
+// past the end may hold anything) and for groups stored as NaN; which (key, group) those were goes to
+// the softmax threads, whose units that see the key answer NaN in the group's dims.
+//
+// Every wait is bounded; one that runs out raises the CTA's abort flag, which ends the others; MMAs
+// and copies in flight are waited for (bounded again) and the rows answer NaN.
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "capi_util.h"
+#include "kv4_attn.cuh"
+#include "mega_ptx.cuh"
+
+using namespace pulsar;
+
+namespace {
+
+constexpr int THREADS = 14 * 32;
+constexpr float FULL = 16384.f;   // a chunk's weights are taken again when their sum passes this
+
+template <int HD>
+struct Lay {
+    static constexpr int CK = kv4_pf_chunk(HD), TPC = CK / 16, NG = HD / 32, NB = HD / 64;
+    static constexpr int PS = 3;                                     // stages of the packed ring
+    static constexpr uint32_t QB = 128 * HD * 2, KB = CK * HD * 2;   // bytes of a Q tile, of K^ or V^
+    static constexpr uint32_t PB = TPC * Kv4Tile<HD>::BYTES;
+    static constexpr uint32_t Q = 0, K = 2 * QB, V = K + 2 * KB, P = V + 2 * KB, MISC = P + PS * PB;
+    static constexpr uint32_t BYTES = MISC + 1024;
+    static constexpr uint32_t S_COL = 0, P_COL = 2 * CK, O_COL = 3 * CK;   // TMEM columns, two of each
+    static_assert(O_COL + 2 * HD <= 512 && PB % 1024 == 0 && BYTES + 1024 <= 227 * 1024, "fits");
+};
+
+struct Misc {   // in shared memory after the operands
+    uint64_t packed_full[3], packed_empty[3], kv_full[2], kv_empty[2], s_full[2], p_full[2], o_full[2], drain;
+    uint32_t valid[3];       // tiles of the packed stage that are there
+    uint32_t stop[2][4];     // per chunk parity and unpacking warp: a wait has run out
+    uint32_t top[2][4][2];   // per chunk parity and unpacking warp: largest |K|, |V| as float bits
+    float kscale[2], ev[2];
+    uint32_t bad[2][4];      // per stage and unpacking warp: some group of V is NaN
+    uint8_t bad_groups[2][128];
+    uint32_t tmem;
+    int abort;
+};
+static_assert(sizeof(Misc) <= 1024, "Misc fits its space");
+
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
+    if (mbar_try(bar, parity)) return true;
+    const unsigned long long t0 = globaltimer();
+    while (!mbar_try(bar, parity)) {
+        if (*abort) return false;
+        if (globaltimer() - t0 > WAIT_NS) {
+            *abort = 1;
+            return false;
+        }
+    }
+    return true;
+}
+
+// K-major SWIZZLE_128B operand: rows of 128 bytes, atoms of 8 rows.
+__device__ __forceinline__ uint64_t desc(uint32_t addr) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
+           (2ull << 61);
+}
+// kind::f16: fp32 accumulator, fp16 operands, both K-major, M = 128.
+constexpr uint32_t idesc(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | (8u << 24); }
+
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(id), "r"((uint32_t)acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, bool acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(id), "r"((uint32_t)acc)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// 32 columns of the thread's TMEM lane (no wait) and 16 back.
+__device__ __forceinline__ void ld32(uint32_t at, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(at));
+}
+__device__ __forceinline__ void st16(uint32_t at, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16};" ::"r"(at),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+// Waits for the loads; the registers pass through it, so that nothing reads them earlier.
+__device__ __forceinline__ void ld_wait(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                   "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                   "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                   "+r"(r[30]), "+r"(r[31])::"memory");
+}
+__device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Two fp32 lanes in one instruction.
+using f32x2 = unsigned long long;
+__device__ __forceinline__ f32x2 two(float a, float b) {
+    f32x2 v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ void parts(f32x2 v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+    f32x2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+    f32x2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
+
+// The four operand registers of a code word as s c + z: codes under the exponent of 1024 (c, or 16 c).
+__device__ __forceinline__ void unpack4(uint32_t w, uint32_t s, uint32_t z, uint32_t* r) {
+    const uint32_t v = w >> 8;
+    const __half2 one = __floats2half2_rn(1024.f, 1024.f), inv = __floats2half2_rn(0.0625f, 0.0625f),
+                  sub = __floats2half2_rn(-64.f, -64.f);
+    const __half2 c0 = __hsub2(as_half2((w & 0x000f000fu) | 0x64006400u), one);
+    const __half2 c1 = __hfma2(as_half2((w & 0x00f000f0u) | 0x64006400u), inv, sub);
+    const __half2 c2 = __hsub2(as_half2((v & 0x000f000fu) | 0x64006400u), one);
+    const __half2 c3 = __hfma2(as_half2((v & 0x00f000f0u) | 0x64006400u), inv, sub);
+    const __half2 x[4] = {__hfma2(c0, as_half2(s), as_half2(z)), __hfma2(c1, as_half2(s), as_half2(z)),
+                          __hfma2(c2, as_half2(s), as_half2(z)), __hfma2(c3, as_half2(s), as_half2(z))};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = *reinterpret_cast<const uint32_t*>(&x[i]);
+}
+
+__device__ __forceinline__ void sts(uint32_t at, uint32_t v) {
+    asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
+
+// Power of two that brings a largest magnitude (float bits) to [2^9, 2^10): the exponent taken out.
+__device__ __forceinline__ int exponent_out(uint32_t bits) {
+    return min(max((int)(bits >> 23) - 127 - 9, -100), 100);
+}
+__device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
+template <int HD>
+__global__ void __launch_bounds__(THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a) {
+    using L = Lay<HD>;
+    using T = Kv4Tile<HD>;
+    constexpr int CK = L::CK, TPC = L::TPC, NG = L::NG, NB = L::NB, PS = L::PS;
+    extern __shared__ unsigned char raw[];
+    unsigned char* sm = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
+    const uint32_t sb = smem_u32(sm);
+    Misc& ms = *reinterpret_cast<Misc*>(sm + L::MISC);
+    volatile int* abort = &ms.abort;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int split = blockIdx.x % a.nsplit, u0 = blockIdx.x / a.nsplit * KV4_PF_UNITS;
+    const int h = blockIdx.y, b = blockIdx.z;
+
+    int row0, nq;
+    kv4_rows(a, b, row0, nq);
+    const int units = nq * a.group;
+    if (u0 >= units) return;
+    const int len = min(max(a.kv_lens[b], 0), a.width << a.page_shift);
+    const int ulast = min(u0 + KV4_PF_UNITS, units) - 1;
+    const int tiles = ulast - u0 >= 128 ? 2 : 1;
+    const int first = len - nq + u0 / a.group, last = len - nq + ulast / a.group;
+    auto low = [&](int pos) { return a.window > 0 ? max(0, pos - a.window + 1) : 0; };
+    const int kmin = low(first), kmax = max(last + 1, 0);
+    const int chunk0 = kmin / CK + split * a.split_len;
+    const int chunk1 = split == a.nsplit - 1 ? (kmax + CK - 1) / CK : min((kmax + CK - 1) / CK, chunk0 + a.split_len);
+    const int n = max(chunk1 - chunk0, 0);
+
+    if (tid == 0) {
+        for (int i = 0; i < PS; ++i) {
+            mbar_init(&ms.packed_full[i], 1);
+            mbar_init(&ms.packed_empty[i], 4);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&ms.kv_full[i], 4);
+            mbar_init(&ms.kv_empty[i], 1);
+            mbar_init(&ms.s_full[i], 1);
+            mbar_init(&ms.p_full[i], 4);
+            mbar_init(&ms.o_full[i], 1);
+        }
+        mbar_init(&ms.drain, 1);
+        ms.abort = 0;
+        fence_mbar_init();
+    }
+    if (warp == 13) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&ms.tmem))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    // the tiles' queries, a thread a unit: q 2^-eq in fp16, its largest |dim| in [2^3, 2^4)
+    float qscale = 0.f;
+    const int u = u0 + tid;   // softmax threads only
+    if (warp < 8) {
+        float x[HD];
+        const bool ok = u < units;
+        const int j = ok ? u / a.group : 0, g = ok ? u - j * a.group : 0;
+        const __nv_bfloat16* src = a.q + (row0 + j) * a.q_row + (h * a.group + g) * a.q_head;
+        const uint32_t* src2 = reinterpret_cast<const uint32_t*>(src);
+        const bool wide = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (ok) {
+                if (wide) {
+                    v = *reinterpret_cast<const uint4*>(src + 8 * i);
+                } else {
+                    v.x = src2[4 * i];
+                    v.y = src2[4 * i + 1];
+                    v.z = src2[4 * i + 2];
+                    v.w = src2[4 * i + 3];
+                }
+            }
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[8 * i + 2 * e] = kv4_s(w[e]);
+                x[8 * i + 2 * e + 1] = kv4_z(w[e]);
+                top = max(top, max(w[e] << 16 & 0x7fffffffu, w[e] & 0x7fff0000u));
+            }
+        }
+        const int eq = min(max((int)(top >> 23) - 127 - 3, -100), 100);
+        const float f = exp2i(-eq);
+        qscale = a.scale_log2 * exp2i(eq);
+        const int row = tid & 127;
+        const uint32_t qt = sb + L::Q + (uint32_t)(tid >> 7) * L::QB + (row >> 3) * 1024 + (row & 7) * 128;
+#pragma unroll
+        for (int i = 0; i < HD / 8; ++i) {
+            const uint32_t at = qt + (i >> 3) * (128 * 128) + (((i & 7) ^ (row & 7)) << 4);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at),
+                         "r"(half2_bits(x[8 * i] * f, x[8 * i + 1] * f)), "r"(half2_bits(x[8 * i + 2] * f, x[8 * i + 3] * f)),
+                         "r"(half2_bits(x[8 * i + 4] * f, x[8 * i + 5] * f)),
+                         "r"(half2_bits(x[8 * i + 6] * f, x[8 * i + 7] * f))
+                         : "memory");
+        }
+        fence_async();
+    }
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem = ms.tmem;
+
+    if (warp == 12) {
+        // copies: lane i a piece of the chunk (the part of it in one page, or all of it)
+        const int page_tiles = 1 << (a.page_shift - 4), piece = min(page_tiles, TPC), pieces = TPC / piece;
+        auto page_of = [&](int c) { return lane < pieces && c < n ? kv4_page(a, b, (chunk0 + c) * TPC + lane * piece) : -1; };
+        int next = page_of(0);
+        int c = 0;
+        for (; c < n; ++c) {
+            const int page = next, st = c % PS;
+            next = page_of(c + 1);
+            bool ok = true;
+            if (c >= PS) ok = wait(&ms.packed_empty[st], (c / PS - 1) & 1, abort);
+            if (!__all_sync(0xffffffffu, ok)) break;
+            const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
+            if (lane == 0) {
+                uint32_t v = 0;
+                for (int i = 0; i < pieces; ++i)
+                    if (there >> i & 1) v |= ((1u << piece) - 1) << (i * piece);
+                ms.valid[st] = v;
+                const uint32_t bytes = __popc(there) * piece * T::BYTES;
+                if (bytes)
+                    mbar_arrive_expect_tx(&ms.packed_full[st], bytes);
+                else
+                    mbar_arrive(&ms.packed_full[st]);
+            }
+            __syncwarp();
+            if (page >= 0)
+                tma_load_1d(sm + L::P + st * L::PB + lane * piece * T::BYTES,
+                            a.pages + ((int64_t)page * a.hkv + h) * a.page_bytes +
+                                (int64_t)(((chunk0 + c) * TPC + lane * piece) & (page_tiles - 1)) * T::BYTES,
+                            piece * T::BYTES, &ms.packed_full[st]);
+        }
+        // what was issued lands before the CTA ends
+        for (int i = max(0, c - PS); i < c; ++i) mbar_wait(&ms.packed_full[i % PS], (i / PS) & 1);
+    } else if (warp == 13) {
+        if (lane == 0 && n > 0) {
+            auto mma_s = [&](int t, int c) {
+                const uint32_t kt = sb + L::K + (c & 1) * L::KB, qt = sb + L::Q + t * L::QB;
+#pragma unroll
+                for (int ks = 0; ks < HD / 16; ++ks)
+                    mma_ss(tmem + L::S_COL + t * CK, desc(qt + (ks >> 2) * (128 * 128) + (ks & 3) * 32),
+                           desc(kt + (ks >> 2) * (CK * 128) + (ks & 3) * 32), idesc(CK), ks > 0);
+                commit(&ms.s_full[t]);
+            };
+            bool ok = wait(&ms.kv_full[0], 0, abort);
+            fence_after();
+            if (ok)
+                for (int t = 0; t < tiles; ++t) mma_s(t, 0);
+            for (int c = 0; ok && c < n; ++c) {
+                const uint32_t vt = sb + L::V + (c & 1) * L::KB;
+                for (int t = 0; ok && t < tiles; ++t) {
+                    if (!(ok = wait(&ms.p_full[t], c & 1, abort))) break;
+                    fence_after();
+#pragma unroll
+                    for (int ks = 0; ks < CK / 16; ++ks)
+                        mma_ts(tmem + L::O_COL + t * HD, tmem + L::P_COL + t * (CK / 2) + ks * 8,
+                               desc(vt + (ks >> 2) * (HD * 128) + (ks & 3) * 32), idesc(HD), c > 0 || ks > 0);
+                    if (t == tiles - 1) commit(&ms.kv_empty[c & 1]);
+                    if (c + 1 < n) {
+                        if (t == 0) {
+                            if (!(ok = wait(&ms.kv_full[(c + 1) & 1], ((c + 1) >> 1) & 1, abort))) break;
+                            fence_after();
+                        }
+                        mma_s(t, c + 1);   // its commit also says that this chunk's P V has completed
+                    } else {
+                        commit(&ms.o_full[t]);
+                    }
+                }
+            }
+            commit(&ms.drain);   // every MMA issued has completed
+            mbar_wait(&ms.drain, 0);
+        }
+        __syncwarp();
+    } else if (warp >= 8) {
+        // unpacking: warp w takes tiles w, w + 4 of the chunk
+        const int w = warp - 8, r = lane >> 2, t = lane & 3;
+        bool good = true;   // no wait of this warp has run out; the four warps leave together
+        for (int c = 0; c < n; ++c) {
+            const int st = c % PS, sg = c & 1, k0 = (chunk0 + c) * CK;
+            if (good) good = __all_sync(0xffffffffu, wait(&ms.packed_full[st], (c / PS) & 1, abort));
+            const unsigned char* pk = sm + L::P + st * L::PB;
+            const uint32_t valid = ms.valid[st];
+            // the largest magnitudes that the chunk's s and z allow, and its NaN groups of V
+            uint32_t topk = 0, topv = 0;
+            bool bad[TPC / 4][NB], any_bad = false;
+#pragma unroll
+            for (int y = 0; y < TPC / 4; ++y) {
+                const int tl = w + 4 * y;
+                const uint32_t* kp = reinterpret_cast<const uint32_t*>(pk + tl * T::BYTES + T::KP);
+                const uint32_t* vp = reinterpret_cast<const uint32_t*>(pk + tl * T::BYTES + T::VP);
+#pragma unroll
+                for (int x = 0; x < NB; ++x) {
+                    const int at = x * 32 + lane, slot = at / NG, key = k0 + 16 * tl + (slot >> 1) + 8 * (slot & 1);
+                    const bool in = (valid >> tl & 1) && key >= kmin && key < kmax;
+                    const uint32_t kw = kp[at], vw = vp[at];
+                    const float ka = fmaxf(fabsf(kv4_z(kw)), fabsf(fmaf(15.f, kv4_s(kw), kv4_z(kw))));
+                    const float va = fmaxf(fabsf(kv4_z(vw)), fabsf(fmaf(15.f, kv4_s(vw), kv4_z(vw))));
+                    topk = max(topk, in && ka == ka ? __float_as_uint(ka) : 0u);
+                    topv = max(topv, in && va == va ? __float_as_uint(va) : 0u);
+                    bad[y][x] = in && !(kv4_z(vw) == kv4_z(vw));
+                    any_bad |= bad[y][x];
+                }
+            }
+            topk = __reduce_max_sync(0xffffffffu, topk);
+            topv = __reduce_max_sync(0xffffffffu, topv);
+            any_bad = __any_sync(0xffffffffu, any_bad);
+            if (lane == 0) {
+                ms.top[sg][w][0] = topk;
+                ms.top[sg][w][1] = topv;
+                ms.stop[sg][w] = !good;
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            bool stop = false;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                topk = max(topk, ms.top[sg][y][0]);
+                topv = max(topv, ms.top[sg][y][1]);
+                stop |= ms.stop[sg][y] != 0;
+            }
+            if (stop) break;
+            const int ek = exponent_out(topk), ev = exponent_out(topv);
+            const float fk = exp2i(-ek), fv = exp2i(-ev);
+            if (c >= 2) {   // the stage's readers: both tiles' MMAs and softmax of chunk c - 2
+                good = __all_sync(0xffffffffu, wait(&ms.kv_empty[sg], (c / 2 - 1) & 1, abort));
+                if (!good) continue;
+            }
+            if (any_bad) {   // rare: which groups of which keys
+#pragma unroll
+                for (int y = 0; y < TPC / 4; ++y)
+#pragma unroll
+                    for (int x = 0; x < NB; ++x) {
+                        uint32_t bits = bad[y][x] ? 1u << (lane % NG) : 0u;
+#pragma unroll
+                        for (int o = 1; o < NG; o <<= 1) bits |= __shfl_xor_sync(0xffffffffu, bits, o);
+                        const int slot = (x * 32 + lane) / NG;
+                        if (lane % NG == 0)
+                            ms.bad_groups[sg][16 * (w + 4 * y) + (slot >> 1) + 8 * (slot & 1)] = (uint8_t)bits;
+                    }
+            }
+            const uint32_t kt = sb + L::K + sg * L::KB, vt = sb + L::V + sg * L::KB;
+#pragma unroll
+            for (int y = 0; y < TPC / 4; ++y) {
+                const int tl = w + 4 * y;
+                const unsigned char* tp = pk + tl * T::BYTES;
+                const bool there = valid >> tl & 1;
+                uint32_t code[NB][4], par[2 * NG];
+#pragma unroll
+                for (int x = 0; x < NB; ++x)
+                    *reinterpret_cast<uint4*>(code[x]) = *reinterpret_cast<const uint4*>(tp + x * T::BLK + lane * 16);
+#pragma unroll
+                for (int x = 0; x < 2 * NG; x += 4)
+                    *reinterpret_cast<uint4*>(par + x) = *reinterpret_cast<const uint4*>(tp + T::KP + r * 8 * NG + x * 4);
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    const int key = k0 + 16 * tl + r + 8 * hf;
+                    const bool in = there && key >= kmin && key < kmax;
+                    const uint32_t row = kt + (2 * tl + hf) * 1024 + r * 128 + 4 * t;
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        const float s = in ? kv4_s(par[hf * NG + g]) * fk : 0.f, z = in ? kv4_z(par[hf * NG + g]) * fk : 0.f;
+                        uint32_t x[4];
+                        unpack4(code[g >> 1][2 * hf + (g & 1)], half2_bits(s, s), half2_bits(z, z), x);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            sts(row + (g >> 1) * (CK * 128) + (((4 * (g & 1) + i) ^ r) << 4), x[i]);
+                    }
+                }
+                uint32_t vpar[4 * NG];   // tokens 2t, 2t + 8, 2t + 1, 2t + 9
+#pragma unroll
+                for (int x = 0; x < NB; ++x)
+                    *reinterpret_cast<uint4*>(code[x]) = *reinterpret_cast<const uint4*>(tp + T::V + x * T::BLK + lane * 16);
+#pragma unroll
+                for (int x = 0; x < 4 * NG; x += 4)
+                    *reinterpret_cast<uint4*>(vpar + x) = *reinterpret_cast<const uint4*>(tp + T::VP + t * 16 * NG + x * 4);
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    const int key = k0 + 16 * tl + 2 * t + 8 * hf;
+                    const bool in0 = there && key >= kmin && key < kmax, in1 = there && key + 1 >= kmin && key + 1 < kmax;
+                    const int col = 16 * tl + 8 * hf;   // of the 8 keys that a 16-byte piece holds
+                    const uint32_t blk = vt + (col >> 6) * (HD * 128) + r * 128 + ((((col & 63) >> 3) ^ r) << 4) + 4 * t;
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        const uint32_t p0 = vpar[hf * NG + g], p1 = vpar[(2 + hf) * NG + g];
+                        const bool ok0 = in0 && kv4_z(p0) == kv4_z(p0), ok1 = in1 && kv4_z(p1) == kv4_z(p1);
+                        const uint32_t s = half2_bits(ok0 ? kv4_s(p0) * fv : 0.f, ok1 ? kv4_s(p1) * fv : 0.f);
+                        const uint32_t z = half2_bits(ok0 ? kv4_z(p0) * fv : 0.f, ok1 ? kv4_z(p1) * fv : 0.f);
+                        uint32_t x[4];
+                        unpack4(code[g >> 1][2 * (g & 1) + hf], s, z, x);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sts(blk + (4 * g + i) * 1024, x[i]);
+                    }
+                }
+            }
+            if (lane == 0) {
+                ms.bad[sg][w] = any_bad;
+                if (w == 0) {
+                    ms.kscale[sg] = exp2i(ek);
+                    ms.ev[sg] = (float)ev;
+                }
+            }
+            fence_async();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&ms.kv_full[sg]);
+                mbar_arrive(&ms.packed_empty[st]);
+            }
+        }
+    } else {
+        // softmax: this thread's unit u, tile warp / 4, TMEM lane (warp % 4) 32 + lane
+        const int tile = warp >> 2;
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t s_at = tmem + lanes + L::S_COL + tile * CK, p_at = tmem + lanes + L::P_COL + tile * (CK / 2),
+                       o_at = tmem + lanes + L::O_COL + tile * HD;
+        const int pos = len - nq + min(u, units - 1) / a.group;
+        const int lo = low(pos), hi = pos + 1;
+        // keys that every unit of the warp sees
+        const int uw = u - lane, ua = min(uw, units - 1), ub = min(uw + 31, units - 1);
+        const int all_lo = low(len - nq + ub / a.group), all_hi = len - nq + ua / a.group + 1;
+        float m = KV4_NEG, l = 0.f;
+        uint32_t bad = 0;
+        bool ok = tile < tiles;
+        for (int c = 0; ok && c < n; ++c) {
+            const int sg = c & 1, k0 = (chunk0 + c) * CK;
+            ok = wait(&ms.s_full[tile], c & 1, abort) && wait(&ms.kv_full[sg], (c >> 1) & 1, abort);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            fence_after();
+            const float kq = ms.kscale[sg] * qscale, ev = ms.ev[sg];
+            const bool edge = k0 < all_lo || k0 + CK > all_hi;
+            const int lo_c = lo - k0, hi_c = hi - k0;
+            // weights with the reference m into P; their sum
+            auto weigh = [&](auto edge_tag) {
+                constexpr bool EDGE = decltype(edge_tag)::value;
+                const f32x2 f2 = two(kq, kq), b2 = two(ev - m, ev - m);
+                f32x2 sum = two(0.f, 0.f);
+                uint32_t v[2][32];
+                ld32(s_at, v[0]);
+#pragma unroll
+                for (int q = 0; q < CK / 32; ++q) {
+                    ld_wait(v[q & 1]);
+                    if (q + 1 < CK / 32) ld32(s_at + 32 * (q + 1), v[(q + 1) & 1]);
+                    uint32_t p[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        float x, y;
+                        parts(fma2(two(__uint_as_float(v[q & 1][2 * i]), __uint_as_float(v[q & 1][2 * i + 1])), f2, b2), x, y);
+                        if (EDGE) {
+                            const int k = 32 * q + 2 * i;
+                            x = k >= lo_c && k < hi_c ? x : -INFINITY;
+                            y = k + 1 >= lo_c && k + 1 < hi_c ? y : -INFINITY;
+                        }
+                        x = kv4_ex2(x);
+                        y = kv4_ex2(y);
+                        sum = add2(sum, two(x, y));
+                        p[i] = half2_bits(x, y);
+                    }
+                    st16(p_at + 16 * q, p);
+                }
+                float x, y;
+                parts(sum, x, y);
+                return x + y;
+            };
+            auto raise = [&]() {   // m to the largest score so far, the row of O with it
+                float top = KV4_NEG;
+#pragma unroll
+                for (int q = 0; q < CK / 32; ++q) {
+                    uint32_t v[32];
+                    ld32(s_at + 32 * q, v);
+                    ld_wait(v);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int k = 32 * q + i;
+                        const float x = fmaf(__uint_as_float(v[i]), kq, ev);
+                        if (k >= lo_c && k < hi_c) top = fmaxf(top, x);
+                    }
+                }
+                const float to = fmaxf(m, top), f = kv4_ex2(m - to);
+                m = to;
+                l *= f;
+                if (c > 0) {
+#pragma unroll
+                    for (int q = 0; q < HD / 32; ++q) {
+                        uint32_t v[32];
+                        ld32(o_at + 32 * q, v);
+                        ld_wait(v);
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
+                        st16(o_at + 32 * q, v);
+                        st16(o_at + 32 * q + 16, v + 16);
+                    }
+                }
+            };
+            if (c == 0) raise();
+            float sum = edge ? weigh(std::true_type{}) : weigh(std::false_type{});
+            if (__any_sync(0xffffffffu, sum > FULL)) {
+                raise();
+                sum = edge ? weigh(std::true_type{}) : weigh(std::false_type{});
+            }
+            l = fmaf(sum, kv4_ex2(-ev), l);
+            if (ms.bad[sg][0] | ms.bad[sg][1] | ms.bad[sg][2] | ms.bad[sg][3]) {
+                for (int k = max(lo_c, 0); k < min(hi_c, CK); ++k)
+                    if (ms.bad[sg][(k >> 4) & 3]) bad |= ms.bad_groups[sg][k];
+            }
+            st_wait();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&ms.p_full[tile]);
+        }
+        if (tile < tiles) {
+            if (ok && n > 0) {
+                ok = __all_sync(0xffffffffu, wait(&ms.o_full[tile], 0, abort));
+                fence_after();
+            }
+            const bool row_ok = u < units;
+            const int j = row_ok ? u / a.group : 0, g = row_ok ? u - j * a.group : 0;
+            const int64_t at = (int64_t)(row0 + j) * a.hq + h * a.group + g;
+            const float inv = a.nsplit > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+            if (!ok) bad = 0xffu;
+#pragma unroll
+            for (int q = 0; q < NG; ++q) {
+                uint32_t v[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) v[i] = 0;
+                if (ok && n > 0) {
+                    ld32(o_at + 32 * q, v);
+                    ld_wait(v);
+                }
+                float x[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i)
+                    x[i] = bad >> q & 1 ? __int_as_float(0x7fffffff) : __uint_as_float(v[i]) * inv;
+                if (!row_ok) continue;
+                if (a.nsplit > 1) {
+                    float4* o = reinterpret_cast<float4*>(a.part_o + (at * a.nsplit + split) * HD + 32 * q);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) o[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+                } else {
+                    uint4* o = reinterpret_cast<uint4*>(a.out + at * HD + 32 * q);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        __nv_bfloat162 y[4];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) y[e] = __floats2bfloat162_rn(x[8 * i + 2 * e], x[8 * i + 2 * e + 1]);
+                        o[i] = *reinterpret_cast<uint4*>(y);
+                    }
+                }
+            }
+            if (row_ok && a.nsplit > 1) {
+                a.part_ml[(at * a.nsplit + split) * 2] = m;
+                a.part_ml[(at * a.nsplit + split) * 2 + 1] = l;
+            }
+        }
+    }
+    fence_before();
+    __syncthreads();
+    if (warp == 13)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+}  // namespace
+
+namespace pulsar {
+
+int kv4_prefill_launch(const Kv4AttnArgs& a, int head_dim, int64_t sequences, int utiles, cudaStream_t stream) {
+    const dim3 grid((unsigned)(utiles * a.nsplit), (unsigned)a.hkv, (unsigned)sequences);
+    if (head_dim == 64) {
+        constexpr int bytes = Lay<64>::BYTES + 1024;
+        PULSAR_TRY(ensure_smem_attr((const void*)k_kv4_prefill<64>, bytes, "k_kv4_prefill shared memory"));
+        k_kv4_prefill<64><<<grid, THREADS, bytes, stream>>>(a);
+    } else {
+        constexpr int bytes = Lay<128>::BYTES + 1024;
+        PULSAR_TRY(ensure_smem_attr((const void*)k_kv4_prefill<128>, bytes, "k_kv4_prefill shared memory"));
+        k_kv4_prefill<128><<<grid, THREADS, bytes, stream>>>(a);
+    }
+    PULSAR_LAUNCH_CHECK("k_kv4_prefill");
+    return PULSAR_OK;
+}
+
+}  // namespace pulsar

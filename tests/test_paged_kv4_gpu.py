@@ -3,7 +3,9 @@
 Tolerances. A bf16 result is rounded once: relative 2^-9, taken as 2^-8 with the 32-bit work before
 it. A stored value is off by half a step s / 2 plus what the rounding of s (15 s 2^-9) and of the
 minimum z (|z| 2^-9) to bf16 add. Attention accumulates in 32 bits with operands good to 2^-16:
-2^-12 of the largest value that a row sees, besides the rounding of the result."""
+2^-12 of the largest value that a row sees, besides the rounding of the result. Above 32 units a kv
+head the operands are fp16 (keys and values rounded twice, weights once, at 2^-12): 3 2^-12 of the
+largest value, and 2 2^-12 scale sum |q k| in a score, so twice that in a weight over their sum."""
 
 from __future__ import annotations
 
@@ -77,6 +79,7 @@ def plain_attention(q, k, v, table, lens, cu, scale, window):
     group, page = q.shape[1] // k.shape[2], k.shape[1]
     out = torch.zeros_like(q)
     top = torch.zeros(q.shape[0], q.shape[1], 1, dtype=torch.double)   # the largest value a row sees
+    amp = torch.zeros_like(top)                                        # the largest scale sum |q k|
     for b, n in enumerate(lens):
         rows = range(cu[b], cu[b + 1])
         for j, row in enumerate(rows):
@@ -92,13 +95,15 @@ def plain_attention(q, k, v, table, lens, cu, scale, window):
                 p = torch.softmax(kk[:, h // group] @ q[row, h] * scale, 0)
                 out[row, h] = p @ vv[:, h // group]
                 top[row, h] = vv[:, h // group].abs().max()
-    return out, top
+                amp[row, h] = (kk[:, h // group].abs() @ q[row, h].abs()).max() * scale
+    return out, top, amp
 
 
-def assert_attention(got, ref, top):
+def assert_attention(got, ref, top, amp, many=False):
     err = (got.cpu().double() - ref).abs()
     assert torch.isfinite(got.float()).all()
-    worst = (err - (2.0 ** -8 * ref.abs() + 2.0 ** -12 * top)).max().item()
+    rel = 3 * 2.0 ** -12 + 4 * 2.0 ** -12 * amp if many else 2.0 ** -12
+    worst = (err - (2.0 ** -8 * ref.abs() + rel * top)).max().item()
     assert worst <= 0, f"off by {err.max().item():.3e}, {worst:.3e} over the bound"
 
 
@@ -264,8 +269,8 @@ def _attend(paged, lens, counts, hq, hkv, d, page, window=0, scale=None, seed=0,
                               None if one else torch.tensor(cu, dtype=torch.int32).cuda(),
                               max_q=max(1, max(counts)), window=window, scale=scale, **kw)
     k, v = held(pages, d)
-    ref, top = plain_attention(q, k, v, table, lens, cu, d ** -0.5 if scale is None else scale, window)
-    assert_attention(got, ref, top)
+    ref, top, amp = plain_attention(q, k, v, table, lens, cu, d ** -0.5 if scale is None else scale, window)
+    assert_attention(got, ref, top, amp, max(counts) * (hq // hkv) > 32)
     return got
 
 
@@ -292,10 +297,42 @@ def test_verify_rows(paged, hq, hkv, d, window):
     _attend(paged, [5, 40, 70, 3, 129, 64, 0, 9], [5, 1, 8, 5, 3, 0, 2, 7], hq, hkv, d, 16, window=window)
 
 
-@pytest.mark.parametrize("hq,hkv,d,window", [(4, 1, 64, 0), (4, 1, 64, 70), (8, 4, 128, 0), (3, 3, 64, 50)])
-def test_prompt_rows(paged, hq, hkv, d, window):
-    """Whole prompts and chunks behind cached keys: more units than one tile holds."""
-    _attend(paged, [100, 75, 150, 33], [100, 40, 65, 1], hq, hkv, d, 64, window=window)
+@pytest.mark.parametrize("hq,hkv,d,page,window", [(4, 1, 64, 64, 0), (4, 1, 64, 16, 70), (8, 4, 128, 32, 0),
+                                                  (3, 3, 64, 128, 50), (7, 1, 128, 16, 33), (8, 2, 64, 32, 1)])
+def test_prompt_rows(paged, hq, hkv, d, page, window):
+    """Whole prompts and chunks behind cached keys: more units than one tile holds, few, none."""
+    _attend(paged, [100, 75, 150, 33, 20], [100, 40, 65, 1, 0], hq, hkv, d, page, window=window)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_prompt_rows_longer_than_their_keys(paged, d):
+    """Rows before the first key see none of them."""
+    got = _attend(paged, [50, 0, 129], [90, 33, 140], 4, 2, d, 16)
+    assert (got[:40] == 0).all() and (got[90:123] == 0).all() and (got[123:134] == 0).all()
+
+
+@pytest.mark.parametrize("d,window", [(64, 0), (128, 0), (64, 300)])
+def test_prompt_rows_behind_many_keys(paged, d, window):
+    """A few dozen rows on a long context: the keys are split over CTAs."""
+    _attend(paged, [1500, 700], [20, 9], 4, 2, d, 64, window=window)
+    _attend(paged, [2600], [40], 2, 2, d, 16, window=window)
+
+
+def test_prompt_values_of_any_size(paged):
+    """Keys and values far from 1, and of unequal size along the sequence, keep their precision."""
+    lens, page, d = [400], 64, 64
+    for kx, vx in ((2.0 ** -20, 2.0 ** 25), (2.0 ** 12, 2.0 ** -30)):
+        pages, table = _filled(paged, lens, 1, d, page)
+        k = _randn(1, 400, 1, d) * kx
+        v = _randn(2, 400, 1, d) * vx * torch.linspace(-3, 3, 400).exp2()[:, None, None]
+        slots = torch.tensor([table[0][i // page] * page + i % page for i in range(400)])
+        paged.kv4_append(None, k.cuda().bfloat16(), v.cuda().bfloat16(), pages, slots.cuda())
+        q = _randn(3, 60, 2, d).bfloat16().cuda()
+        got = paged.kv4_attention(q, pages, torch.tensor(table, dtype=torch.int32).cuda(),
+                                  torch.tensor(lens, dtype=torch.int32).cuda(),
+                                  torch.tensor([0, 60], dtype=torch.int32).cuda(), max_q=60, scale=0.2 / kx)
+        hk, hv = held(pages, d)
+        assert_attention(got, *plain_attention(q, hk, hv, table, lens, [0, 60], 0.2 / kx, 0), many=True)
 
 
 @pytest.mark.parametrize("d,window,max_kv", [(64, 0, None), (64, 0, 2500), (128, 0, None), (64, 900, None), (64, 0, 64)])
@@ -320,8 +357,7 @@ def test_pages_outside_the_cache_are_masked(paged):
     got = paged.kv4_attention(q, pages, torch.tensor(table, dtype=torch.int32).cuda(),
                               torch.tensor(lens, dtype=torch.int32).cuda())
     k, v = held(pages, 64)
-    ref, top = plain_attention(q, k, v, table, lens, [0, 1, 2], 0.125, 0)
-    assert_attention(got, ref, top)
+    assert_attention(got, *plain_attention(q, k, v, table, lens, [0, 1, 2], 0.125, 0))
 
 
 def test_lengths_and_rows_outside_the_tensors(paged):
@@ -357,6 +393,21 @@ def test_nan_stays_where_it_is_seen(paged):
     assert torch.isfinite(got[:3].float()).all() and torch.isnan(got[3:].float()).all()
     got = paged.kv4_attention(q, pages, t, n, cu, max_q=6, window=2)
     assert torch.isnan(got[3:5].float()).all() and torch.isfinite(got[[0, 1, 2, 5]].float()).all()
+    q = _randn(5, 20, 4, 64).bfloat16().cuda()                  # positions 20 .. 39
+    cu = torch.tensor([0, 20], dtype=torch.int32).cuda()
+    got = paged.kv4_attention(q, pages, t, n, cu, max_q=20)
+    assert torch.isfinite(got[:17].float()).all() and torch.isnan(got[17:].float()).all()
+    # a value that is none in 32 of its dims, its key sound: those dims only
+    good, half = torch.ones_like(bad), torch.ones_like(bad)
+    half[..., 40] = float("inf")
+    paged.kv4_append(None, good, half, pages, torch.tensor([table[0][2] * page + 5]).cuda())
+    for rows, window in ((6, 0), (20, 0), (20, 2)):
+        got = paged.kv4_attention(q[:rows], pages, t, n, torch.tensor([0, rows], dtype=torch.int32).cuda(), max_q=rows,
+                                  window=window).float()
+        sees = torch.zeros(rows, dtype=torch.bool)
+        sees[rows - 3:rows - 1 if window else rows] = True
+        assert torch.isfinite(got[..., :32]).all() and torch.isfinite(got[~sees]).all()
+        assert torch.isnan(got[sees][..., 32:]).all()
 
 
 def test_strided_queries_streams_and_repeats(paged):
