@@ -500,7 +500,7 @@ struct Plan {
 // How a call is cut. More than MANY units of a sequence's rows go to k_kv4_prefill in tiles of 256.
 // Others: the fewest columns that hold max_q rows of a group (four: both halves of the weights in
 // one operand), at most 32 (heads of 128: 16, for the registers). Splits of the keys: until about
-// four CTAs an SM are there (k_kv4_prefill: one), of at least 8 pairs of tiles (two a warp; 4 chunks).
+// four CTAs an SM are there (k_kv4_prefill: one), of at least 8 pairs of tiles (two a warp; two steps).
 constexpr int64_t MANY = 32;
 Plan make_plan(int64_t B, int64_t Hkv, int64_t group, int64_t head_dim, int64_t max_q, int64_t max_kv,
                int64_t window) {
@@ -510,7 +510,7 @@ Plan make_plan(int64_t B, int64_t Hkv, int64_t group, int64_t head_dim, int64_t 
     p.dup = units <= 4;
     p.nt = (int)(units > 8 * cap ? cap : (units + 7) / 8);
     const int64_t ut = p.many ? KV4_PF_UNITS : p.dup ? 4 : 8 * p.nt;
-    const int64_t step = p.many ? kv4_pf_chunk((int)head_dim) : 32, least = p.many ? 4 : 8, full = p.many ? 148 : 148 * 4;
+    const int64_t step = p.many ? KV4_PF_STEP : 32, least = p.many ? 2 : 8, full = p.many ? 148 : 148 * 4;
     p.utiles = (int)((units + ut - 1) / ut);
     int64_t span = max_kv;
     if (window > 0) {

@@ -52,7 +52,7 @@ __device__ __forceinline__ float kv4_z(uint32_t param) { return __uint_as_float(
 
 // Many query rows (kv4_prefill.cu): units = query rows x heads of a group.
 constexpr int KV4_PF_UNITS = 256;   // units of a CTA
-constexpr int kv4_pf_chunk(int head_dim) { return head_dim == 64 ? 128 : 64; }   // keys of a step
+constexpr int KV4_PF_STEP = 128;    // keys of a step
 int kv4_prefill_launch(const Kv4AttnArgs& a, int head_dim, int64_t sequences, int utiles, cudaStream_t stream);
 
 }  // namespace pulsar

@@ -2,18 +2,20 @@
 // half of pulsar_op_kv4_attention: prompts and chunks of prompts.
 //
 // CTA: 256 units (query rows x heads of one kv head's group) of a sequence as two tiles of 128, one
-// TMEM lane a unit, over a range of its keys in chunks of CK (128, for heads of 128: 64). Per chunk
+// TMEM lane a unit, over a range of its keys in chunks of 64, two to a step of the copies:
 //   copy      the packed tiles into a ring, 1-D bulk copies of whole pages' parts (warp 12)
-//   unpack    K^ [CK keys][HD] and V^T^ [HD][CK keys] in fp16, K-major SWIZZLE_128B (warps 8-11): the
+//   unpack    K^ [64 keys][HD] and V^T^ [HD][64 keys] in fp16, K-major SWIZZLE_128B (warps 8-11): the
 //             cache keeps codes so that a word's halves are neighbours in the operand's rows
-//   S = Q K^  tcgen05.mma kind::f16, M 128, N CK, fp32 in TMEM (one lane of warp 13 issues every MMA)
-//   softmax   a thread per unit (warps 0-3: tile 0, 4-7: tile 1): weights in fp16 back to TMEM
+//   S = Q K^  tcgen05.mma kind::f16, M 128, N 64, fp32 in TMEM (warp 13 issues every MMA)
+//   softmax   a thread per unit (warps 0-3: tile 0, 4-7: tile 1): weights in fp16 back to TMEM, over
+//             the scores they came from
 //   O += P V^ with P read from TMEM as the A operand, O in TMEM
-// The two tiles take turns: while one tile's weights are computed, the other's MMAs run.
+// Scores have two buffers a tile: a chunk's are there before the weights of the one before are done,
+// so the softmax threads, whose exponentials bound the kernel, do not wait for the tensor cores.
 //
 // Exactness. fp16 has the significand for it (values s c + z of 8-bit s, z and 4-bit c are rounded
 // at 2^-12, weights too) but not the range, so powers of two move out: queries by their row, keys and
-// values by their chunk (2^eK, 2^eV from the largest |value| that s and z allow, over the keys that
+// values by their step of 128 (2^eK, 2^eV from the largest |value| that s and z allow, over the keys that
 // some unit sees). Score and weight: x = 2^eK 2^eq scale log2(e) S + eV - m, P = 2^x; P V^ = 2^(s - m) V
 // and l = sum 2^-eV P. The reference m of a unit moves when a chunk's sum of weights passes 2^14
 // (then the row of O is rescaled and the chunk's weights taken again), so P stays inside fp16 and no
@@ -42,24 +44,24 @@ constexpr float FULL = 16384.f;   // a chunk's weights are taken again when thei
 
 template <int HD>
 struct Lay {
-    static constexpr int CK = kv4_pf_chunk(HD), TPC = CK / 16, NG = HD / 32, NB = HD / 64;
-    static constexpr int PS = 3;                                     // stages of the packed ring
-    static constexpr uint32_t QB = 128 * HD * 2, KB = CK * HD * 2;   // bytes of a Q tile, of K^ or V^
-    static constexpr uint32_t PB = TPC * Kv4Tile<HD>::BYTES;
-    static constexpr uint32_t Q = 0, K = 2 * QB, V = K + 2 * KB, P = V + 2 * KB, MISC = P + PS * PB;
+    static constexpr int CK = 64, SK = KV4_PF_STEP, TPS = SK / 16, NG = HD / 32, NB = HD / 64;
+    static constexpr int PS = HD == 64 ? 3 : 2, KS = HD == 64 ? 4 : 3;   // stages: packed steps, unpacked chunks
+    static constexpr uint32_t QB = 128 * HD * 2, KB = CK * HD * 2;       // bytes of a Q tile, of K^ or V^
+    static constexpr uint32_t PB = TPS * Kv4Tile<HD>::BYTES;
+    static constexpr uint32_t Q = 0, K = 2 * QB, V = K + KS * KB, P = V + KS * KB, MISC = P + PS * PB;
     static constexpr uint32_t BYTES = MISC + 1024;
-    static constexpr uint32_t S_COL = 0, P_COL = 2 * CK, O_COL = 3 * CK;   // TMEM columns, two of each
+    static constexpr uint32_t S_COL = 0, O_COL = 4 * CK;   // TMEM columns: [tile][2] scores, [tile] O
     static_assert(O_COL + 2 * HD <= 512 && PB % 1024 == 0 && BYTES + 1024 <= 227 * 1024, "fits");
 };
 
 struct Misc {   // in shared memory after the operands
-    uint64_t packed_full[3], packed_empty[3], kv_full[2], kv_empty[2], s_full[2], p_full[2], o_full[2], drain;
+    uint64_t packed_full[3], packed_empty[3], kv_full[4], kv_empty[4], s_full[2][2], p_full[2][2], pv_done[2], drain;
     uint32_t valid[3];       // tiles of the packed stage that are there
-    uint32_t stop[2][4];     // per chunk parity and unpacking warp: a wait has run out
-    uint32_t top[2][4][2];   // per chunk parity and unpacking warp: largest |K|, |V| as float bits
-    float kscale[2], ev[2];
-    uint32_t bad[2][4];      // per stage and unpacking warp: some group of V is NaN
-    uint8_t bad_groups[2][128];
+    uint32_t stop[2][4];     // per step parity and unpacking warp: a wait has run out
+    uint32_t top[2][4][2];   // largest |K|, |V| as float bits
+    float kscale[4], ev[4];  // per unpacked stage
+    uint32_t bad[4][4];      // and unpacking warp: some group of V is NaN
+    uint8_t bad_groups[4][64];
     uint32_t tmem;
     int abort;
 };
@@ -78,31 +80,43 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile in
     return true;
 }
 
-// K-major SWIZZLE_128B operand: rows of 128 bytes, atoms of 8 rows.
-__device__ __forceinline__ uint64_t desc(uint32_t addr) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) |
-           (2ull << 61);
-}
+// K-major SWIZZLE_128B operand (rows of 128 bytes, atoms of 8 rows): the descriptor's upper word is a
+// constant, the lower one the address.
+constexpr uint32_t DESC_HI = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t desc(uint32_t addr) { return ((addr >> 4) & 0x3FFF) | (1u << 16); }
 // kind::f16: fp32 accumulator, fp16 operands, both K-major, M = 128.
 constexpr uint32_t idesc(int n) { return (1u << 4) | ((uint32_t)(n >> 3) << 17) | (8u << 24); }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t id, bool acc) {
+// The whole warp comes here with the same operands, which then sit in uniform registers; the elected
+// lane (one nonzero) issues. (An MMA issued inside a branch on the lane takes about 70 cycles.)
+__device__ __forceinline__ void mma_ss(uint32_t one, uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(id), "r"((uint32_t)acc)
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %0, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "mov.b64 x, {%2, %6};\n\tmov.b64 y, {%3, %6};\n\t"
+        "@p tcgen05.mma.cta_group::1.kind::f16 [%1], x, y, %4, q;\n\t}" ::"r"(one),
+        "r"(d), "r"(a), "r"(b), "r"(id), "r"(acc), "n"(DESC_HI)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t id, bool acc) {
+__device__ __forceinline__ void mma_ts(uint32_t one, uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(id), "r"((uint32_t)acc)
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %0, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "mov.b64 y, {%3, %6};\n\t"
+        "@p tcgen05.mma.cta_group::1.kind::f16 [%1], [%2], y, %4, q;\n\t}" ::"r"(one),
+        "r"(d), "r"(a), "r"(b), "r"(id), "r"(acc), "n"(DESC_HI)
         : "memory");
 }
-__device__ __forceinline__ void commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
+__device__ __forceinline__ void commit(uint32_t one, uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %0, 0;\n\t"
+        "@p tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%1];\n\t}" ::"r"(one),
+        "r"(smem_u32(bar))
+        : "memory");
+}
+__device__ __forceinline__ uint32_t elect() {
+    uint32_t one;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one;
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -191,7 +205,7 @@ template <int HD>
 __global__ void __launch_bounds__(THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a) {
     using L = Lay<HD>;
     using T = Kv4Tile<HD>;
-    constexpr int CK = L::CK, TPC = L::TPC, NG = L::NG, NB = L::NB, PS = L::PS;
+    constexpr int CK = L::CK, SK = L::SK, TPS = L::TPS, NG = L::NG, NB = L::NB, PS = L::PS, KS = L::KS;
     extern __shared__ unsigned char raw[];
     unsigned char* sm = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
     const uint32_t sb = smem_u32(sm);
@@ -211,21 +225,25 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a)
     const int first = len - nq + u0 / a.group, last = len - nq + ulast / a.group;
     auto low = [&](int pos) { return a.window > 0 ? max(0, pos - a.window + 1) : 0; };
     const int kmin = low(first), kmax = max(last + 1, 0);
-    const int chunk0 = kmin / CK + split * a.split_len;
-    const int chunk1 = split == a.nsplit - 1 ? (kmax + CK - 1) / CK : min((kmax + CK - 1) / CK, chunk0 + a.split_len);
-    const int n = max(chunk1 - chunk0, 0);
+    const int step0 = kmin / SK + split * a.split_len, base = step0 * SK;
+    const int kend = split == a.nsplit - 1 ? kmax : min(kmax, base + a.split_len * SK);
+    const int n = kend > base ? (kend - base + CK - 1) / CK : 0, steps = (n + 1) / 2;   // chunks, steps
 
     if (tid == 0) {
         for (int i = 0; i < PS; ++i) {
             mbar_init(&ms.packed_full[i], 1);
             mbar_init(&ms.packed_empty[i], 4);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < KS; ++i) {
             mbar_init(&ms.kv_full[i], 4);
             mbar_init(&ms.kv_empty[i], 1);
-            mbar_init(&ms.s_full[i], 1);
-            mbar_init(&ms.p_full[i], 4);
-            mbar_init(&ms.o_full[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            for (int j = 0; j < 2; ++j) {
+                mbar_init(&ms.s_full[i][j], 1);
+                mbar_init(&ms.p_full[i][j], 4);
+            }
+            mbar_init(&ms.pv_done[i], 1);
         }
         mbar_init(&ms.drain, 1);
         ms.abort = 0;
@@ -290,12 +308,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a)
     const uint32_t tmem = ms.tmem;
 
     if (warp == 12) {
-        // copies: lane i a piece of the chunk (the part of it in one page, or all of it)
-        const int page_tiles = 1 << (a.page_shift - 4), piece = min(page_tiles, TPC), pieces = TPC / piece;
-        auto page_of = [&](int c) { return lane < pieces && c < n ? kv4_page(a, b, (chunk0 + c) * TPC + lane * piece) : -1; };
+        // copies: lane i a piece of the step (the part of it in one page, or all of it)
+        const int page_tiles = 1 << (a.page_shift - 4), piece = min(page_tiles, TPS), pieces = TPS / piece;
+        auto page_of = [&](int c) { return lane < pieces && c < steps ? kv4_page(a, b, (step0 + c) * TPS + lane * piece) : -1; };
         int next = page_of(0);
         int c = 0;
-        for (; c < n; ++c) {
+        for (; c < steps; ++c) {
             const int page = next, st = c % PS;
             next = page_of(c + 1);
             bool ok = true;
@@ -317,64 +335,67 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a)
             if (page >= 0)
                 tma_load_1d(sm + L::P + st * L::PB + lane * piece * T::BYTES,
                             a.pages + ((int64_t)page * a.hkv + h) * a.page_bytes +
-                                (int64_t)(((chunk0 + c) * TPC + lane * piece) & (page_tiles - 1)) * T::BYTES,
+                                (int64_t)(((step0 + c) * TPS + lane * piece) & (page_tiles - 1)) * T::BYTES,
                             piece * T::BYTES, &ms.packed_full[st]);
         }
         // what was issued lands before the CTA ends
         for (int i = max(0, c - PS); i < c; ++i) mbar_wait(&ms.packed_full[i % PS], (i / PS) & 1);
     } else if (warp == 13) {
-        if (lane == 0 && n > 0) {
+        if (n > 0) {
+            const uint32_t one = elect(), tm = __shfl_sync(0xffffffffu, tmem, 0);
+            auto ready = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity, abort)); };
             auto mma_s = [&](int t, int c) {
-                const uint32_t kt = sb + L::K + (c & 1) * L::KB, qt = sb + L::Q + t * L::QB;
+                const uint32_t kt = desc(sb + L::K + (c % KS) * L::KB), qt = desc(sb + L::Q + t * L::QB);
 #pragma unroll
                 for (int ks = 0; ks < HD / 16; ++ks)
-                    mma_ss(tmem + L::S_COL + t * CK, desc(qt + (ks >> 2) * (128 * 128) + (ks & 3) * 32),
-                           desc(kt + (ks >> 2) * (CK * 128) + (ks & 3) * 32), idesc(CK), ks > 0);
-                commit(&ms.s_full[t]);
+                    mma_ss(one, tm + L::S_COL + (2 * t + (c & 1)) * CK,
+                           qt + (((ks >> 2) * (128 * 128) + (ks & 3) * 32) >> 4),
+                           kt + (((ks >> 2) * (CK * 128) + (ks & 3) * 32) >> 4), idesc(CK), ks > 0);
+                commit(one, &ms.s_full[t][c & 1]);
             };
-            bool ok = wait(&ms.kv_full[0], 0, abort);
+            bool ok = ready(&ms.kv_full[0], 0);
             fence_after();
             if (ok)
                 for (int t = 0; t < tiles; ++t) mma_s(t, 0);
             for (int c = 0; ok && c < n; ++c) {
-                const uint32_t vt = sb + L::V + (c & 1) * L::KB;
+                if (c + 1 < n) {   // the next chunk's scores: over those (and the weights) of chunk c - 1
+                    if (!(ok = ready(&ms.kv_full[(c + 1) % KS], ((c + 1) / KS) & 1))) break;
+                    for (int t = 0; ok && t < tiles; ++t) {
+                        if (c > 0 && !(ok = ready(&ms.pv_done[t], (c - 1) & 1))) break;
+                        fence_after();
+                        mma_s(t, c + 1);
+                    }
+                }
+                const uint32_t vt = desc(sb + L::V + (c % KS) * L::KB);
                 for (int t = 0; ok && t < tiles; ++t) {
-                    if (!(ok = wait(&ms.p_full[t], c & 1, abort))) break;
+                    if (!(ok = ready(&ms.p_full[t][c & 1], (c >> 1) & 1))) break;
                     fence_after();
 #pragma unroll
                     for (int ks = 0; ks < CK / 16; ++ks)
-                        mma_ts(tmem + L::O_COL + t * HD, tmem + L::P_COL + t * (CK / 2) + ks * 8,
-                               desc(vt + (ks >> 2) * (HD * 128) + (ks & 3) * 32), idesc(HD), c > 0 || ks > 0);
-                    if (t == tiles - 1) commit(&ms.kv_empty[c & 1]);
-                    if (c + 1 < n) {
-                        if (t == 0) {
-                            if (!(ok = wait(&ms.kv_full[(c + 1) & 1], ((c + 1) >> 1) & 1, abort))) break;
-                            fence_after();
-                        }
-                        mma_s(t, c + 1);   // its commit also says that this chunk's P V has completed
-                    } else {
-                        commit(&ms.o_full[t]);
-                    }
+                        mma_ts(one, tm + L::O_COL + t * HD, tm + L::S_COL + (2 * t + (c & 1)) * CK + ks * 8, vt + ks * 2,
+                               idesc(HD), c > 0 || ks > 0);
+                    commit(one, &ms.pv_done[t]);
+                    if (t == tiles - 1) commit(one, &ms.kv_empty[c % KS]);
                 }
             }
-            commit(&ms.drain);   // every MMA issued has completed
+            commit(one, &ms.drain);   // every MMA issued has completed
             mbar_wait(&ms.drain, 0);
         }
         __syncwarp();
     } else if (warp >= 8) {
-        // unpacking: warp w takes tiles w, w + 4 of the chunk
+        // unpacking: warp w takes tile w of each of a step's two chunks
         const int w = warp - 8, r = lane >> 2, t = lane & 3;
         bool good = true;   // no wait of this warp has run out; the four warps leave together
-        for (int c = 0; c < n; ++c) {
-            const int st = c % PS, sg = c & 1, k0 = (chunk0 + c) * CK;
+        for (int c = 0; c < steps; ++c) {
+            const int st = c % PS, sg = c & 1, k0 = base + c * SK;
             if (good) good = __all_sync(0xffffffffu, wait(&ms.packed_full[st], (c / PS) & 1, abort));
             const unsigned char* pk = sm + L::P + st * L::PB;
             const uint32_t valid = ms.valid[st];
             // the largest magnitudes that the chunk's s and z allow, and its NaN groups of V
             uint32_t topk = 0, topv = 0;
-            bool bad[TPC / 4][NB], any_bad = false;
+            bool bad[2][NB], any_bad[2] = {false, false};
 #pragma unroll
-            for (int y = 0; y < TPC / 4; ++y) {
+            for (int y = 0; y < 2; ++y) {
                 const int tl = w + 4 * y;
                 const uint32_t* kp = reinterpret_cast<const uint32_t*>(pk + tl * T::BYTES + T::KP);
                 const uint32_t* vp = reinterpret_cast<const uint32_t*>(pk + tl * T::BYTES + T::VP);
@@ -388,12 +409,12 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a)
                     topk = max(topk, in && ka == ka ? __float_as_uint(ka) : 0u);
                     topv = max(topv, in && va == va ? __float_as_uint(va) : 0u);
                     bad[y][x] = in && !(kv4_z(vw) == kv4_z(vw));
-                    any_bad |= bad[y][x];
+                    any_bad[y] |= bad[y][x];
                 }
+                any_bad[y] = __any_sync(0xffffffffu, any_bad[y]);
             }
             topk = __reduce_max_sync(0xffffffffu, topk);
             topv = __reduce_max_sync(0xffffffffu, topv);
-            any_bad = __any_sync(0xffffffffu, any_bad);
             if (lane == 0) {
                 ms.top[sg][w][0] = topk;
                 ms.top[sg][w][1] = topv;
@@ -410,26 +431,25 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a)
             if (stop) break;
             const int ek = exponent_out(topk), ev = exponent_out(topv);
             const float fk = exp2i(-ek), fv = exp2i(-ev);
-            if (c >= 2) {   // the stage's readers: both tiles' MMAs and softmax of chunk c - 2
-                good = __all_sync(0xffffffffu, wait(&ms.kv_empty[sg], (c / 2 - 1) & 1, abort));
-                if (!good) continue;
-            }
-            if (any_bad) {   // rare: which groups of which keys
 #pragma unroll
-                for (int y = 0; y < TPC / 4; ++y)
+            for (int y = 0; y < 2; ++y) {
+                const int ch = 2 * c + y, sk = ch % KS;
+                if (ch >= n) break;
+                if (ch >= KS) {   // the stage's readers: both tiles' MMAs and softmax of chunk ch - KS
+                    if (good) good = __all_sync(0xffffffffu, wait(&ms.kv_empty[sk], (ch / KS - 1) & 1, abort));
+                    if (!good) break;
+                }
+                if (any_bad[y]) {   // rare: which groups of which keys
 #pragma unroll
                     for (int x = 0; x < NB; ++x) {
                         uint32_t bits = bad[y][x] ? 1u << (lane % NG) : 0u;
 #pragma unroll
                         for (int o = 1; o < NG; o <<= 1) bits |= __shfl_xor_sync(0xffffffffu, bits, o);
                         const int slot = (x * 32 + lane) / NG;
-                        if (lane % NG == 0)
-                            ms.bad_groups[sg][16 * (w + 4 * y) + (slot >> 1) + 8 * (slot & 1)] = (uint8_t)bits;
+                        if (lane % NG == 0) ms.bad_groups[sk][16 * w + (slot >> 1) + 8 * (slot & 1)] = (uint8_t)bits;
                     }
-            }
-            const uint32_t kt = sb + L::K + sg * L::KB, vt = sb + L::V + sg * L::KB;
-#pragma unroll
-            for (int y = 0; y < TPC / 4; ++y) {
+                }
+                const uint32_t kt = sb + L::K + sk * L::KB, vt = sb + L::V + sk * L::KB;
                 const int tl = w + 4 * y;
                 const unsigned char* tp = pk + tl * T::BYTES;
                 const bool there = valid >> tl & 1;
@@ -444,7 +464,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a)
                 for (int hf = 0; hf < 2; ++hf) {
                     const int key = k0 + 16 * tl + r + 8 * hf;
                     const bool in = there && key >= kmin && key < kmax;
-                    const uint32_t row = kt + (2 * tl + hf) * 1024 + r * 128 + 4 * t;
+                    const uint32_t row = kt + (2 * w + hf) * 1024 + r * 128 + 4 * t;
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
                         const float s = in ? kv4_s(par[hf * NG + g]) * fk : 0.f, z = in ? kv4_z(par[hf * NG + g]) * fk : 0.f;
@@ -466,8 +486,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a)
                 for (int hf = 0; hf < 2; ++hf) {
                     const int key = k0 + 16 * tl + 2 * t + 8 * hf;
                     const bool in0 = there && key >= kmin && key < kmax, in1 = there && key + 1 >= kmin && key + 1 < kmax;
-                    const int col = 16 * tl + 8 * hf;   // of the 8 keys that a 16-byte piece holds
-                    const uint32_t blk = vt + (col >> 6) * (HD * 128) + r * 128 + ((((col & 63) >> 3) ^ r) << 4) + 4 * t;
+                    const uint32_t blk = vt + r * 128 + (((2 * w + hf) ^ r) << 4) + 4 * t;
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
                         const uint32_t p0 = vpar[hf * NG + g], p1 = vpar[(2 + hf) * NG + g];
@@ -480,27 +499,24 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a)
                         for (int i = 0; i < 4; ++i) sts(blk + (4 * g + i) * 1024, x[i]);
                     }
                 }
-            }
-            if (lane == 0) {
-                ms.bad[sg][w] = any_bad;
-                if (w == 0) {
-                    ms.kscale[sg] = exp2i(ek);
-                    ms.ev[sg] = (float)ev;
+                if (lane == 0) {
+                    ms.bad[sk][w] = any_bad[y];
+                    if (w == 0) {
+                        ms.kscale[sk] = exp2i(ek);
+                        ms.ev[sk] = (float)ev;
+                    }
                 }
+                fence_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ms.kv_full[sk]);
             }
-            fence_async();
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&ms.kv_full[sg]);
-                mbar_arrive(&ms.packed_empty[st]);
-            }
+            if (lane == 0) mbar_arrive(&ms.packed_empty[st]);
         }
     } else {
         // softmax: this thread's unit u, tile warp / 4, TMEM lane (warp % 4) 32 + lane
         const int tile = warp >> 2;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t s_at = tmem + lanes + L::S_COL + tile * CK, p_at = tmem + lanes + L::P_COL + tile * (CK / 2),
-                       o_at = tmem + lanes + L::O_COL + tile * HD;
+        const uint32_t o_at = tmem + lanes + L::O_COL + tile * HD;
         const int pos = len - nq + min(u, units - 1) / a.group;
         const int lo = low(pos), hi = pos + 1;
         // keys that every unit of the warp sees
@@ -510,95 +526,85 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a)
         uint32_t bad = 0;
         bool ok = tile < tiles;
         for (int c = 0; ok && c < n; ++c) {
-            const int sg = c & 1, k0 = (chunk0 + c) * CK;
-            ok = wait(&ms.s_full[tile], c & 1, abort) && wait(&ms.kv_full[sg], (c >> 1) & 1, abort);
+            const int sk = c % KS, k0 = base + c * CK;
+            const uint32_t s_at = tmem + lanes + L::S_COL + (2 * tile + (c & 1)) * CK;
+            ok = wait(&ms.s_full[tile][c & 1], (c >> 1) & 1, abort) && wait(&ms.kv_full[sk], (c / KS) & 1, abort);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             fence_after();
-            const float kq = ms.kscale[sg] * qscale, ev = ms.ev[sg];
+            const float kq = ms.kscale[sk] * qscale, ev = ms.ev[sk];
             const bool edge = k0 < all_lo || k0 + CK > all_hi;
             const int lo_c = lo - k0, hi_c = hi - k0;
-            // weights with the reference m into P; their sum
-            auto weigh = [&](auto edge_tag) {
-                constexpr bool EDGE = decltype(edge_tag)::value;
+            uint32_t v[CK], p[CK / 2];
+            ld32(s_at, v);
+            ld32(s_at + 32, v + 32);
+            ld_wait(v);
+            ld_wait(v + 32);
+            if (edge) {   // scores of keys that the unit does not see
+#pragma unroll
+                for (int k = 0; k < CK; ++k)
+                    if (k < lo_c || k >= hi_c) v[k] = 0xff800000u;
+            }
+            // weights with the reference m; their sum
+            auto weigh = [&]() {
                 const f32x2 f2 = two(kq, kq), b2 = two(ev - m, ev - m);
                 f32x2 sum = two(0.f, 0.f);
-                uint32_t v[2][32];
-                ld32(s_at, v[0]);
 #pragma unroll
-                for (int q = 0; q < CK / 32; ++q) {
-                    ld_wait(v[q & 1]);
-                    if (q + 1 < CK / 32) ld32(s_at + 32 * (q + 1), v[(q + 1) & 1]);
-                    uint32_t p[16];
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        float x, y;
-                        parts(fma2(two(__uint_as_float(v[q & 1][2 * i]), __uint_as_float(v[q & 1][2 * i + 1])), f2, b2), x, y);
-                        if (EDGE) {
-                            const int k = 32 * q + 2 * i;
-                            x = k >= lo_c && k < hi_c ? x : -INFINITY;
-                            y = k + 1 >= lo_c && k + 1 < hi_c ? y : -INFINITY;
-                        }
-                        x = kv4_ex2(x);
-                        y = kv4_ex2(y);
-                        sum = add2(sum, two(x, y));
-                        p[i] = half2_bits(x, y);
-                    }
-                    st16(p_at + 16 * q, p);
+                for (int i = 0; i < CK / 2; ++i) {
+                    float x, y;
+                    parts(fma2(two(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), f2, b2), x, y);
+                    x = kv4_ex2(x);
+                    y = kv4_ex2(y);
+                    sum = add2(sum, two(x, y));
+                    p[i] = half2_bits(x, y);
                 }
                 float x, y;
                 parts(sum, x, y);
                 return x + y;
             };
             auto raise = [&]() {   // m to the largest score so far, the row of O with it
-                float top = KV4_NEG;
+                float top = m;
 #pragma unroll
-                for (int q = 0; q < CK / 32; ++q) {
-                    uint32_t v[32];
-                    ld32(s_at + 32 * q, v);
-                    ld_wait(v);
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const int k = 32 * q + i;
-                        const float x = fmaf(__uint_as_float(v[i]), kq, ev);
-                        if (k >= lo_c && k < hi_c) top = fmaxf(top, x);
-                    }
-                }
-                const float to = fmaxf(m, top), f = kv4_ex2(m - to);
-                m = to;
+                for (int k = 0; k < CK; ++k) top = fmaxf(top, fmaf(__uint_as_float(v[k]), kq, ev));
+                const float f = kv4_ex2(m - top);
+                m = top;
                 l *= f;
                 if (c > 0) {
+                    if (!__all_sync(0xffffffffu, wait(&ms.pv_done[tile], (c - 1) & 1, abort))) return;   // aborted
+                    fence_after();
 #pragma unroll
                     for (int q = 0; q < HD / 32; ++q) {
-                        uint32_t v[32];
-                        ld32(o_at + 32 * q, v);
-                        ld_wait(v);
+                        uint32_t o[32];
+                        ld32(o_at + 32 * q, o);
+                        ld_wait(o);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = __float_as_uint(__uint_as_float(v[i]) * f);
-                        st16(o_at + 32 * q, v);
-                        st16(o_at + 32 * q + 16, v + 16);
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        st16(o_at + 32 * q, o);
+                        st16(o_at + 32 * q + 16, o + 16);
                     }
                 }
             };
             if (c == 0) raise();
-            float sum = edge ? weigh(std::true_type{}) : weigh(std::false_type{});
+            float sum = weigh();
             if (__any_sync(0xffffffffu, sum > FULL)) {
                 raise();
-                sum = edge ? weigh(std::true_type{}) : weigh(std::false_type{});
+                sum = weigh();
             }
+            st16(s_at, p);
+            st16(s_at + 16, p + 16);
             l = fmaf(sum, kv4_ex2(-ev), l);
-            if (ms.bad[sg][0] | ms.bad[sg][1] | ms.bad[sg][2] | ms.bad[sg][3]) {
+            if (ms.bad[sk][0] | ms.bad[sk][1] | ms.bad[sk][2] | ms.bad[sk][3]) {
                 for (int k = max(lo_c, 0); k < min(hi_c, CK); ++k)
-                    if (ms.bad[sg][(k >> 4) & 3]) bad |= ms.bad_groups[sg][k];
+                    if (ms.bad[sk][k >> 4]) bad |= ms.bad_groups[sk][k];
             }
             st_wait();
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&ms.p_full[tile]);
+            if (lane == 0) mbar_arrive(&ms.p_full[tile][c & 1]);
         }
         if (tile < tiles) {
             if (ok && n > 0) {
-                ok = __all_sync(0xffffffffu, wait(&ms.o_full[tile], 0, abort));
+                ok = __all_sync(0xffffffffu, wait(&ms.pv_done[tile], (n - 1) & 1, abort) && !*abort);
                 fence_after();
             }
             const bool row_ok = u < units;
