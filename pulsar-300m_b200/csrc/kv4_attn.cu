@@ -497,7 +497,7 @@ struct Plan {
     int nt, dup, utiles, nsplit, split_len;
 };
 
-// How a call is cut. More than MANY units of a sequence's rows go to k_kv4_prefill in tiles of 256.
+// How a call is cut. More than MANY units of a sequence's rows go to k_kv4_prefill, 512 or 256 a CTA.
 // Others: the fewest columns that hold max_q rows of a group (four: both halves of the weights in
 // one operand), at most 32 (heads of 128: 16, for the registers). Splits of the keys: until about
 // four CTAs an SM are there (k_kv4_prefill: one), of at least 8 pairs of tiles (two a warp; two steps).
@@ -509,7 +509,7 @@ Plan make_plan(int64_t B, int64_t Hkv, int64_t group, int64_t head_dim, int64_t 
     p.many = units > MANY;
     p.dup = units <= 4;
     p.nt = (int)(units > 8 * cap ? cap : (units + 7) / 8);
-    const int64_t ut = p.many ? KV4_PF_UNITS : p.dup ? 4 : 8 * p.nt;
+    const int64_t ut = p.many ? kv4_pf_units((int)head_dim) : p.dup ? 4 : 8 * p.nt;
     const int64_t step = p.many ? KV4_PF_STEP : 32, least = p.many ? 2 : 8, full = p.many ? 148 : 148 * 4;
     p.utiles = (int)((units + ut - 1) / ut);
     int64_t span = max_kv;

@@ -51,8 +51,8 @@ __device__ __forceinline__ float kv4_s(uint32_t param) { return __uint_as_float(
 __device__ __forceinline__ float kv4_z(uint32_t param) { return __uint_as_float(param & 0xffff0000u); }
 
 // Many query rows (kv4_prefill.cu): units = query rows x heads of a group.
-constexpr int KV4_PF_UNITS = 256;   // units of a CTA
-constexpr int KV4_PF_STEP = 128;    // keys of a step
+constexpr int kv4_pf_units(int head_dim) { return head_dim == 64 ? 512 : 256; }   // units of a CTA
+constexpr int KV4_PF_STEP = 128;   // keys of a step
 int kv4_prefill_launch(const Kv4AttnArgs& a, int head_dim, int64_t sequences, int utiles, cudaStream_t stream);
 
 }  // namespace pulsar

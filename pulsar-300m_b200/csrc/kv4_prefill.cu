@@ -1,17 +1,17 @@
 // Attention of many query rows over the paged 4-bit KV cache (layout: kv4.cuh), the tensor-core
 // half of pulsar_op_kv4_attention: prompts and chunks of prompts.
 //
-// CTA: 256 units (query rows x heads of one kv head's group) of a sequence as two tiles of 128, one
-// TMEM lane a unit, over a range of its keys in chunks of 64, two to a step of the copies:
-//   copy      the packed tiles into a ring, 1-D bulk copies of whole pages' parts (warp 12)
-//   unpack    K^ [64 keys][HD] and V^T^ [HD][64 keys] in fp16, K-major SWIZZLE_128B (warps 8-11): the
-//             cache keeps codes so that a word's halves are neighbours in the operand's rows
-//   S = Q K^  tcgen05.mma kind::f16, M 128, N 64, fp32 in TMEM (warp 13 issues every MMA)
-//   softmax   a thread per unit (warps 0-3: tile 0, 4-7: tile 1): weights in fp16 back to TMEM, over
-//             the scores they came from
+// CTA: 512 units (query rows x heads of one kv head's group; heads of 128: 256) of a sequence as
+// tiles of 128, one TMEM lane a unit, over a range of its keys in chunks of 64, two to a step:
+//   unpack    a warp takes tiles of 16 tokens through a ring of its own (1-D bulk copies, page ids
+//             prefetched) to K^ [64 keys][HD] and V^T^ [HD][64 keys] in fp16, K-major SWIZZLE_128B:
+//             the cache keeps codes so that a word's halves are neighbours in the operand's rows
+//   S = Q K^  tcgen05.mma kind::f16, M 128, N 64, fp32 in TMEM (a warp for each tile of units)
+//   softmax   a thread per unit (four warps a tile): weights in fp16 back to TMEM, over the scores
 //   O += P V^ with P read from TMEM as the A operand, O in TMEM
-// Scores have two buffers a tile: a chunk's are there before the weights of the one before are done,
-// so the softmax threads, whose exponentials bound the kernel, do not wait for the tensor cores.
+// What bounds the kernel are the exponentials (16 a clock and SM). A tile's chain of MMA, scores,
+// weights and MMA is longer than its exponentials take, so four tiles are in flight at different
+// places of it, each with a softmax warp on every scheduler (heads of 128: the two that TMEM holds).
 //
 // Exactness. fp16 has the significand for it (values s c + z of 8-bit s, z and 4-bit c are rounded
 // at 2^-12, weights too) but not the range, so powers of two move out: queries by their row, keys and
@@ -39,33 +39,36 @@ using namespace pulsar;
 
 namespace {
 
-constexpr int THREADS = 14 * 32;
 constexpr float FULL = 16384.f;   // a chunk's weights are taken again when their sum passes this
 
 template <int HD>
 struct Lay {
-    static constexpr int CK = 64, SK = KV4_PF_STEP, TPS = SK / 16, NG = HD / 32, NB = HD / 64;
-    static constexpr int PS = HD == 64 ? 3 : 2, KS = HD == 64 ? 4 : 3;   // stages: packed steps, unpacked chunks
-    static constexpr uint32_t QB = 128 * HD * 2, KB = CK * HD * 2;       // bytes of a Q tile, of K^ or V^
-    static constexpr uint32_t PB = TPS * Kv4Tile<HD>::BYTES;
-    static constexpr uint32_t Q = 0, K = 2 * QB, V = K + KS * KB, P = V + KS * KB, MISC = P + PS * PB;
-    static constexpr uint32_t BYTES = MISC + 1024;
-    static constexpr uint32_t S_COL = 0, O_COL = 4 * CK;   // TMEM columns: [tile][2] scores, [tile] O
-    static_assert(O_COL + 2 * HD <= 512 && PB % 1024 == 0 && BYTES + 1024 <= 227 * 1024, "fits");
+    static constexpr int NT = HD == 64 ? 4 : 2;                              // tiles of 128 units
+    static constexpr int UNITS = 128 * NT;
+    static constexpr int SOFT = 4 * NT, UNPACK = HD == 64 ? 4 : 8, MMA = SOFT + UNPACK;   // warps; MMA + t: tile t
+    static constexpr int THREADS = (MMA + 4) * 32;
+    static constexpr int CK = 64, SK = KV4_PF_STEP, NG = HD / 32, NB = HD / 64;
+    static constexpr int YT = 8 / UNPACK;                                    // tiles of a step an unpacking warp takes
+    static constexpr int PS = HD == 64 ? 3 : 2, KS = HD == 64 ? 4 : 3;       // stages: packed steps, unpacked chunks
+    static constexpr uint32_t QB = 128 * HD * 2, KB = CK * HD * 2;           // bytes of a Q tile, of K^ or V^
+    static constexpr uint32_t TB = Kv4Tile<HD>::BYTES, PB = PS * YT * TB;    // of a warp's packed ring
+    static constexpr uint32_t Q = 0, K = NT * QB, V = K + KS * KB, P = V + KS * KB, MISC = P + UNPACK * PB;
+    static constexpr uint32_t BYTES = MISC + 2048;
+    static constexpr uint32_t S_COL = 0, O_COL = NT * CK;   // TMEM columns of the tiles' scores and of O
+    static_assert(O_COL + NT * HD <= 512 && MISC % 1024 == 0 && BYTES + 1024 <= 227 * 1024, "fits");
 };
 
 struct Misc {   // in shared memory after the operands
-    uint64_t packed_full[3], packed_empty[3], kv_full[4], kv_empty[4], s_full[2][2], p_full[2][2], pv_done[2], drain;
-    uint32_t valid[3];       // tiles of the packed stage that are there
-    uint32_t stop[2][4];     // per step parity and unpacking warp: a wait has run out
-    uint32_t top[2][4][2];   // largest |K|, |V| as float bits
+    uint64_t packed[8][3], kv_full[4], kv_empty[4], s_full[4], p_full[4], pv_done[4], drain[4];
+    uint32_t stop[2][8];     // per step parity and unpacking warp: a wait has run out
+    uint32_t top[2][8][2];   // largest |K|, |V| as float bits
     float kscale[4], ev[4];  // per unpacked stage
-    uint32_t bad[4][4];      // and unpacking warp: some group of V is NaN
+    uint32_t bad[4][4];      // and tile of 16 tokens: some group of V is NaN
     uint8_t bad_groups[4][64];
     uint32_t tmem;
     int abort;
 };
-static_assert(sizeof(Misc) <= 1024, "Misc fits its space");
+static_assert(sizeof(Misc) <= 2048, "Misc fits its space");
 
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
     if (mbar_try(bar, parity)) return true;
@@ -141,6 +144,15 @@ __device__ __forceinline__ void st16(uint32_t at, const uint32_t* r) {
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
+__device__ __forceinline__ void ld16(uint32_t at, uint32_t* r) {   // (waits)
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15}, [%16];\n\ttcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(at)
+        : "memory");
+}
 // Waits for the loads; the registers pass through it, so that nothing reads them earlier.
 __device__ __forceinline__ void ld_wait(uint32_t* r) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
@@ -202,17 +214,17 @@ __device__ __forceinline__ int exponent_out(uint32_t bits) {
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
 template <int HD>
-__global__ void __launch_bounds__(THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a) {
+__global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a) {
     using L = Lay<HD>;
     using T = Kv4Tile<HD>;
-    constexpr int CK = L::CK, SK = L::SK, TPS = L::TPS, NG = L::NG, NB = L::NB, PS = L::PS, KS = L::KS;
+    constexpr int CK = L::CK, SK = L::SK, NG = L::NG, NB = L::NB, PS = L::PS, KS = L::KS;
     extern __shared__ unsigned char raw[];
     unsigned char* sm = raw + ((1024 - (smem_u32(raw) & 1023)) & 1023);
     const uint32_t sb = smem_u32(sm);
     Misc& ms = *reinterpret_cast<Misc*>(sm + L::MISC);
     volatile int* abort = &ms.abort;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int split = blockIdx.x % a.nsplit, u0 = blockIdx.x / a.nsplit * KV4_PF_UNITS;
+    const int split = blockIdx.x % a.nsplit, u0 = blockIdx.x / a.nsplit * L::UNITS;
     const int h = blockIdx.y, b = blockIdx.z;
 
     int row0, nq;
@@ -220,8 +232,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a)
     const int units = nq * a.group;
     if (u0 >= units) return;
     const int len = min(max(a.kv_lens[b], 0), a.width << a.page_shift);
-    const int ulast = min(u0 + KV4_PF_UNITS, units) - 1;
-    const int tiles = ulast - u0 >= 128 ? 2 : 1;
+    const int ulast = min(u0 + L::UNITS, units) - 1;
+    const int tiles = (ulast - u0) / 128 + 1;
     const int first = len - nq + u0 / a.group, last = len - nq + ulast / a.group;
     auto low = [&](int pos) { return a.window > 0 ? max(0, pos - a.window + 1) : 0; };
     const int kmin = low(first), kmax = max(last + 1, 0);
@@ -230,74 +242,65 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a)
     const int n = kend > base ? (kend - base + CK - 1) / CK : 0, steps = (n + 1) / 2;   // chunks, steps
 
     if (tid == 0) {
-        for (int i = 0; i < PS; ++i) {
-            mbar_init(&ms.packed_full[i], 1);
-            mbar_init(&ms.packed_empty[i], 4);
-        }
+        for (int i = 0; i < L::UNPACK; ++i)
+            for (int j = 0; j < PS; ++j) mbar_init(&ms.packed[i][j], 1);
         for (int i = 0; i < KS; ++i) {
             mbar_init(&ms.kv_full[i], 4);
-            mbar_init(&ms.kv_empty[i], 1);
+            mbar_init(&ms.kv_empty[i], tiles);
         }
-        for (int i = 0; i < 2; ++i) {
-            for (int j = 0; j < 2; ++j) {
-                mbar_init(&ms.s_full[i][j], 1);
-                mbar_init(&ms.p_full[i][j], 4);
-            }
+        for (int i = 0; i < L::NT; ++i) {
+            mbar_init(&ms.s_full[i], 1);
+            mbar_init(&ms.p_full[i], 4);
             mbar_init(&ms.pv_done[i], 1);
+            mbar_init(&ms.drain[i], 1);
         }
-        mbar_init(&ms.drain, 1);
         ms.abort = 0;
         fence_mbar_init();
     }
-    if (warp == 13) {
+    if (warp == L::MMA) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&ms.tmem))
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    // the tiles' queries, a thread a unit: q 2^-eq in fp16, its largest |dim| in [2^3, 2^4)
     float qscale = 0.f;
-    const int u = u0 + tid;   // softmax threads only
-    if (warp < 8) {
-        float x[HD];
+    // the tiles' queries, a thread a unit: q 2^-eq in fp16, its largest |dim| in [2^3, 2^4)
+    if (warp < L::SOFT) {
+        const int u = u0 + tid;
         const bool ok = u < units;
         const int j = ok ? u / a.group : 0, g = ok ? u - j * a.group : 0;
         const __nv_bfloat16* src = a.q + (row0 + j) * a.q_row + (h * a.group + g) * a.q_head;
-        const uint32_t* src2 = reinterpret_cast<const uint32_t*>(src);
         const bool wide = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
-        uint32_t top = 0;
+        auto dims = [&](int i, uint32_t* w) {   // 8 i ..
+            const uint32_t* src2 = reinterpret_cast<const uint32_t*>(src) + 4 * i;
+            if (!ok) {
+                w[0] = w[1] = w[2] = w[3] = 0;
+            } else if (wide) {
+                *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(src2);
+            } else {
 #pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = src2[e];
+            }
+        };
+        uint32_t top = 0, w[4];
+#pragma unroll 4
         for (int i = 0; i < HD / 8; ++i) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (ok) {
-                if (wide) {
-                    v = *reinterpret_cast<const uint4*>(src + 8 * i);
-                } else {
-                    v.x = src2[4 * i];
-                    v.y = src2[4 * i + 1];
-                    v.z = src2[4 * i + 2];
-                    v.w = src2[4 * i + 3];
-                }
-            }
-            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            dims(i, w);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[8 * i + 2 * e] = kv4_s(w[e]);
-                x[8 * i + 2 * e + 1] = kv4_z(w[e]);
-                top = max(top, max(w[e] << 16 & 0x7fffffffu, w[e] & 0x7fff0000u));
-            }
+            for (int e = 0; e < 4; ++e) top = max(top, max(w[e] << 16 & 0x7fffffffu, w[e] & 0x7fff0000u));
         }
         const int eq = min(max((int)(top >> 23) - 127 - 3, -100), 100);
         const float f = exp2i(-eq);
         qscale = a.scale_log2 * exp2i(eq);
         const int row = tid & 127;
         const uint32_t qt = sb + L::Q + (uint32_t)(tid >> 7) * L::QB + (row >> 3) * 1024 + (row & 7) * 128;
-#pragma unroll
+#pragma unroll 4
         for (int i = 0; i < HD / 8; ++i) {
-            const uint32_t at = qt + (i >> 3) * (128 * 128) + (((i & 7) ^ (row & 7)) << 4);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at),
-                         "r"(half2_bits(x[8 * i] * f, x[8 * i + 1] * f)), "r"(half2_bits(x[8 * i + 2] * f, x[8 * i + 3] * f)),
-                         "r"(half2_bits(x[8 * i + 4] * f, x[8 * i + 5] * f)),
-                         "r"(half2_bits(x[8 * i + 6] * f, x[8 * i + 7] * f))
+            dims(i, w);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = half2_bits(kv4_s(w[e]) * f, kv4_z(w[e]) * f);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(qt + (i >> 3) * (128 * 128) +
+                                                                          (((i & 7) ^ (row & 7)) << 4)),
+                         "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
                          : "memory");
         }
         fence_async();
@@ -307,102 +310,103 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a)
     fence_after();
     const uint32_t tmem = ms.tmem;
 
-    if (warp == 12) {
-        // copies: lane i a piece of the step (the part of it in one page, or all of it)
-        const int page_tiles = 1 << (a.page_shift - 4), piece = min(page_tiles, TPS), pieces = TPS / piece;
-        auto page_of = [&](int c) { return lane < pieces && c < steps ? kv4_page(a, b, (step0 + c) * TPS + lane * piece) : -1; };
-        int next = page_of(0);
-        int c = 0;
-        for (; c < steps; ++c) {
-            const int page = next, st = c % PS;
-            next = page_of(c + 1);
-            bool ok = true;
-            if (c >= PS) ok = wait(&ms.packed_empty[st], (c / PS - 1) & 1, abort);
-            if (!__all_sync(0xffffffffu, ok)) break;
-            const uint32_t there = __ballot_sync(0xffffffffu, page >= 0);
-            if (lane == 0) {
-                uint32_t v = 0;
-                for (int i = 0; i < pieces; ++i)
-                    if (there >> i & 1) v |= ((1u << piece) - 1) << (i * piece);
-                ms.valid[st] = v;
-                const uint32_t bytes = __popc(there) * piece * T::BYTES;
-                if (bytes)
-                    mbar_arrive_expect_tx(&ms.packed_full[st], bytes);
-                else
-                    mbar_arrive(&ms.packed_full[st]);
-            }
-            __syncwarp();
-            if (page >= 0)
-                tma_load_1d(sm + L::P + st * L::PB + lane * piece * T::BYTES,
-                            a.pages + ((int64_t)page * a.hkv + h) * a.page_bytes +
-                                (int64_t)(((step0 + c) * TPS + lane * piece) & (page_tiles - 1)) * T::BYTES,
-                            piece * T::BYTES, &ms.packed_full[st]);
-        }
-        // what was issued lands before the CTA ends
-        for (int i = max(0, c - PS); i < c; ++i) mbar_wait(&ms.packed_full[i % PS], (i / PS) & 1);
-    } else if (warp == 13) {
-        if (n > 0) {
+    if (warp >= L::MMA) {
+        const int t = warp - L::MMA;
+        if (n > 0 && t < tiles) {
             const uint32_t one = elect(), tm = __shfl_sync(0xffffffffu, tmem, 0);
-            auto ready = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity, abort)); };
-            auto mma_s = [&](int t, int c) {
+            auto ready = [&](uint64_t* bar, uint32_t parity) {
+                const bool ok = __all_sync(0xffffffffu, wait(bar, parity, abort));
+                fence_after();
+                return ok;
+            };
+            bool ok = true;
+            for (int c = 0; c < n; ++c) {
+                // scores, over the weights of chunk c - 1
+                ok = ready(&ms.kv_full[c % KS], (c / KS) & 1) && (c == 0 || ready(&ms.pv_done[t], (c - 1) & 1));
+                if (!ok) break;
                 const uint32_t kt = desc(sb + L::K + (c % KS) * L::KB), qt = desc(sb + L::Q + t * L::QB);
 #pragma unroll
                 for (int ks = 0; ks < HD / 16; ++ks)
-                    mma_ss(one, tm + L::S_COL + (2 * t + (c & 1)) * CK,
-                           qt + (((ks >> 2) * (128 * 128) + (ks & 3) * 32) >> 4),
+                    mma_ss(one, tm + L::S_COL + t * CK, qt + (((ks >> 2) * (128 * 128) + (ks & 3) * 32) >> 4),
                            kt + (((ks >> 2) * (CK * 128) + (ks & 3) * 32) >> 4), idesc(CK), ks > 0);
-                commit(one, &ms.s_full[t][c & 1]);
-            };
-            bool ok = ready(&ms.kv_full[0], 0);
-            fence_after();
-            if (ok)
-                for (int t = 0; t < tiles; ++t) mma_s(t, 0);
-            for (int c = 0; ok && c < n; ++c) {
-                if (c + 1 < n) {   // the next chunk's scores: over those (and the weights) of chunk c - 1
-                    if (!(ok = ready(&ms.kv_full[(c + 1) % KS], ((c + 1) / KS) & 1))) break;
-                    for (int t = 0; ok && t < tiles; ++t) {
-                        if (c > 0 && !(ok = ready(&ms.pv_done[t], (c - 1) & 1))) break;
-                        fence_after();
-                        mma_s(t, c + 1);
-                    }
-                }
+                commit(one, &ms.s_full[t]);
+                if (!(ok = ready(&ms.p_full[t], c & 1))) break;
                 const uint32_t vt = desc(sb + L::V + (c % KS) * L::KB);
-                for (int t = 0; ok && t < tiles; ++t) {
-                    if (!(ok = ready(&ms.p_full[t][c & 1], (c >> 1) & 1))) break;
-                    fence_after();
 #pragma unroll
-                    for (int ks = 0; ks < CK / 16; ++ks)
-                        mma_ts(one, tm + L::O_COL + t * HD, tm + L::S_COL + (2 * t + (c & 1)) * CK + ks * 8, vt + ks * 2,
-                               idesc(HD), c > 0 || ks > 0);
-                    commit(one, &ms.pv_done[t]);
-                    if (t == tiles - 1) commit(one, &ms.kv_empty[c % KS]);
-                }
+                for (int ks = 0; ks < CK / 16; ++ks)
+                    mma_ts(one, tm + L::O_COL + t * HD, tm + L::S_COL + t * CK + ks * 8, vt + ks * 2, idesc(HD),
+                           c > 0 || ks > 0);
+                commit(one, &ms.pv_done[t]);
+                commit(one, &ms.kv_empty[c % KS]);
             }
-            commit(one, &ms.drain);   // every MMA issued has completed
-            mbar_wait(&ms.drain, 0);
+            commit(one, &ms.drain[t]);   // every MMA issued has completed
+            mbar_wait(&ms.drain[t], 0);
         }
         __syncwarp();
-    } else if (warp >= 8) {
-        // unpacking: warp w takes tile w of each of a step's two chunks
-        const int w = warp - 8, r = lane >> 2, t = lane & 3;
-        bool good = true;   // no wait of this warp has run out; the four warps leave together
-        for (int c = 0; c < steps; ++c) {
-            const int st = c % PS, sg = c & 1, k0 = base + c * SK;
-            if (good) good = __all_sync(0xffffffffu, wait(&ms.packed_full[st], (c / PS) & 1, abort));
-            const unsigned char* pk = sm + L::P + st * L::PB;
-            const uint32_t valid = ms.valid[st];
-            // the largest magnitudes that the chunk's s and z allow, and its NaN groups of V
-            uint32_t topk = 0, topv = 0;
-            bool bad[2][NB], any_bad[2] = {false, false};
+    } else if (warp >= L::SOFT) {
+        // unpacking: warp w of four takes tile w of each chunk; with eight, warp 4 y + w of chunk y of the steps
+        constexpr int YT = L::YT;
+        const int uw = warp - L::SOFT, y0 = uw >> 2, w = uw & 3, r = lane >> 2, t = lane & 3;
+        unsigned char* ring = sm + L::P + uw * L::PB;
+        uint64_t* packed = ms.packed[uw];
+        // pages of the warp's tiles, those of 32 steps at a time (lane i: step i)
+        auto pages_of = [&](int c0, int* pg) {
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                const int tl = w + 4 * y;
-                const uint32_t* kp = reinterpret_cast<const uint32_t*>(pk + tl * T::BYTES + T::KP);
-                const uint32_t* vp = reinterpret_cast<const uint32_t*>(pk + tl * T::BYTES + T::VP);
+            for (int y = 0; y < YT; ++y) pg[y] = c0 + lane < steps ? kv4_page(a, b, (step0 + c0 + lane) * 8 + 4 * (y0 + y) + w) : -1;
+        };
+        int pg[YT], nextpg[YT];
+        auto issue = [&](int c, const int* page) {   // lane 0
+            uint64_t* bar = &packed[c % PS];
+            uint32_t bytes = 0;
+#pragma unroll
+            for (int y = 0; y < YT; ++y) bytes += page[y] >= 0 ? L::TB : 0;
+            if (bytes == 0) {
+                mbar_arrive(bar);
+                return;
+            }
+            mbar_arrive_expect_tx(bar, bytes);
+#pragma unroll
+            for (int y = 0; y < YT; ++y)
+                if (page[y] >= 0)
+                    tma_load_1d(ring + ((c % PS) * YT + y) * L::TB,
+                                a.pages + ((int64_t)page[y] * a.hkv + h) * a.page_bytes +
+                                    (int64_t)(((step0 + c) * 8 + 4 * (y0 + y) + w) & ((1 << (a.page_shift - 4)) - 1)) * L::TB,
+                                L::TB, bar);
+        };
+        pages_of(0, pg);
+#pragma unroll
+        for (int y = 0; y < YT; ++y) nextpg[y] = pg[y];
+        for (int c = 0; c < min(PS, steps); ++c) {
+            int page[YT];
+#pragma unroll
+            for (int y = 0; y < YT; ++y) page[y] = __shfl_sync(0xffffffffu, pg[y], c);
+            if (lane == 0) issue(c, page);
+        }
+        bool good = true;   // no wait of this warp has run out; the warps leave together
+        int c = 0;
+        for (; c < steps; ++c) {
+            const int st = c % PS, sg = c & 1, k0 = base + c * SK;
+            if (c > 0 && (c & 31) == 0)
+#pragma unroll
+                for (int y = 0; y < YT; ++y) pg[y] = nextpg[y];
+            bool there[YT];
+#pragma unroll
+            for (int y = 0; y < YT; ++y) there[y] = __shfl_sync(0xffffffffu, pg[y], c & 31) >= 0;
+            if (good) good = __all_sync(0xffffffffu, wait(&packed[st], (c / PS) & 1, abort));
+            const unsigned char* pk = ring + st * YT * L::TB;
+            // the largest magnitudes that the step's s and z allow, and the tiles' NaN groups of V
+            uint32_t topk = 0, topv = 0;
+            bool bad[YT][NB], any_bad[YT];
+#pragma unroll
+            for (int y = 0; y < YT; ++y) {
+                const uint32_t* kp = reinterpret_cast<const uint32_t*>(pk + y * L::TB + T::KP);
+                const uint32_t* vp = reinterpret_cast<const uint32_t*>(pk + y * L::TB + T::VP);
+                any_bad[y] = false;
 #pragma unroll
                 for (int x = 0; x < NB; ++x) {
-                    const int at = x * 32 + lane, slot = at / NG, key = k0 + 16 * tl + (slot >> 1) + 8 * (slot & 1);
-                    const bool in = (valid >> tl & 1) && key >= kmin && key < kmax;
+                    const int at = x * 32 + lane, slot = at / NG;
+                    const int key = k0 + 16 * (4 * (y0 + y) + w) + (slot >> 1) + 8 * (slot & 1);
+                    const bool in = there[y] && key >= kmin && key < kmax;
                     const uint32_t kw = kp[at], vw = vp[at];
                     const float ka = fmaxf(fabsf(kv4_z(kw)), fabsf(fmaf(15.f, kv4_s(kw), kv4_z(kw))));
                     const float va = fmaxf(fabsf(kv4_z(vw)), fabsf(fmaf(15.f, kv4_s(vw), kv4_z(vw))));
@@ -416,29 +420,23 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a)
             topk = __reduce_max_sync(0xffffffffu, topk);
             topv = __reduce_max_sync(0xffffffffu, topv);
             if (lane == 0) {
-                ms.top[sg][w][0] = topk;
-                ms.top[sg][w][1] = topv;
-                ms.stop[sg][w] = !good;
+                ms.top[sg][uw][0] = topk;
+                ms.top[sg][uw][1] = topv;
+                ms.stop[sg][uw] = !good;
             }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            bool stop = false;
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-                topk = max(topk, ms.top[sg][y][0]);
-                topv = max(topv, ms.top[sg][y][1]);
-                stop |= ms.stop[sg][y] != 0;
-            }
-            if (stop) break;
+            asm volatile("bar.sync 1, %0;" ::"n"(L::UNPACK * 32) : "memory");
+            topk = __reduce_max_sync(0xffffffffu, ms.top[sg][lane % L::UNPACK][0]);
+            topv = __reduce_max_sync(0xffffffffu, ms.top[sg][lane % L::UNPACK][1]);
+            if (__any_sync(0xffffffffu, ms.stop[sg][lane % L::UNPACK] != 0)) break;
             const int ek = exponent_out(topk), ev = exponent_out(topv);
             const float fk = exp2i(-ek), fv = exp2i(-ev);
 #pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                const int ch = 2 * c + y, sk = ch % KS;
-                if (ch >= n) break;
-                if (ch >= KS) {   // the stage's readers: both tiles' MMAs and softmax of chunk ch - KS
-                    if (good) good = __all_sync(0xffffffffu, wait(&ms.kv_empty[sk], (ch / KS - 1) & 1, abort));
-                    if (!good) break;
-                }
+            for (int y = 0; y < YT; ++y) {
+                const int ch = 2 * c + y0 + y, sk = ch % KS, tl = 4 * (y0 + y) + w;
+                // the stage's readers: every tile's MMAs and softmax of chunk ch - KS
+                if (good && ch < n && ch >= KS)
+                    good = __all_sync(0xffffffffu, wait(&ms.kv_empty[sk], (ch / KS - 1) & 1, abort));
+                if (!good || ch >= n) continue;
                 if (any_bad[y]) {   // rare: which groups of which keys
 #pragma unroll
                     for (int x = 0; x < NB; ++x) {
@@ -450,9 +448,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a)
                     }
                 }
                 const uint32_t kt = sb + L::K + sk * L::KB, vt = sb + L::V + sk * L::KB;
-                const int tl = w + 4 * y;
-                const unsigned char* tp = pk + tl * T::BYTES;
-                const bool there = valid >> tl & 1;
+                const unsigned char* tp = pk + y * L::TB;
                 uint32_t code[NB][4], par[2 * NG];
 #pragma unroll
                 for (int x = 0; x < NB; ++x)
@@ -463,7 +459,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a)
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
                     const int key = k0 + 16 * tl + r + 8 * hf;
-                    const bool in = there && key >= kmin && key < kmax;
+                    const bool in = there[y] && key >= kmin && key < kmax;
                     const uint32_t row = kt + (2 * w + hf) * 1024 + r * 128 + 4 * t;
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
@@ -485,7 +481,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a)
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
                     const int key = k0 + 16 * tl + 2 * t + 8 * hf;
-                    const bool in0 = there && key >= kmin && key < kmax, in1 = there && key + 1 >= kmin && key + 1 < kmax;
+                    const bool in0 = there[y] && key >= kmin && key < kmax, in1 = there[y] && key + 1 >= kmin && key + 1 < kmax;
                     const uint32_t blk = vt + r * 128 + (((2 * w + hf) ^ r) << 4) + 4 * t;
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
@@ -510,77 +506,96 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a)
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ms.kv_full[sk]);
             }
-            if (lane == 0) mbar_arrive(&ms.packed_empty[st]);
+            __syncwarp();   // every lane has read the stage
+            const int nx = c + PS;
+            if (nx < steps) {
+                if ((nx & 31) == 0) pages_of(nx, nextpg);
+                int page[YT];
+#pragma unroll
+                for (int y = 0; y < YT; ++y)
+                    page[y] = __shfl_sync(0xffffffffu, (nx >> 5) == (c >> 5) ? pg[y] : nextpg[y], nx & 31);
+                if (lane == 0) issue(nx, page);
+            }
         }
+        // what was issued lands before the CTA ends
+        for (int i = c; i < min(steps, c + PS); ++i) mbar_wait(&packed[i % PS], (i / PS) & 1);
     } else {
-        // softmax: this thread's unit u, tile warp / 4, TMEM lane (warp % 4) 32 + lane
-        const int tile = warp >> 2;
+        // softmax: unit u, TMEM lane (warp % 4) 32 + lane of tile warp / 4
+        const int tile = warp >> 2, u = u0 + tid;
         const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t o_at = tmem + lanes + L::O_COL + tile * HD;
+        const uint32_t s_at = tmem + lanes + L::S_COL + tile * CK, o_at = tmem + lanes + L::O_COL + tile * HD;
         const int pos = len - nq + min(u, units - 1) / a.group;
         const int lo = low(pos), hi = pos + 1;
         // keys that every unit of the warp sees
-        const int uw = u - lane, ua = min(uw, units - 1), ub = min(uw + 31, units - 1);
+        const int ua = min(u - lane, units - 1), ub = min(u - lane + 31, units - 1);
         const int all_lo = low(len - nq + ub / a.group), all_hi = len - nq + ua / a.group + 1;
         float m = KV4_NEG, l = 0.f;
         uint32_t bad = 0;
         bool ok = tile < tiles;
         for (int c = 0; ok && c < n; ++c) {
             const int sk = c % KS, k0 = base + c * CK;
-            const uint32_t s_at = tmem + lanes + L::S_COL + (2 * tile + (c & 1)) * CK;
-            ok = wait(&ms.s_full[tile][c & 1], (c >> 1) & 1, abort) && wait(&ms.kv_full[sk], (c / KS) & 1, abort);
+            ok = wait(&ms.s_full[tile], c & 1, abort) && wait(&ms.kv_full[sk], (c / KS) & 1, abort);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             fence_after();
             const float kq = ms.kscale[sk] * qscale, ev = ms.ev[sk];
             const bool edge = k0 < all_lo || k0 + CK > all_hi;
             const int lo_c = lo - k0, hi_c = hi - k0;
-            uint32_t v[CK], p[CK / 2];
-            ld32(s_at, v);
-            ld32(s_at + 32, v + 32);
-            ld_wait(v);
-            ld_wait(v + 32);
-            if (edge) {   // scores of keys that the unit does not see
+            // scores of keys 32 q .. of the chunk; those that the unit does not see: -inf
+            auto scores = [&](int q, uint32_t* v) {
+                ld32(s_at + 32 * q, v);
+                ld_wait(v);
+                if (edge) {
 #pragma unroll
-                for (int k = 0; k < CK; ++k)
-                    if (k < lo_c || k >= hi_c) v[k] = 0xff800000u;
-            }
+                    for (int k = 0; k < 32; ++k)
+                        if (32 * q + k < lo_c || 32 * q + k >= hi_c) v[k] = 0xff800000u;
+                }
+            };
             // weights with the reference m; their sum
+            uint32_t p[CK / 2];
             auto weigh = [&]() {
                 const f32x2 f2 = two(kq, kq), b2 = two(ev - m, ev - m);
                 f32x2 sum = two(0.f, 0.f);
 #pragma unroll
-                for (int i = 0; i < CK / 2; ++i) {
-                    float x, y;
-                    parts(fma2(two(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), f2, b2), x, y);
-                    x = kv4_ex2(x);
-                    y = kv4_ex2(y);
-                    sum = add2(sum, two(x, y));
-                    p[i] = half2_bits(x, y);
+                for (int q = 0; q < CK / 32; ++q) {
+                    uint32_t v[32];
+                    scores(q, v);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        float x, y;
+                        parts(fma2(two(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), f2, b2), x, y);
+                        x = kv4_ex2(x);
+                        y = kv4_ex2(y);
+                        sum = add2(sum, two(x, y));
+                        p[16 * q + i] = half2_bits(x, y);
+                    }
                 }
                 float x, y;
                 parts(sum, x, y);
                 return x + y;
             };
-            auto raise = [&]() {   // m to the largest score so far, the row of O with it
+            // m to the largest score so far, the row of O with it (the scores say that P V of the chunk
+            // before has completed)
+            auto raise = [&]() {
                 float top = m;
 #pragma unroll
-                for (int k = 0; k < CK; ++k) top = fmaxf(top, fmaf(__uint_as_float(v[k]), kq, ev));
+                for (int q = 0; q < CK / 32; ++q) {
+                    uint32_t v[32];
+                    scores(q, v);
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) top = fmaxf(top, fmaf(__uint_as_float(v[k]), kq, ev));
+                }
                 const float f = kv4_ex2(m - top);
                 m = top;
                 l *= f;
                 if (c > 0) {
-                    if (!__all_sync(0xffffffffu, wait(&ms.pv_done[tile], (c - 1) & 1, abort))) return;   // aborted
-                    fence_after();
 #pragma unroll
-                    for (int q = 0; q < HD / 32; ++q) {
-                        uint32_t o[32];
-                        ld32(o_at + 32 * q, o);
-                        ld_wait(o);
+                    for (int q = 0; q < HD / 16; ++q) {
+                        uint32_t o[16];
+                        ld16(o_at + 16 * q, o);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                        st16(o_at + 32 * q, o);
-                        st16(o_at + 32 * q + 16, o + 16);
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        st16(o_at + 16 * q, o);
                     }
                 }
             };
@@ -600,40 +615,36 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a)
             st_wait();
             fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&ms.p_full[tile][c & 1]);
+            if (lane == 0) mbar_arrive(&ms.p_full[tile]);
         }
         if (tile < tiles) {
-            if (ok && n > 0) {
-                ok = __all_sync(0xffffffffu, wait(&ms.pv_done[tile], (n - 1) & 1, abort) && !*abort);
-                fence_after();
-            }
+            if (ok && n > 0) ok = wait(&ms.pv_done[tile], (n - 1) & 1, abort) && !*abort;
+            ok = __all_sync(0xffffffffu, ok);
+            fence_after();
+            if (!ok) bad = 0xffu;
             const bool row_ok = u < units;
             const int j = row_ok ? u / a.group : 0, g = row_ok ? u - j * a.group : 0;
             const int64_t at = (int64_t)(row0 + j) * a.hq + h * a.group + g;
             const float inv = a.nsplit > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-            if (!ok) bad = 0xffu;
 #pragma unroll
-            for (int q = 0; q < NG; ++q) {
-                uint32_t v[32];
+            for (int q = 0; q < HD / 16; ++q) {
+                uint32_t v[16];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) v[i] = 0;
-                if (ok && n > 0) {
-                    ld32(o_at + 32 * q, v);
-                    ld_wait(v);
-                }
-                float x[32];
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                    x[i] = bad >> q & 1 ? __int_as_float(0x7fffffff) : __uint_as_float(v[i]) * inv;
+                for (int i = 0; i < 16; ++i) v[i] = 0;
+                if (ok && n > 0) ld16(o_at + 16 * q, v);
                 if (!row_ok) continue;
+                float x[16];
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    x[i] = bad >> (q / 2) & 1 ? __int_as_float(0x7fffffff) : __uint_as_float(v[i]) * inv;
                 if (a.nsplit > 1) {
-                    float4* o = reinterpret_cast<float4*>(a.part_o + (at * a.nsplit + split) * HD + 32 * q);
+                    float4* o = reinterpret_cast<float4*>(a.part_o + (at * a.nsplit + split) * HD + 16 * q);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) o[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+                    for (int i = 0; i < 4; ++i) o[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
                 } else {
-                    uint4* o = reinterpret_cast<uint4*>(a.out + at * HD + 32 * q);
+                    uint4* o = reinterpret_cast<uint4*>(a.out + at * HD + 16 * q);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < 2; ++i) {
                         __nv_bfloat162 y[4];
 #pragma unroll
                         for (int e = 0; e < 4; ++e) y[e] = __floats2bfloat162_rn(x[8 * i + 2 * e], x[8 * i + 2 * e + 1]);
@@ -649,7 +660,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a)
     }
     fence_before();
     __syncthreads();
-    if (warp == 13)
+    if (warp == L::MMA)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
 }
 
@@ -662,11 +673,11 @@ int kv4_prefill_launch(const Kv4AttnArgs& a, int head_dim, int64_t sequences, in
     if (head_dim == 64) {
         constexpr int bytes = Lay<64>::BYTES + 1024;
         PULSAR_TRY(ensure_smem_attr((const void*)k_kv4_prefill<64>, bytes, "k_kv4_prefill shared memory"));
-        k_kv4_prefill<64><<<grid, THREADS, bytes, stream>>>(a);
+        k_kv4_prefill<64><<<grid, Lay<64>::THREADS, bytes, stream>>>(a);
     } else {
         constexpr int bytes = Lay<128>::BYTES + 1024;
         PULSAR_TRY(ensure_smem_attr((const void*)k_kv4_prefill<128>, bytes, "k_kv4_prefill shared memory"));
-        k_kv4_prefill<128><<<grid, THREADS, bytes, stream>>>(a);
+        k_kv4_prefill<128><<<grid, Lay<128>::THREADS, bytes, stream>>>(a);
     }
     PULSAR_LAUNCH_CHECK("k_kv4_prefill");
     return PULSAR_OK;
