@@ -500,7 +500,8 @@ struct Plan {
 // How a call is cut. More than MANY units of a sequence's rows go to k_kv4_prefill, 512 or 256 a CTA.
 // Others: the fewest columns that hold max_q rows of a group (four: both halves of the weights in
 // one operand), at most 32 (heads of 128: 16, for the registers). Splits of the keys: until about
-// four CTAs an SM are there (k_kv4_prefill: one), of at least 8 pairs of tiles (two a warp; two steps).
+// four CTAs an SM are there, of at least 8 pairs of tiles (two a warp); k_kv4_prefill: the number
+// that fills the last wave best, of at least two steps.
 constexpr int64_t MANY = 32;
 Plan make_plan(int64_t B, int64_t Hkv, int64_t group, int64_t head_dim, int64_t max_q, int64_t max_kv,
                int64_t window) {
@@ -520,9 +521,22 @@ Plan make_plan(int64_t B, int64_t Hkv, int64_t group, int64_t head_dim, int64_t 
     }
     const int64_t steps = (span + step - 1) / step;
     const int64_t ctas = B * Hkv * p.utiles;
-    int64_t ns = p.many ? full / ctas : (full + ctas - 1) / ctas;
-    if (ns > steps / least) ns = steps / least;
-    if (ns > 64) ns = 64;
+    int64_t ns = (full + ctas - 1) / ctas, most = steps / least < 64 ? steps / least : 64;
+    if (p.many) {
+        // in units of a step (about 1.8 us): waves of CTAs, each with the start and end of one, then the
+        // partials' way through memory and the merge
+        double best = 1e30;
+        for (int64_t s = 1, pick = 1; s <= most || s == 1; ns = pick, ++s) {
+            const double waves = (double)((ctas * s + full - 1) / full), len = (double)((steps + s - 1) / s);
+            const double merge = s > 1 ? 2 + (double)(B * Hkv * units) * s * (head_dim + 2) * 8 / 7.2e6 : 0;
+            if (waves * (len + 2) + merge < best) {
+                best = waves * (len + 2) + merge;
+                pick = s;
+            }
+        }
+    } else if (ns > most) {
+        ns = most;
+    }
     if (ns < 1) ns = 1;
     p.split_len = (int)((steps + ns - 1) / ns);
     if (p.split_len < 1) p.split_len = 1;
