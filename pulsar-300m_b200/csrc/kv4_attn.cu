@@ -38,7 +38,6 @@ using namespace pulsar;
 
 namespace {
 
-constexpr int WARPS = 4;
 constexpr int LAZY = 30;
 constexpr float NEG = KV4_NEG;
 
@@ -84,14 +83,16 @@ __device__ __forceinline__ uint32_t pack(float a, float b) {
 __device__ __forceinline__ float lo_of(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float hi_of(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
-// A stage holds two tiles (32 tokens); bytes in flight per warp: 10 KB.
+// A stage holds two tiles (32 tokens): 10 KB in flight a warp.
 template <int HD>
-constexpr int stages() { return HD == 64 ? 4 : 3; }
-template <int HD>
-constexpr int ring_bytes() { return WARPS * stages<HD>() * 2 * Kv4Tile<HD>::BYTES; }
+constexpr int stages() { return HD == 64 ? 4 : 2; }
 
-template <int HD, int NT, bool DUP>
-__global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const Kv4AttnArgs a) {
+// CTAs that an SM should hold: 16 warps where the registers allow it.
+template <int HD, int NT, int WARPS>
+constexpr int resident() { return NT == 1 ? 16 / WARPS : 1; }
+
+template <int HD, int NT, bool DUP, int WARPS>
+__global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_attn(const Kv4AttnArgs a) {
     using T = Kv4Tile<HD>;
     constexpr int NG = T::NG, NB = HD / 64, S = stages<HD>(), MT = HD / 16, TB = T::BYTES;
     constexpr int UT = DUP ? 4 : 8 * NT;
@@ -101,19 +102,14 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const Kv4AttnArgs a) {
     const int split = blockIdx.x % a.nsplit, u0 = blockIdx.x / a.nsplit * UT;
     const int h = blockIdx.y, b = blockIdx.z;
 
-    int row0, nq;
-    kv4_rows(a, b, row0, nq);
-    const int units = nq * a.group;
-    if (u0 >= units) return;
-    const int len = min(max(a.kv_lens[b], 0), a.width << a.page_shift);
-    const int ulast = min(u0 + UT, units) - 1;
-    const int first = len - nq + u0 / a.group, last = len - nq + ulast / a.group;   // their positions
-    auto low = [&](int pos) { return a.window > 0 ? max(0, pos - a.window + 1) : 0; };
-    const int kmin = low(first), kmax = last + 1;   // keys that some unit sees: [kmin, kmax)
-    // pairs of tiles (32 tokens, aligned): the split's range, of which the warp takes every fourth
-    const int pair0 = kmin / 32, npairs = kmax > 0 ? (kmax + 31) / 32 : 0;
-    const int p_begin = pair0 + split * a.split_len + warp;
-    const int p_end = split == a.nsplit - 1 ? npairs : min(npairs, pair0 + (split + 1) * a.split_len);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the merge may be set up meanwhile
+    Kv4Range rg;
+    if (!kv4_range(a, b, u0, UT, 32, rg) || split >= rg.used) return;
+    const int row0 = rg.row0, units = rg.units, ulast = rg.ulast;
+    // steps are pairs of tiles (32 tokens, aligned): the split's range, of which the warp takes every WARPS-th
+    int s_begin, s_end;
+    kv4_split(a, rg, split, s_begin, s_end);
+    const int p_begin = rg.step0 + s_begin + warp, p_end = rg.step0 + s_end;
     const int mine = p_end > p_begin ? (p_end - p_begin + WARPS - 1) / WARPS : 0;
 
     if (lane == 0) {
@@ -172,7 +168,7 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const Kv4AttnArgs a) {
     for (int nt = 0; nt < NT; ++nt) {
         const int u = u0 + (DUP ? (r & 3) : nt * 8 + r);
         const bool ok = u < units;
-        const int j = ok ? u / a.group : 0, g = ok ? u - j * a.group : 0;
+        const int j = ok ? kv4_row(a, u) : 0, g = ok ? u - j * a.group : 0;
         const __nv_bfloat16* src = a.q + (row0 + j) * a.q_row + (h * a.group + g) * a.q_head;
 #pragma unroll
         for (int i = 0; i < 2 * MT; ++i) qf[nt][i] = ok ? *reinterpret_cast<const uint32_t*>(src + 8 * i + 2 * t) : 0u;
@@ -199,11 +195,11 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const Kv4AttnArgs a) {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
             const int u = min(u0 + (DUP ? ((2 * t + c) & 3) : nt * 8 + 2 * t + c), units - 1);
-            const int pos = len - nq + u / a.group;
+            const int pos = rg.len - rg.nq + kv4_row(a, u);
             hi[nt][c] = pos + 1;
-            lo[nt][c] = low(pos);
+            lo[nt][c] = kv4_low(a, pos);
         }
-    const int all_lo = low(last), all_hi = first + 1;   // keys in [all_lo, all_hi) are seen by every unit
+    const int all_lo = kv4_low(a, rg.last), all_hi = rg.first + 1;   // keys in [all_lo, all_hi) are seen by every unit
 
     // Scores come in units of 2^(LIFT - CODE_EXP); m: their running maximum, nm = LIFT - scale m, so
     // that weights are 2^LIFT exp2(scale (s - m))
@@ -458,9 +454,9 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const Kv4AttnArgs a) {
             ll = fmaf(f, p[HD + 1], ll);
             oo = fmaf(f, p[d], oo);
         }
-        const int j = (u0 + u) / a.group, g = (u0 + u) - j * a.group;
+        const int j = kv4_row(a, u0 + u), g = (u0 + u) - j * a.group;
         const int64_t at = (int64_t)(row0 + j) * a.hq + h * a.group + g;
-        if (a.nsplit == 1) {
+        if (rg.used == 1) {
             a.out[at * HD + d] = __float2bfloat16(ll == 0.f ? 0.f : oo / ll);
         } else {
             a.part_o[(at * a.nsplit + split) * HD + d] = oo;
@@ -472,36 +468,82 @@ __global__ void __launch_bounds__(WARPS * 32) k_kv4_attn(const Kv4AttnArgs a) {
     }
 }
 
-// out of one (sequence row, head) from its splits' partials, in split order: a block of HD threads.
+// out of one (sequence row, head) from its splits' partials (where there is more than one): 128
+// threads, HD / 4 to a partial, which go through every 512 / HD-th split; these are joined in shared
+// memory. Both orders are fixed.
 template <int HD>
-__global__ void __launch_bounds__(HD) k_kv4_merge(const Kv4AttnArgs a) {
-    const int j = blockIdx.x / a.hq, b = blockIdx.y;
-    int row0, nq;
-    kv4_rows(a, b, row0, nq);
-    if (j >= nq) return;
-    const int64_t at = (int64_t)(row0 + j) * a.hq + blockIdx.x % a.hq;
-    const float* ml = a.part_ml + at * a.nsplit * 2;
-    float mm = NEG;
-    for (int s = 0; s < a.nsplit; ++s) mm = fmaxf(mm, ml[2 * s]);
-    float ll = 0.f, oo = 0.f;
-    for (int s = 0; s < a.nsplit; ++s) {
-        const float f = kv4_ex2(ml[2 * s] - mm);
-        ll = fmaf(f, ml[2 * s + 1], ll);
-        oo = fmaf(f, a.part_o[(at * a.nsplit + s) * HD + threadIdx.x], oo);
+__global__ void __launch_bounds__(128) k_kv4_merge(const Kv4AttnArgs a) {
+    constexpr int LN = HD / 4, NG = 128 / LN;
+    __shared__ float4 os[NG][LN];
+    __shared__ float2 mls[NG];
+    const int j = blockIdx.x / a.hq, head = blockIdx.x % a.hq, b = blockIdx.y;
+    const int u = j * a.group + head % a.group, g = threadIdx.x / LN, d = threadIdx.x % LN;
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // the attention kernel's partials are there
+    Kv4Range rg;
+    if (!kv4_range(a, b, u - u % a.unit_tile, a.unit_tile, a.step, rg) || u >= rg.units || rg.used == 1) return;
+    const int64_t at = (int64_t)(rg.row0 + j) * a.hq + head;
+    const float2* ml = reinterpret_cast<const float2*>(a.part_ml) + at * a.nsplit;
+    const float4* po = reinterpret_cast<const float4*>(a.part_o) + at * a.nsplit * LN + d;
+    float m = NEG, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = g; s0 < rg.used; s0 += 4 * NG) {
+        float2 x[4];
+        float4 y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int s = s0 + i * NG;
+            x[i] = s < rg.used ? ml[s] : make_float2(NEG, 0.f);
+            y[i] = s < rg.used ? po[(int64_t)s * LN] : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        const float top = fmaxf(fmaxf(fmaxf(x[0].x, x[1].x), fmaxf(x[2].x, x[3].x)), m);
+        float f = kv4_ex2(m - top);
+        m = top;
+        l *= f;
+        o = make_float4(o.x * f, o.y * f, o.z * f, o.w * f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            f = kv4_ex2(x[i].x - top);
+            l = fmaf(f, x[i].y, l);
+            o = make_float4(fmaf(f, y[i].x, o.x), fmaf(f, y[i].y, o.y), fmaf(f, y[i].z, o.z), fmaf(f, y[i].w, o.w));
+        }
     }
-    a.out[at * HD + threadIdx.x] = __float2bfloat16(ll == 0.f ? 0.f : oo / ll);
+    os[g][d] = o;
+    if (d == 0) mls[g] = make_float2(m, l);
+    __syncthreads();
+    if (g > 0) return;
+    float top = NEG;
+#pragma unroll
+    for (int i = 0; i < NG; ++i) top = fmaxf(top, mls[i].x);
+    l = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+        const float f = kv4_ex2(mls[i].x - top);
+        const float4 y = os[i][d];
+        l = fmaf(f, mls[i].y, l);
+        o = make_float4(fmaf(f, y.x, o.x), fmaf(f, y.y, o.y), fmaf(f, y.z, o.z), fmaf(f, y.w, o.w));
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const __nv_bfloat162 lo2 = __floats2bfloat162_rn(o.x * inv, o.y * inv), hi2 = __floats2bfloat162_rn(o.z * inv, o.w * inv);
+    uint2 v;
+    v.x = *reinterpret_cast<const uint32_t*>(&lo2);
+    v.y = *reinterpret_cast<const uint32_t*>(&hi2);
+    *reinterpret_cast<uint2*>(a.out + at * HD + 4 * d) = v;
 }
 
 struct Plan {
     bool many;   // k_kv4_prefill
-    int nt, dup, utiles, nsplit, split_len;
+    int nt, dup, warps, unit_tile, utiles, step, nsplit, split_len;
 };
 
 // How a call is cut. More than MANY units of a sequence's rows go to k_kv4_prefill, 512 or 256 a CTA.
 // Others: the fewest columns that hold max_q rows of a group (four: both halves of the weights in
-// one operand), at most 32 (heads of 128: 16, for the registers). Splits of the keys: until about
-// four CTAs an SM are there, of at least 8 pairs of tiles (two a warp); k_kv4_prefill: the number
-// that fills the last wave best, of at least two steps.
+// one operand), at most 32 (heads of 128: 16, for the registers).
+// Splits of the keys: until four CTAs an SM are there, of at least 8 pairs of tiles (two a warp); where
+// there are many keys, of 32 to 64 pairs, so that sequences shorter than max_kv even out (the splits
+// that they lack end at once). k_kv4_prefill: the number that fills the last wave best.
+// Two warps instead of four where there is a CTA for every unit tile and each has few keys: what a CTA
+// costs besides its keys is paid per warp.
 constexpr int64_t MANY = 32;
 Plan make_plan(int64_t B, int64_t Hkv, int64_t group, int64_t head_dim, int64_t max_q, int64_t max_kv,
                int64_t window) {
@@ -511,7 +553,9 @@ Plan make_plan(int64_t B, int64_t Hkv, int64_t group, int64_t head_dim, int64_t 
     p.dup = units <= 4;
     p.nt = (int)(units > 8 * cap ? cap : (units + 7) / 8);
     const int64_t ut = p.many ? kv4_pf_units((int)head_dim) : p.dup ? 4 : 8 * p.nt;
-    const int64_t step = p.many ? KV4_PF_STEP : 32, least = p.many ? 2 : 8, full = p.many ? 148 : 148 * 4;
+    const int64_t step = p.many ? KV4_PF_STEP : 32;
+    p.unit_tile = (int)ut;
+    p.step = (int)step;
     p.utiles = (int)((units + ut - 1) / ut);
     int64_t span = max_kv;
     if (window > 0) {
@@ -521,23 +565,29 @@ Plan make_plan(int64_t B, int64_t Hkv, int64_t group, int64_t head_dim, int64_t 
     }
     const int64_t steps = (span + step - 1) / step;
     const int64_t ctas = B * Hkv * p.utiles;
-    int64_t ns = (full + ctas - 1) / ctas, most = steps / least < 64 ? steps / least : 64;
+    int64_t ns = 1;
     if (p.many) {
         // in units of a step (about 1.8 us): waves of CTAs, each with the start and end of one, then the
         // partials' way through memory and the merge
+        const int64_t most = steps / 2 < 64 ? steps / 2 : 64;
         double best = 1e30;
-        for (int64_t s = 1, pick = 1; s <= most || s == 1; ns = pick, ++s) {
-            const double waves = (double)((ctas * s + full - 1) / full), len = (double)((steps + s - 1) / s);
+        for (int64_t s = 1; s <= most || s == 1; ++s) {
+            const double waves = (double)((ctas * s + 147) / 148), len = (double)((steps + s - 1) / s);
             const double merge = s > 1 ? 2 + (double)(B * Hkv * units) * s * (head_dim + 2) * 8 / 7.2e6 : 0;
             if (waves * (len + 2) + merge < best) {
                 best = waves * (len + 2) + merge;
-                pick = s;
+                ns = s;
             }
         }
-    } else if (ns > most) {
-        ns = most;
+    } else {
+        const int64_t fill = 148 * 4;
+        ns = (fill + ctas - 1) / ctas;
+        if (ns > steps / 8) ns = steps / 8;
+        if (ctas * ((steps + 63) / 64) > fill && ns < (steps + 63) / 64) ns = (steps + 31) / 32;
+        if (ns > 128) ns = 128;
+        if (ns < 1) ns = 1;
     }
-    if (ns < 1) ns = 1;
+    p.warps = !p.many && p.nt == 1 && ns == 1 && ctas > 148 * 4 && steps <= 64 ? 2 : 4;
     p.split_len = (int)((steps + ns - 1) / ns);
     if (p.split_len < 1) p.split_len = 1;
     p.nsplit = (int)((steps + p.split_len - 1) / p.split_len);
@@ -545,15 +595,30 @@ Plan make_plan(int64_t B, int64_t Hkv, int64_t group, int64_t head_dim, int64_t 
     return p;
 }
 
-template <int HD, int NT, bool DUP>
+template <int HD, int NT, bool DUP, int WARPS>
 int launch(const Kv4AttnArgs& a, const Plan& p, int64_t B, cudaStream_t st) {
-    constexpr int merge = WARPS * (DUP ? 4 : 8 * NT) * (HD + 2) * 4;
-    constexpr int bytes = ring_bytes<HD>() > merge ? ring_bytes<HD>() : merge;
-    PULSAR_TRY(ensure_smem_attr((const void*)k_kv4_attn<HD, NT, DUP>, bytes, "k_kv4_attn shared memory"));
+    constexpr int ring = WARPS * stages<HD>() * 2 * Kv4Tile<HD>::BYTES, merge = WARPS * (DUP ? 4 : 8 * NT) * (HD + 2) * 4;
+    constexpr int bytes = ring > merge ? ring : merge;
+    PULSAR_TRY(ensure_smem_attr((const void*)k_kv4_attn<HD, NT, DUP, WARPS>, bytes, "k_kv4_attn shared memory"));
     const dim3 grid((unsigned)(p.utiles * p.nsplit), (unsigned)a.hkv, (unsigned)B);
-    k_kv4_attn<HD, NT, DUP><<<grid, WARPS * 32, bytes, st>>>(a);
+    k_kv4_attn<HD, NT, DUP, WARPS><<<grid, WARPS * 32, bytes, st>>>(a);
     PULSAR_LAUNCH_CHECK("k_kv4_attn");
     return PULSAR_OK;
+}
+
+// The merge is launched under the attention kernel's end; it waits for that before it reads.
+template <int HD>
+int launch_merge(const Kv4AttnArgs& a, int64_t B, cudaStream_t st) {
+    cudaLaunchAttribute early{};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)((int64_t)a.max_q * a.hq), (unsigned)B);
+    cfg.blockDim = dim3(128);
+    cfg.stream = st;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    return cuda_status(cudaLaunchKernelEx(&cfg, k_kv4_merge<HD>, a), "k_kv4_merge");
 }
 
 int check_shape(int64_t N, int64_t Hq, int64_t Hkv, int64_t head_dim, int64_t B, int64_t max_q, int64_t max_kv,
@@ -610,26 +675,23 @@ extern "C" int pulsar_op_kv4_attention(const void* q, int64_t q_row_stride, int6
                p.nsplit > 1 ? ws + N * Hq * p.nsplit * head_dim : nullptr, q_row_stride, q_head_stride,
                page_size / KV4_TILE * 20 * head_dim, (int)N, (int)Hq, (int)Hkv, (int)(Hq / Hkv), (int)num_pages,
                (int)width, __builtin_ctzll((unsigned long long)page_size), (int)max_q, (int)window, p.nsplit,
-               p.split_len, scale * 1.4426950408889634f};
+               p.split_len, p.unit_tile, p.step, scale * 1.4426950408889634f};
     cudaStream_t st = (cudaStream_t)stream;
     int rc;
     if (p.many)
         rc = kv4_prefill_launch(a, (int)head_dim, B, p.utiles, st);
+    else if (head_dim == 64 && p.warps == 2)
+        rc = p.dup ? launch<64, 1, true, 2>(a, p, B, st) : launch<64, 1, false, 2>(a, p, B, st);
     else if (head_dim == 64)
-        rc = p.dup ? launch<64, 1, true>(a, p, B, st) : p.nt == 1 ? launch<64, 1, false>(a, p, B, st)
-           : p.nt == 2 ? launch<64, 2, false>(a, p, B, st) : p.nt == 3 ? launch<64, 3, false>(a, p, B, st)
-           : launch<64, 4, false>(a, p, B, st);
+        rc = p.dup ? launch<64, 1, true, 4>(a, p, B, st) : p.nt == 1 ? launch<64, 1, false, 4>(a, p, B, st)
+           : p.nt == 2 ? launch<64, 2, false, 4>(a, p, B, st) : p.nt == 3 ? launch<64, 3, false, 4>(a, p, B, st)
+           : launch<64, 4, false, 4>(a, p, B, st);
+    else if (p.warps == 2)
+        rc = p.dup ? launch<128, 1, true, 2>(a, p, B, st) : launch<128, 1, false, 2>(a, p, B, st);
     else
-        rc = p.dup ? launch<128, 1, true>(a, p, B, st) : p.nt == 1 ? launch<128, 1, false>(a, p, B, st)
-           : launch<128, 2, false>(a, p, B, st);
+        rc = p.dup ? launch<128, 1, true, 4>(a, p, B, st) : p.nt == 1 ? launch<128, 1, false, 4>(a, p, B, st)
+           : launch<128, 2, false, 4>(a, p, B, st);
     PULSAR_TRY(rc);
-    if (p.nsplit > 1) {
-        const dim3 grid((unsigned)(max_q * Hq), (unsigned)B);
-        if (head_dim == 64)
-            k_kv4_merge<64><<<grid, 64, 0, st>>>(a);
-        else
-            k_kv4_merge<128><<<grid, 128, 0, st>>>(a);
-        PULSAR_LAUNCH_CHECK("k_kv4_merge");
-    }
+    if (p.nsplit > 1) return head_dim == 64 ? launch_merge<64>(a, B, st) : launch_merge<128>(a, B, st);
     return PULSAR_OK;
 }

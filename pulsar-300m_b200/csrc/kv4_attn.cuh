@@ -21,18 +21,46 @@ struct Kv4AttnArgs {
     // exponent m (base 2) and the sum l of the weights relative to it
     float *part_o, *part_ml;
     int64_t q_row, q_head, page_bytes;
-    int rows, hq, hkv, group, num_pages, width, page_shift, max_q, window, nsplit, split_len;
+    int rows, hq, hkv, group, num_pages, width, page_shift, max_q, window, nsplit, split_len, unit_tile, step;
     float scale_log2;
 };
 
-// The rows of sequence b, held inside q whatever cu_q says.
-__device__ __forceinline__ void kv4_rows(const Kv4AttnArgs& a, int b, int& row0, int& nq) {
-    row0 = b;
-    nq = 1;
+// The part of sequence b that a unit tile (units u0 .. u0 + ut - 1) concerns. Everything stays inside
+// the tensors whatever cu_q and kv_lens say.
+struct Kv4Range {
+    int row0, nq, units, ulast;   // the sequence's rows and units, the tile's last unit
+    int len, first, last;         // keys; positions of the tile's first and last unit
+    int kmin, kmax;               // keys that some unit of the tile sees: [kmin, kmax)
+    int step0, steps, used;       // in steps of `step` keys from step0 on; splits that have some (at least 1)
+};
+__device__ __forceinline__ int kv4_low(const Kv4AttnArgs& a, int pos) {   // first key that position pos sees
+    return a.window > 0 ? max(0, pos - a.window + 1) : 0;
+}
+__device__ __forceinline__ int kv4_row(const Kv4AttnArgs& a, int u) { return a.max_q == 1 ? 0 : u / a.group; }
+__device__ __forceinline__ bool kv4_range(const Kv4AttnArgs& a, int b, int u0, int ut, int step, Kv4Range& r) {
+    r.row0 = b;
+    r.nq = 1;
     if (a.cu_q) {
-        row0 = min(max(a.cu_q[b], 0), a.rows);
-        nq = min(max(a.cu_q[b + 1] - row0, 0), min(a.max_q, a.rows - row0));
+        r.row0 = min(max(a.cu_q[b], 0), a.rows);
+        r.nq = min(max(a.cu_q[b + 1] - r.row0, 0), min(a.max_q, a.rows - r.row0));
     }
+    r.len = min(max(a.kv_lens[b], 0), a.width << a.page_shift);
+    r.units = r.nq * a.group;
+    if (u0 >= r.units) return false;
+    r.ulast = min(u0 + ut, r.units) - 1;
+    r.first = r.len - r.nq + kv4_row(a, u0);
+    r.last = r.len - r.nq + kv4_row(a, r.ulast);
+    r.kmin = kv4_low(a, r.first);
+    r.kmax = max(r.last + 1, 0);
+    r.step0 = r.kmin / step;
+    r.steps = max((r.kmax + step - 1) / step - r.step0, 0);
+    r.used = min(max((r.steps + a.split_len - 1) / a.split_len, 1), a.nsplit);
+    return true;
+}
+// Steps [begin, end) of split sp < used, counted from step0: the last one takes what is left.
+__device__ __forceinline__ void kv4_split(const Kv4AttnArgs& a, const Kv4Range& r, int sp, int& begin, int& end) {
+    begin = sp * a.split_len;
+    end = sp == r.used - 1 ? r.steps : min(r.steps, begin + a.split_len);
 }
 
 // Page of tile `tile` of sequence b (-1: none, or outside the cache).

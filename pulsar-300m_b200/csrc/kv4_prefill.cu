@@ -227,18 +227,15 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
     const int split = blockIdx.x % a.nsplit, u0 = blockIdx.x / a.nsplit * L::UNITS;
     const int h = blockIdx.y, b = blockIdx.z;
 
-    int row0, nq;
-    kv4_rows(a, b, row0, nq);
-    const int units = nq * a.group;
-    if (u0 >= units) return;
-    const int len = min(max(a.kv_lens[b], 0), a.width << a.page_shift);
-    const int ulast = min(u0 + L::UNITS, units) - 1;
-    const int tiles = (ulast - u0) / 128 + 1;
-    const int first = len - nq + u0 / a.group, last = len - nq + ulast / a.group;
-    auto low = [&](int pos) { return a.window > 0 ? max(0, pos - a.window + 1) : 0; };
-    const int kmin = low(first), kmax = max(last + 1, 0);
-    const int step0 = kmin / SK + split * a.split_len, base = step0 * SK;
-    const int kend = split == a.nsplit - 1 ? kmax : min(kmax, base + a.split_len * SK);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the merge may be set up meanwhile
+    Kv4Range rg;
+    if (!kv4_range(a, b, u0, L::UNITS, SK, rg) || split >= rg.used) return;
+    const int row0 = rg.row0, nq = rg.nq, units = rg.units, len = rg.len, kmin = rg.kmin, kmax = rg.kmax;
+    const int tiles = (rg.ulast - u0) / 128 + 1;
+    auto low = [&](int pos) { return kv4_low(a, pos); };
+    int s_begin, s_end;
+    kv4_split(a, rg, split, s_begin, s_end);
+    const int step0 = rg.step0 + s_begin, base = step0 * SK, kend = min(kmax, (rg.step0 + s_end) * SK);
     const int n = kend > base ? (kend - base + CK - 1) / CK : 0, steps = (n + 1) / 2;   // chunks, steps
 
     if (tid == 0) {
@@ -625,7 +622,7 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
             const bool row_ok = u < units;
             const int j = row_ok ? u / a.group : 0, g = row_ok ? u - j * a.group : 0;
             const int64_t at = (int64_t)(row0 + j) * a.hq + h * a.group + g;
-            const float inv = a.nsplit > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
+            const float inv = rg.used > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
             for (int q = 0; q < HD / 16; ++q) {
                 uint32_t v[16];
@@ -637,7 +634,7 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
 #pragma unroll
                 for (int i = 0; i < 16; ++i)
                     x[i] = bad >> (q / 2) & 1 ? __int_as_float(0x7fffffff) : __uint_as_float(v[i]) * inv;
-                if (a.nsplit > 1) {
+                if (rg.used > 1) {
                     float4* o = reinterpret_cast<float4*>(a.part_o + (at * a.nsplit + split) * HD + 16 * q);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) o[i] = make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
@@ -652,7 +649,7 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
                     }
                 }
             }
-            if (row_ok && a.nsplit > 1) {
+            if (row_ok && rg.used > 1) {
                 a.part_ml[(at * a.nsplit + split) * 2] = m;
                 a.part_ml[(at * a.nsplit + split) * 2 + 1] = l;
             }
