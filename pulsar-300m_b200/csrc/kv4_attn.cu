@@ -50,6 +50,14 @@ __device__ __forceinline__ void mma16816(float* d, const uint32_t* a, uint32_t b
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 
+__device__ __forceinline__ void mma16816h(float* d, const uint32_t* a, uint32_t b0, uint32_t b1, const float* c) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%10,%11,%12,%13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+
 __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -96,6 +104,7 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
     using T = Kv4Tile<HD>;
     constexpr int NG = T::NG, NB = HD / 64, S = stages<HD>(), MT = HD / 16, TB = T::BYTES;
     constexpr int UT = DUP ? 4 : 8 * NT;
+    constexpr bool WIDE = NT > 1;
     extern __shared__ __align__(128) unsigned char sm[];
     __shared__ uint64_t bars[WARPS][S];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, t = lane & 3;
@@ -163,7 +172,8 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
 
     // queries: B operand of step j (dims 16 j ..): unit n = lane / 4, dims 2t, 2t + 1 and 8 further
     uint32_t qf[NT][2 * MT];
-    float qsum[NT][NG][2];   // sum of q over the group (in the units of the scores), for the thread's columns
+    // sum of q over the group, in the units of the scores; WIDE: exponent taken out of q times scale, in [0]
+    float qsum[NT][NG][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int u = u0 + (DUP ? (r & 3) : nt * 8 + r);
@@ -172,21 +182,36 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
         const __nv_bfloat16* src = a.q + (row0 + j) * a.q_row + (h * a.group + g) * a.q_head;
 #pragma unroll
         for (int i = 0; i < 2 * MT; ++i) qf[nt][i] = ok ? *reinterpret_cast<const uint32_t*>(src + 8 * i + 2 * t) : 0u;
+        if constexpr (WIDE) {   // q 2^-eq in fp16, its largest |dim| in [2^3, 2^4)
+            uint32_t top = 0;
 #pragma unroll
-        for (int g4 = 0; g4 < NG; ++g4) {
-            float s = 0.f;
+            for (int i = 0; i < 2 * MT; ++i)
+                top = max(top, max(qf[nt][i] << 16 & 0x7fffffffu, qf[nt][i] & 0x7fff0000u));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int eq = min(max((int)(top >> 23) - 127 - 3, -100), 100);
+            const float f = kv4_exp2i(-eq), s = a.scale_log2 * kv4_exp2i(eq);
+            qsum[nt][0][0] = __shfl_sync(0xffffffffu, s, 8 * t);
+            qsum[nt][0][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s += lo_of(qf[nt][4 * g4 + i]) + hi_of(qf[nt][4 * g4 + i]);
-            s += __shfl_xor_sync(0xffffffffu, s, 1);
-            s += __shfl_xor_sync(0xffffffffu, s, 2);
-            s *= pow2(LIFT - CODE_EXP);
-            qsum[nt][g4][0] = __shfl_sync(0xffffffffu, s, 8 * t);
-            qsum[nt][g4][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
-        }
+            for (int i = 0; i < 2 * MT; ++i) qf[nt][i] = kv4_half2(lo_of(qf[nt][i]) * f, hi_of(qf[nt][i]) * f);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 2 * MT; ++i) {   // odd registers meet 16 c
-            const float f = i & 1 ? pow2(LIFT - 4) : pow2(LIFT);
-            qf[nt][i] = pack(lo_of(qf[nt][i]) * f, hi_of(qf[nt][i]) * f);
+            for (int g4 = 0; g4 < NG; ++g4) {
+                float s = 0.f;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s += lo_of(qf[nt][4 * g4 + i]) + hi_of(qf[nt][4 * g4 + i]);
+                s += __shfl_xor_sync(0xffffffffu, s, 1);
+                s += __shfl_xor_sync(0xffffffffu, s, 2);
+                s *= pow2(LIFT - CODE_EXP);
+                qsum[nt][g4][0] = __shfl_sync(0xffffffffu, s, 8 * t);
+                qsum[nt][g4][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
+            }
+#pragma unroll
+            for (int i = 0; i < 2 * MT; ++i) {   // odd registers meet 16 c
+                const float f = i & 1 ? pow2(LIFT - 4) : pow2(LIFT);
+                qf[nt][i] = pack(lo_of(qf[nt][i]) * f, hi_of(qf[nt][i]) * f);
+            }
         }
     }
     int hi[NT][2], lo[NT][2];   // keys that the thread's columns see
@@ -202,21 +227,22 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
     const int all_lo = kv4_low(a, rg.last), all_hi = rg.first + 1;   // keys in [all_lo, all_hi) are seen by every unit
 
     // Scores come in units of 2^(LIFT - CODE_EXP); m: their running maximum, nm = LIFT - scale m, so
-    // that weights are 2^LIFT exp2(scale (s - m))
+    // that weights are 2^LIFT exp2(scale (s - m)). WIDE: m is the reference of the weights 2^(x - m), base 2
     float o[MT][NT][4], zacc[NT][NG][2], m[NT][2], nm[NT][2], l[NT][2];
-    const float scale = a.scale_log2 * pow2(CODE_EXP - LIFT);
+    const float scale = WIDE ? 1.f : a.scale_log2 * pow2(CODE_EXP - LIFT);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int i = 0; i < MT; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
 #pragma unroll
         for (int g = 0; g < NG; ++g) zacc[nt][g][0] = zacc[nt][g][1] = 0.f;
-        m[nt][0] = m[nt][1] = NEG * pow2(LIFT - CODE_EXP);
+        m[nt][0] = m[nt][1] = WIDE ? NEG : NEG * pow2(LIFT - CODE_EXP);
         nm[nt][0] = nm[nt][1] = -NEG * a.scale_log2;
         l[nt][0] = l[nt][1] = 0.f;
     }
     // columns 4..7 of the doubled units (t >= 2) carry the lo halves: x = w lo_w + hi lo_h
     const float lo_w = t < 2 ? 0.f : 1.f, lo_h = t < 2 ? 1.f : -1.f;
+    uint32_t bad[NT][2] = {};   // WIDE: groups of V stored as NaN that the column sees
     int failed = -1;   // the pair whose copy did not land within the bound
 
     // one pair of tiles; EDGE: some of its keys are not seen by some unit, or a page is missing
@@ -376,6 +402,184 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
         }
     };
 
+    // The same with keys and values unpacked to fp16 numbers, s and z applied: more work a tile and less
+    // a unit (no s and z on scores, one operand of weights instead of two a group). 2^ek, 2^ev come
+    // out of the pair's keys and values: x = 2^ek q.k scale + ev, weights 2^(x - m), l = sum 2^-ev weight
+    auto wide_step = [&](auto edge_tag, const unsigned char* tp, int k0, bool ok0, bool ok1) {
+        constexpr bool EDGE = decltype(edge_tag)::value;
+        auto known = [&](int x, int token) {   // some unit sees the token
+            const int key = k0 + 16 * x + token;
+            return !EDGE || ((x ? ok1 : ok0) && key >= rg.kmin && key < rg.kmax);
+        };
+        uint32_t topk = 0, topv = 0;
+        bool nan_v = false;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int y = 0; y < NB; ++y) {
+                const int at = 32 * y + lane, slot = at / NG;
+                const bool in = known(x, (slot >> 1) + 8 * (slot & 1));
+                const uint32_t kw = *reinterpret_cast<const uint32_t*>(tp + x * TB + T::KP + 4 * at);
+                const uint32_t vw = *reinterpret_cast<const uint32_t*>(tp + x * TB + T::VP + 4 * at);
+                topk = max(topk, in ? kv4_top(kw) : 0u);
+                topv = max(topv, in ? kv4_top(vw) : 0u);
+                if (EDGE) nan_v |= in && !(kv4_z(vw) == kv4_z(vw));
+            }
+        topk = __reduce_max_sync(0xffffffffu, topk);
+        topv = __reduce_max_sync(0xffffffffu, topv);
+        if (EDGE) nan_v = __any_sync(0xffffffffu, nan_v);
+        const int ek = kv4_exponent_out(topk), evi = kv4_exponent_out(topv);
+        const float fk = kv4_exp2i(-ek), fv = kv4_exp2i(-evi), ev = (float)evi;
+        float sc[2][NT][4], kq[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            kq[nt][0] = qsum[nt][0][0] * kv4_exp2i(ek);
+            kq[nt][1] = qsum[nt][0][1] * kv4_exp2i(ek);
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const unsigned char* kt = tp + x * TB;
+            uint32_t kp[2][NG], kc[NB][4];
+#pragma unroll
+            for (int y = 0; y < NB; ++y)
+                *reinterpret_cast<uint4*>(kc[y]) = *reinterpret_cast<const uint4*>(kt + y * T::BLK + lane * 16);
+#pragma unroll
+            for (int y = 0; y < 2 * NG; y += 4)
+                *reinterpret_cast<uint4*>(&kp[0][0] + y) = *reinterpret_cast<const uint4*>(kt + T::KP + r * 8 * NG + y * 4);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) sc[x][nt][0] = sc[x][nt][1] = sc[x][nt][2] = sc[x][nt][3] = 0.f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                uint32_t w0[4], w8[4];
+                const float s0 = kv4_s(kp[0][g]) * fk, z0 = kv4_z(kp[0][g]) * fk, s8 = kv4_s(kp[1][g]) * fk,
+                            z8 = kv4_z(kp[1][g]) * fk;
+                kv4_unpack4(kc[g >> 1][g & 1], kv4_half2(s0, s0), kv4_half2(z0, z0), w0);
+                kv4_unpack4(kc[g >> 1][2 + (g & 1)], kv4_half2(s8, s8), kv4_half2(z8, z8), w8);
+                const uint32_t a0[4] = {w0[0], w8[0], w0[1], w8[1]}, a1[4] = {w0[2], w8[2], w0[3], w8[3]};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    mma16816h(sc[x][nt], a0, qf[nt][4 * g], qf[nt][4 * g + 1], sc[x][nt]);
+                    mma16816h(sc[x][nt], a1, qf[nt][4 * g + 2], qf[nt][4 * g + 3], sc[x][nt]);
+                }
+            }
+        }
+        if (EDGE) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int k = k0 + 16 * x + r + (e < 2 ? 0 : 8);
+                        const bool see = (x ? ok1 : ok0) && k >= lo[nt][e & 1] && k < hi[nt][e & 1];
+                        if (!see) sc[x][nt][e] = -INFINITY;
+                        if (nan_v && see) {   // rare
+#pragma unroll
+                            for (int g = 0; g < NG; ++g) {
+                                const float z = kv4_z(*reinterpret_cast<const uint32_t*>(
+                                    tp + x * TB + T::VP + ((2 * r + (e < 2 ? 0 : 1)) * NG + g) * 4));
+                                if (!(z == z)) bad[nt][e & 1] |= 1u << g;
+                            }
+                        }
+                    }
+        }
+        uint32_t p[2][NT][2];   // weights, fp16 pairs (token r; token r + 8)
+        float ls[NT][2];
+        auto weigh = [&]() {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                ls[nt][0] = ls[nt][1] = 0.f;
+                const float b0 = ev - m[nt][0], b1 = ev - m[nt][1];
+#pragma unroll
+                for (int x = 0; x < 2; ++x)
+#pragma unroll
+                    for (int y = 0; y < 2; ++y) {
+                        const float w0 = kv4_ex2(fmaf(sc[x][nt][2 * y], kq[nt][0], b0));
+                        const float w1 = kv4_ex2(fmaf(sc[x][nt][2 * y + 1], kq[nt][1], b1));
+                        ls[nt][0] += w0;
+                        ls[nt][1] += w1;
+                        p[x][nt][y] = kv4_half2(w0, w1);
+                    }
+            }
+        };
+        weigh();
+        bool up = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) up |= ls[nt][0] > pow2(14) || ls[nt][1] > pow2(14);
+        if (__any_sync(0xffffffffu, up)) {   // fp16 would soon be left: move the references, weigh again
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float x = fmaxf(fmaxf(sc[0][nt][c], sc[0][nt][c + 2]), fmaxf(sc[1][nt][c], sc[1][nt][c + 2]));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                    x = fmaxf(fmaf(x, kq[nt][c], ev), m[nt][c]);
+                    const float f = kv4_ex2(m[nt][c] - x);
+                    m[nt][c] = x;
+                    l[nt][c] *= f;
+#pragma unroll
+                    for (int y = 0; y < MT; ++y) {
+                        o[y][nt][c] *= f;
+                        o[y][nt][c + 2] *= f;
+                    }
+                }
+            weigh();
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            l[nt][0] = fmaf(ls[nt][0], kv4_exp2i(-evi), l[nt][0]);
+            l[nt][1] = fmaf(ls[nt][1], kv4_exp2i(-evi), l[nt][1]);
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const unsigned char* vt = tp + x * TB;
+            uint32_t vp[4 * NG], vc[NB][4], b0[NT], b1[NT];
+#pragma unroll
+            for (int y = 0; y < NB; ++y)
+                *reinterpret_cast<uint4*>(vc[y]) = *reinterpret_cast<const uint4*>(vt + T::V + y * T::BLK + lane * 16);
+#pragma unroll
+            for (int y = 0; y < 4 * NG; y += 4)   // tokens 2t, 2t + 8, 2t + 1, 2t + 9
+                *reinterpret_cast<uint4*>(vp + y) = *reinterpret_cast<const uint4*>(vt + T::VP + t * 16 * NG + y * 4);
+            if (EDGE) {   // what no unit sees, and NaN groups (in bad): zero
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+#pragma unroll
+                    for (int g = 0; g < NG; ++g)
+                        if (!known(x, 2 * t + (y >> 1) + 8 * (y & 1)) || !(kv4_z(vp[y * NG + g]) == kv4_z(vp[y * NG + g])))
+                            vp[y * NG + g] = 0u;
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                b0[nt] = movmatrix(p[x][nt][0]);
+                b1[nt] = movmatrix(p[x][nt][1]);
+            }
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                uint32_t w[2][4];
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {   // tokens 2t, 2t + 1 and 8 further
+                    const uint32_t p0 = vp[y * NG + g], p1 = vp[(2 + y) * NG + g];
+                    kv4_unpack4(vc[g >> 1][2 * (g & 1) + y], kv4_half2(kv4_s(p0) * fv, kv4_s(p1) * fv),
+                                kv4_half2(kv4_z(p0) * fv, kv4_z(p1) * fv), w[y]);
+                }
+                const uint32_t a0[4] = {w[0][0], w[0][1], w[1][0], w[1][1]}, a1[4] = {w[0][2], w[0][3], w[1][2], w[1][3]};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    mma16816h(o[2 * g][nt], a0, b0[nt], b1[nt], o[2 * g][nt]);
+                    mma16816h(o[2 * g + 1][nt], a1, b0[nt], b1[nt], o[2 * g + 1][nt]);
+                }
+            }
+        }
+    };
+    auto step = [&](auto edge_tag, const unsigned char* tp, int k0, bool ok0, bool ok1) {
+        if constexpr (WIDE)
+            wide_step(edge_tag, tp, k0, ok0, ok1);
+        else
+            pair_step(edge_tag, tp, k0, ok0, ok1);
+    };
+
     for (int i = 0; i < mine; ++i) {
         const int st = i % S;
         if (i > 0 && (i & 31) == 0) {
@@ -390,9 +594,9 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
         const int k0 = (p_begin + i * WARPS) * 32;
         const unsigned char* tp = ring + st * 2 * TB;
         if (k0 >= all_lo && k0 + 32 <= all_hi && ok0 && ok1)
-            pair_step(std::false_type{}, tp, k0, true, true);
+            step(std::false_type{}, tp, k0, true, true);
         else if (ok0 || ok1)
-            pair_step(std::true_type{}, tp, k0, ok0, ok1);
+            step(std::true_type{}, tp, k0, ok0, ok1);
         __syncwarp();   // every lane has read the stage
         const int nx = i + S;
         if (nx < mine) {
@@ -420,14 +624,20 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
             if (failed >= 0) s = __int_as_float(0x7fffffff);
             if (r == 0 && (!DUP || t < 2)) {
                 wo[u * (HD + 2) + HD] = m[nt][c] * scale;
-                wo[u * (HD + 2) + HD + 1] = s * pow2(-LIFT);
+                wo[u * (HD + 2) + HD + 1] = WIDE ? s : s * pow2(-LIFT);
             }
+            uint32_t none = bad[nt][c];
+            if (WIDE) none = __reduce_or_sync(0x11111111u << t, none);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 float z = zacc[nt][g][c];
+                if (WIDE) {
+                    z = none >> g & 1 ? __int_as_float(0x7fffffff) : 0.f;
+                } else {
 #pragma unroll
-                for (int x = 4; x < 32; x <<= 1) z += __shfl_xor_sync(0xffffffffu, z, x);
-                z *= pow2(-LIFT);
+                    for (int x = 4; x < 32; x <<= 1) z += __shfl_xor_sync(0xffffffffu, z, x);
+                    z *= pow2(-LIFT);
+                }
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -436,7 +646,7 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
                         if (DUP) v += __shfl_xor_sync(0xffffffffu, v, 2);
                         if (!DUP || t < 2)
                             wo[u * (HD + 2) + 32 * g + 16 * x + 8 * e + r] =
-                                fmaf(v, pow2(CODE_EXP - LIFT - 4 * e), z);
+                                fmaf(v, WIDE ? 1.f : pow2(CODE_EXP - LIFT - 4 * e), z);
                     }
             }
         }
@@ -469,15 +679,16 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
 }
 
 // out of one (sequence row, head) from its splits' partials (where there is more than one): 128
-// threads, HD / 4 to a partial, which go through every 512 / HD-th split; these are joined in shared
-// memory. Both orders are fixed.
-template <int HD>
+// threads, HD / 4 to a partial; NG groups of these go through every NG-th split of one (row, head) and
+// are joined in shared memory, the others of the block have rows of their own. Both orders are fixed.
+template <int HD, int NG>
 __global__ void __launch_bounds__(128) k_kv4_merge(const Kv4AttnArgs a) {
-    constexpr int LN = HD / 4, NG = 128 / LN;
-    __shared__ float4 os[NG][LN];
+    constexpr int LN = HD / 4, PER = 128 / LN / NG;   // (row, head) pairs of a block
+    __shared__ float4 os[NG > 1 ? NG : 1][LN];
     __shared__ float2 mls[NG];
-    const int j = blockIdx.x / a.hq, head = blockIdx.x % a.hq, b = blockIdx.y;
-    const int u = j * a.group + head % a.group, g = threadIdx.x / LN, d = threadIdx.x % LN;
+    const int d = threadIdx.x % LN, g = threadIdx.x / LN % NG, b = blockIdx.y;
+    const int jh = blockIdx.x * PER + threadIdx.x / (LN * NG), j = jh / a.hq, head = jh % a.hq;
+    const int u = j * a.group + head % a.group;
     asm volatile("griddepcontrol.wait;" ::: "memory");   // the attention kernel's partials are there
     Kv4Range rg;
     if (!kv4_range(a, b, u - u % a.unit_tile, a.unit_tile, a.step, rg) || u >= rg.units || rg.used == 1) return;
@@ -507,21 +718,23 @@ __global__ void __launch_bounds__(128) k_kv4_merge(const Kv4AttnArgs a) {
             o = make_float4(fmaf(f, y[i].x, o.x), fmaf(f, y[i].y, o.y), fmaf(f, y[i].z, o.z), fmaf(f, y[i].w, o.w));
         }
     }
-    os[g][d] = o;
-    if (d == 0) mls[g] = make_float2(m, l);
-    __syncthreads();
-    if (g > 0) return;
-    float top = NEG;
+    if (NG > 1) {   // (the block has one pair: all its threads are here)
+        os[g][d] = o;
+        if (d == 0) mls[g] = make_float2(m, l);
+        __syncthreads();
+        if (g > 0) return;
+        float top = NEG;
 #pragma unroll
-    for (int i = 0; i < NG; ++i) top = fmaxf(top, mls[i].x);
-    l = 0.f;
-    o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = 0; i < NG; ++i) top = fmaxf(top, mls[i].x);
+        l = 0.f;
+        o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < NG; ++i) {
-        const float f = kv4_ex2(mls[i].x - top);
-        const float4 y = os[i][d];
-        l = fmaf(f, mls[i].y, l);
-        o = make_float4(fmaf(f, y.x, o.x), fmaf(f, y.y, o.y), fmaf(f, y.z, o.z), fmaf(f, y.w, o.w));
+        for (int i = 0; i < NG; ++i) {
+            const float f = kv4_ex2(mls[i].x - top);
+            const float4 y = os[i][d];
+            l = fmaf(f, mls[i].y, l);
+            o = make_float4(fmaf(f, y.x, o.x), fmaf(f, y.y, o.y), fmaf(f, y.z, o.z), fmaf(f, y.w, o.w));
+        }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const __nv_bfloat162 lo2 = __floats2bfloat162_rn(o.x * inv, o.y * inv), hi2 = __floats2bfloat162_rn(o.z * inv, o.w * inv);
@@ -539,7 +752,8 @@ struct Plan {
 // How a call is cut. More than MANY units of a sequence's rows go to k_kv4_prefill, 512 or 256 a CTA.
 // Others: the fewest columns that hold max_q rows of a group (four: both halves of the weights in
 // one operand), at most 32 (heads of 128: 16, for the registers).
-// Splits of the keys: until four CTAs an SM are there, of at least 8 pairs of tiles (two a warp); where
+// Splits of the keys: until the SMs are full (four CTAs each; two above 8 units), of at least 8 pairs of
+// tiles (two a warp); where
 // there are many keys, of 32 to 64 pairs, so that sequences shorter than max_kv even out (the splits
 // that they lack end at once). k_kv4_prefill: the number that fills the last wave best.
 // Two warps instead of four where there is a CTA for every unit tile and each has few keys: what a CTA
@@ -580,8 +794,8 @@ Plan make_plan(int64_t B, int64_t Hkv, int64_t group, int64_t head_dim, int64_t 
             }
         }
     } else {
-        const int64_t fill = 148 * 4;
-        ns = (fill + ctas - 1) / ctas;
+        const int64_t fill = 148 * (p.nt == 1 ? 4 : 2);   // CTAs that the GPU holds at once
+        ns = ctas * 4 > fill * 3 ? 1 : (fill + ctas - 1) / ctas;
         if (ns > steps / 8) ns = steps / 8;
         if (ctas * ((steps + 63) / 64) > fill && ns < (steps + 63) / 64) ns = (steps + 31) / 32;
         if (ns > 128) ns = 128;
@@ -606,19 +820,24 @@ int launch(const Kv4AttnArgs& a, const Plan& p, int64_t B, cudaStream_t st) {
     return PULSAR_OK;
 }
 
-// The merge is launched under the attention kernel's end; it waits for that before it reads.
+// The merge is launched under the attention kernel's end; it waits for that before it reads. Up to
+// four splits a group of threads takes them all.
 template <int HD>
 int launch_merge(const Kv4AttnArgs& a, int64_t B, cudaStream_t st) {
+    constexpr int ALL = 512 / HD;   // groups of a block
+    const bool few = a.nsplit <= 4;
+    const int64_t rows = (int64_t)a.max_q * a.hq;
     cudaLaunchAttribute early{};
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     early.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)((int64_t)a.max_q * a.hq), (unsigned)B);
+    cfg.gridDim = dim3((unsigned)(few ? (rows + ALL - 1) / ALL : rows), (unsigned)B);
     cfg.blockDim = dim3(128);
     cfg.stream = st;
     cfg.attrs = &early;
     cfg.numAttrs = 1;
-    return cuda_status(cudaLaunchKernelEx(&cfg, k_kv4_merge<HD>, a), "k_kv4_merge");
+    return cuda_status(few ? cudaLaunchKernelEx(&cfg, k_kv4_merge<HD, 1>, a) : cudaLaunchKernelEx(&cfg, k_kv4_merge<HD, ALL>, a),
+                       "k_kv4_merge");
 }
 
 int check_shape(int64_t N, int64_t Hq, int64_t Hkv, int64_t head_dim, int64_t B, int64_t max_q, int64_t max_kv,

@@ -3,6 +3,7 @@
 #pragma once
 
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -77,6 +78,41 @@ __device__ __forceinline__ float kv4_ex2(float x) {
 }
 __device__ __forceinline__ float kv4_s(uint32_t param) { return __uint_as_float(param << 16); }
 __device__ __forceinline__ float kv4_z(uint32_t param) { return __uint_as_float(param & 0xffff0000u); }
+
+// Operands in fp16 (values s c + z of 8-bit s, z and 4-bit c, rounded twice at 2^-12): fp16 has the
+// significand but not the range, so powers of two are taken out of keys and values.
+__device__ __forceinline__ uint32_t kv4_half2(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ __half2 kv4_as_half2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
+
+// The four operand registers of a code word as s c + z: codes under the exponent of 1024 (c, or 16 c).
+__device__ __forceinline__ void kv4_unpack4(uint32_t w, uint32_t s, uint32_t z, uint32_t* r) {
+    const uint32_t v = w >> 8;
+    const __half2 one = __floats2half2_rn(1024.f, 1024.f), inv = __floats2half2_rn(0.0625f, 0.0625f),
+                  sub = __floats2half2_rn(-64.f, -64.f);
+    const __half2 c0 = __hsub2(kv4_as_half2((w & 0x000f000fu) | 0x64006400u), one);
+    const __half2 c1 = __hfma2(kv4_as_half2((w & 0x00f000f0u) | 0x64006400u), inv, sub);
+    const __half2 c2 = __hsub2(kv4_as_half2((v & 0x000f000fu) | 0x64006400u), one);
+    const __half2 c3 = __hfma2(kv4_as_half2((v & 0x00f000f0u) | 0x64006400u), inv, sub);
+    const __half2 x[4] = {__hfma2(c0, kv4_as_half2(s), kv4_as_half2(z)), __hfma2(c1, kv4_as_half2(s), kv4_as_half2(z)),
+                          __hfma2(c2, kv4_as_half2(s), kv4_as_half2(z)), __hfma2(c3, kv4_as_half2(s), kv4_as_half2(z))};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = *reinterpret_cast<const uint32_t*>(&x[i]);
+}
+
+// Power of two that brings a largest magnitude (float bits) to [2^9, 2^10): the exponent taken out.
+__device__ __forceinline__ int kv4_exponent_out(uint32_t bits) {
+    return min(max((int)(bits >> 23) - 127 - 9, -100), 100);
+}
+__device__ __forceinline__ float kv4_exp2i(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
+// The largest |value| that a parameter pair allows, as float bits (0 for NaN).
+__device__ __forceinline__ uint32_t kv4_top(uint32_t param) {
+    const float x = fmaxf(fabsf(kv4_z(param)), fabsf(fmaf(15.f, kv4_s(param), kv4_z(param))));
+    return x == x ? __float_as_uint(x) : 0u;
+}
 
 // Many query rows (kv4_prefill.cu): units = query rows x heads of a group.
 constexpr int kv4_pf_units(int head_dim) { return head_dim == 64 ? 512 : 256; }   // units of a CTA

@@ -27,8 +27,6 @@
 //
 // Every wait is bounded; one that runs out raises the CTA's abort flag, which ends the others; MMAs
 // and copies in flight are waited for (bounded again) and the rows answer NaN.
-#include <cuda_fp16.h>
-
 #include <type_traits>
 
 #include "capi_util.h"
@@ -182,36 +180,9 @@ __device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
-__device__ __forceinline__ uint32_t half2_bits(float a, float b) {
-    const __half2 v = __floats2half2_rn(a, b);
-    return *reinterpret_cast<const uint32_t*>(&v);
-}
-__device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
-
-// The four operand registers of a code word as s c + z: codes under the exponent of 1024 (c, or 16 c).
-__device__ __forceinline__ void unpack4(uint32_t w, uint32_t s, uint32_t z, uint32_t* r) {
-    const uint32_t v = w >> 8;
-    const __half2 one = __floats2half2_rn(1024.f, 1024.f), inv = __floats2half2_rn(0.0625f, 0.0625f),
-                  sub = __floats2half2_rn(-64.f, -64.f);
-    const __half2 c0 = __hsub2(as_half2((w & 0x000f000fu) | 0x64006400u), one);
-    const __half2 c1 = __hfma2(as_half2((w & 0x00f000f0u) | 0x64006400u), inv, sub);
-    const __half2 c2 = __hsub2(as_half2((v & 0x000f000fu) | 0x64006400u), one);
-    const __half2 c3 = __hfma2(as_half2((v & 0x00f000f0u) | 0x64006400u), inv, sub);
-    const __half2 x[4] = {__hfma2(c0, as_half2(s), as_half2(z)), __hfma2(c1, as_half2(s), as_half2(z)),
-                          __hfma2(c2, as_half2(s), as_half2(z)), __hfma2(c3, as_half2(s), as_half2(z))};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r[i] = *reinterpret_cast<const uint32_t*>(&x[i]);
-}
-
 __device__ __forceinline__ void sts(uint32_t at, uint32_t v) {
     asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
 }
-
-// Power of two that brings a largest magnitude (float bits) to [2^9, 2^10): the exponent taken out.
-__device__ __forceinline__ int exponent_out(uint32_t bits) {
-    return min(max((int)(bits >> 23) - 127 - 9, -100), 100);
-}
-__device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
 template <int HD>
 __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4AttnArgs a) {
@@ -286,15 +257,15 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
             for (int e = 0; e < 4; ++e) top = max(top, max(w[e] << 16 & 0x7fffffffu, w[e] & 0x7fff0000u));
         }
         const int eq = min(max((int)(top >> 23) - 127 - 3, -100), 100);
-        const float f = exp2i(-eq);
-        qscale = a.scale_log2 * exp2i(eq);
+        const float f = kv4_exp2i(-eq);
+        qscale = a.scale_log2 * kv4_exp2i(eq);
         const int row = tid & 127;
         const uint32_t qt = sb + L::Q + (uint32_t)(tid >> 7) * L::QB + (row >> 3) * 1024 + (row & 7) * 128;
 #pragma unroll 4
         for (int i = 0; i < HD / 8; ++i) {
             dims(i, w);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = half2_bits(kv4_s(w[e]) * f, kv4_z(w[e]) * f);
+            for (int e = 0; e < 4; ++e) w[e] = kv4_half2(kv4_s(w[e]) * f, kv4_z(w[e]) * f);
             asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(qt + (i >> 3) * (128 * 128) +
                                                                           (((i & 7) ^ (row & 7)) << 4)),
                          "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
@@ -405,10 +376,8 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
                     const int key = k0 + 16 * (4 * (y0 + y) + w) + (slot >> 1) + 8 * (slot & 1);
                     const bool in = there[y] && key >= kmin && key < kmax;
                     const uint32_t kw = kp[at], vw = vp[at];
-                    const float ka = fmaxf(fabsf(kv4_z(kw)), fabsf(fmaf(15.f, kv4_s(kw), kv4_z(kw))));
-                    const float va = fmaxf(fabsf(kv4_z(vw)), fabsf(fmaf(15.f, kv4_s(vw), kv4_z(vw))));
-                    topk = max(topk, in && ka == ka ? __float_as_uint(ka) : 0u);
-                    topv = max(topv, in && va == va ? __float_as_uint(va) : 0u);
+                    topk = max(topk, in ? kv4_top(kw) : 0u);
+                    topv = max(topv, in ? kv4_top(vw) : 0u);
                     bad[y][x] = in && !(kv4_z(vw) == kv4_z(vw));
                     any_bad[y] |= bad[y][x];
                 }
@@ -425,8 +394,8 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
             topk = __reduce_max_sync(0xffffffffu, ms.top[sg][lane % L::UNPACK][0]);
             topv = __reduce_max_sync(0xffffffffu, ms.top[sg][lane % L::UNPACK][1]);
             if (__any_sync(0xffffffffu, ms.stop[sg][lane % L::UNPACK] != 0)) break;
-            const int ek = exponent_out(topk), ev = exponent_out(topv);
-            const float fk = exp2i(-ek), fv = exp2i(-ev);
+            const int ek = kv4_exponent_out(topk), ev = kv4_exponent_out(topv);
+            const float fk = kv4_exp2i(-ek), fv = kv4_exp2i(-ev);
 #pragma unroll
             for (int y = 0; y < YT; ++y) {
                 const int ch = 2 * c + y0 + y, sk = ch % KS, tl = 4 * (y0 + y) + w;
@@ -462,7 +431,7 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
                     for (int g = 0; g < NG; ++g) {
                         const float s = in ? kv4_s(par[hf * NG + g]) * fk : 0.f, z = in ? kv4_z(par[hf * NG + g]) * fk : 0.f;
                         uint32_t x[4];
-                        unpack4(code[g >> 1][2 * hf + (g & 1)], half2_bits(s, s), half2_bits(z, z), x);
+                        kv4_unpack4(code[g >> 1][2 * hf + (g & 1)], kv4_half2(s, s), kv4_half2(z, z), x);
 #pragma unroll
                         for (int i = 0; i < 4; ++i)
                             sts(row + (g >> 1) * (CK * 128) + (((4 * (g & 1) + i) ^ r) << 4), x[i]);
@@ -484,10 +453,10 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
                     for (int g = 0; g < NG; ++g) {
                         const uint32_t p0 = vpar[hf * NG + g], p1 = vpar[(2 + hf) * NG + g];
                         const bool ok0 = in0 && kv4_z(p0) == kv4_z(p0), ok1 = in1 && kv4_z(p1) == kv4_z(p1);
-                        const uint32_t s = half2_bits(ok0 ? kv4_s(p0) * fv : 0.f, ok1 ? kv4_s(p1) * fv : 0.f);
-                        const uint32_t z = half2_bits(ok0 ? kv4_z(p0) * fv : 0.f, ok1 ? kv4_z(p1) * fv : 0.f);
+                        const uint32_t s = kv4_half2(ok0 ? kv4_s(p0) * fv : 0.f, ok1 ? kv4_s(p1) * fv : 0.f);
+                        const uint32_t z = kv4_half2(ok0 ? kv4_z(p0) * fv : 0.f, ok1 ? kv4_z(p1) * fv : 0.f);
                         uint32_t x[4];
-                        unpack4(code[g >> 1][2 * (g & 1) + hf], s, z, x);
+                        kv4_unpack4(code[g >> 1][2 * (g & 1) + hf], s, z, x);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) sts(blk + (4 * g + i) * 1024, x[i]);
                     }
@@ -495,7 +464,7 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
                 if (lane == 0) {
                     ms.bad[sk][w] = any_bad[y];
                     if (w == 0) {
-                        ms.kscale[sk] = exp2i(ek);
+                        ms.kscale[sk] = kv4_exp2i(ek);
                         ms.ev[sk] = (float)ev;
                     }
                 }
@@ -564,7 +533,7 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
                         x = kv4_ex2(x);
                         y = kv4_ex2(y);
                         sum = add2(sum, two(x, y));
-                        p[16 * q + i] = half2_bits(x, y);
+                        p[16 * q + i] = kv4_half2(x, y);
                     }
                 }
                 float x, y;

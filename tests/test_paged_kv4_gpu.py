@@ -3,7 +3,7 @@
 Tolerances. A bf16 result is rounded once: relative 2^-9, taken as 2^-8 with the 32-bit work before
 it. A stored value is off by half a step s / 2 plus what the rounding of s (15 s 2^-9) and of the
 minimum z (|z| 2^-9) to bf16 add. Attention accumulates in 32 bits with operands good to 2^-16:
-2^-12 of the largest value that a row sees, besides the rounding of the result. Above 32 units a kv
+2^-12 of the largest value that a row sees, besides the rounding of the result. Above 8 units a kv
 head the operands are fp16 (keys and values rounded twice, weights once, at 2^-12, and a quarter of
 the weights good to 2^-13): 4 2^-12 of the largest value, and 2 2^-12 scale sum |q k| in a score, so
 twice that in a weight over their sum."""
@@ -271,7 +271,7 @@ def _attend(paged, lens, counts, hq, hkv, d, page, window=0, scale=None, seed=0,
                               max_q=max(1, max(counts)), window=window, scale=scale, **kw)
     k, v = held(pages, d)
     ref, top, amp = plain_attention(q, k, v, table, lens, cu, d ** -0.5 if scale is None else scale, window)
-    assert_attention(got, ref, top, amp, max(counts) * (hq // hkv) > 32)
+    assert_attention(got, ref, top, amp, max(counts) * (hq // hkv) > 8)
     return got
 
 
