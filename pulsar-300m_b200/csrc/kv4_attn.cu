@@ -12,8 +12,7 @@
 //
 // A unit is a (query row, head of the kv head's group). CTA (split and unit tile, kv head,
 // sequence): four warps, each walking every fourth pair of 16-token tiles of the split's range
-// through a ring of its own (1-D bulk copies of whole tiles, issued by its lane 0; page ids are
-// prefetched 32 pairs at a time, one a lane). Tokens are the M rows of S^T = K Q^T and units its N
+// through a ring of its own (1-D bulk copies of whole tiles; each lane looks after every 32nd pair). Tokens are the M rows of S^T = K Q^T and units its N
 // columns, so a tile's codes are unpacked once for all units, straight into operand registers; the
 // weights pass through movmatrix into the B operand of O^T = V^T P^T. Up to four units the eight
 // columns hold every unit twice and the copies carry the hi and the lo halves.
@@ -127,48 +126,48 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
     }
     __syncwarp();
 
-    // pages of the warp's i-th pair (-1: none): lane i % 32 holds them for the current 32; a page of
-    // 16 tokens holds one tile of the pair only
+    // Lane i % 32 looks after the warp's i-th pair: it knows where the pair lies (null: no page) and
+    // issues its copy. A page of 16 tokens holds one tile of the pair only.
     const bool two = a.page_shift == 4;
-    auto fetch_pages = [&](int i0, int& pg, int& pg2) {
-        pg = pg2 = -1;
-        if (i0 + lane < mine) {
-            const int tile = 2 * (p_begin + (i0 + lane) * WARPS);
-            pg = pg2 = kv4_page(a, b, tile);
-            if (two) pg2 = kv4_page(a, b, tile + 1);
-        }
-    };
     unsigned char* ring = sm + warp * S * 2 * TB;
-    auto issue = [&](int i, int pg, int pg2) {   // lane 0; a pair of no page completes its phase at once
+    struct Where {
+        const uint8_t *t0, *t1;   // the pair's tiles
+        uint32_t ok0, ok1;        // of the 32 pairs: which tiles are there
+    };
+    auto locate = [&](int i0) {   // pairs i0 .. i0 + 31
+        Where w;
+        const int tile = 2 * (p_begin + (i0 + lane) * WARPS);
+        auto at = [&](int page, int tl) {
+            return page < 0 ? nullptr
+                            : a.pages + ((int64_t)page * a.hkv + h) * a.page_bytes +
+                                  (int64_t)(tl & ((1 << (a.page_shift - 4)) - 1)) * TB;
+        };
+        w.t0 = w.t1 = nullptr;
+        if (i0 + lane < mine) {
+            const int page = kv4_page(a, b, tile);
+            w.t0 = at(page, tile);
+            w.t1 = two ? at(kv4_page(a, b, tile + 1), tile + 1) : page < 0 ? nullptr : w.t0 + TB;
+        }
+        w.ok0 = __ballot_sync(0xffffffffu, w.t0 != nullptr);
+        w.ok1 = __ballot_sync(0xffffffffu, w.t1 != nullptr);
+        return w;
+    };
+    auto issue = [&](int i, const Where& w) {   // one lane; a pair of no page completes its phase at once
         uint64_t* bar = &bars[warp][i % S];
         unsigned char* dst = ring + (i % S) * 2 * TB;
-        const int tile = 2 * (p_begin + i * WARPS) & ((1 << (a.page_shift - 4)) - 1);
-        if (!two) {
-            if (pg < 0) {
-                mbar_arrive(bar);
-                return;
-            }
+        if (w.t0 == nullptr && w.t1 == nullptr) {
+            mbar_arrive(bar);
+        } else if (!two) {
             mbar_arrive_expect_tx(bar, 2 * TB);
-            tma_load_1d(dst, a.pages + ((int64_t)pg * a.hkv + h) * a.page_bytes + tile * TB, 2 * TB, bar);
+            tma_load_1d(dst, w.t0, 2 * TB, bar);
         } else {
-            const uint32_t bytes = (pg >= 0 ? TB : 0) + (pg2 >= 0 ? TB : 0);
-            if (bytes == 0) {
-                mbar_arrive(bar);
-                return;
-            }
-            mbar_arrive_expect_tx(bar, bytes);
-            if (pg >= 0) tma_load_1d(dst, a.pages + ((int64_t)pg * a.hkv + h) * a.page_bytes, TB, bar);
-            if (pg2 >= 0) tma_load_1d(dst + TB, a.pages + ((int64_t)pg2 * a.hkv + h) * a.page_bytes, TB, bar);
+            mbar_arrive_expect_tx(bar, (w.t0 ? TB : 0) + (w.t1 ? TB : 0));
+            if (w.t0) tma_load_1d(dst, w.t0, TB, bar);
+            if (w.t1) tma_load_1d(dst + TB, w.t1, TB, bar);
         }
     };
-    int pg, pg2, next, next2;   // of the 32 pairs that hold the current one, and the next one to issue
-    fetch_pages(0, pg, pg2);
-    next = pg;
-    next2 = pg2;
-    for (int i = 0; i < min(S, mine); ++i) {
-        const int p = __shfl_sync(0xffffffffu, pg, i), p2 = __shfl_sync(0xffffffffu, pg2, i);
-        if (lane == 0) issue(i, p, p2);
-    }
+    Where here = locate(0), next = here;   // of the 32 pairs that hold the current one, the next one to issue
+    if (lane < min(S, mine)) issue(lane, here);
 
     // queries: B operand of step j (dims 16 j ..): unit n = lane / 4, dims 2t, 2t + 1 and 8 further
     uint32_t qf[NT][2 * MT];
@@ -582,11 +581,8 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
 
     for (int i = 0; i < mine; ++i) {
         const int st = i % S;
-        if (i > 0 && (i & 31) == 0) {
-            pg = next;
-            pg2 = next2;
-        }
-        const bool ok0 = __shfl_sync(0xffffffffu, pg, i & 31) >= 0, ok1 = __shfl_sync(0xffffffffu, pg2, i & 31) >= 0;
+        if (i > 0 && (i & 31) == 0) here = next;
+        const bool ok0 = here.ok0 >> (i & 31) & 1, ok1 = here.ok1 >> (i & 31) & 1;
         if (!mbar_wait(&bars[warp][st], (i / S) & 1)) {
             failed = i;
             break;
@@ -600,11 +596,8 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
         __syncwarp();   // every lane has read the stage
         const int nx = i + S;
         if (nx < mine) {
-            if ((nx & 31) == 0) fetch_pages(nx, next, next2);
-            const bool same = (nx >> 5) == (i >> 5);
-            const int p = __shfl_sync(0xffffffffu, same ? pg : next, nx & 31);
-            const int p2 = __shfl_sync(0xffffffffu, same ? pg2 : next2, nx & 31);
-            if (lane == 0) issue(nx, p, p2);
+            if ((nx & 31) == 0) next = locate(nx);
+            if (lane == (nx & 31)) issue(nx, (nx >> 5) == (i >> 5) ? here : next);
         }
     }
     if (failed >= 0)   // let the copies in flight land (bounded again) and answer NaN
