@@ -22,7 +22,8 @@
 // Keys that a unit does not see get weight 0 by selection, not by multiplication: pages past a
 // sequence's end may hold anything, NaN included. Tiles of a page outside the cache are skipped.
 //
-// Splits write (m, l, O) partials; k_kv4_merge joins them in split order.
+// Splits of the keys end in (m, l, O) partials, joined in split order: up to eight splits that fit the
+// GPU at once are a cluster and read each other's shared memory, else k_kv4_merge follows.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -90,6 +91,18 @@ __device__ __forceinline__ uint32_t pack(float a, float b) {
 __device__ __forceinline__ float lo_of(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float hi_of(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
 
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// *p of the cluster's CTA `rank`.
+__device__ __forceinline__ float ld_cluster(const float* p, int rank) {
+    uint32_t at;
+    float v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+
 // A stage holds two tiles (32 tokens): 10 KB in flight a warp.
 template <int HD>
 constexpr int stages() { return HD == 64 ? 4 : 2; }
@@ -112,11 +125,12 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the merge may be set up meanwhile
     Kv4Range rg;
-    if (!kv4_range(a, b, u0, UT, 32, rg) || split >= rg.used) return;
+    if (!kv4_range(a, b, u0, UT, 32, rg) || (split >= rg.used && !a.cluster)) return;   // (the same for a cluster)
     const int row0 = rg.row0, units = rg.units, ulast = rg.ulast;
     // steps are pairs of tiles (32 tokens, aligned): the split's range, of which the warp takes every WARPS-th
     int s_begin, s_end;
     kv4_split(a, rg, split, s_begin, s_end);
+    if (split >= rg.used) s_begin = s_end = 0;
     const int p_begin = rg.step0 + s_begin + warp, p_end = rg.step0 + s_end;
     const int mine = p_end > p_begin ? (p_end - p_begin + WARPS - 1) / WARPS : 0;
 
@@ -645,7 +659,13 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
         }
     __syncthreads();
     const float* all = reinterpret_cast<const float*>(sm);
-    for (int i = tid; i < (ulast - u0 + 1) * HD; i += WARPS * 32) {
+    float* mine_o = reinterpret_cast<float*>(sm) + WARPS * UT * (HD + 2);   // cluster: the CTA's own, for the others
+    const int items = (ulast - u0 + 1) * HD;
+    auto place = [&](int u) {
+        const int j = kv4_row(a, u0 + u), g = (u0 + u) - j * a.group;
+        return (int64_t)(row0 + j) * a.hq + h * a.group + g;
+    };
+    for (int i = tid; i < items; i += WARPS * 32) {
         const int u = i / HD, d = i % HD;
         float mm = NEG, ll = 0.f, oo = 0.f;
 #pragma unroll
@@ -657,8 +677,16 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
             ll = fmaf(f, p[HD + 1], ll);
             oo = fmaf(f, p[d], oo);
         }
-        const int j = kv4_row(a, u0 + u), g = (u0 + u) - j * a.group;
-        const int64_t at = (int64_t)(row0 + j) * a.hq + h * a.group + g;
+        if (a.cluster) {
+            float* p = mine_o + u * (HD + 2);
+            p[d] = oo;
+            if (d == 0) {
+                p[HD] = mm;
+                p[HD + 1] = ll;
+            }
+            continue;
+        }
+        const int64_t at = place(u);
         if (rg.used == 1) {
             a.out[at * HD + d] = __float2bfloat16(ll == 0.f ? 0.f : oo / ll);
         } else {
@@ -669,6 +697,22 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
             }
         }
     }
+    if (!a.cluster) return;
+    // the splits are a cluster: each CTA joins a part of the dims from all of their shared memories
+    cluster_sync();
+    for (int i = split * WARPS * 32 + tid; i < items; i += a.nsplit * WARPS * 32) {
+        const int u = i / HD, d = i % HD;
+        const float* p = mine_o + u * (HD + 2);
+        float mm = NEG, ll = 0.f, oo = 0.f;
+        for (int sp = 0; sp < a.nsplit; ++sp) mm = fmaxf(mm, ld_cluster(p + HD, sp));
+        for (int sp = 0; sp < a.nsplit; ++sp) {
+            const float f = kv4_ex2(ld_cluster(p + HD, sp) - mm);
+            ll = fmaf(f, ld_cluster(p + HD + 1, sp), ll);
+            oo = fmaf(f, ld_cluster(p + d, sp), oo);
+        }
+        a.out[place(u) * HD + d] = __float2bfloat16(ll == 0.f ? 0.f : oo / ll);
+    }
+    cluster_sync();   // nobody leaves while its shared memory is read
 }
 
 // out of one (sequence row, head) from its splits' partials (where there is more than one): 128
@@ -739,7 +783,7 @@ __global__ void __launch_bounds__(128) k_kv4_merge(const Kv4AttnArgs a) {
 
 struct Plan {
     bool many;   // k_kv4_prefill
-    int nt, dup, warps, unit_tile, utiles, step, nsplit, split_len;
+    int nt, dup, warps, unit_tile, utiles, step, nsplit, split_len, cluster;
 };
 
 // How a call is cut. More than MANY units of a sequence's rows go to k_kv4_prefill, 512 or 256 a CTA.
@@ -799,18 +843,33 @@ Plan make_plan(int64_t B, int64_t Hkv, int64_t group, int64_t head_dim, int64_t 
     if (p.split_len < 1) p.split_len = 1;
     p.nsplit = (int)((steps + p.split_len - 1) / p.split_len);
     if (p.nsplit < 1) p.nsplit = 1;
+    p.cluster = !p.many && p.nsplit > 1 && p.nsplit <= 8 && ctas * p.nsplit <= 148 * (p.nt == 1 ? 4 : 2);
     return p;
 }
 
 template <int HD, int NT, bool DUP, int WARPS>
 int launch(const Kv4AttnArgs& a, const Plan& p, int64_t B, cudaStream_t st) {
-    constexpr int ring = WARPS * stages<HD>() * 2 * Kv4Tile<HD>::BYTES, merge = WARPS * (DUP ? 4 : 8 * NT) * (HD + 2) * 4;
+    constexpr int ring = WARPS * stages<HD>() * 2 * Kv4Tile<HD>::BYTES, merge = (WARPS + 1) * (DUP ? 4 : 8 * NT) * (HD + 2) * 4;
     constexpr int bytes = ring > merge ? ring : merge;
     PULSAR_TRY(ensure_smem_attr((const void*)k_kv4_attn<HD, NT, DUP, WARPS>, bytes, "k_kv4_attn shared memory"));
     const dim3 grid((unsigned)(p.utiles * p.nsplit), (unsigned)a.hkv, (unsigned)B);
-    k_kv4_attn<HD, NT, DUP, WARPS><<<grid, WARPS * 32, bytes, st>>>(a);
-    PULSAR_LAUNCH_CHECK("k_kv4_attn");
-    return PULSAR_OK;
+    if (!p.cluster) {
+        k_kv4_attn<HD, NT, DUP, WARPS><<<grid, WARPS * 32, bytes, st>>>(a);
+        PULSAR_LAUNCH_CHECK("k_kv4_attn");
+        return PULSAR_OK;
+    }
+    cudaLaunchAttribute splits{};
+    splits.id = cudaLaunchAttributeClusterDimension;
+    splits.val.clusterDim.x = (unsigned)p.nsplit;
+    splits.val.clusterDim.y = splits.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(WARPS * 32);
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = st;
+    cfg.attrs = &splits;
+    cfg.numAttrs = 1;
+    return cuda_status(cudaLaunchKernelEx(&cfg, k_kv4_attn<HD, NT, DUP, WARPS>, a), "k_kv4_attn");
 }
 
 // The merge is launched under the attention kernel's end; it waits for that before it reads. Up to
@@ -853,7 +912,7 @@ extern "C" int pulsar_op_kv4_attention_workspace(int64_t N, int64_t Hq, int64_t 
     PULSAR_CHECK_ARG(bytes, "kv4_attention_workspace: null pointer");
     PULSAR_TRY(check_shape(N, Hq, Hkv, head_dim, B, max_q, max_kv, window));
     const Plan p = make_plan(B > 0 ? B : 1, Hkv, Hq / Hkv, head_dim, max_q, max_kv, window);
-    *bytes = p.nsplit > 1 ? N * Hq * p.nsplit * (head_dim + 2) * 4 : 0;
+    *bytes = p.nsplit > 1 && !p.cluster ? N * Hq * p.nsplit * (head_dim + 2) * 4 : 0;
     return PULSAR_OK;
 }
 
@@ -878,16 +937,16 @@ extern "C" int pulsar_op_kv4_attention(const void* q, int64_t q_row_stride, int6
                        reinterpret_cast<uintptr_t>(workspace)) & 15) == 0,
                      "kv4_attention: pages, out and the workspace must be 16-byte aligned");
     const Plan p = make_plan(B, Hkv, Hq / Hkv, head_dim, max_q, max_kv, window);
-    const int64_t need = p.nsplit > 1 ? N * Hq * p.nsplit * (head_dim + 2) * 4 : 0;
+    const int64_t need = p.nsplit > 1 && !p.cluster ? N * Hq * p.nsplit * (head_dim + 2) * 4 : 0;
     PULSAR_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need),
                      "kv4_attention: workspace of %lld bytes needed, got %lld", (long long)need,
                      (long long)workspace_bytes);
     float* ws = (float*)workspace;
     Kv4AttnArgs a{(const __nv_bfloat16*)q, (const uint8_t*)pages, block_table, kv_lens, cu_q, (__nv_bfloat16*)out, ws,
-               p.nsplit > 1 ? ws + N * Hq * p.nsplit * head_dim : nullptr, q_row_stride, q_head_stride,
+               need > 0 ? ws + N * Hq * p.nsplit * head_dim : nullptr, q_row_stride, q_head_stride,
                page_size / KV4_TILE * 20 * head_dim, (int)N, (int)Hq, (int)Hkv, (int)(Hq / Hkv), (int)num_pages,
                (int)width, __builtin_ctzll((unsigned long long)page_size), (int)max_q, (int)window, p.nsplit,
-               p.split_len, p.unit_tile, p.step, scale * 1.4426950408889634f};
+               p.split_len, p.unit_tile, p.step, p.cluster, scale * 1.4426950408889634f};
     cudaStream_t st = (cudaStream_t)stream;
     int rc;
     if (p.many)
@@ -904,6 +963,6 @@ extern "C" int pulsar_op_kv4_attention(const void* q, int64_t q_row_stride, int6
         rc = p.dup ? launch<128, 1, true, 4>(a, p, B, st) : p.nt == 1 ? launch<128, 1, false, 4>(a, p, B, st)
            : launch<128, 2, false, 4>(a, p, B, st);
     PULSAR_TRY(rc);
-    if (p.nsplit > 1) return head_dim == 64 ? launch_merge<64>(a, B, st) : launch_merge<128>(a, B, st);
+    if (need > 0) return head_dim == 64 ? launch_merge<64>(a, B, st) : launch_merge<128>(a, B, st);
     return PULSAR_OK;
 }

@@ -22,7 +22,7 @@ struct Kv4AttnArgs {
     // exponent m (base 2) and the sum l of the weights relative to it
     float *part_o, *part_ml;
     int64_t q_row, q_head, page_bytes;
-    int rows, hq, hkv, group, num_pages, width, page_shift, max_q, window, nsplit, split_len, unit_tile, step;
+    int rows, hq, hkv, group, num_pages, width, page_shift, max_q, window, nsplit, split_len, unit_tile, step, cluster;
     float scale_log2;
 };
 
