@@ -43,26 +43,45 @@ __device__ __forceinline__ float lanes_sum(float v) {
     return v;
 }
 
-// x / s, correctly rounded, for s with 1 / s = inv correctly rounded: one step of Markstein's division
-// (IBM J. Res. Dev. 34, 1990). s has a bf16 significand, which is none of the method's exceptions.
-__device__ __forceinline__ float divide(float x, float s, float inv) {
-    const float q = __fmul_rn(x, inv);
-    return __fmaf_rn(__fmaf_rn(-q, s, x), inv, q);
-}
-
 constexpr float WHOLE = 12582912.f;   // 1.5 2^23: adding it rounds to a whole number, ties to even
 
-// Codes, s and z of the group of 32 dims whose 8-dim quarter this lane holds (x: its values).
-// Returns the lane's 8 codes, nibble j = dim j.
-__device__ __forceinline__ uint32_t quantise(const float* x, uint32_t& param) {
-    float mn = x[0], mx = x[0], bad = __fmul_rn(x[0], 0.f);
+// A lane's 8 dims, two to a register pair: every packed operation rounds each half on its own.
+struct Dims {
+    f32x2 v[4];
+    __device__ __forceinline__ void load(const void* p) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int j = 1; j < 8; ++j) {
-        mn = fminf(mn, x[j]);
-        mx = fmaxf(mx, x[j]);
-        bad = __fmaf_rn(x[j], 0.f, bad);   // NaN once a value is none or infinite
+        for (int i = 0; i < 4; ++i) v[i] = two(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
     }
-    if (!(bad == 0.f)) mx = INFINITY;
+    __device__ __forceinline__ uint4 bf16() const {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float x, y;
+            parts(v[i], x, y);
+            const __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
+            w[i] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+};
+
+// Codes, s and z of the group of 32 dims whose 8-dim quarter this lane holds. Returns the lane's 8
+// codes, nibble j = dim j.
+__device__ __forceinline__ uint32_t quantise(const Dims& x, uint32_t& param) {
+    float lo[8];
+    f32x2 bad2 = two(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        parts(x.v[i], lo[2 * i], lo[2 * i + 1]);
+        bad2 = fma2(x.v[i], two(0.f, 0.f), bad2);   // NaN once a value is none or infinite
+    }
+    float mn = fminf(fminf(fminf(lo[0], lo[1]), fminf(lo[2], lo[3])), fminf(fminf(lo[4], lo[5]), fminf(lo[6], lo[7])));
+    float mx = fmaxf(fmaxf(fmaxf(lo[0], lo[1]), fmaxf(lo[2], lo[3])), fmaxf(fmaxf(lo[4], lo[5]), fmaxf(lo[6], lo[7])));
+    float b0, b1;
+    parts(bad2, b0, b1);
+    if (!(b0 + b1 == 0.f)) mx = INFINITY;
 #pragma unroll
     for (int o = 1; o < 4; o <<= 1) {
         mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
@@ -81,11 +100,19 @@ __device__ __forceinline__ uint32_t quantise(const float* x, uint32_t& param) {
         return 0u;
     }
     param = (uint32_t)__bfloat16_as_ushort(zb) << 16 | __bfloat16_as_ushort(sb);
+    // (x - z) / s, correctly rounded: the reciprocal and one step of Markstein's division (IBM J. Res.
+    // Dev. 34, 1990; s has a bf16 significand, which is none of the method's exceptions). At most
+    // 15 (1 + 2^-8) since s is rounded, so no code passes 15; z is rounded too and may lie above x.
     const float inv = __frcp_rn(s);
+    const f32x2 z2 = two(-z, -z), s2 = two(-s, -s), i2 = two(inv, inv);
     float c[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-        c[j] = __fsub_rn(__fadd_rn(fminf(fmaxf(divide(__fsub_rn(x[j], z), s, inv), 0.f), 15.f), WHOLE), WHOLE);
+    for (int i = 0; i < 4; ++i) {
+        const f32x2 d = add2(x.v[i], z2), q = mul2(d, i2), r = fma2(q, s2, d);
+        float u, v;
+        parts(fma2(r, i2, q), u, v);
+        parts(add2(add2(two(fmaxf(u, 0.f), fmaxf(v, 0.f)), two(WHOLE, WHOLE)), two(-WHOLE, -WHOLE)), c[2 * i], c[2 * i + 1]);
+    }
     // four codes at a time as the digits of one whole number
     uint32_t p[2];
 #pragma unroll
@@ -108,46 +135,47 @@ __device__ __forceinline__ uint32_t quad_word(uint32_t p, int lane) {
     return __byte_perm(e0 | e0 >> 4, e1 | e1 >> 4, 0x6420);
 }
 
-__device__ __forceinline__ void load4(const float* p, float* x) {
+__device__ __forceinline__ void load4(const float* p, f32x2* x) {
     const float4 v = __ldg(reinterpret_cast<const float4*>(p));
-    x[0] = v.x;
-    x[1] = v.y;
-    x[2] = v.z;
-    x[3] = v.w;
+    x[0] = two(v.x, v.y);
+    x[1] = two(v.z, v.w);
 }
 
 // x: the 8 dims (8 l ..) of a head vector that this lane holds, normed (weights w, or none) and
 // turned. Every lane of the warp takes part.
 template <int HD>
-__device__ __forceinline__ void norm_rotate(const AppendArgs& a, const float* w, int pos, bool pos_ok, int lane,
-                                            float* x) {
+__device__ __forceinline__ void norm_rotate(const AppendArgs& a, const float* w, int pos, bool pos_ok, int lane, Dims& x) {
     constexpr int L = HD / 8;
     const int l = lane % L;
     if (w) {
-        float t[8];
+        float t[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) t[j] = __fmul_rn(x[j], x[j]);
-        float ss = __fadd_rn(__fadd_rn(__fadd_rn(t[0], t[1]), __fadd_rn(t[2], t[3])),
-                             __fadd_rn(__fadd_rn(t[4], t[5]), __fadd_rn(t[6], t[7])));
-        ss = lanes_sum<L>(ss);
+        for (int i = 0; i < 4; ++i) {
+            float u, v;
+            parts(mul2(x.v[i], x.v[i]), u, v);
+            t[i] = __fadd_rn(u, v);
+        }
+        const float ss = lanes_sum<L>(__fadd_rn(__fadd_rn(t[0], t[1]), __fadd_rn(t[2], t[3])));
         const float inv = __frcp_rn(__fsqrt_rn(__fadd_rn(__fmul_rn(ss, 1.f / HD), a.eps)));
-        float wv[8];
+        f32x2 wv[4];
         load4(w + 8 * l, wv);
-        load4(w + 8 * l + 4, wv + 4);
+        load4(w + 8 * l + 4, wv + 2);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = __fmul_rn(wv[j], __fmul_rn(x[j], inv));
+        for (int i = 0; i < 4; ++i) x.v[i] = mul2(wv[i], mul2(x.v[i], two(inv, inv)));
     }
     if (a.rot == 0) return;
     const int half = a.rot >> 1;
     const int64_t row = (int64_t)(pos_ok ? pos : 0) * half;
     const float *cs = a.cs + row, *sn = a.sn + row;
     const bool turn = 8 * l < a.rot;
-    float c[8], s[8];
     if (a.interleaved) {
         if (!turn) return;
+        float c[4], s[4];
         if ((a.rot & 7) == 0) {   // rows of the tables are multiples of 16 bytes
-            load4(cs + 4 * l, c);
-            load4(sn + 4 * l, s);
+            const float4 c4 = __ldg(reinterpret_cast<const float4*>(cs + 4 * l));
+            const float4 s4 = __ldg(reinterpret_cast<const float4*>(sn + 4 * l));
+            c[0] = c4.x; c[1] = c4.y; c[2] = c4.z; c[3] = c4.w;
+            s[0] = s4.x; s[1] = s4.y; s[2] = s4.z; s[3] = s4.w;
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
@@ -158,29 +186,29 @@ __device__ __forceinline__ void norm_rotate(const AppendArgs& a, const float* w,
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            if (8 * l + 2 * j < a.rot) {
-                const float u = x[2 * j], v = x[2 * j + 1];
-                x[2 * j] = __fsub_rn(__fmul_rn(u, c[j]), __fmul_rn(v, s[j]));
-                x[2 * j + 1] = __fadd_rn(__fmul_rn(v, c[j]), __fmul_rn(u, s[j]));
+            if (8 * l + 2 * j < a.rot) {   // (u c - v s, v c + u s)
+                float u, v;
+                parts(x.v[j], u, v);
+                x.v[j] = add2(mul2(x.v[j], two(c[j], c[j])), mul2(two(v, u), two(-s[j], s[j])));
             }
         }
     } else {   // rot % 16 == 0: the partner's dims are the same 8 of another lane, rows multiples of 32 bytes
         const int hl = half >> 3;
         const bool first = l < hl;
         const int from = (lane - l) + (turn ? (first ? l + hl : l - hl) : l);
-        float o[8];
+        f32x2 o[4];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) o[j] = __shfl_sync(0xffffffffu, x[j], from);
+        for (int i = 0; i < 4; ++i) o[i] = __shfl_sync(0xffffffffu, x.v[i], from);
         if (turn) {
             const int b = 8 * (first ? l : l - hl);
+            f32x2 c[4], s[4];
             load4(cs + b, c);
-            load4(cs + b + 4, c + 4);
+            load4(cs + b + 4, c + 2);
             load4(sn + b, s);
-            load4(sn + b + 4, s + 4);
+            load4(sn + b + 4, s + 2);
+            const float sign = first ? -1.f : 1.f;   // x c - o s, or x c + o s
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                x[j] = first ? __fsub_rn(__fmul_rn(x[j], c[j]), __fmul_rn(o[j], s[j]))
-                             : __fadd_rn(__fmul_rn(x[j], c[j]), __fmul_rn(o[j], s[j]));
+            for (int i = 0; i < 4; ++i) x.v[i] = add2(mul2(x.v[i], c[i]), mul2(o[i], mul2(s[i], two(sign, sign))));
         }
     }
 }
@@ -195,24 +223,23 @@ __device__ __forceinline__ void append_queries(const AppendArgs& a, uint32_t vb,
     const uint32_t tk = live ? vi / (uint32_t)a.hq : 0u;
     const int64_t tok = tk;
     const int h = live ? (int)(vi - tk * a.hq) : 0;
-    float x[8];
-    bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(a.q + tok * a.qs + h * a.qh) + l), x);
+    Dims x;
+    x.load(a.q + tok * a.qs + h * a.qh + 8 * l);
     const int pos = a.pos ? a.pos[tok] : 0;
     const bool ok = !a.pos || (pos >= 0 && pos < a.max_pos);
     norm_rotate<HD>(a, a.qw ? a.qw + h * HD : nullptr, pos, ok, lane, x);
     if (a.gain) {
         const float g = ok ? a.gain[pos] : 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = __fmul_rn(x[j], g);
+        for (int i = 0; i < 4; ++i) x.v[i] = mul2(x.v[i], two(g, g));
     }
-    if (live)
-        reinterpret_cast<uint4*>(a.qo + (tok * a.hq + h) * HD)[l] = ok ? f32_to_bf16x8(x) : make_uint4(0, 0, 0, 0);
+    if (live) reinterpret_cast<uint4*>(a.qo + (tok * a.hq + h) * HD)[l] = ok ? x.bf16() : make_uint4(0, 0, 0, 0);
 }
 
 // One (token, kv head) vector for each group of HD / 8 lanes: its codes and parameters, to those of
 // the token's tile (in global or shared memory); t: the token's place in the tile.
 template <int HD>
-__device__ __forceinline__ void store_vector(const float* x, bool is_k, int t, bool put, uint8_t* codes, uint8_t* params,
+__device__ __forceinline__ void store_vector(const Dims& x, bool is_k, int t, bool put, uint8_t* codes, uint8_t* params,
                                              int lane) {
     using T = Kv4Tile<HD>;
     const int l = lane % (HD / 8), r = t & 7, hf = t >> 3, g = l >> 2, j = l & 3;
@@ -238,11 +265,11 @@ __device__ __forceinline__ int64_t tile_at(int64_t slot, int h, int hkv, int pag
 
 // A head vector of k or v, normed and turned for keys; put: whether it is stored, at slot.
 template <int HD>
-__device__ __forceinline__ bool load_kv(const AppendArgs& a, bool is_k, int64_t tok, int h, int lane, float* x,
+__device__ __forceinline__ bool load_kv(const AppendArgs& a, bool is_k, int64_t tok, int h, int lane, Dims& x,
                                         int64_t& slot) {
     const int l = lane % (HD / 8);
     const __nv_bfloat16* src = is_k ? a.k + tok * a.ks + h * a.kh : a.v + tok * a.vs + h * a.vh;
-    bf16x8_to_f32(__ldg(reinterpret_cast<const uint4*>(src) + l), x);
+    x.load(src + 8 * l);
     const int pos = a.pos ? a.pos[tok] : 0;
     const bool ok = !a.pos || (pos >= 0 && pos < a.max_pos);
     slot = a.slots[tok];
@@ -267,7 +294,7 @@ __global__ void __launch_bounds__(128) k_kv4_append(const AppendArgs a) {
         const bool live = vi < a.n * (uint32_t)a.hkv;
         const uint32_t tok = live ? vi / (uint32_t)a.hkv : 0u;
         const int h = live ? (int)(vi - tok * a.hkv) : 0;
-        float x[8];
+        Dims x;
         int64_t slot;
         const bool put = load_kv<HD>(a, is_k, tok, h, lane, x, slot) && live;
         uint8_t* tile = a.pages + (put ? tile_at<HD>(slot, h, a.hkv, a.page_shift, a.page_bytes) : 0);
@@ -316,7 +343,7 @@ __global__ void __launch_bounds__(BULK_WARPS * 32) k_kv4_append_bulk(const Appen
         for (int i = 0; i < 16; i += VW) {
             const int64_t tk = tok0 + i + lane / L;
             const bool live = tk >= 0 && tk < a.n;
-            float x[8];
+            Dims x;
             int64_t slot;
             const bool put = load_kv<HD>(a, is_k, live ? tk : 0, h, lane, x, slot) && live;
             uint8_t *codes = images[warp], *params = images[warp] + 8 * HD;

@@ -344,6 +344,14 @@ def test_decode_splits(paged, d, window, max_kv):
     _attend(paged, lens, [3, 1, 2, 1, 0], 4, 1, d, 64, window=window, max_kv=max_kv)
 
 
+@pytest.mark.parametrize("hq,hkv,d,rows,window", [(4, 1, 64, 1, 0), (16, 4, 64, 1, 700), (8, 1, 128, 1, 0), (4, 1, 64, 3, 0),
+                                                  (4, 2, 128, 5, 600)])
+def test_decode_few_splits(paged, hq, hkv, d, rows, window):
+    """Few enough splits to be joined inside one launch; sequences that need fewer of them, or none."""
+    for lens in ([1300], [1290, 3, 700], [0, 1100]):
+        _attend(paged, lens, [rows] * len(lens), hq, hkv, d, 32, window=window, one=rows == 1)
+
+
 def test_peaked_and_flat_scores(paged):
     _attend(paged, [700, 1500], [1, 1], 4, 1, 64, 64, scale=6.0, one=True)
     _attend(paged, [700, 1500], [1, 1], 4, 1, 64, 64, scale=1e-4, one=True)
