@@ -48,8 +48,7 @@ constexpr float WHOLE = 12582912.f;   // 1.5 2^23: adding it rounds to a whole n
 // A lane's 8 dims, two to a register pair: every packed operation rounds each half on its own.
 struct Dims {
     f32x2 v[4];
-    __device__ __forceinline__ void load(const void* p) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(p));
+    __device__ __forceinline__ void take(const uint4& u) {
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = two(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
@@ -189,7 +188,7 @@ __device__ __forceinline__ void norm_rotate(const AppendArgs& a, const float* w,
             if (8 * l + 2 * j < a.rot) {   // (u c - v s, v c + u s)
                 float u, v;
                 parts(x.v[j], u, v);
-                x.v[j] = add2(mul2(x.v[j], two(c[j], c[j])), mul2(two(v, u), two(-s[j], s[j])));
+                x.v[j] = two(__fsub_rn(__fmul_rn(u, c[j]), __fmul_rn(v, s[j])), __fadd_rn(__fmul_rn(v, c[j]), __fmul_rn(u, s[j])));
             }
         }
     } else {   // rot % 16 == 0: the partner's dims are the same 8 of another lane, rows multiples of 32 bytes
@@ -208,32 +207,50 @@ __device__ __forceinline__ void norm_rotate(const AppendArgs& a, const float* w,
             load4(sn + b + 4, s + 2);
             const float sign = first ? -1.f : 1.f;   // x c - o s, or x c + o s
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x.v[i] = add2(mul2(x.v[i], c[i]), mul2(o[i], mul2(s[i], two(sign, sign))));
+            for (int i = 0; i < 4; ++i) {   // (the products in pairs; the sums not, which would be contracted with them)
+                float u0, u1, v0, v1;
+                parts(mul2(x.v[i], c[i]), u0, u1);
+                parts(mul2(o[i], mul2(s[i], two(sign, sign))), v0, v1);
+                x.v[i] = two(__fadd_rn(u0, v0), __fadd_rn(u1, v1));
+            }
         }
     }
 }
 
-// The warp's 256 / HD query vectors from vb on (of the call's n hq).
-template <int HD>
+// N times the warp's 256 / HD query vectors from vb on (of the call's n hq). What they need from
+// memory is asked for before any of it is used.
+template <int HD, int N>
 __device__ __forceinline__ void append_queries(const AppendArgs& a, uint32_t vb, int lane) {
-    constexpr int L = HD / 8;
+    constexpr int L = HD / 8, VW = 256 / HD;
     const int l = lane % L;
-    const uint32_t vi = vb + lane / L;
-    const bool live = vi < a.n * (uint32_t)a.hq;
-    const uint32_t tk = live ? vi / (uint32_t)a.hq : 0u;
-    const int64_t tok = tk;
-    const int h = live ? (int)(vi - tk * a.hq) : 0;
-    Dims x;
-    x.load(a.q + tok * a.qs + h * a.qh + 8 * l);
-    const int pos = a.pos ? a.pos[tok] : 0;
-    const bool ok = !a.pos || (pos >= 0 && pos < a.max_pos);
-    norm_rotate<HD>(a, a.qw ? a.qw + h * HD : nullptr, pos, ok, lane, x);
-    if (a.gain) {
-        const float g = ok ? a.gain[pos] : 0.f;
+    uint4 raw[N];
+    int pos[N], head[N];
+    const uint32_t first = vb + lane / L;
+    int64_t tok = first / (uint32_t)a.hq;
+    int h = (int)(first - (uint32_t)tok * a.hq);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x.v[i] = mul2(x.v[i], two(g, g));
+    for (int i = 0; i < N; ++i) {
+        if (tok >= a.n) tok = 0;   // past the last vector: any valid one, not stored
+        head[i] = h;
+        raw[i] = __ldg(reinterpret_cast<const uint4*>(a.q + tok * a.qs + h * a.qh) + l);
+        pos[i] = a.pos ? a.pos[tok] : 0;
+        for (h += VW; h >= a.hq; h -= a.hq) ++tok;
     }
-    if (live) reinterpret_cast<uint4*>(a.qo + (tok * a.hq + h) * HD)[l] = ok ? x.bf16() : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const uint32_t vi = first + i * VW;
+        Dims x;
+        x.take(raw[i]);
+        const bool ok = !a.pos || (pos[i] >= 0 && pos[i] < a.max_pos);
+        norm_rotate<HD>(a, a.qw ? a.qw + head[i] * HD : nullptr, pos[i], ok, lane, x);
+        if (a.gain) {
+            const float g = ok ? a.gain[pos[i]] : 0.f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x.v[j] = mul2(x.v[j], two(g, g));
+        }
+        if (vi < a.n * (uint32_t)a.hq)
+            reinterpret_cast<uint4*>(a.qo)[(int64_t)vi * L + l] = ok ? x.bf16() : make_uint4(0, 0, 0, 0);
+    }
 }
 
 // One (token, kv head) vector for each group of HD / 8 lanes: its codes and parameters, to those of
@@ -263,18 +280,11 @@ __device__ __forceinline__ int64_t tile_at(int64_t slot, int h, int hkv, int pag
            (int64_t)((slot & ((1 << page_shift) - 1)) >> 4) * Kv4Tile<HD>::BYTES;
 }
 
-// A head vector of k or v, normed and turned for keys; put: whether it is stored, at slot.
+// Where the lane's 8 dims of a head vector of k or v are.
 template <int HD>
-__device__ __forceinline__ bool load_kv(const AppendArgs& a, bool is_k, int64_t tok, int h, int lane, Dims& x,
-                                        int64_t& slot) {
-    const int l = lane % (HD / 8);
-    const __nv_bfloat16* src = is_k ? a.k + tok * a.ks + h * a.kh : a.v + tok * a.vs + h * a.vh;
-    x.load(src + 8 * l);
-    const int pos = a.pos ? a.pos[tok] : 0;
-    const bool ok = !a.pos || (pos >= 0 && pos < a.max_pos);
-    slot = a.slots[tok];
-    if (is_k) norm_rotate<HD>(a, a.kw ? a.kw + h * HD : nullptr, pos, ok, lane, x);
-    return ok && slot >= 0 && slot < a.num_slots;
+__device__ __forceinline__ const uint4* kv_source(const AppendArgs& a, bool is_k, int64_t tok, int h, int lane) {
+    return reinterpret_cast<const uint4*>(is_k ? a.k + tok * a.ks + h * a.kh : a.v + tok * a.vs + h * a.vh) +
+           lane % (HD / 8);
 }
 
 // Few tokens: a warp per 32 / L head vectors of one kind (queries, keys or values), so that no warp
@@ -287,16 +297,20 @@ __global__ void __launch_bounds__(128) k_kv4_append(const AppendArgs a) {
     const uint32_t nq = (a.n * (uint32_t)a.hq + VW - 1) / VW, nk = (a.n * (uint32_t)a.hkv + VW - 1) / VW;
     const uint32_t w = blockIdx.x * 4 + (threadIdx.x >> 5);
     if (w < nq) {
-        append_queries<HD>(a, w * VW, lane);
+        append_queries<HD, 1>(a, w * VW, lane);
     } else if (w < nq + 2 * nk) {
         const bool is_k = w < nq + nk;
         const uint32_t vi = (w - nq - (is_k ? 0 : nk)) * VW + lane / (HD / 8);
         const bool live = vi < a.n * (uint32_t)a.hkv;
         const uint32_t tok = live ? vi / (uint32_t)a.hkv : 0u;
         const int h = live ? (int)(vi - tok * a.hkv) : 0;
+        const uint4 raw = __ldg(kv_source<HD>(a, is_k, tok, h, lane));
+        const int pos = a.pos ? a.pos[tok] : 0;
+        const int64_t slot = a.slots[tok];
+        const bool ok = !a.pos || (pos >= 0 && pos < a.max_pos), put = live && ok && slot >= 0 && slot < a.num_slots;
         Dims x;
-        int64_t slot;
-        const bool put = load_kv<HD>(a, is_k, tok, h, lane, x, slot) && live;
+        x.take(raw);
+        if (is_k) norm_rotate<HD>(a, a.kw ? a.kw + h * HD : nullptr, pos, ok, lane, x);
         uint8_t* tile = a.pages + (put ? tile_at<HD>(slot, h, a.hkv, a.page_shift, a.page_bytes) : 0);
         store_vector<HD>(x, is_k, (int)(slot & 15), put, tile + (is_k ? 0 : T::V), tile + (is_k ? T::KP : T::VP), lane);
     }
@@ -308,7 +322,7 @@ __global__ void __launch_bounds__(128) k_kv4_append(const AppendArgs a) {
 // of 16 start so that the first token's page lines up with them. Queries: 16 vectors a warp.
 constexpr int BULK_WARPS = 8;
 template <int HD>
-__global__ void __launch_bounds__(BULK_WARPS * 32) k_kv4_append_bulk(const AppendArgs a) {
+__global__ void __launch_bounds__(BULK_WARPS * 32, 4) k_kv4_append_bulk(const AppendArgs a) {
     using T = Kv4Tile<HD>;
     constexpr int VW = 256 / HD, L = HD / 8;
     __shared__ __align__(16) uint8_t images[BULK_WARPS][10 * HD];
@@ -317,35 +331,49 @@ __global__ void __launch_bounds__(BULK_WARPS * 32) k_kv4_append_bulk(const Appen
     const uint32_t groups = (a.n + lead + 15) / 16, nkv = groups * 2 * a.hkv;
     const uint32_t nq = (a.n * (uint32_t)a.hq + 15) / 16, w = blockIdx.x * BULK_WARPS + warp;
     if (w >= nkv) {
-#pragma unroll 2
-        for (int i = 0; i < 16; i += VW)
-            if (w < nkv + nq && (w - nkv) * 16 + i < a.n * (uint32_t)a.hq) append_queries<HD>(a, (w - nkv) * 16 + i, lane);
+        if (w < nkv + nq)
+#pragma unroll 1
+            for (int i = 0; i < 16; i += 4 * VW) append_queries<HD, 4>(a, (w - nkv) * 16 + i, lane);
     } else {
         const uint32_t grp = w / (2u * a.hkv);
         const int kh = (int)(w - grp * 2 * a.hkv);
         const bool is_k = kh < a.hkv;
         const int h = is_k ? kh : kh - a.hkv;
         const int64_t tok0 = (int64_t)grp * 16 - lead;
-        // a whole tile: 16 tokens in the 16 consecutive slots of one, all of them stored
-        bool fits = true;
-        int64_t s0 = -1;
-        {
-            const int64_t tk = tok0 + (lane & 15);
-            const bool in = tk >= 0 && tk < a.n;
-            const int64_t s = in ? a.slots[tk] : -1;
-            const int pos = in && a.pos ? a.pos[tk] : 0;
-            s0 = __shfl_sync(0xffffffffu, s, 0);
-            fits = in && s == s0 + (lane & 15) && s0 >= 0 && (s0 & 15) == 0 && s < a.num_slots &&
-                   (!a.pos || (pos >= 0 && pos < a.max_pos));
-        }
-        const bool whole = __all_sync(0xffffffffu, fits);
+        constexpr int N = 4;   // vectors of a lane asked for at a time
+        uint4 raw[N];
+        auto ask = [&](int i0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int64_t tk = tok0 + (i0 + i) * VW + lane / L;
+                raw[i] = __ldg(kv_source<HD>(a, is_k, tk >= 0 && tk < a.n ? tk : 0, h, lane));
+            }
+        };
+        ask(0);
+        // lane t % 16 knows token t's slot and position. A whole tile: 16 tokens in the 16 consecutive
+        // slots of one, all of them stored
+        const int64_t mine = tok0 + (lane & 15);
+        const bool in = mine >= 0 && mine < a.n;
+        const int64_t my_slot = in ? a.slots[mine] : -1;
+        const int my_pos = in && a.pos ? a.pos[mine] : 0;
+        const bool my_ok = !a.pos || (my_pos >= 0 && my_pos < a.max_pos);
+        const bool my_put = in && my_ok && my_slot >= 0 && my_slot < a.num_slots;
+        const int64_t s0 = __shfl_sync(0xffffffffu, my_slot, 0);
+        const bool whole = __all_sync(0xffffffffu, my_put && my_slot == s0 + (lane & 15) && (s0 & 15) == 0);
+        const uint32_t puts = __ballot_sync(0xffffffffu, my_put), oks = __ballot_sync(0xffffffffu, my_ok);
         uint8_t* dst = a.pages + (whole ? tile_at<HD>(s0, h, a.hkv, a.page_shift, a.page_bytes) : 0);
-        for (int i = 0; i < 16; i += VW) {
-            const int64_t tk = tok0 + i + lane / L;
-            const bool live = tk >= 0 && tk < a.n;
+#pragma unroll 1
+        for (int i0 = 0; i0 < 16 / VW; i0 += N) {
+          if (i0 > 0) ask(i0);
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const int t = (i0 + i) * VW + lane / L;
+            const int pos = __shfl_sync(0xffffffffu, my_pos, t);
+            const int64_t slot = __shfl_sync(0xffffffffu, my_slot, t);
+            const bool put = puts >> t & 1;
             Dims x;
-            int64_t slot;
-            const bool put = load_kv<HD>(a, is_k, live ? tk : 0, h, lane, x, slot) && live;
+            x.take(raw[i]);
+            if (is_k) norm_rotate<HD>(a, a.kw ? a.kw + h * HD : nullptr, pos, oks >> t & 1, lane, x);
             uint8_t *codes = images[warp], *params = images[warp] + 8 * HD;
             if (!whole) {
                 codes = a.pages + (put ? tile_at<HD>(slot, h, a.hkv, a.page_shift, a.page_bytes) : 0);
@@ -353,6 +381,7 @@ __global__ void __launch_bounds__(BULK_WARPS * 32) k_kv4_append_bulk(const Appen
                 codes += is_k ? 0 : T::V;
             }
             store_vector<HD>(x, is_k, (int)(slot & 15), put, codes, params, lane);
+          }
         }
         if (whole) {
             __syncwarp();

@@ -198,6 +198,45 @@ def test_stored_codes_follow_the_definition(paged):
     assert torch.equal(ref.nan_to_num(7.0), hv.nan_to_num(7.0)) and torch.equal(hk.nan_to_num(7.0), hv.nan_to_num(7.0))
 
 
+@pytest.mark.parametrize("n,d,rot,interleaved", [(300, 64, 64, False), (2000, 64, 32, False), (300, 128, 128, True),
+                                                 (1500, 128, 64, False), (1200, 64, 64, True)])
+def test_queries_and_codes_match_plain_32_bits(paged, n, d, rot, interleaved):
+    """Every operation is rounded on its own and sums run neighbours first, so 32-bit torch operations in
+    that order give the same bits (a contracted product and sum would not)."""
+    hq, hkv = 4, 2
+    q, k = _randn(1, n, hq, d).bfloat16().cuda(), _randn(2, n, hkv, d).bfloat16().cuda()
+    qw, kw = 1 + 0.1 * _randn(3, hq, d).cuda(), 1 + 0.1 * _randn(4, hkv, d).cuda()
+    cos, sin = paged.rope_tables(n, rot)
+    pos = torch.randperm(n, generator=torch.Generator().manual_seed(1)).int().cuda()
+    gain = 1 + torch.rand(n, generator=torch.Generator().manual_seed(2)).cuda()
+    pages = paged.kv4_pages(n // 64 + 1, hkv, d)
+    slots = torch.arange(n).cuda()
+    out = paged.kv4_append(q, k, k, pages, slots, pos, cos, sin, q_norm=qw, k_norm=kw, interleaved=interleaved,
+                           q_gain=gain)
+
+    def plain(x, w):
+        x = x.float()
+        s = x * x
+        while s.shape[-1] > 1:
+            s = s[..., ::2] + s[..., 1::2]
+        x = w * (x * (1.0 / torch.sqrt(s * (1.0 / d) + 1e-6)))
+        c, s = cos[pos.long()][:, None], sin[pos.long()][:, None]
+        a, b = (x[..., 0:rot:2], x[..., 1:rot:2]) if interleaved else (x[..., :rot // 2], x[..., rot // 2:rot])
+        y = x.clone()
+        if interleaved:
+            y[..., 0:rot:2], y[..., 1:rot:2] = a * c - b * s, b * c + a * s
+        else:
+            y[..., :rot // 2], y[..., rot // 2:rot] = a * c - b * s, b * c + a * s
+        return y
+
+    assert torch.equal(out, (plain(q, qw) * gain[pos.long()][:, None, None]).bfloat16())
+    g = plain(k, kw).unflatten(-1, (-1, 32))
+    z = g.amin(-1, keepdim=True).bfloat16().float()
+    s = ((g.amax(-1, keepdim=True) - z) / g.new_full((), 15.0)).bfloat16().float()
+    c = torch.round((g - z) / s).clamp(0, 15)
+    assert torch.equal(paged.kv4_read(pages, slots, d)[0], (c * s + z).flatten(-2).bfloat16())
+
+
 @pytest.mark.parametrize("d,page,start,shuffle", [(64, 64, 0, False), (64, 16, 5, False), (128, 32, 0, False),
                                                   (128, 64, 15, False), (64, 64, 0, True)])
 def test_many_tokens_match_few(paged, d, page, start, shuffle):
