@@ -269,17 +269,19 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
                 fence_after();
                 return ok;
             };
-            bool ok = true;
-            for (int c = 0; c < n; ++c) {
+            const uint32_t qt = desc(sb + L::Q + t * L::QB);
+            bool ok = ready(&ms.kv_full[0], 0);
+            for (int c = 0; ok && c < n; ++c) {
                 // scores, over the weights of chunk c - 1
-                ok = ready(&ms.kv_full[c % KS], (c / KS) & 1) && (c == 0 || ready(&ms.pv_done[t], (c - 1) & 1));
-                if (!ok) break;
-                const uint32_t kt = desc(sb + L::K + (c % KS) * L::KB), qt = desc(sb + L::Q + t * L::QB);
+                if (c > 0 && !(ok = ready(&ms.pv_done[t], (c - 1) & 1))) break;
+                const uint32_t kt = desc(sb + L::K + (c % KS) * L::KB);
 #pragma unroll
                 for (int ks = 0; ks < HD / 16; ++ks)
                     mma_ss(one, tm + L::S_COL + t * CK, qt + (((ks >> 2) * (128 * 128) + (ks & 3) * 32) >> 4),
                            kt + (((ks >> 2) * (CK * 128) + (ks & 3) * 32) >> 4), idesc(CK), ks > 0);
                 commit(one, &ms.s_full[t]);
+                // (the next chunk's operands are waited for here, off the way from weights to scores)
+                if (c + 1 < n && !(ok = ready(&ms.kv_full[(c + 1) % KS], ((c + 1) / KS) & 1))) break;
                 if (!(ok = ready(&ms.p_full[t], c & 1))) break;
                 const uint32_t vt = desc(sb + L::V + (c % KS) * L::KB);
 #pragma unroll
@@ -479,14 +481,24 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
         const int all_lo = low(len - nq + ub / a.group), all_hi = len - nq + ua / a.group + 1;
         float m = KV4_NEG, l = 0.f;
         uint32_t bad = 0;
-        bool ok = tile < tiles;
+        // the chunk's scale of scores, exponent of values and NaN marks, taken while its scores are computed
+        float kq = 0.f, ev = 0.f;
+        uint32_t odd = 0;
+        auto chunk = [&](int c) {
+            const int sk = c % KS;
+            const bool there = __all_sync(0xffffffffu, wait(&ms.kv_full[sk], (c / KS) & 1, abort));
+            kq = ms.kscale[sk] * qscale;
+            ev = ms.ev[sk];
+            odd = ms.bad[sk][0] | ms.bad[sk][1] | ms.bad[sk][2] | ms.bad[sk][3];
+            return there;
+        };
+        bool ok = tile < tiles && n > 0;
+        if (ok) ok = chunk(0);
         for (int c = 0; ok && c < n; ++c) {
             const int sk = c % KS, k0 = base + c * CK;
-            ok = wait(&ms.s_full[tile], c & 1, abort) && wait(&ms.kv_full[sk], (c / KS) & 1, abort);
-            ok = __all_sync(0xffffffffu, ok);
+            ok = __all_sync(0xffffffffu, wait(&ms.s_full[tile], c & 1, abort));
             if (!ok) break;
             fence_after();
-            const float kq = ms.kscale[sk] * qscale, ev = ms.ev[sk];
             const bool edge = k0 < all_lo || k0 + CK > all_hi;
             const int lo_c = lo - k0, hi_c = hi - k0;
             // scores of keys 32 q .. of the chunk; those that the unit does not see: -inf
@@ -556,7 +568,7 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
             st16(s_at, p);
             st16(s_at + 16, p + 16);
             l = fmaf(sum, kv4_ex2(-ev), l);
-            if (ms.bad[sk][0] | ms.bad[sk][1] | ms.bad[sk][2] | ms.bad[sk][3]) {
+            if (odd) {
                 for (int k = max(lo_c, 0); k < min(hi_c, CK); ++k)
                     if (ms.bad[sk][k >> 4]) bad |= ms.bad_groups[sk][k];
             }
@@ -564,9 +576,11 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
             fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&ms.p_full[tile]);
+            if (c + 1 < n) ok = chunk(c + 1);
         }
         if (tile < tiles) {
-            if (ok && n > 0) ok = wait(&ms.pv_done[tile], (n - 1) & 1, abort) && !*abort;
+            if (n == 0) ok = true;
+            else if (ok) ok = wait(&ms.pv_done[tile], (n - 1) & 1, abort) && !*abort;
             ok = __all_sync(0xffffffffu, ok);
             fence_after();
             if (!ok) bad = 0xffu;
