@@ -30,18 +30,10 @@ struct AppendArgs {
     uint8_t* pages;
     __nv_bfloat16* qo;
     int64_t num_slots, page_bytes;
-    uint32_t n;   // n (hq + 2 hkv) < 2^31
-    int hq, hkv, page_shift, rot, max_pos, interleaved;
+    uint32_t n, warps;   // n (hq + 2 hkv) < 2^31
+    int hq, hkv, page_shift, rot, max_pos, heads;
     float eps;
 };
-
-// Sum of v over the L lanes of a vector, lane l ending with the sum that starts from neighbours.
-template <int L>
-__device__ __forceinline__ float lanes_sum(float v) {
-#pragma unroll
-    for (int o = 1; o < L; o <<= 1) v = __fadd_rn(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
 
 constexpr float WHOLE = 12582912.f;   // 1.5 2^23: adding it rounds to a whole number, ties to even
 
@@ -66,43 +58,36 @@ struct Dims {
     }
 };
 
-// Codes, s and z of the group of 32 dims whose 8-dim quarter this lane holds. Returns the lane's 8
-// codes, nibble j = dim j.
-__device__ __forceinline__ uint32_t quantise(const Dims& x, uint32_t& param) {
-    float lo[8];
-    f32x2 bad2 = two(0.f, 0.f);
+// How a call's queries and keys are turned: not at all; pairs (i, i + D/2) of the whole vector, whose
+// halves a lane holds; neighbours; pairs (i, i + rot/2) of a part, which other lanes hold.
+enum { TURN_NONE, TURN_WHOLE, TURN_NEIGHBOURS, TURN_PART };
+
+__device__ __forceinline__ float min3(float a, float b, float c) {
+    float d;
+    asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// The largest, NaN where there is one.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ void range(const Dims& x, float& mn, float& mx) {
+    float v[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        parts(x.v[i], lo[2 * i], lo[2 * i + 1]);
-        bad2 = fma2(x.v[i], two(0.f, 0.f), bad2);   // NaN once a value is none or infinite
-    }
-    float mn = fminf(fminf(fminf(lo[0], lo[1]), fminf(lo[2], lo[3])), fminf(fminf(lo[4], lo[5]), fminf(lo[6], lo[7])));
-    float mx = fmaxf(fmaxf(fmaxf(lo[0], lo[1]), fmaxf(lo[2], lo[3])), fmaxf(fmaxf(lo[4], lo[5]), fmaxf(lo[6], lo[7])));
-    float b0, b1;
-    parts(bad2, b0, b1);
-    if (!(b0 + b1 == 0.f)) mx = INFINITY;
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-        mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, o));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    }
-    const __nv_bfloat16 zb = __float2bfloat16(mn);
-    const float z = __bfloat162float(zb);
-    const __nv_bfloat16 sb = __float2bfloat16(__fdiv_rn(__fsub_rn(mx, z), 15.f));
-    const float s = __bfloat162float(sb);
-    if (!(fabsf(z) < INFINITY && s < INFINITY)) {   // the whole group reads back as NaN
-        param = 0x7fff7fffu;
-        return 0u;
-    }
-    if (!(s >= 1.17549435e-38f)) {   // a constant group (or a span below the normal range)
-        param = (uint32_t)__bfloat16_as_ushort(zb) << 16;
-        return 0u;
-    }
-    param = (uint32_t)__bfloat16_as_ushort(zb) << 16 | __bfloat16_as_ushort(sb);
+    for (int i = 0; i < 4; ++i) parts(x.v[i], v[2 * i], v[2 * i + 1]);
+    mn = min3(min3(min3(v[0], v[1], v[2]), v[3], v[4]), min3(v[5], v[6], v[7]), v[7]);
+    mx = max3(max3(max3(v[0], v[1], v[2]), v[3], v[4]), max3(v[5], v[6], v[7]), v[7]);
+}
+
+// The 8 codes (nibble j = dim j) of a lane's quarter of a group with parameters par and inv = 1 / s, 0
+// for a group of one value; a group of NaN has codes 0.
+__device__ __forceinline__ uint32_t codes_of(const Dims& x, uint32_t par, float inv) {
     // (x - z) / s, correctly rounded: the reciprocal and one step of Markstein's division (IBM J. Res.
     // Dev. 34, 1990; s has a bf16 significand, which is none of the method's exceptions). At most
     // 15 (1 + 2^-8) since s is rounded, so no code passes 15; z is rounded too and may lie above x.
-    const float inv = __frcp_rn(s);
+    const float s = __uint_as_float(par << 16), z = __uint_as_float(par & 0xffff0000u);
     const f32x2 z2 = two(-z, -z), s2 = two(-s, -s), i2 = two(inv, inv);
     float c[8];
 #pragma unroll
@@ -121,17 +106,56 @@ __device__ __forceinline__ uint32_t quantise(const Dims& x, uint32_t& param) {
     return __byte_perm(p[0], p[1], 0x5410);
 }
 
-// Transpose among the quad of lanes that holds a group: lane j = 2 b + n comes with the codes of
-// dims 16 b + 8 n + x (nibble x) and leaves with the word of x = 2j, 2j + 1: half e = x % 2, byte
-// b of the half, nibble n of the byte.
-__device__ __forceinline__ uint32_t quad_word(uint32_t p, int lane) {
-    uint32_t o[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = __shfl_sync(0xffffffffu, p, (lane & ~3) | i);
-    const uint32_t j = lane & 3, sel = j | (4 + j) << 4;   // byte j of each of the four
-    const uint32_t v = __byte_perm(__byte_perm(o[0], o[1], sel), __byte_perm(o[2], o[3], sel), 0x5410);
-    const uint32_t e0 = v & 0x0f0f0f0fu, e1 = (v >> 4) & 0x0f0f0f0fu;
+// Codes and parameters (s, z above it) of the two groups of 32 dims of which the quad of lanes holds the
+// quarters lo and hi. Even lanes look after the first group's parameters, odd lanes after the other's.
+__device__ __forceinline__ void quantise(const Dims& lo, const Dims& hi, int lane, uint32_t* code, uint32_t* param) {
+    const bool odd = lane & 1;
+    float mn0, mx0, mn1, mx1;
+    range(lo, mn0, mx0);
+    range(hi, mn1, mx1);
+    float mn = odd ? mn1 : mn0, mx = odd ? mx1 : mx0;
+    const float mn_up = __shfl_xor_sync(0xffffffffu, odd ? mn0 : mn1, 1), mx_up = __shfl_xor_sync(0xffffffffu, odd ? mx0 : mx1, 1);
+    const float mn2 = fminf(mn, mn_up), mx2 = max3(mx, mx_up, mx_up);
+    mn = fminf(mn2, __shfl_xor_sync(0xffffffffu, mn2, 2));
+    const float mx3 = __shfl_xor_sync(0xffffffffu, mx2, 2);
+    mx = max3(mx2, mx3, mx3);
+    const __nv_bfloat16 zb = __float2bfloat16(mn);
+    const float z = __bfloat162float(zb);
+    // (mx - z) / 15, correctly rounded in the same way
+    const float span = __fsub_rn(mx, z), part = __fmul_rn(span, 1.f / 15.f);
+    const __nv_bfloat16 sb = __float2bfloat16(__fmaf_rn(__fmaf_rn(part, -15.f, span), 1.f / 15.f, part));
+    const float s = __bfloat162float(sb);
+    uint32_t par = (uint32_t)__bfloat16_as_ushort(zb) << 16;
+    float inv = 0.f;
+    if (!(fabsf(z) < INFINITY && s < INFINITY)) {   // the whole group reads back as NaN
+        par = 0x7fff7fffu;
+    } else if (s >= 1.17549435e-38f) {   // else a group of one value (or a span below the normal range)
+        par |= __bfloat16_as_ushort(sb);
+        inv = __frcp_rn(s);
+    }
+    const uint32_t par_up = __shfl_xor_sync(0xffffffffu, par, 1);
+    const float inv_up = __shfl_xor_sync(0xffffffffu, inv, 1);
+    param[0] = odd ? par_up : par;
+    param[1] = odd ? par : par_up;
+    code[0] = codes_of(lo, param[0], odd ? inv_up : inv);
+    code[1] = codes_of(hi, param[1], odd ? inv : inv_up);
+}
+
+// Byte j of each of the four lanes' words, for lane j of the quad.
+__device__ __forceinline__ uint32_t quad_transpose(uint32_t p, int lane) {
+    p = __byte_perm(p, __shfl_xor_sync(0xffffffffu, p, 2), lane & 2 ? 0x3276 : 0x5410);
+    return __byte_perm(p, __shfl_xor_sync(0xffffffffu, p, 1), lane & 1 ? 0x3715 : 0x6240);
+}
+// Among the quad of lanes that holds a group: lane j = 2 b + n comes with the codes of dims
+// 16 b + 8 n + x (nibble x) and leaves with the word of x = 2j, 2j + 1: half e = x % 2, byte b of the
+// half, nibble n of the byte.
+__device__ __forceinline__ uint32_t to_word(uint32_t p, int lane) {
+    const uint32_t v = quad_transpose(p, lane), e0 = v & 0x0f0f0f0fu, e1 = (v >> 4) & 0x0f0f0f0fu;
     return __byte_perm(e0 | e0 >> 4, e1 | e1 >> 4, 0x6420);
+}
+__device__ __forceinline__ uint32_t from_word(uint32_t w, int lane) {
+    const uint32_t a = __byte_perm(w, 0, 0x1100), b = __byte_perm(w, 0, 0x3322);
+    return quad_transpose((a & 0x000f000fu) | ((a >> 4) & 0x0f000f00u) | ((b << 4) & 0x00f000f0u) | (b & 0xf000f000u), lane);
 }
 
 __device__ __forceinline__ void load4(const float* p, f32x2* x) {
@@ -139,14 +163,16 @@ __device__ __forceinline__ void load4(const float* p, f32x2* x) {
     x[0] = two(v.x, v.y);
     x[1] = two(v.z, v.w);
 }
+__device__ __forceinline__ void load8(const float* p, f32x2* x) {
+    load4(p, x);
+    load4(p + 4, x + 2);
+}
 
-// x: the 8 dims (8 l ..) of a head vector that this lane holds, normed (weights w, or none) and
-// turned. Every lane of the warp takes part.
+// x = w x / sqrt(mean x^2 + eps) of the vector whose parts lo and hi this lane holds.
 template <int HD>
-__device__ __forceinline__ void norm_rotate(const AppendArgs& a, const float* w, int pos, bool pos_ok, int lane, Dims& x) {
-    constexpr int L = HD / 8;
-    const int l = lane % L;
-    if (w) {
+__device__ __forceinline__ void norm(Dims& lo, Dims& hi, const f32x2* w, float eps, int lane) {
+    constexpr int L = HD / 16;
+    auto sum8 = [](const Dims& x) {
         float t[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -154,123 +180,123 @@ __device__ __forceinline__ void norm_rotate(const AppendArgs& a, const float* w,
             parts(mul2(x.v[i], x.v[i]), u, v);
             t[i] = __fadd_rn(u, v);
         }
-        const float ss = lanes_sum<L>(__fadd_rn(__fadd_rn(t[0], t[1]), __fadd_rn(t[2], t[3])));
-        const float inv = __frcp_rn(__fsqrt_rn(__fadd_rn(__fmul_rn(ss, 1.f / HD), a.eps)));
-        f32x2 wv[4];
-        load4(w + 8 * l, wv);
-        load4(w + 8 * l + 4, wv + 2);
+        return __fadd_rn(__fadd_rn(t[0], t[1]), __fadd_rn(t[2], t[3]));
+    };
+    // sums of neighbours first; even lanes add up the first half's, odd lanes the other's
+    const bool odd = lane & 1;
+    const float a = sum8(lo), b = sum8(hi);
+    float ss = __fadd_rn(odd ? b : a, __shfl_xor_sync(0xffffffffu, odd ? a : b, 1));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) x.v[i] = mul2(wv[i], mul2(x.v[i], two(inv, inv)));
+    for (int o = 2; o < L; o <<= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, o));
+    ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, 1));
+    const float inv = __frcp_rn(__fsqrt_rn(__fadd_rn(__fmul_rn(ss, 1.f / HD), eps)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        lo.v[i] = mul2(w[i], mul2(lo.v[i], two(inv, inv)));
+        hi.v[i] = mul2(w[4 + i], mul2(hi.v[i], two(inv, inv)));
     }
-    if (a.rot == 0) return;
-    const int half = a.rot >> 1;
-    const int64_t row = (int64_t)(pos_ok ? pos : 0) * half;
+}
+
+// What a token's vectors are turned by: cos in t[0..3] and sin in t[4..7] of a lane's 8 pairs. Pairs of
+// neighbours: the first four pairs (of lo) in t[0..1] and t[4..5].
+template <int HD, int TURN>
+__device__ __forceinline__ void load_turn(const AppendArgs& a, int pos, int l, f32x2* t) {
+    if (TURN != TURN_WHOLE && TURN != TURN_NEIGHBOURS) return;
+    const int64_t row = (int64_t)pos * (a.rot >> 1);
     const float *cs = a.cs + row, *sn = a.sn + row;
-    const bool turn = 8 * l < a.rot;
-    if (a.interleaved) {
-        if (!turn) return;
-        float c[4], s[4];
-        if ((a.rot & 7) == 0) {   // rows of the tables are multiples of 16 bytes
-            const float4 c4 = __ldg(reinterpret_cast<const float4*>(cs + 4 * l));
-            const float4 s4 = __ldg(reinterpret_cast<const float4*>(sn + 4 * l));
-            c[0] = c4.x; c[1] = c4.y; c[2] = c4.z; c[3] = c4.w;
-            s[0] = s4.x; s[1] = s4.y; s[2] = s4.z; s[3] = s4.w;
-        } else {
+    if (TURN == TURN_WHOLE) {
+        load8(cs + 8 * l, t);
+        load8(sn + 8 * l, t + 4);
+    } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const bool in = 8 * l + 2 * j < a.rot;
-                c[j] = in ? cs[4 * l + j] : 1.f;
-                s[j] = in ? sn[4 * l + j] : 0.f;
+        for (int hf = 0; hf < 2; ++hf) {
+            const int p = hf * (HD / 4) + 4 * l;   // the first pair
+            if (a.rot % 8 == 0) {   // rows of the tables are multiples of 16 bytes
+                if (2 * p < a.rot) {
+                    load4(cs + p, t + 2 * hf);
+                    load4(sn + p, t + 4 + 2 * hf);
+                }
+            } else {
+                float c[4], s[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const bool in = 2 * (p + j) < a.rot;
+                    c[j] = in ? cs[p + j] : 1.f;
+                    s[j] = in ? sn[p + j] : 0.f;
+                }
+                t[2 * hf] = two(c[0], c[1]);
+                t[2 * hf + 1] = two(c[2], c[3]);
+                t[4 + 2 * hf] = two(s[0], s[1]);
+                t[5 + 2 * hf] = two(s[2], s[3]);
             }
         }
+    }
+}
+
+// The products are taken in pairs; the sums are not, which would be contracted with them.
+template <int HD, int TURN>
+__device__ __forceinline__ void turn(const AppendArgs& a, Dims& lo, Dims& hi, const f32x2* t, int pos, int lane) {
+    constexpr int L = HD / 16;
+    const int l = lane % L;
+    if (TURN == TURN_WHOLE) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            if (8 * l + 2 * j < a.rot) {   // (u c - v s, v c + u s)
-                float u, v;
-                parts(x.v[j], u, v);
-                x.v[j] = two(__fsub_rn(__fmul_rn(u, c[j]), __fmul_rn(v, s[j])), __fadd_rn(__fmul_rn(v, c[j]), __fmul_rn(u, s[j])));
-            }
+        for (int i = 0; i < 4; ++i) {
+            float u0, u1, v0, v1;
+            parts(mul2(lo.v[i], t[i]), u0, u1);
+            parts(mul2(hi.v[i], t[4 + i]), v0, v1);
+            const f32x2 x = two(__fsub_rn(u0, v0), __fsub_rn(u1, v1));
+            parts(mul2(hi.v[i], t[i]), u0, u1);
+            parts(mul2(lo.v[i], t[4 + i]), v0, v1);
+            hi.v[i] = two(__fadd_rn(u0, v0), __fadd_rn(u1, v1));
+            lo.v[i] = x;
         }
-    } else {   // rot % 16 == 0: the partner's dims are the same 8 of another lane, rows multiples of 32 bytes
-        const int hl = half >> 3;
-        const bool first = l < hl;
-        const int from = (lane - l) + (turn ? (first ? l + hl : l - hl) : l);
-        f32x2 o[4];
+    } else if (TURN == TURN_NEIGHBOURS) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = __shfl_sync(0xffffffffu, x.v[i], from);
-        if (turn) {
-            const int b = 8 * (first ? l : l - hl);
-            f32x2 c[4], s[4];
-            load4(cs + b, c);
-            load4(cs + b + 4, c + 2);
-            load4(sn + b, s);
-            load4(sn + b + 4, s + 2);
+        for (int j = 0; j < 8; ++j) {   // (u c - v s, v c + u s)
+            f32x2& x = j < 4 ? lo.v[j] : hi.v[j - 4];
+            if ((j < 4 ? 0 : HD / 2) + 8 * l + 2 * (j & 3) >= a.rot) continue;
+            float c[2], s[2], u, v, uc, vc, us, vs;
+            parts(t[j / 2], c[0], c[1]);
+            parts(t[4 + j / 2], s[0], s[1]);
+            parts(x, u, v);
+            parts(mul2(x, two(c[j & 1], c[j & 1])), uc, vc);
+            parts(mul2(x, two(s[j & 1], s[j & 1])), us, vs);
+            x = two(__fsub_rn(uc, vs), __fadd_rn(vc, us));
+        }
+    } else if (TURN == TURN_PART) {   // rot % 16 == 0: the partners of 8 dims are 8 of one lane
+        const int hl = a.rot >> 4;
+        const int64_t row = (int64_t)pos * (a.rot >> 1);
+        const Dims x[2] = {lo, hi};
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+            if (hf * (HD / 2) >= a.rot) break;
+            const int c = hf * L + l;   // which 8 dims
+            const bool on = c < 2 * hl, first = c < hl;
+            const int pc = on ? (first ? c + hl : c - hl) : 0, from = (lane - l) + pc % L;
+            f32x2 o[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                o[i] = __shfl_sync(0xffffffffu, x[0].v[i], from);
+                if (a.rot > HD / 2) {
+                    const f32x2 up = __shfl_sync(0xffffffffu, x[1].v[i], from);
+                    if (pc >= L) o[i] = up;
+                }
+            }
+            if (!on) continue;
+            const int64_t at = row + 8 * (first ? c : c - hl);
+            f32x2 cs[4], sn[4];
+            load8(a.cs + at, cs);
+            load8(a.sn + at, sn);
             const float sign = first ? -1.f : 1.f;   // x c - o s, or x c + o s
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {   // (the products in pairs; the sums not, which would be contracted with them)
+            for (int i = 0; i < 4; ++i) {
                 float u0, u1, v0, v1;
-                parts(mul2(x.v[i], c[i]), u0, u1);
-                parts(mul2(o[i], mul2(s[i], two(sign, sign))), v0, v1);
-                x.v[i] = two(__fadd_rn(u0, v0), __fadd_rn(u1, v1));
+                parts(mul2(x[hf].v[i], cs[i]), u0, u1);
+                parts(mul2(o[i], mul2(sn[i], two(sign, sign))), v0, v1);
+                (hf ? hi : lo).v[i] = two(__fadd_rn(u0, v0), __fadd_rn(u1, v1));
             }
         }
     }
-}
-
-// N times the warp's 256 / HD query vectors from vb on (of the call's n hq). What they need from
-// memory is asked for before any of it is used.
-template <int HD, int N>
-__device__ __forceinline__ void append_queries(const AppendArgs& a, uint32_t vb, int lane) {
-    constexpr int L = HD / 8, VW = 256 / HD;
-    const int l = lane % L;
-    uint4 raw[N];
-    int pos[N], head[N];
-    const uint32_t first = vb + lane / L;
-    int64_t tok = first / (uint32_t)a.hq;
-    int h = (int)(first - (uint32_t)tok * a.hq);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        if (tok >= a.n) tok = 0;   // past the last vector: any valid one, not stored
-        head[i] = h;
-        raw[i] = __ldg(reinterpret_cast<const uint4*>(a.q + tok * a.qs + h * a.qh) + l);
-        pos[i] = a.pos ? a.pos[tok] : 0;
-        for (h += VW; h >= a.hq; h -= a.hq) ++tok;
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-        const uint32_t vi = first + i * VW;
-        Dims x;
-        x.take(raw[i]);
-        const bool ok = !a.pos || (pos[i] >= 0 && pos[i] < a.max_pos);
-        norm_rotate<HD>(a, a.qw ? a.qw + head[i] * HD : nullptr, pos[i], ok, lane, x);
-        if (a.gain) {
-            const float g = ok ? a.gain[pos[i]] : 0.f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) x.v[j] = mul2(x.v[j], two(g, g));
-        }
-        if (vi < a.n * (uint32_t)a.hq)
-            reinterpret_cast<uint4*>(a.qo)[(int64_t)vi * L + l] = ok ? x.bf16() : make_uint4(0, 0, 0, 0);
-    }
-}
-
-// One (token, kv head) vector for each group of HD / 8 lanes: its codes and parameters, to those of
-// the token's tile (in global or shared memory); t: the token's place in the tile.
-template <int HD>
-__device__ __forceinline__ void store_vector(const Dims& x, bool is_k, int t, bool put, uint8_t* codes, uint8_t* params,
-                                             int lane) {
-    using T = Kv4Tile<HD>;
-    const int l = lane % (HD / 8), r = t & 7, hf = t >> 3, g = l >> 2, j = l & 3;
-    uint32_t param;
-    const uint32_t word = quad_word(quantise(x, param), lane);
-    if (!put) return;
-    if (is_k) {
-        *reinterpret_cast<uint32_t*>(codes + (g >> 1) * T::BLK + (4 * r + j) * 16 + hf * 8 + (g & 1) * 4) = word;
-    } else {
-        uint8_t* p = codes + (g >> 1) * T::BLK + (8 * j + (r >> 1)) * 16 + (g & 1) * 8 + hf * 4 + (r & 1) * 2;
-        *reinterpret_cast<uint16_t*>(p) = (uint16_t)word;
-        *reinterpret_cast<uint16_t*>(p + 64) = (uint16_t)(word >> 16);
-    }
-    if (j == 0) *reinterpret_cast<uint32_t*>(params + ((2 * r + hf) * T::NG + g) * 4) = param;
 }
 
 // The tile of a slot (0 .. num_slots - 1) and kv head.
@@ -280,148 +306,158 @@ __device__ __forceinline__ int64_t tile_at(int64_t slot, int h, int hkv, int pag
            (int64_t)((slot & ((1 << page_shift) - 1)) >> 4) * Kv4Tile<HD>::BYTES;
 }
 
-// Where the lane's 8 dims of a head vector of k or v are.
+// Where the bytes of token t of a tile are: a lane's word of key codes, its two halves of a word of value
+// codes (64 bytes apart), the parameters; of group g, lane j of the quad.
 template <int HD>
-__device__ __forceinline__ const uint4* kv_source(const AppendArgs& a, bool is_k, int64_t tok, int h, int lane) {
-    return reinterpret_cast<const uint4*>(is_k ? a.k + tok * a.ks + h * a.kh : a.v + tok * a.vs + h * a.vh) +
-           lane % (HD / 8);
+__device__ __forceinline__ int key_at(int t, int g, int j) {
+    return (g >> 1) * Kv4Tile<HD>::BLK + (4 * (t & 7) + j) * 16 + (t >> 3) * 8 + (g & 1) * 4;
+}
+template <int HD>
+__device__ __forceinline__ int value_at(int t, int g, int j) {
+    return Kv4Tile<HD>::V + (g >> 1) * Kv4Tile<HD>::BLK + (8 * j + ((t & 7) >> 1)) * 16 + (g & 1) * 8 + (t >> 3) * 4 + (t & 1) * 2;
+}
+template <int HD>
+__device__ __forceinline__ int params_at(int t, int g) {
+    return ((2 * (t & 7) + (t >> 3)) * Kv4Tile<HD>::NG + g) * 4;
 }
 
-// Few tokens: a warp per 32 / L head vectors of one kind (queries, keys or values), so that no warp
-// quantises what it does not store.
+// The words of a lane's two groups, `apart` bytes from each other: neighbours with heads of 64.
 template <int HD>
-__global__ void __launch_bounds__(128) k_kv4_append(const AppendArgs a) {
-    using T = Kv4Tile<HD>;
-    constexpr int VW = 256 / HD;   // vectors a warp
-    const int lane = threadIdx.x & 31;
-    const uint32_t nq = (a.n * (uint32_t)a.hq + VW - 1) / VW, nk = (a.n * (uint32_t)a.hkv + VW - 1) / VW;
-    const uint32_t w = blockIdx.x * 4 + (threadIdx.x >> 5);
-    if (w < nq) {
-        append_queries<HD, 1>(a, w * VW, lane);
-    } else if (w < nq + 2 * nk) {
-        const bool is_k = w < nq + nk;
-        const uint32_t vi = (w - nq - (is_k ? 0 : nk)) * VW + lane / (HD / 8);
-        const bool live = vi < a.n * (uint32_t)a.hkv;
-        const uint32_t tok = live ? vi / (uint32_t)a.hkv : 0u;
-        const int h = live ? (int)(vi - tok * a.hkv) : 0;
-        const uint4 raw = __ldg(kv_source<HD>(a, is_k, tok, h, lane));
-        const int pos = a.pos ? a.pos[tok] : 0;
-        const int64_t slot = a.slots[tok];
-        const bool ok = !a.pos || (pos >= 0 && pos < a.max_pos), put = live && ok && slot >= 0 && slot < a.num_slots;
-        Dims x;
-        x.take(raw);
-        if (is_k) norm_rotate<HD>(a, a.kw ? a.kw + h * HD : nullptr, pos, ok, lane, x);
-        uint8_t* tile = a.pages + (put ? tile_at<HD>(slot, h, a.hkv, a.page_shift, a.page_bytes) : 0);
-        store_vector<HD>(x, is_k, (int)(slot & 15), put, tile + (is_k ? 0 : T::V), tile + (is_k ? T::KP : T::VP), lane);
-    }
-}
-
-// Many tokens: a warp per 16 tokens of one kv head's keys or values. Where they fill one tile of the
-// cache, its codes and parameters are put together in shared memory and written in 16-byte pieces
-// (value codes of a token are 2-byte pieces 64 bytes apart); others are written one by one. Groups
-// of 16 start so that the first token's page lines up with them. Queries: 16 vectors a warp.
-constexpr int BULK_WARPS = 8;
-template <int HD>
-__global__ void __launch_bounds__(BULK_WARPS * 32, 4) k_kv4_append_bulk(const AppendArgs a) {
-    using T = Kv4Tile<HD>;
-    constexpr int VW = 256 / HD, L = HD / 8;
-    __shared__ __align__(16) uint8_t images[BULK_WARPS][10 * HD];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int lead = (int)(a.slots[0] & 15);   // tokens of the first group that lie before token 0
-    const uint32_t groups = (a.n + lead + 15) / 16, nkv = groups * 2 * a.hkv;
-    const uint32_t nq = (a.n * (uint32_t)a.hq + 15) / 16, w = blockIdx.x * BULK_WARPS + warp;
-    if (w >= nkv) {
-        if (w < nkv + nq)
-#pragma unroll 1
-            for (int i = 0; i < 16; i += 4 * VW) append_queries<HD, 4>(a, (w - nkv) * 16 + i, lane);
+__device__ __forceinline__ void store_two(uint8_t* p, int apart, uint32_t x, uint32_t y) {
+    if (HD == 64) {
+        *reinterpret_cast<uint2*>(p) = make_uint2(x, y);
     } else {
-        const uint32_t grp = w / (2u * a.hkv);
-        const int kh = (int)(w - grp * 2 * a.hkv);
-        const bool is_k = kh < a.hkv;
-        const int h = is_k ? kh : kh - a.hkv;
-        const int64_t tok0 = (int64_t)grp * 16 - lead;
-        constexpr int N = 4;   // vectors of a lane asked for at a time
-        uint4 raw[N];
-        auto ask = [&](int i0) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-                const int64_t tk = tok0 + (i0 + i) * VW + lane / L;
-                raw[i] = __ldg(kv_source<HD>(a, is_k, tk >= 0 && tk < a.n ? tk : 0, h, lane));
-            }
-        };
-        ask(0);
-        // lane t % 16 knows token t's slot and position. A whole tile: 16 tokens in the 16 consecutive
-        // slots of one, all of them stored
-        const int64_t mine = tok0 + (lane & 15);
-        const bool in = mine >= 0 && mine < a.n;
-        const int64_t my_slot = in ? a.slots[mine] : -1;
-        const int my_pos = in && a.pos ? a.pos[mine] : 0;
-        const bool my_ok = !a.pos || (my_pos >= 0 && my_pos < a.max_pos);
-        const bool my_put = in && my_ok && my_slot >= 0 && my_slot < a.num_slots;
-        const int64_t s0 = __shfl_sync(0xffffffffu, my_slot, 0);
-        const bool whole = __all_sync(0xffffffffu, my_put && my_slot == s0 + (lane & 15) && (s0 & 15) == 0);
-        const uint32_t puts = __ballot_sync(0xffffffffu, my_put), oks = __ballot_sync(0xffffffffu, my_ok);
-        uint8_t* dst = a.pages + (whole ? tile_at<HD>(s0, h, a.hkv, a.page_shift, a.page_bytes) : 0);
+        *reinterpret_cast<uint32_t*>(p) = x;
+        *reinterpret_cast<uint32_t*>(p + apart) = y;
+    }
+}
+template <int HD>
+__device__ __forceinline__ uint2 load_two(const uint8_t* p, int apart) {
+    if (HD == 64) return *reinterpret_cast<const uint2*>(p);
+    return make_uint2(*reinterpret_cast<const uint32_t*>(p), *reinterpret_cast<const uint32_t*>(p + apart));
+}
+
+// A warp's work: 512 / HD tokens (a lane holds dims 8 l .. and HD / 2 + 8 l .. of one's vector, l = lane %
+// (HD / 16): both halves of the rotation's pairs, and quarters of two groups), and up to `heads` heads
+// of one kind, one after the other: slots, positions and tables are looked up once for them.
+struct Item {
+    int64_t tok;
+    int kind, h0, h1;   // 0 queries, 1 keys, 2 values; heads h0 .. h1 - 1
+    bool live;
+};
+template <int HD>
+__device__ __forceinline__ Item item_of(uint32_t w, uint32_t n, int hq, int hkv, int heads, int lane) {
+    const uint32_t iq = (uint32_t)(hq + heads - 1) / heads, ik = (uint32_t)(hkv + heads - 1) / heads, per = iq + 2 * ik;
+    const uint32_t grp = w / per;
+    uint32_t i = w - grp * per;
+    Item it;
+    it.kind = i < iq ? 0 : i < iq + ik ? 1 : 2;
+    i -= it.kind == 0 ? 0 : it.kind == 1 ? iq : iq + ik;
+    it.h0 = (int)i * heads;
+    const int all = it.kind == 0 ? hq : hkv;
+    it.h1 = it.h0 + heads < all ? it.h0 + heads : all;
+    it.tok = (int64_t)grp * (512 / HD) + lane / (HD / 16);
+    it.live = it.tok < n;
+    if (!it.live) it.tok = 0;   // any valid one, not stored
+    return it;
+}
+
+// 16384 tokens of 16 query and 4 kv heads of 64 take 31 us: 89 MB, 2.8 TB/s. One token: 2.5 us. What
+// bounds it is the arithmetic (some 290 instructions for a lane's 16 dims, 14 M in all, two a clock and
+// SM) behind the chain slot, position, table, vector; 24 warps an SM (80 registers, a few spilled) hide
+// that better than the 16 that fit without a bound: 32 us against 40. Tokens run along the warp so
+// that neighbouring slots share sectors of a tile: a token's value codes are 2-byte pieces 64 bytes
+// apart. Gathering whole tiles in shared memory to write them in 16-byte pieces gained nothing.
+template <int HD, int TURN>
+__global__ void __launch_bounds__(128, 6) k_kv4_append(const AppendArgs a) {
+    constexpr int L = HD / 16, NG = Kv4Tile<HD>::NG;
+    const int lane = threadIdx.x & 31, l = lane % L;
+    const uint32_t w = blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (w >= a.warps) return;
+    const Item it = item_of<HD>(w, a.n, a.hq, a.hkv, a.heads, lane);
+    const __nv_bfloat16* src = it.kind == 0 ? a.q + it.tok * a.qs + it.h0 * a.qh
+                             : it.kind == 1 ? a.k + it.tok * a.ks + it.h0 * a.kh : a.v + it.tok * a.vs + it.h0 * a.vh;
+    const int64_t next = it.kind == 0 ? a.qh : it.kind == 1 ? a.kh : a.vh;
+    uint4 raw0 = __ldg(reinterpret_cast<const uint4*>(src) + l), raw1 = __ldg(reinterpret_cast<const uint4*>(src) + L + l);
+    int pos = a.pos ? a.pos[it.tok] : 0;
+    const bool ok = !a.pos || (pos >= 0 && pos < a.max_pos);
+    if (!ok) pos = 0;
+    const int64_t slot = it.kind ? a.slots[it.tok] : 0;
+    f32x2 t[8] = {};
+    if (it.kind != 2) load_turn<HD, TURN>(a, pos, l, t);
+    const float* wn = it.kind == 0 ? a.qw : it.kind == 1 ? a.kw : nullptr;
+    const float gain = it.kind == 0 && a.gain ? a.gain[pos] : 1.f;
+    const bool put = it.live && ok && slot >= 0 && slot < a.num_slots;
+    uint8_t* tile = a.pages + (put && it.kind ? tile_at<HD>(slot, it.h0, a.hkv, a.page_shift, a.page_bytes) : 0);
+    __nv_bfloat16* dst = a.qo + (it.tok * a.hq + it.h0) * HD;
 #pragma unroll 1
-        for (int i0 = 0; i0 < 16 / VW; i0 += N) {
-          if (i0 > 0) ask(i0);
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const int t = (i0 + i) * VW + lane / L;
-            const int pos = __shfl_sync(0xffffffffu, my_pos, t);
-            const int64_t slot = __shfl_sync(0xffffffffu, my_slot, t);
-            const bool put = puts >> t & 1;
-            Dims x;
-            x.take(raw[i]);
-            if (is_k) norm_rotate<HD>(a, a.kw ? a.kw + h * HD : nullptr, pos, oks >> t & 1, lane, x);
-            uint8_t *codes = images[warp], *params = images[warp] + 8 * HD;
-            if (!whole) {
-                codes = a.pages + (put ? tile_at<HD>(slot, h, a.hkv, a.page_shift, a.page_bytes) : 0);
-                params = codes + (is_k ? T::KP : T::VP);
-                codes += is_k ? 0 : T::V;
-            }
-            store_vector<HD>(x, is_k, (int)(slot & 15), put, codes, params, lane);
-          }
+    for (int h = it.h0; h < it.h1; ++h) {
+        f32x2 weight[8];
+        if (wn) {
+            load8(wn + h * HD + 8 * l, weight);
+            load8(wn + h * HD + HD / 2 + 8 * l, weight + 4);
         }
-        if (whole) {
-            __syncwarp();
-            const uint4* src = reinterpret_cast<const uint4*>(images[warp]);
-            uint4* codes = reinterpret_cast<uint4*>(dst + (is_k ? 0 : T::V));
-            uint4* par = reinterpret_cast<uint4*>(dst + (is_k ? T::KP : T::VP));
+        Dims lo, hi;
+        lo.take(raw0);
+        hi.take(raw1);
+        src += next;
+        if (h + 1 < it.h1) {
+            raw0 = __ldg(reinterpret_cast<const uint4*>(src) + l);
+            raw1 = __ldg(reinterpret_cast<const uint4*>(src) + L + l);
+        }
+        if (wn) norm<HD>(lo, hi, weight, a.eps, lane);
+        if (it.kind != 2) turn<HD, TURN>(a, lo, hi, t, pos, lane);
+        if (it.kind == 0) {
+            if (a.gain) {
 #pragma unroll
-            for (int i = lane; i < HD / 2; i += 32) codes[i] = src[i];
-            if (lane < HD / 8) par[lane] = src[HD / 2 + lane];
+                for (int i = 0; i < 4; ++i) {
+                    lo.v[i] = mul2(lo.v[i], two(gain, gain));
+                    hi.v[i] = mul2(hi.v[i], two(gain, gain));
+                }
+            }
+            if (it.live) {
+                reinterpret_cast<uint4*>(dst)[l] = ok ? lo.bf16() : make_uint4(0, 0, 0, 0);
+                reinterpret_cast<uint4*>(dst)[L + l] = ok ? hi.bf16() : make_uint4(0, 0, 0, 0);
+            }
+            dst += HD;
+        } else {
+            uint32_t code[2], param[2];
+            quantise(lo, hi, lane, code, param);
+            const uint32_t w0 = to_word(code[0], lane), w1 = to_word(code[1], lane);
+            const int tt = (int)(slot & 15), g0 = l >> 2, g1 = g0 + NG / 2, j = l & 3;
+            if (put) {
+                if (it.kind == 1) {
+                    store_two<HD>(tile + key_at<HD>(tt, g0, j), key_at<HD>(tt, g1, j) - key_at<HD>(tt, g0, j), w0, w1);
+                } else {
+                    uint8_t *v0 = tile + value_at<HD>(tt, g0, j), *v1 = tile + value_at<HD>(tt, g1, j);
+                    *reinterpret_cast<uint16_t*>(v0) = (uint16_t)w0;
+                    *reinterpret_cast<uint16_t*>(v0 + 64) = (uint16_t)(w0 >> 16);
+                    *reinterpret_cast<uint16_t*>(v1) = (uint16_t)w1;
+                    *reinterpret_cast<uint16_t*>(v1 + 64) = (uint16_t)(w1 >> 16);
+                }
+                if (j == 0) {
+                    uint8_t* p = tile + (it.kind == 1 ? Kv4Tile<HD>::KP : Kv4Tile<HD>::VP);
+                    store_two<HD>(p + params_at<HD>(tt, g0), params_at<HD>(tt, g1) - params_at<HD>(tt, g0), param[0], param[1]);
+                }
+            }
+            tile += a.page_bytes;
         }
     }
 }
 
-// The inverse of quantise and quad_word: bf16(s c + z) of the lane's 8 dims of each group of lanes'
-// head vector, from the codes and parameters of its tile (ok false: zeros).
-template <int HD>
-__device__ __forceinline__ uint4 fetch_vector(const uint8_t* codes, const uint8_t* params, bool is_k, int t, bool ok,
-                                              int lane) {
-    using T = Kv4Tile<HD>;
-    const int l = lane % (HD / 8), g = l >> 2, j = l & 3, r = t & 7, hf = t >> 3;
-    uint32_t word = 0, par = 0;
-    if (ok) {
-        if (is_k) {
-            word = *reinterpret_cast<const uint32_t*>(codes + (g >> 1) * T::BLK + (4 * r + j) * 16 + hf * 8 + (g & 1) * 4);
-        } else {
-            const uint8_t* p = codes + (g >> 1) * T::BLK + (8 * j + (r >> 1)) * 16 + (g & 1) * 8 + hf * 4 + (r & 1) * 2;
-            word = *reinterpret_cast<const uint16_t*>(p) | (uint32_t)*reinterpret_cast<const uint16_t*>(p + 64) << 16;
-        }
-        par = *reinterpret_cast<const uint32_t*>(params + ((2 * r + hf) * T::NG + g) * 4);
-    }
+// bf16(s c + z) of a lane's 8 dims, from its codes (nibble j = dim j).
+__device__ __forceinline__ uint4 values_of(uint32_t p, uint32_t par) {
     const float s = __uint_as_float(par << 16), z = __uint_as_float(par & 0xffff0000u);
-    float x[8];
+    const uint32_t even = p & 0x0f0f0f0fu, odd = (p >> 4) & 0x0f0f0f0fu;
+    Dims x;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {   // dims 32 g + 8 j + 2 q, + 1: nibble (j / 2, j % 2) of quad lane q's word
-        const uint32_t o = __shfl_sync(0xffffffffu, word, (lane & ~3) | q) >> (4 * j);
+    for (int i = 0; i < 4; ++i) {
         // a code under the exponent of 2^23 is 2^23 + c; s c is exact, so the sum is rounded once
-        x[2 * q] = fmaf(__uint_as_float((o & 15u) | 0x4b000000u) - 8388608.f, s, z);
-        x[2 * q + 1] = fmaf(__uint_as_float(((o >> 16) & 15u) | 0x4b000000u) - 8388608.f, s, z);
+        const f32x2 c = two(__uint_as_float(__byte_perm(even, 0x4b000000u, 0x7440 + i)),
+                            __uint_as_float(__byte_perm(odd, 0x4b000000u, 0x7440 + i)));
+        x.v[i] = fma2(add2(c, two(-8388608.f, -8388608.f)), two(s, s), two(z, z));
     }
-    return f32_to_bf16x8(x);
+    return x.bf16();
 }
 
 struct ReadArgs {
@@ -429,79 +465,63 @@ struct ReadArgs {
     const int64_t* slots;
     __nv_bfloat16 *k, *v;
     int64_t page_bytes, num_slots;
-    uint32_t n;   // 2 n hkv < 2^31
-    int hkv, page_shift;
+    uint32_t n, warps;   // 2 n hkv < 2^31
+    int hkv, page_shift, heads;
 };
 
-// Few positions: a warp per 32 / L head vectors.
+// 32768 positions of 4 kv heads of 64: 44 MB in 11.4 us, 3.9 TB/s (8 heads of 128: 176 MB in 34 us,
+// 5.2 TB/s); 777 positions 2.3 us. Bound by instructions (80 for a lane's 16 dims) and, past that, by the
+// writes. Through shared memory in whole tiles it took 14.2 us; two heads' bytes asked for at a time cost
+// more registers than waiting: 12.
 template <int HD>
 __global__ void __launch_bounds__(128) k_kv4_read(const ReadArgs a) {
-    using T = Kv4Tile<HD>;
-    constexpr int L = HD / 8;
-    const int lane = threadIdx.x & 31;
-    const uint32_t vi = (blockIdx.x * 128 + threadIdx.x) / L;
-    const bool live = vi < a.n * 2 * a.hkv;
-    const uint32_t tok = live ? vi / (2u * a.hkv) : 0u;
-    const int kh = live ? (int)(vi - tok * 2 * a.hkv) : 0;
-    const bool is_k = kh < a.hkv;
-    const int h = is_k ? kh : kh - a.hkv;
-    const int64_t slot = a.slots[tok];
+    constexpr int L = HD / 16, NG = Kv4Tile<HD>::NG;
+    const int lane = threadIdx.x & 31, l = lane % L;
+    const uint32_t w = blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (w >= a.warps) return;
+    const Item it = item_of<HD>(w, a.n, 0, a.hkv, a.heads, lane);
+    const int64_t slot = a.slots[it.tok];
     const bool ok = slot >= 0 && slot < a.num_slots;
-    const uint8_t* tile = a.pages + (ok ? tile_at<HD>(slot, h, a.hkv, a.page_shift, a.page_bytes) : 0);
-    const uint4 x = fetch_vector<HD>(tile + (is_k ? 0 : T::V), tile + (is_k ? T::KP : T::VP), is_k, (int)(slot & 15), ok,
-                                     lane);
-    if (live) reinterpret_cast<uint4*>((is_k ? a.k : a.v) + ((int64_t)tok * a.hkv + h) * HD)[lane % L] = x;
-}
-
-// Many positions: a warp per 16 of one kv head's keys or values; where they are one whole tile, its
-// bytes come through shared memory in 16-byte pieces. Groups of 16 start so that the first
-// position's tile lines up with them.
-template <int HD>
-__global__ void __launch_bounds__(BULK_WARPS * 32) k_kv4_read_bulk(const ReadArgs a) {
-    using T = Kv4Tile<HD>;
-    constexpr int VW = 256 / HD, L = HD / 8;
-    __shared__ __align__(16) uint8_t images[BULK_WARPS][10 * HD];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int lead = (int)(a.slots[0] & 15);
-    const uint32_t w = blockIdx.x * BULK_WARPS + warp;
-    if (w >= (a.n + lead + 15) / 16 * 2 * a.hkv) return;
-    const uint32_t grp = w / (2u * a.hkv);
-    const int kh = (int)(w - grp * 2 * a.hkv);
-    const bool is_k = kh < a.hkv;
-    const int h = is_k ? kh : kh - a.hkv;
-    const int64_t tok0 = (int64_t)grp * 16 - lead, mine = tok0 + (lane & 15);
-    const int64_t s = mine >= 0 && mine < a.n ? a.slots[mine] : -1;
-    const int64_t s0 = __shfl_sync(0xffffffffu, s, 0);
-    const bool whole = __all_sync(0xffffffffu, s0 >= 0 && (s0 & 15) == 0 && s == s0 + (lane & 15) && s < a.num_slots);
-    if (whole) {
-        const uint8_t* src = a.pages + tile_at<HD>(s0, h, a.hkv, a.page_shift, a.page_bytes);
-        const uint4* codes = reinterpret_cast<const uint4*>(src + (is_k ? 0 : T::V));
-        const uint4* par = reinterpret_cast<const uint4*>(src + (is_k ? T::KP : T::VP));
-        uint4* img = reinterpret_cast<uint4*>(images[warp]);
-#pragma unroll
-        for (int i = lane; i < HD / 2; i += 32) img[i] = __ldg(codes + i);
-        if (lane < HD / 8) img[HD / 2 + lane] = __ldg(par + lane);
-        __syncwarp();
-    }
-#pragma unroll 4
-    for (int i = 0; i < 16; i += VW) {
-        const int64_t slot = __shfl_sync(0xffffffffu, s, i + lane / L), tk = tok0 + i + lane / L;
-        const bool ok = slot >= 0 && slot < a.num_slots;
-        const uint8_t *codes = images[warp], *params = images[warp] + 8 * HD;
-        if (!whole) {
-            codes = a.pages + (ok ? tile_at<HD>(slot, h, a.hkv, a.page_shift, a.page_bytes) : 0);
-            params = codes + (is_k ? T::KP : T::VP);
-            codes += is_k ? 0 : T::V;
+    const uint8_t* tile = a.pages + (ok ? tile_at<HD>(slot, it.h0, a.hkv, a.page_shift, a.page_bytes) : 0);
+    const int tt = (int)(slot & 15), g0 = l >> 2, g1 = g0 + NG / 2, j = l & 3;
+    uint4* dst = reinterpret_cast<uint4*>((it.kind == 1 ? a.k : a.v) + (it.tok * a.hkv + it.h0) * HD);
+#pragma unroll 1
+    for (int h = it.h0; h < it.h1; ++h) {
+        uint2 w = {}, par = {};
+        if (ok) {
+            if (it.kind == 1) {
+                w = load_two<HD>(tile + key_at<HD>(tt, g0, j), key_at<HD>(tt, g1, j) - key_at<HD>(tt, g0, j));
+            } else {
+                const uint16_t *v0 = reinterpret_cast<const uint16_t*>(tile + value_at<HD>(tt, g0, j)),
+                               *v1 = reinterpret_cast<const uint16_t*>(tile + value_at<HD>(tt, g1, j));
+                w = make_uint2(v0[0] | (uint32_t)v0[32] << 16, v1[0] | (uint32_t)v1[32] << 16);
+            }
+            const uint8_t* p = tile + (it.kind == 1 ? Kv4Tile<HD>::KP : Kv4Tile<HD>::VP);
+            par = load_two<HD>(p + params_at<HD>(tt, g0), params_at<HD>(tt, g1) - params_at<HD>(tt, g0));
         }
-        const uint4 x = fetch_vector<HD>(codes, params, is_k, (int)(slot & 15), ok, lane);
-        if (tk >= 0 && tk < a.n) reinterpret_cast<uint4*>((is_k ? a.k : a.v) + (tk * a.hkv + h) * HD)[lane % L] = x;
+        const uint4 x0 = values_of(from_word(w.x, lane), par.x), x1 = values_of(from_word(w.y, lane), par.y);
+        if (it.live) {
+            dst[l] = x0;
+            dst[L + l] = x1;
+        }
+        dst += HD / 8;
+        tile += a.page_bytes;
     }
 }
 
-// From this many tokens on a warp takes 16 of them.
-constexpr int64_t BULK_TOKENS = 1024;
+template <int HD>
+auto append_kernel(int turn) {
+    return turn == TURN_NONE ? k_kv4_append<HD, TURN_NONE> : turn == TURN_WHOLE ? k_kv4_append<HD, TURN_WHOLE>
+         : turn == TURN_NEIGHBOURS ? k_kv4_append<HD, TURN_NEIGHBOURS> : k_kv4_append<HD, TURN_PART>;
+}
 
-int bulk_grid(int64_t warps) { return (int)((warps + BULK_WARPS - 1) / BULK_WARPS); }
+// Heads of a warp's work, from the warps that one head each would take: one until those fill the SMs
+// (24 warps each), then more, which share the look-ups. Measured with 1 / 2 / 4 heads, 16 query and 4 kv
+// heads of 64: 1024 tokens 4.1 / 4.1 / 6.6 us, 2048 6.6 / 5.6 / 6.6, 6144 16.9 / 13.9 /
+// 14.7, 8192 (24576 warps) 24 / 20 / 18, 16384 46 / 36 / 32, with 8 heads 35; reading 16384 positions
+// 7.3 / 6.2 / 5.7.
+constexpr int64_t HEADS_2 = 3552, HEADS_4 = 21312;
+int heads_of(int64_t warps) { return warps < HEADS_2 ? 1 : warps < HEADS_4 ? 2 : 4; }
 
 int page_geometry(const char* what, int64_t head_dim, int64_t page_size, int64_t num_pages, int64_t hkv,
                   const void* pages, int* shift, int64_t* page_bytes) {
@@ -544,25 +564,19 @@ extern "C" int pulsar_op_kv4_append(const void* q, const void* k, const void* v,
                           (const void*)sin})
         PULSAR_CHECK_ARG((reinterpret_cast<uintptr_t>(p) & 15) == 0,
                          "kv4_append: q, k, v, norm weights and tables must be 16-byte aligned");
-    AppendArgs a{(const __nv_bfloat16*)q, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, strides[0], strides[2],
-                 strides[4], strides[1], strides[3], strides[5], q_norm, k_norm, cos, sin, q_gain, slots,
-                 (rot > 0 || q_gain) ? positions : nullptr, (uint8_t*)pages, (__nv_bfloat16*)q_out,
-                 num_pages * page_size, pb, (uint32_t)N, (int)Hq, (int)Hkv, shift, (int)rot, (int)max_pos, interleaved, eps};
+    const int64_t groups = (N * head_dim + 511) / 512;
+    const int heads = heads_of(groups * (Hq + 2 * Hkv));
+    const int64_t warps = groups * ((Hq + heads - 1) / heads + 2 * ((Hkv + heads - 1) / heads));
+    const int turn = rot == 0 ? TURN_NONE : interleaved ? TURN_NEIGHBOURS : rot == head_dim ? TURN_WHOLE : TURN_PART;
+    const AppendArgs a{(const __nv_bfloat16*)q, (const __nv_bfloat16*)k, (const __nv_bfloat16*)v, strides[0], strides[2],
+                       strides[4], strides[1], strides[3], strides[5], q_norm, k_norm, cos, sin, q_gain, slots,
+                       (rot > 0 || q_gain) ? positions : nullptr, (uint8_t*)pages, (__nv_bfloat16*)q_out,
+                       num_pages * page_size, pb, (uint32_t)N, (uint32_t)warps, (int)Hq, (int)Hkv, shift, (int)rot,
+                       (int)max_pos, heads, eps};
     cudaStream_t st = (cudaStream_t)stream;
-    if (N >= BULK_TOKENS) {
-        const int grid = bulk_grid((N + 30) / 16 * 2 * Hkv + (N * Hq + 15) / 16);
-        if (head_dim == 64)
-            k_kv4_append_bulk<64><<<grid, BULK_WARPS * 32, 0, st>>>(a);
-        else
-            k_kv4_append_bulk<128><<<grid, BULK_WARPS * 32, 0, st>>>(a);
-    } else {
-        const int64_t vw = 256 / head_dim, warps = (N * Hq + vw - 1) / vw + 2 * ((N * Hkv + vw - 1) / vw);
-        const int grid = (int)((warps + 3) / 4);
-        if (head_dim == 64)
-            k_kv4_append<64><<<grid, 128, 0, st>>>(a);
-        else
-            k_kv4_append<128><<<grid, 128, 0, st>>>(a);
-    }
+    const int grid = (int)((warps + 3) / 4);
+    auto* kernel = head_dim == 64 ? append_kernel<64>(turn) : append_kernel<128>(turn);
+    kernel<<<grid, 128, 0, st>>>(a);
     PULSAR_LAUNCH_CHECK("k_kv4_append");
     return PULSAR_OK;
 }
@@ -579,22 +593,17 @@ extern "C" int pulsar_op_kv4_read(const void* pages, int64_t num_pages, int64_t 
     for (const void* p : {(const void*)k_out, (const void*)v_out})
         PULSAR_CHECK_ARG((reinterpret_cast<uintptr_t>(p) & 15) == 0, "kv4_read: outputs must be 16-byte aligned");
     PULSAR_CHECK_ARG(N <= INT32_MAX / (2 * Hkv) - 64, "kv4_read: invalid shape (%lld positions)", (long long)N);
+    const int64_t groups = (N * head_dim + 511) / 512;
+    const int heads = heads_of(groups * 2 * Hkv);
+    const int64_t warps = groups * 2 * ((Hkv + heads - 1) / heads);
     const ReadArgs a{(const uint8_t*)pages, slots, (__nv_bfloat16*)k_out, (__nv_bfloat16*)v_out, pb,
-                     num_pages * page_size, (uint32_t)N, (int)Hkv, shift};
+                     num_pages * page_size, (uint32_t)N, (uint32_t)warps, (int)Hkv, shift, heads};
     cudaStream_t st = (cudaStream_t)stream;
-    if (N >= BULK_TOKENS) {
-        const int grid = bulk_grid((N + 30) / 16 * 2 * Hkv);
-        if (head_dim == 64)
-            k_kv4_read_bulk<64><<<grid, BULK_WARPS * 32, 0, st>>>(a);
-        else
-            k_kv4_read_bulk<128><<<grid, BULK_WARPS * 32, 0, st>>>(a);
-    } else {
-        const int grid = (int)((N * 2 * Hkv * (head_dim / 8) + 127) / 128);
-        if (head_dim == 64)
-            k_kv4_read<64><<<grid, 128, 0, st>>>(a);
-        else
-            k_kv4_read<128><<<grid, 128, 0, st>>>(a);
-    }
+    const int grid = (int)((warps + 3) / 4);
+    if (head_dim == 64)
+        k_kv4_read<64><<<grid, 128, 0, st>>>(a);
+    else
+        k_kv4_read<128><<<grid, 128, 0, st>>>(a);
     PULSAR_LAUNCH_CHECK("k_kv4_read");
     return PULSAR_OK;
 }

@@ -269,6 +269,44 @@ def test_many_tokens_match_few(paged, d, page, start, shuffle):
     assert (out[[40, 1111]] == 0).all() and (many[0][[7, 600, 601, 2050]] == 0).all()
 
 
+@pytest.mark.parametrize("n,d,rot", [(70, 64, 48), (70, 128, 96), (40, 128, 112), (40, 128, 32), (9, 64, 16)])
+def test_partial_rotation_matches_plain_32_bits(paged, n, d, rot):
+    """Pairs (i, i + rot / 2) of the first dims: a partner's dims lie anywhere in the vector."""
+    q = _randn(1, n, 5, d).bfloat16().cuda()
+    k = _randn(2, n, 1, d).bfloat16().cuda()
+    cos, sin = paged.rope_tables(n, rot)
+    pos = torch.randperm(n, generator=torch.Generator().manual_seed(1)).int().cuda()
+    pages = paged.kv4_pages(n // 16 + 1, 1, d, 16)
+    out = paged.kv4_append(q, k, k, pages, torch.arange(n).cuda(), pos, cos, sin)
+    c, s = cos[pos.long()][:, None], sin[pos.long()][:, None]
+    y = q.float()
+    a, b = y[..., :rot // 2].clone(), y[..., rot // 2:rot].clone()
+    y[..., :rot // 2], y[..., rot // 2:rot] = a * c - b * s, b * c + a * s
+    assert torch.equal(out, y.bfloat16())
+
+
+@pytest.mark.parametrize("n,d", [(2501, 64), (4001, 64), (2003, 128)])
+def test_several_heads_a_warp(paged, n, d):
+    """Head counts that fill a warp's share of heads or leave a part of one: the same bits as in calls of
+    few tokens."""
+    hq, hkv, page = 41, 9, 64
+    q, k, v = (_randn(i, n, h, d).bfloat16().cuda() for i, h in ((1, hq), (2, hkv), (3, hkv)))
+    pages = paged.kv4_pages(n // page + 1, hkv, d, page)
+    slots, pos = torch.arange(n).flip(0).cuda(), torch.arange(n).int().cuda()
+    cos, sin = paged.rope_tables(n, d)
+    qw, kw = 1 + 0.1 * _randn(4, hq, d).cuda(), 1 + 0.1 * _randn(5, hkv, d).cuda()
+    few, parts = pages.clone(), []
+    out = paged.kv4_append(q, k, v, pages, slots, pos, cos, sin, q_norm=qw, k_norm=kw)
+    for a in range(0, n, 300):
+        b = slice(a, a + 300)
+        parts.append(paged.kv4_append(q[b], k[b], v[b], few, slots[b], pos[b], cos, sin, q_norm=qw, k_norm=kw))
+    assert torch.equal(out, torch.cat(parts)) and torch.equal(pages, few)
+    many = paged.kv4_read(pages, slots, d)
+    few = [paged.kv4_read(pages, slots[a:a + 300], d) for a in range(0, n, 300)]
+    for i in (0, 1):
+        assert torch.equal(many[i], torch.cat([x[i] for x in few]))
+
+
 def test_append_empty_and_no_queries(paged):
     pages = paged.kv4_pages(2, 2)
     e = torch.empty(0, 2, 64, dtype=torch.bfloat16, device="cuda")
