@@ -34,10 +34,16 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
-_Strides = C.c_int64 * 6
+@functools.lru_cache(maxsize=64)
+def _strides(*of):
+    return (C.c_int64 * len(of))(*of)
+
+
 # The current stream's handle; torch's own function for it, where it has one, costs 2 us less than
-# building a Stream object, as much as a small kernel takes.
+# building a Stream object, as much as a small kernel takes. A CUDA tensor is there when they are
+# asked, so torch's state is set up.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _entries: dict = {}
 
 
@@ -48,7 +54,7 @@ def _call(name, dev, *args):
         fn = _entries[name] = getattr(_lib.load(), name)
     index = dev.index
     stream = _raw_stream(index) if _raw_stream else torch.cuda.current_stream(dev).cuda_stream
-    if torch.cuda.current_device() == index:
+    if _current_device() == index:
         status = fn(*args, stream)
     else:
         with torch.cuda.device(dev):
@@ -91,9 +97,8 @@ def _cache(pages, head_dim):
     if pages.dtype != _U8 or pages.dim() != 3 or not pages.is_cuda or not pages.is_contiguous():
         _refuse("pages must be a contiguous uint8 CUDA tensor [num_pages, kv heads, page bytes]")
     num, hkv, nbytes = pages.shape
-    page_size = nbytes * 16 // (20 * head_dim) if head_dim > 0 else 0
-    if head_dim not in (64, 128) or page_size < 16 or page_size & (page_size - 1) or (
-            page_size * 20 * head_dim != nbytes * 16):
+    page_size = nbytes * 4 // (5 * head_dim) if head_dim > 0 else 0
+    if head_dim not in (64, 128) or page_size < 16 or page_size & (page_size - 1) or page_size * 5 * head_dim != nbytes * 4:
         _refuse(f"pages of {nbytes} bytes a kv head: no cache of head_dim {head_dim} (64 or 128) with a power of two "
                 "of tokens, at least 16, in a page")
     return num, hkv, page_size
@@ -193,7 +198,7 @@ def kv4_append(q, k, v, pages, slots, positions=None, cos=None, sin=None, *, q_n
         if w is not None and (w.dtype != _F32 or w.shape != (heads, hd) or w.device != dev or not w.is_contiguous()):
             _refuse(f"{name} must be a contiguous float32 tensor [{heads}, {hd}] on {dev}")
     if n:
-        _call("pulsar_op_kv4_append", dev, _p(q), k.data_ptr(), v.data_ptr(), _Strides(qt, qh, kt, kh, vt, vh), n, hq,
+        _call("pulsar_op_kv4_append", dev, _p(q), k.data_ptr(), v.data_ptr(), _strides(qt, qh, kt, kh, vt, vh), n, hq,
               hkv, hd, _p(q_norm), _p(k_norm), eps, _p(cos), _p(sin), rot, max_pos, int(interleaved), _p(q_gain),
               _p(positions), slots.data_ptr(), pages.data_ptr(), num, page_size, _p(out))
     return out
@@ -207,7 +212,7 @@ def kv4_read(pages, slots, head_dim: int = 64):
     _vector(slots, "slots", _I64, None, dev)
     n = slots.shape[0]
     k = torch.empty(n, hkv, head_dim, dtype=_BF16, device=dev)
-    v = torch.empty(n, hkv, head_dim, dtype=_BF16, device=dev)
+    v = torch.empty_like(k)
     if n:
         _call("pulsar_op_kv4_read", dev, pages.data_ptr(), num, page_size, hkv, head_dim, slots.data_ptr(), n,
               k.data_ptr(), v.data_ptr())
@@ -263,7 +268,7 @@ def kv4_attention(q, pages, block_table, kv_lens, cu_q=None, *, max_q: int = 1, 
     elif not scale > 0:
         _refuse(f"scale must be positive, got {scale}")
     if out is None:
-        out = torch.empty(n, hq, hd, dtype=_BF16, device=dev)
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(n, hq, hd, dtype=_BF16, device=dev)
     elif out.dtype != _BF16 or out.shape != q.shape or out.device != dev or not out.is_contiguous():
         _refuse("out must be a contiguous bfloat16 tensor of q's shape")
     if n and b:
