@@ -12,10 +12,13 @@
 //
 // A unit is a (query row, head of the kv head's group). CTA (split and unit tile, kv head,
 // sequence): four warps, each walking every fourth pair of 16-token tiles of the split's range
-// through a ring of its own (1-D bulk copies of whole tiles; each lane looks after every 32nd pair). Tokens are the M rows of S^T = K Q^T and units its N
-// columns, so a tile's codes are unpacked once for all units, straight into operand registers; the
-// weights pass through movmatrix into the B operand of O^T = V^T P^T. Up to four units the eight
-// columns hold every unit twice and the copies carry the hi and the lo halves.
+// through a ring of its own (1-D bulk copies of whole tiles; each lane looks after every 32nd
+// pair). Tokens are the M rows of S^T = K Q^T and units its N columns, so a tile's codes are
+// unpacked once for all units, straight into operand registers; the weights pass through movmatrix
+// into the B operand of O^T = V^T P^T. Up to four units the eight columns hold every unit twice and
+// the copies carry the hi and the lo halves (256 sequences of 640 keys: 19.5 us, with both halves
+// multiplied one after the other 20.0). Above eight units keys and values are unpacked to fp16 numbers
+// instead (see wide_step): 64 x 5 rows of 4 heads on 1024 keys take 24 us, with codes as operands 38.
 //
 // The softmax keeps a maximum per unit that moves only when a sum of weights relative to it passes
 // 2^LAZY (l and O use the same maximum, so the result does not depend on when it moves).
@@ -24,6 +27,12 @@
 //
 // Splits of the keys end in (m, l, O) partials, joined in split order: up to eight splits that fit the
 // GPU at once are a cluster and read each other's shared memory, else k_kv4_merge follows.
+//
+// Time and what bounds it (4 kv heads of 64, 16 query heads): 4 x 32768 keys 19.3 us, 2.2 TB/s of cache;
+// 256 x 513..767 21.9 us; 48 x 1..8191, 8 kv heads of 128, 77 us, 3.3 TB/s; 1 x 2048 6.5 us. The
+// copies alone take 13.7, 13.3, 50 and 5.8 us. The rest is issue slots: about 400 instructions for a pair of
+// tiles (heads of 128: 740) and 1000 a warp for its start and end, at 2 to 2.6 a clock and SM with 16
+// warps there.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -87,6 +96,11 @@ constexpr float pow2(int e) {   // 2^e (constant expressions only)
 __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ uint32_t cut(float a, float b) {   // both towards zero
+    uint32_t v;
+    asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(b), "f"(a));
+    return v;
 }
 __device__ __forceinline__ float lo_of(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float hi_of(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
@@ -185,8 +199,10 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
 
     // queries: B operand of step j (dims 16 j ..): unit n = lane / 4, dims 2t, 2t + 1 and 8 further
     uint32_t qf[NT][2 * MT];
-    // sum of q over the group, in the units of the scores; WIDE: exponent taken out of q times scale, in [0]
-    float qsum[NT][NG][2];
+    // Sums of q over the groups, in the units of the scores: B operand that meets the keys' z, k = 2t and
+    // 2t + 1 (and 8 further) groups 0 and 1 (2 and 3), the three bf16 terms of their sums on t = 0..2.
+    uint32_t zq[NT][2] = {};
+    float q_scale[NT][2];   // WIDE: scale times the power of two taken out of q
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const int u = u0 + (DUP ? (r & 3) : nt * 8 + r);
@@ -204,8 +220,8 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const int eq = min(max((int)(top >> 23) - 127 - 3, -100), 100);
             const float f = kv4_exp2i(-eq), s = a.scale_log2 * kv4_exp2i(eq);
-            qsum[nt][0][0] = __shfl_sync(0xffffffffu, s, 8 * t);
-            qsum[nt][0][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
+            q_scale[nt][0] = __shfl_sync(0xffffffffu, s, 8 * t);
+            q_scale[nt][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
 #pragma unroll
             for (int i = 0; i < 2 * MT; ++i) qf[nt][i] = kv4_half2(lo_of(qf[nt][i]) * f, hi_of(qf[nt][i]) * f);
         } else {
@@ -217,8 +233,9 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
                 s += __shfl_xor_sync(0xffffffffu, s, 1);
                 s += __shfl_xor_sync(0xffffffffu, s, 2);
                 s *= pow2(LIFT - CODE_EXP);
-                qsum[nt][g4][0] = __shfl_sync(0xffffffffu, s, 8 * t);
-                qsum[nt][g4][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
+                const float s1 = s - lo_of(pack(s, s)), s2 = s1 - lo_of(pack(s1, s1));
+                const uint32_t term = t == 0 ? pack(s, s) : t == 1 ? pack(s1, s1) : t == 2 ? pack(s2, s2) : 0u;
+                zq[nt][g4 >> 1] = g4 & 1 ? __byte_perm(zq[nt][g4 >> 1], term, 0x5410) : term;
             }
 #pragma unroll
             for (int i = 0; i < 2 * MT; ++i) {   // odd registers meet 16 c
@@ -253,8 +270,7 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
         nm[nt][0] = nm[nt][1] = -NEG * a.scale_log2;
         l[nt][0] = l[nt][1] = 0.f;
     }
-    // columns 4..7 of the doubled units (t >= 2) carry the lo halves: x = w lo_w + hi lo_h
-    const float lo_w = t < 2 ? 0.f : 1.f, lo_h = t < 2 ? 1.f : -1.f;
+    const uint32_t hi_mask = DUP && t < 2 ? 0u : 0xffff0000u;   // columns 4..7 of the doubled units (t >= 2) carry the lo halves
     uint32_t bad[NT][2] = {};   // WIDE: groups of V stored as NaN that the column sees
     int failed = -1;   // the pair whose copy did not land within the bound
 
@@ -272,23 +288,26 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
 #pragma unroll
             for (int y = 0; y < 2 * NG; y += 4)
                 *reinterpret_cast<uint4*>(&kp[0][0] + y) = *reinterpret_cast<const uint4*>(kt + T::KP + r * 8 * NG + y * 4);
+            uint32_t az[4] = {};   // z of the keys
+#pragma unroll
+            for (int y = 0; y < NG; ++y) az[y] = __byte_perm(kp[y & 1][y & 2], kp[y & 1][(y & 2) + 1], 0x7632);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                sc[x][nt][0] = sc[x][nt][1] = sc[x][nt][2] = sc[x][nt][3] = 0.f;
+                mma16816(sc[x][nt], az, zq[nt][0], zq[nt][1], sc[x][nt]);
+            }
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 uint32_t a0[4], a1[4];
                 unpack(kc[g >> 1][g & 1], a0[0], a0[2], a1[0], a1[2]);
                 unpack(kc[g >> 1][2 + (g & 1)], a0[1], a0[3], a1[1], a1[3]);
-                const float s0 = kv4_s(kp[0][g]), y0 = kv4_z(kp[0][g]), s8 = kv4_s(kp[1][g]), y8 = kv4_z(kp[1][g]);
+                const float s0 = kv4_s(kp[0][g]), s8 = kv4_s(kp[1][g]);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     float acc[4] = {0.f, 0.f, 0.f, 0.f};
                     mma16816(acc, a0, qf[nt][4 * g], qf[nt][4 * g + 1], acc);
                     mma16816(acc, a1, qf[nt][4 * g + 2], qf[nt][4 * g + 3], acc);
-                    const float q0 = qsum[nt][g][0], q1 = qsum[nt][g][1];
                     float* c = sc[x][nt];
-                    c[0] = g == 0 ? y0 * q0 : fmaf(y0, q0, c[0]);
-                    c[1] = g == 0 ? y0 * q1 : fmaf(y0, q1, c[1]);
-                    c[2] = g == 0 ? y8 * q0 : fmaf(y8, q0, c[2]);
-                    c[3] = g == 0 ? y8 * q1 : fmaf(y8, q1, c[3]);
                     c[0] = fmaf(s0, acc[0], c[0]);
                     c[1] = fmaf(s0, acc[1], c[1]);
                     c[2] = fmaf(s8, acc[2], c[2]);
@@ -388,15 +407,13 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
                         za[0] = fmaf(pp[0], z0, fmaf(pp[2], z8, za[0]));
                         za[1] = fmaf(pp[1], z0, fmaf(pp[3], z8, za[1]));
                     }
-                    float wh[4];   // hi halves, cut
+                    float wh[4];   // hi halves, cut (DUP: of the columns that carry the lo halves, else 0)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) wh[e] = hi_of(__float_as_uint(w[e]));
+                    for (int e = 0; e < 4; ++e) wh[e] = __uint_as_float(__float_as_uint(w[e]) & hi_mask);
                     uint32_t pa, pb;
                     if (DUP) {
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) w[e] = fmaf(wh[e], lo_h, w[e] * lo_w);
-                        pa = pack(w[0], w[1]);
-                        pb = pack(w[2], w[3]);
+                        pa = cut(w[0] - wh[0], w[1] - wh[1]);
+                        pb = cut(w[2] - wh[2], w[3] - wh[3]);
                     } else {
                         pa = __byte_perm(__float_as_uint(w[0]), __float_as_uint(w[1]), 0x7632);
                         pb = __byte_perm(__float_as_uint(w[2]), __float_as_uint(w[3]), 0x7632);
@@ -446,8 +463,8 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
         float sc[2][NT][4], kq[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            kq[nt][0] = qsum[nt][0][0] * kv4_exp2i(ek);
-            kq[nt][1] = qsum[nt][0][1] * kv4_exp2i(ek);
+            kq[nt][0] = q_scale[nt][0] * kv4_exp2i(ek);
+            kq[nt][1] = q_scale[nt][1] * kv4_exp2i(ek);
         }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
@@ -787,14 +804,24 @@ struct Plan {
 };
 
 // How a call is cut. More than MANY units of a sequence's rows go to k_kv4_prefill, 512 or 256 a CTA.
+// Measured (this kernel / that one, us), heads of 64: 8 x 4096 keys, 16 units 24 / 29, 32 36 / 30, 48 43 /
+// 31, 128 60 / 33; 1 x 16384, 32 units 20 / 22, 64 25 / 23, 128 44 / 25; 64 x 2048, 32 units 38 / 87, 64 75
+// / 88, 96 113 / 88; heads of 128: 8 x 4096, 16 units 34 / 35, 32 45 / 38, 64 60 / 39; 64 x 2048, 32
+// units 87 / 109, 48 128 / 110.
 // Others: the fewest columns that hold max_q rows of a group (four: both halves of the weights in
 // one operand), at most 32 (heads of 128: 16, for the registers).
 // Splits of the keys: until the SMs are full (four CTAs each; two above 8 units), of at least 8 pairs of
-// tiles (two a warp); where
-// there are many keys, of 32 to 64 pairs, so that sequences shorter than max_kv even out (the splits
-// that they lack end at once). k_kv4_prefill: the number that fills the last wave best.
+// tiles (two a warp); where there are many keys, of 32 to 64 pairs, so that sequences shorter than
+// max_kv even out (the splits that they lack end at once). Measured: 4 x 32768, 18 to 37 splits 19 to 19.6
+// us, 8 31, 74 23; 256 x 640, one 21.8, two 27; 48 x 1..8191 of heads of 128, 2 / 4 / 8 / 12 / 16 splits 93 /
+// 81 / 77 / 81 / 83; 64 x 5 rows on 1024 keys, 1 / 2 / 3 splits 24 / 38 / 45. k_kv4_prefill: the number
+// that fills the last wave best.
 // Two warps instead of four where there is a CTA for every unit tile and each has few keys: what a CTA
-// costs besides its keys is paid per warp.
+// costs besides its keys is paid per warp (256 x 640: 21.8 us, with four 22.6).
+// A cluster joins its splits through shared memory where there are at most eight and all fit at once.
+// Measured against partials in memory and k_kv4_merge: 1 x 2048 6.2 / 6.5 us (on the host 12 / 22 a
+// call: one launch and no workspace), 16 x 1024 6.7 / 7.7, 4 x 1024 with 5 rows 13.4 / 14.9, heads of
+// 128, 16 x 2048 12.4 / 13.4, 1 x 512 8.4 / 7.8.
 constexpr int64_t MANY = 32;
 Plan make_plan(int64_t B, int64_t Hkv, int64_t group, int64_t head_dim, int64_t max_q, int64_t max_kv,
                int64_t window) {
@@ -873,7 +900,9 @@ int launch(const Kv4AttnArgs& a, const Plan& p, int64_t B, cudaStream_t st) {
 }
 
 // The merge is launched under the attention kernel's end; it waits for that before it reads. Up to
-// four splits a group of threads takes them all.
+// four splits a group of threads takes them all, above all groups of a block share those of one row:
+// with one group / all, 64 x 2048 in 4 splits 18.9 / 20.4 us, 2048 rows on 16384 in 2 240 / 277,
+// 4 x 32768 in 37 25.7 / 20.2, 8 splits even.
 template <int HD>
 int launch_merge(const Kv4AttnArgs& a, int64_t B, cudaStream_t st) {
     constexpr int ALL = 512 / HD;   // groups of a block
@@ -927,7 +956,7 @@ extern "C" int pulsar_op_kv4_attention(const void* q, int64_t q_row_stride, int6
                      "kv4_attention: page_size must be a power of two of at least 16, got %lld", (long long)page_size);
     PULSAR_CHECK_ARG(num_pages >= 0 && num_pages < (int64_t)1 << 31 && width >= 0 && width * page_size < (int64_t)1 << 30,
                      "kv4_attention: invalid page table");
-    PULSAR_CHECK_ARG(scale > 0.f, "kv4_attention: scale must be positive");
+    PULSAR_CHECK_ARG(scale > 0.f && scale < INFINITY, "kv4_attention: scale must be positive and finite");
     PULSAR_CHECK_ARG(cu_q || (N == B && max_q == 1), "kv4_attention: without cu_q every sequence has one row");
     if (N == 0 || B == 0) return PULSAR_OK;
     PULSAR_CHECK_ARG(q && pages && kv_lens && out && (block_table || width == 0), "kv4_attention: null pointer");

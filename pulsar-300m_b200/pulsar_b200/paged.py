@@ -265,8 +265,8 @@ def kv4_attention(q, pages, block_table, kv_lens, cu_q=None, *, max_q: int = 1, 
         _refuse("max_q and max_kv must be at least 1, window at least 0")
     if scale is None:
         scale = hd ** -0.5
-    elif not scale > 0:
-        _refuse(f"scale must be positive, got {scale}")
+    elif not 0 < scale < math.inf:
+        _refuse(f"scale must be positive and finite, got {scale}")
     if out is None:
         out = torch.empty_like(q) if q.is_contiguous() else torch.empty(n, hq, hd, dtype=_BF16, device=dev)
     elif out.dtype != _BF16 or out.shape != q.shape or out.device != dev or not out.is_contiguous():
