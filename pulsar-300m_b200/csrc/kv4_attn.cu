@@ -5,10 +5,10 @@
 // max(0, pos - window + 1) .. pos (window 0: all of 0 .. pos):
 //   out = sum_k p_k v_k / sum_k p_k,  p_k = exp(scale q.k_k - m)
 // with k = s c + z per group of 32 dims, so q.k = sum_g s_g (q.c)_g + z_g sum(q)_g: the codes enter
-// the matrix instruction as they are (exact, see unpack) and s, z are applied in fp32 to its
-// results. Values: O = sum_k (p_k s_kg) c + sum_k p_k z_kg: s goes into the weights, whose bf16 hi
-// and lo halves are both multiplied (|x - hi - lo| <= 2^-16 |x|), and the second sum is a scalar per
-// (row, group).
+// the matrix instruction as they are (exact, see unpack) and s is applied in fp32 to its results;
+// z meets the three bf16 terms of sum(q) in an instruction of its own. Values: O = sum_k (p_k s_kg) c
+// + sum_k p_k z_kg: s goes into the weights, whose bf16 hi and lo halves (cut, |x - hi - lo| <=
+// 2^-15 |x|) are both multiplied, and the second sum is a scalar per (row, group).
 //
 // A unit is a (query row, head of the kv head's group). CTA (split and unit tile, kv head,
 // sequence): four warps, each walking every fourth pair of 16-token tiles of the split's range
@@ -28,10 +28,10 @@
 // Splits of the keys end in (m, l, O) partials, joined in split order: up to eight splits that fit the
 // GPU at once are a cluster and read each other's shared memory, else k_kv4_merge follows.
 //
-// Time and what bounds it (4 kv heads of 64, 16 query heads): 4 x 32768 keys 19.3 us, 2.2 TB/s of cache;
-// 256 x 513..767 21.9 us; 48 x 1..8191, 8 kv heads of 128, 77 us, 3.3 TB/s; 1 x 2048 6.5 us. The
-// copies alone take 13.7, 13.3, 50 and 5.8 us. The rest is issue slots: about 400 instructions for a pair of
-// tiles (heads of 128: 740) and 1000 a warp for its start and end, at 2 to 2.6 a clock and SM with 16
+// Time and what bounds it (4 kv heads of 64, 16 query heads): 4 x 32768 keys 18.0 us, 2.3 TB/s of cache;
+// 256 x 513..767 20.2 us; 48 x 1..8191, 8 kv heads of 128, 71.5 us, 3.5 TB/s; 1 x 2048 6.5 us. The
+// copies alone took 13.7, 13.3, 50 and 5.8 us. The rest is issue slots: about 380 instructions for a pair of
+// tiles (heads of 128: 680) and 1000 a warp for its start and end, at 2 to 2.6 a clock and SM with 16
 // warps there.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -108,12 +108,12 @@ __device__ __forceinline__ float hi_of(uint32_t v) { return __uint_as_float(v & 
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// *p of the cluster's CTA `rank`.
-__device__ __forceinline__ float ld_cluster(const float* p, int rank) {
+// The pair at p of the cluster's CTA `rank`.
+__device__ __forceinline__ float2 ld_cluster(const float* p, int rank) {
     uint32_t at;
-    float v;
+    float2 v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
     return v;
 }
 
@@ -195,7 +195,10 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
         }
     };
     Where here = locate(0), next = here;   // of the 32 pairs that hold the current one, the next one to issue
-    if (lane < min(S, mine)) issue(lane, here);
+    // The first pair alone, the others of the ring once the queries are there: copies of an SM are served in
+    // the order of issue, so every warp starts after a quarter of the rings instead of all of them
+    // (4 x 32768: 19.3 -> 18.0 us).
+    if (lane == 0 && mine > 0) issue(0, here);
 
     // queries: B operand of step j (dims 16 j ..): unit n = lane / 4, dims 2t, 2t + 1 and 8 further
     uint32_t qf[NT][2 * MT];
@@ -255,6 +258,8 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
             lo[nt][c] = kv4_low(a, pos);
         }
     const int all_lo = kv4_low(a, rg.last), all_hi = rg.first + 1;   // keys in [all_lo, all_hi) are seen by every unit
+
+    if (lane > 0 && lane < min(S, mine)) issue(lane, here);
 
     // Scores come in units of 2^(LIFT - CODE_EXP); m: their running maximum, nm = LIFT - scale m, so
     // that weights are 2^LIFT exp2(scale (s - m)). WIDE: m is the reference of the weights 2^(x - m), base 2
@@ -677,57 +682,59 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
     __syncthreads();
     const float* all = reinterpret_cast<const float*>(sm);
     float* mine_o = reinterpret_cast<float*>(sm) + WARPS * UT * (HD + 2);   // cluster: the CTA's own, for the others
-    const int items = (ulast - u0 + 1) * HD;
+    const int items = (ulast - u0 + 1) * (HD / 2);   // two dims each
     auto place = [&](int u) {
         const int j = kv4_row(a, u0 + u), g = (u0 + u) - j * a.group;
         return (int64_t)(row0 + j) * a.hq + h * a.group + g;
     };
+    auto answer = [&](int u, int d, float ll, float2 oo) {
+        const __nv_bfloat162 v = ll == 0.f ? __floats2bfloat162_rn(0.f, 0.f) : __floats2bfloat162_rn(oo.x / ll, oo.y / ll);
+        *reinterpret_cast<__nv_bfloat162*>(a.out + place(u) * HD + d) = v;
+    };
     for (int i = tid; i < items; i += WARPS * 32) {
-        const int u = i / HD, d = i % HD;
-        float mm = NEG, ll = 0.f, oo = 0.f;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, all[(w * UT + u) * (HD + 2) + HD]);
+        const int u = i / (HD / 2), d = i % (HD / 2) * 2;
+        float mm = NEG, ll = 0.f;
+        float2 oo = make_float2(0.f, 0.f), ml[WARPS];
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
-            const float* p = all + (w * UT + u) * (HD + 2);
-            const float f = kv4_ex2(p[HD] - mm);
-            ll = fmaf(f, p[HD + 1], ll);
-            oo = fmaf(f, p[d], oo);
+            ml[w] = *reinterpret_cast<const float2*>(all + (w * UT + u) * (HD + 2) + HD);
+            mm = fmaxf(mm, ml[w].x);
+        }
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float f = kv4_ex2(ml[w].x - mm);
+            const float2 p = *reinterpret_cast<const float2*>(all + (w * UT + u) * (HD + 2) + d);
+            ll = fmaf(f, ml[w].y, ll);
+            oo = make_float2(fmaf(f, p.x, oo.x), fmaf(f, p.y, oo.y));
         }
         if (a.cluster) {
             float* p = mine_o + u * (HD + 2);
-            p[d] = oo;
-            if (d == 0) {
-                p[HD] = mm;
-                p[HD + 1] = ll;
-            }
-            continue;
-        }
-        const int64_t at = place(u);
-        if (rg.used == 1) {
-            a.out[at * HD + d] = __float2bfloat16(ll == 0.f ? 0.f : oo / ll);
+            *reinterpret_cast<float2*>(p + d) = oo;
+            if (d == 0) *reinterpret_cast<float2*>(p + HD) = make_float2(mm, ll);
+        } else if (rg.used == 1) {
+            answer(u, d, ll, oo);
         } else {
-            a.part_o[(at * a.nsplit + split) * HD + d] = oo;
-            if (d == 0) {
-                a.part_ml[(at * a.nsplit + split) * 2] = mm;
-                a.part_ml[(at * a.nsplit + split) * 2 + 1] = ll;
-            }
+            const int64_t at = place(u) * a.nsplit + split;
+            *reinterpret_cast<float2*>(a.part_o + at * HD + d) = oo;
+            if (d == 0) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(mm, ll);
         }
     }
     if (!a.cluster) return;
     // the splits are a cluster: each CTA joins a part of the dims from all of their shared memories
     cluster_sync();
     for (int i = split * WARPS * 32 + tid; i < items; i += a.nsplit * WARPS * 32) {
-        const int u = i / HD, d = i % HD;
+        const int u = i / (HD / 2), d = i % (HD / 2) * 2;
         const float* p = mine_o + u * (HD + 2);
-        float mm = NEG, ll = 0.f, oo = 0.f;
-        for (int sp = 0; sp < a.nsplit; ++sp) mm = fmaxf(mm, ld_cluster(p + HD, sp));
+        float mm = NEG, ll = 0.f;
+        float2 oo = make_float2(0.f, 0.f);
+        for (int sp = 0; sp < a.nsplit; ++sp) mm = fmaxf(mm, ld_cluster(p + HD, sp).x);
         for (int sp = 0; sp < a.nsplit; ++sp) {
-            const float f = kv4_ex2(ld_cluster(p + HD, sp) - mm);
-            ll = fmaf(f, ld_cluster(p + HD + 1, sp), ll);
-            oo = fmaf(f, ld_cluster(p + d, sp), oo);
+            const float2 ml = ld_cluster(p + HD, sp), x = ld_cluster(p + d, sp);
+            const float f = kv4_ex2(ml.x - mm);
+            ll = fmaf(f, ml.y, ll);
+            oo = make_float2(fmaf(f, x.x, oo.x), fmaf(f, x.y, oo.y));
         }
-        a.out[place(u) * HD + d] = __float2bfloat16(ll == 0.f ? 0.f : oo / ll);
+        answer(u, d, ll, oo);
     }
     cluster_sync();   // nobody leaves while its shared memory is read
 }
