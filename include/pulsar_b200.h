@@ -133,7 +133,7 @@ int pulsar_op_moe_dispatch(const void* x_dev, const int64_t* topk_idx_dev, const
  * first rot dims (rot 0: none): pairs (i, i + rot / 2), rot a multiple of 16, or (2i, 2i + 1) when
  * interleaved, rot even. q_gain [max_pos] f32 or NULL: factor of the queries of a position.
  * positions [N] i32 (may be NULL without tables); slots [N] i64, distinct. q_out [N, Hq, head_dim]
- * bf16 contiguous. A token with a slot outside the cache or a position outside the tables is not
+ * bf16 contiguous. Norm weights, tables and q_out 16-byte aligned. A token with a slot outside the cache or a position outside the tables is not
  * stored; in the latter case its query is zero. */
 int pulsar_op_kv4_append(const void* q_dev, const void* k_dev, const void* v_dev, const int64_t* strides_host,
                          int64_t N, int64_t Hq, int64_t Hkv, int64_t head_dim, const float* q_norm_dev,
@@ -158,8 +158,10 @@ int pulsar_op_kv4_attention_workspace(int64_t N, int64_t Hq, int64_t Hkv, int64_
  * of these. q [N, Hq, head_dim] bf16 with even element strides, Hq a multiple of Hkv. max_kv bounds
  * kv_lens and only decides how the work is split. out [N, Hq, head_dim] bf16: softmax(scale q k^T) v,
  * 0 for a row that sees no key; rows of no sequence are not written. Page numbers outside the cache
- * count as masked. workspace_dev: scratch of at least pulsar_op_kv4_attention_workspace bytes, which
- * calls on different streams must not share. */
+ * count as masked; scale is positive and finite. q 4-byte, out and the workspace 16-byte aligned.
+ * Up to 8 units (max_q times heads of a group) the operands are good to 2^-15, above that to 2^-12
+ * (fp16 with powers of two taken out); sums are 32-bit. workspace_dev: scratch of at least
+ * pulsar_op_kv4_attention_workspace bytes, which calls on different streams must not share. */
 int pulsar_op_kv4_attention(const void* q_dev, int64_t q_row_stride, int64_t q_head_stride, int64_t N, int64_t Hq,
                             int64_t head_dim, const void* pages_dev, int64_t num_pages, int64_t page_size,
                             int64_t Hkv, const int32_t* block_table_dev, int64_t B, int64_t width,

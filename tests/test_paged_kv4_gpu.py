@@ -2,7 +2,7 @@
 
 Tolerances. A bf16 result is rounded once: relative 2^-9, taken as 2^-8 with the 32-bit work before
 it. A stored value is off by half a step s / 2 plus what the rounding of s (15 s 2^-9) and of the
-minimum z (|z| 2^-9) to bf16 add. Attention accumulates in 32 bits with operands good to 2^-16:
+minimum z (|z| 2^-9) to bf16 add. Attention accumulates in 32 bits with operands good to 2^-15:
 2^-12 of the largest value that a row sees, besides the rounding of the result. Above 8 units a kv
 head the operands are fp16 (keys and values rounded twice, weights once, at 2^-12, and a quarter of
 the weights good to 2^-13): 4 2^-12 of the largest value, and 2 2^-12 scale sum |q k| in a score, so
@@ -534,6 +534,50 @@ def test_large_cache_offsets(paged):
     assert torch.equal(big, paged.kv4_attention(q, small, torch.tensor([[2, 0]], dtype=torch.int32).cuda(), n))
 
 
+def test_graph_replays_follow_lengths_and_slots(paged):
+    """A decode step captured once (append, attention in splits with their merge) serves later steps: slots,
+    positions, lengths and inputs are read on the device."""
+    B, hq, hkv, d, page, width = 24, 16, 4, 64, 64, 40
+    pages = paged.kv4_pages(B * width, hkv, d, page)
+    table = torch.randperm(B * width, generator=torch.Generator().manual_seed(1)).int().view(B, width).cuda()
+    start = torch.randint(1500, 2500, (B,), generator=torch.Generator().manual_seed(2)).cuda()
+    old = torch.arange(2500, device="cuda").repeat(B, 1)
+    slots = torch.where(old < start[:, None], table.long().gather(1, old // page) * page + old % page, -1).flatten()
+    k, v = (_randn(i, B * 2500, hkv, d).cuda().bfloat16() for i in (3, 4))
+    paged.kv4_append(None, k, v, pages, slots)
+    cos, sin = paged.rope_tables(width * page)
+    qkv = [_randn(10 + i, B, hq + 2 * hkv, d).cuda().bfloat16() for i in range(3)]
+    x, lens, slot = qkv[0].clone(), start.int(), torch.empty(B, dtype=torch.int64, device="cuda")
+
+    def step():
+        torch.add(table.long().gather(1, (lens.long() // page)[:, None])[:, 0] * page, lens.long() % page, out=slot)
+        q = paged.kv4_append(x[:, :hq], x[:, hq:hq + hkv], x[:, hq + hkv:], pages, slot, lens, cos, sin)
+        lens.add_(1)
+        return paged.kv4_attention(q, pages, table, lens)
+
+    empty = pages.clone()
+    want = []
+    for i in range(3):
+        x.copy_(qkv[i])
+        want.append(step())
+    pages.copy_(empty)
+    lens.copy_(start)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    pages.copy_(empty)
+    lens.copy_(start)
+    for i in range(3):
+        x.copy_(qkv[i])
+        graph.replay()
+        assert torch.equal(got, want[i])
+
+
 # -------------------------------------------------------------------------------------- refusals
 def test_refusals(paged):
     pages = paged.kv4_pages(4, 2, 64, 16)
@@ -567,3 +611,12 @@ def test_refusals(paged):
     refuse("max_q", paged.kv4_attention, x, pages, table, lens, max_q=2)
     refuse("out", paged.kv4_attention, x, pages, table, lens, out=x.float())
     refuse("window", paged.kv4_attention, x, pages, table, lens, window=-1)
+
+
+def test_scale_is_positive_and_finite(paged):
+    pages = paged.kv4_pages(4, 2, 64, 16)
+    x = torch.zeros(3, 2, 64, dtype=torch.bfloat16, device="cuda")
+    table, lens = torch.zeros(3, 1, dtype=torch.int32, device="cuda"), torch.ones(3, dtype=torch.int32, device="cuda")
+    for scale in (0.0, -1.0, math.inf, math.nan):
+        with pytest.raises(RuntimeError, match="scale"):
+            paged.kv4_attention(x, pages, table, lens, scale=scale)
