@@ -159,9 +159,10 @@ int pulsar_op_kv4_attention_workspace(int64_t N, int64_t Hq, int64_t Hkv, int64_
  * kv_lens and only decides how the work is split. out [N, Hq, head_dim] bf16: softmax(scale q k^T) v,
  * 0 for a row that sees no key; rows of no sequence are not written. Page numbers outside the cache
  * count as masked; scale is positive and finite. q 4-byte, out and the workspace 16-byte aligned.
- * Up to 8 units (max_q times heads of a group) the operands are good to 2^-15, above that to 2^-12
- * (fp16 with powers of two taken out); sums are 32-bit. workspace_dev: scratch of at least
- * pulsar_op_kv4_attention_workspace bytes, which calls on different streams must not share. */
+ * Up to 8 units (max_q times heads of a group) the operands are good to 2^-16 and values may reach
+ * 2^37, above that to 2^-12 (fp16 with powers of two taken out); sums are 32-bit. workspace_dev:
+ * scratch of at least pulsar_op_kv4_attention_workspace bytes, which calls on different streams must
+ * not share. */
 int pulsar_op_kv4_attention(const void* q_dev, int64_t q_row_stride, int64_t q_head_stride, int64_t N, int64_t Hq,
                             int64_t head_dim, const void* pages_dev, int64_t num_pages, int64_t page_size,
                             int64_t Hkv, const int32_t* block_table_dev, int64_t B, int64_t width,

@@ -7,8 +7,8 @@
 // with k = s c + z per group of 32 dims, so q.k = sum_g s_g (q.c)_g + z_g sum(q)_g: the codes enter
 // the matrix instruction as they are (exact, see unpack) and s is applied in fp32 to its results;
 // z meets the three bf16 terms of sum(q) in an instruction of its own. Values: O = sum_k (p_k s_kg) c
-// + sum_k p_k z_kg: s goes into the weights, whose bf16 hi and lo halves (cut, |x - hi - lo| <=
-// 2^-15 |x|) are both multiplied, and the second sum is a scalar per (row, group).
+// + sum_k p_k z_kg: s goes into the weights, whose bf16 hi and lo halves (|x - hi - lo| <= 2^-17
+// |x|) are both multiplied, and the second sum is a scalar per (row, group).
 //
 // A unit is a (query row, head of the kv head's group). CTA (split and unit tile, kv head,
 // sequence): four warps, each walking every fourth pair of 16-token tiles of the split's range
@@ -47,7 +47,7 @@ using namespace pulsar;
 
 namespace {
 
-constexpr int LAZY = 30;
+constexpr int LAZY = 30;   // more than log2 of the keys of a row, and weights of 2^(LIFT + LAZY) times values stay in fp32 up to 2^37
 constexpr float NEG = KV4_NEG;
 
 // d = a b + c (d and c may be the same registers)
@@ -96,11 +96,6 @@ constexpr float pow2(int e) {   // 2^e (constant expressions only)
 __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&v);
-}
-__device__ __forceinline__ uint32_t cut(float a, float b) {   // both towards zero
-    uint32_t v;
-    asm("cvt.rz.bf16x2.f32 %0, %1, %2;" : "=r"(v) : "f"(b), "f"(a));
-    return v;
 }
 __device__ __forceinline__ float lo_of(uint32_t v) { return __uint_as_float(v << 16); }
 __device__ __forceinline__ float hi_of(uint32_t v) { return __uint_as_float(v & 0xffff0000u); }
@@ -275,7 +270,7 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
         nm[nt][0] = nm[nt][1] = -NEG * a.scale_log2;
         l[nt][0] = l[nt][1] = 0.f;
     }
-    const uint32_t hi_mask = DUP && t < 2 ? 0u : 0xffff0000u;   // columns 4..7 of the doubled units (t >= 2) carry the lo halves
+    const float minus_hi = t < 2 ? 0.f : -1.f;   // columns 4..7 of the doubled units (t >= 2) carry the lo halves
     uint32_t bad[NT][2] = {};   // WIDE: groups of V stored as NaN that the column sees
     int failed = -1;   // the pair whose copy did not land within the bound
 
@@ -412,23 +407,18 @@ __global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_a
                         za[0] = fmaf(pp[0], z0, fmaf(pp[2], z8, za[0]));
                         za[1] = fmaf(pp[1], z0, fmaf(pp[3], z8, za[1]));
                     }
-                    float wh[4];   // hi halves, cut (DUP: of the columns that carry the lo halves, else 0)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) wh[e] = __uint_as_float(__float_as_uint(w[e]) & hi_mask);
-                    uint32_t pa, pb;
-                    if (DUP) {
-                        pa = cut(w[0] - wh[0], w[1] - wh[1]);
-                        pb = cut(w[2] - wh[2], w[3] - wh[3]);
-                    } else {
-                        pa = __byte_perm(__float_as_uint(w[0]), __float_as_uint(w[1]), 0x7632);
-                        pb = __byte_perm(__float_as_uint(w[2]), __float_as_uint(w[3]), 0x7632);
+                    uint32_t pa = pack(w[0], w[1]), pb = pack(w[2], w[3]);   // hi halves
+                    const uint32_t ha = pa, hb = pb;
+                    if (DUP) {   // of the columns that carry the lo halves: those
+                        pa = pack(fmaf(lo_of(ha), minus_hi, w[0]), fmaf(hi_of(ha), minus_hi, w[1]));
+                        pb = pack(fmaf(lo_of(hb), minus_hi, w[2]), fmaf(hi_of(hb), minus_hi, w[3]));
                     }
                     const uint32_t b0 = movmatrix(pa), b1 = movmatrix(pb);
                     mma16816(o[2 * g][nt], a0, b0, b1, o[2 * g][nt]);
                     mma16816(o[2 * g + 1][nt], a1, b0, b1, o[2 * g + 1][nt]);
                     if (!DUP) {
-                        const uint32_t c0 = movmatrix(pack(w[0] - wh[0], w[1] - wh[1]));
-                        const uint32_t c1 = movmatrix(pack(w[2] - wh[2], w[3] - wh[3]));
+                        const uint32_t c0 = movmatrix(pack(w[0] - lo_of(ha), w[1] - hi_of(ha)));
+                        const uint32_t c1 = movmatrix(pack(w[2] - lo_of(hb), w[3] - hi_of(hb)));
                         mma16816(o[2 * g][nt], a0, c0, c1, o[2 * g][nt]);
                         mma16816(o[2 * g + 1][nt], a1, c0, c1, o[2 * g + 1][nt]);
                     }

@@ -237,6 +237,9 @@ def kv4_attention(q, pages, block_table, kv_lens, cu_q=None, *, max_q: int = 1, 
     there is one row for each sequence. ``max_kv`` bounds kv_lens (default: the table's width); it only
     decides how the work is split. ``scale`` defaults to D ** -0.5.
 
+    Sums are in 32 bits; up to 8 units (max_q times the heads of a group) operands are good to 2^-16 and
+    values may reach 2^37, above that they are good to 2^-12 at any size.
+
     A row that sees no key is zero. Lengths past the table end there; pages numbered outside the cache
     are left out as if masked; rows that no sequence claims are not written.
     """

@@ -2,7 +2,7 @@
 
 Tolerances. A bf16 result is rounded once: relative 2^-9, taken as 2^-8 with the 32-bit work before
 it. A stored value is off by half a step s / 2 plus what the rounding of s (15 s 2^-9) and of the
-minimum z (|z| 2^-9) to bf16 add. Attention accumulates in 32 bits with operands good to 2^-15:
+minimum z (|z| 2^-9) to bf16 add. Attention accumulates in 32 bits with operands good to 2^-16:
 2^-12 of the largest value that a row sees, besides the rounding of the result. Above 8 units a kv
 head the operands are fp16 (keys and values rounded twice, weights once, at 2^-12, and a quarter of
 the weights good to 2^-13): 4 2^-12 of the largest value, and 2 2^-12 scale sum |q k| in a score, so
@@ -411,6 +411,22 @@ def test_prompt_values_of_any_size(paged):
                                   torch.tensor([0, 60], dtype=torch.int32).cuda(), max_q=60, scale=0.2 / kx)
         hk, hv = held(pages, d)
         assert_attention(got, *plain_attention(q, hk, hv, table, lens, [0, 60], 0.2 / kx, 0), many=True)
+
+
+@pytest.mark.parametrize("hq,d", [(4, 64), (7, 128)])
+@pytest.mark.parametrize("kx,vx", [(2.0 ** -20, 2.0 ** 25), (2.0 ** 12, 2.0 ** -30), (1.0, 2.0 ** 32)])
+def test_decode_values_of_any_size(paged, hq, d, kx, vx):
+    lens, page = [400], 64
+    pages, table = _filled(paged, lens, 1, d, page)
+    k = _randn(1, 400, 1, d) * kx
+    v = _randn(2, 400, 1, d) * vx * torch.linspace(-3, 3, 400).exp2()[:, None, None]
+    slots = torch.tensor([table[0][i // page] * page + i % page for i in range(400)])
+    paged.kv4_append(None, k.cuda().bfloat16(), v.cuda().bfloat16(), pages, slots.cuda())
+    q = _randn(3, 1, hq, d).bfloat16().cuda()
+    got = paged.kv4_attention(q, pages, torch.tensor(table, dtype=torch.int32).cuda(),
+                              torch.tensor(lens, dtype=torch.int32).cuda(), scale=0.2 / kx)
+    hk, hv = held(pages, d)
+    assert_attention(got, *plain_attention(q, hk, hv, table, lens, [0, 1], 0.2 / kx, 0))
 
 
 @pytest.mark.parametrize("d,window,max_kv", [(64, 0, None), (64, 0, 2500), (128, 0, None), (64, 900, None), (64, 0, 64)])
