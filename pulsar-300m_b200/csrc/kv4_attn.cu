@@ -812,7 +812,9 @@ struct Plan {
 // max_kv even out (the splits that they lack end at once). Measured: 4 x 32768, 18 to 37 splits 19 to 19.6
 // us, 8 31, 74 23; 256 x 640, one 21.8, two 27; 48 x 1..8191 of heads of 128, 2 / 4 / 8 / 12 / 16 splits 93 /
 // 81 / 77 / 81 / 83; 64 x 5 rows on 1024 keys, 1 / 2 / 3 splits 24 / 38 / 45. k_kv4_prefill: the number
-// that fills the last wave best.
+// that the cost below finds best: 2048 rows on 16384 keys in 1 / 2 / 3 / 4 splits 441 / 241 / 321 / 254 us, on
+// 2048 keys 69 / 53 / 51 / 61, 4096 rows with a window of 1024 52 / 85 / 104 / 102, 1500 with one of 1000 on 16384
+// keys 55 / 48 / 46 / 63, 33 rows on 16000 keys in 1 / 8 / 32 splits 350 / 57 / 28.
 // Two warps instead of four where there is a CTA for every unit tile and each has few keys: what a CTA
 // costs besides its keys is paid per warp (256 x 640: 21.8 us, with four 22.6).
 // A cluster joins its splits through shared memory where there are at most eight and all fit at once.
@@ -842,15 +844,15 @@ Plan make_plan(int64_t B, int64_t Hkv, int64_t group, int64_t head_dim, int64_t 
     const int64_t ctas = B * Hkv * p.utiles;
     int64_t ns = 1;
     if (p.many) {
-        // in units of a step (about 1.8 us): waves of CTAs, each with the start and end of one, then the
-        // partials' way through memory and the merge
+        // in units of a step (3.45 us): waves of CTAs, each with 4 for its start and end, then the partials'
+        // way through memory and the merge
         const int64_t most = steps / 2 < 64 ? steps / 2 : 64;
         double best = 1e30;
         for (int64_t s = 1; s <= most || s == 1; ++s) {
             const double waves = (double)((ctas * s + 147) / 148), len = (double)((steps + s - 1) / s);
-            const double merge = s > 1 ? 2 + (double)(B * Hkv * units) * s * (head_dim + 2) * 8 / 7.2e6 : 0;
-            if (waves * (len + 2) + merge < best) {
-                best = waves * (len + 2) + merge;
+            const double merge = s > 1 ? 0.6 + (double)(B * Hkv * units) * s * (head_dim + 2) * 8 / 13.8e6 : 0;
+            if (waves * (len + 4) + merge < best) {
+                best = waves * (len + 4) + merge;
                 ns = s;
             }
         }

@@ -181,7 +181,8 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
     Misc& ms = *reinterpret_cast<Misc*>(sm + L::MISC);
     volatile int* abort = &ms.abort;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int split = blockIdx.x % a.nsplit, u0 = blockIdx.x / a.nsplit * L::UNITS;
+    // the last units first, which see the most keys (8192 rows on 8192 keys: 352 -> 314 us)
+    const int split = blockIdx.x % a.nsplit, u0 = (gridDim.x / a.nsplit - 1 - blockIdx.x / a.nsplit) * L::UNITS;
     const int h = blockIdx.y, b = blockIdx.z;
 
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the merge may be set up meanwhile
