@@ -12,7 +12,7 @@
 // What bounds the kernel are the exponentials (16 a clock and SM). A tile's chain of MMA, scores,
 // weights and MMA is longer than its exponentials take, so four tiles are in flight at different
 // places of it, each with a softmax warp on every scheduler (heads of 128: the two that TMEM holds).
-// 2048 rows of 16 heads of 64 on 16384 keys (4 kv heads) take 240 us: 0.54 PFLOP/s of products, and
+// 2048 rows of 16 heads of 64 on 16384 keys (4 kv heads) take 238 us: 0.54 PFLOP/s of products, and
 // 5 10^8 exponentials, which take 128 SMs (64 unit tiles x 2 splits) 130 us. Measured instead: three
 // tiles with weights beside the scores 277, two threads a unit 322, chunks of 32 keys 300, a quarter
 // of the exponentials as cubic polynomials 281.
@@ -197,8 +197,6 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
     const int n = kend > base ? (kend - base + CK - 1) / CK : 0, steps = (n + 1) / 2;   // chunks, steps
 
     if (tid == 0) {
-        for (int i = 0; i < L::UNPACK; ++i)
-            for (int j = 0; j < PS; ++j) mbar_init(&ms.packed[i][j], 1);
         for (int i = 0; i < KS; ++i) {
             mbar_init(&ms.kv_full[i], 4);
             mbar_init(&ms.kv_empty[i], tiles);
@@ -217,6 +215,54 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    // unpacking: warp w of four takes tile w of each chunk; with eight, warp 4 y + w of chunk y of the steps.
+    // With heads of 64 its first copies are on their way while the others set up (2048 rows on 2048 keys
+    // 53.0 -> 51.8 us); heads of 128 lost by it (246 -> 256 us on 8192 keys)
+    constexpr int YT = L::YT;
+    const int uw = warp >= L::SOFT && warp < L::MMA ? warp - L::SOFT : 0, y0 = uw >> 2, w = uw & 3;
+    unsigned char* ring = sm + L::P + uw * L::PB;
+    uint64_t* packed = ms.packed[uw];
+    // pages of the warp's tiles, those of 32 steps at a time (lane i: step i)
+    auto pages_of = [&](int c0, int* pg) {
+#pragma unroll
+        for (int y = 0; y < YT; ++y) pg[y] = c0 + lane < steps ? kv4_page(a, b, (step0 + c0 + lane) * 8 + 4 * (y0 + y) + w) : -1;
+    };
+    auto issue = [&](int c, const int* page) {   // lane 0
+        uint64_t* bar = &packed[c % PS];
+        uint32_t bytes = 0;
+#pragma unroll
+        for (int y = 0; y < YT; ++y) bytes += page[y] >= 0 ? L::TB : 0;
+        if (bytes == 0) {
+            mbar_arrive(bar);
+            return;
+        }
+        mbar_arrive_expect_tx(bar, bytes);
+#pragma unroll
+        for (int y = 0; y < YT; ++y)
+            if (page[y] >= 0)
+                tma_load_1d(ring + ((c % PS) * YT + y) * L::TB,
+                            a.pages + ((int64_t)page[y] * a.hkv + h) * a.page_bytes +
+                                (int64_t)(((step0 + c) * 8 + 4 * (y0 + y) + w) & ((1 << (a.page_shift - 4)) - 1)) * L::TB,
+                            L::TB, bar);
+    };
+    int pg[YT], nextpg[YT];
+    auto begin = [&]() {
+        if (lane == 0) {
+            for (int i = 0; i < PS; ++i) mbar_init(&packed[i], 1);
+            fence_mbar_init();
+        }
+        __syncwarp();
+        pages_of(0, pg);
+#pragma unroll
+        for (int y = 0; y < YT; ++y) nextpg[y] = pg[y];
+        for (int c = 0; c < min(PS, steps); ++c) {
+            int page[YT];
+#pragma unroll
+            for (int y = 0; y < YT; ++y) page[y] = __shfl_sync(0xffffffffu, pg[y], c);
+            if (lane == 0) issue(c, page);
+        }
+    };
+    if (HD == 64 && warp >= L::SOFT && warp < L::MMA) begin();
     float qscale = 0.f;
     // the tiles' queries, a thread a unit: q 2^-eq in fp16, its largest |dim| in [2^3, 2^4)
     if (warp < L::SOFT) {
@@ -301,44 +347,8 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
         }
         __syncwarp();
     } else if (warp >= L::SOFT) {
-        // unpacking: warp w of four takes tile w of each chunk; with eight, warp 4 y + w of chunk y of the steps
-        constexpr int YT = L::YT;
-        const int uw = warp - L::SOFT, y0 = uw >> 2, w = uw & 3, r = lane >> 2, t = lane & 3;
-        unsigned char* ring = sm + L::P + uw * L::PB;
-        uint64_t* packed = ms.packed[uw];
-        // pages of the warp's tiles, those of 32 steps at a time (lane i: step i)
-        auto pages_of = [&](int c0, int* pg) {
-#pragma unroll
-            for (int y = 0; y < YT; ++y) pg[y] = c0 + lane < steps ? kv4_page(a, b, (step0 + c0 + lane) * 8 + 4 * (y0 + y) + w) : -1;
-        };
-        int pg[YT], nextpg[YT];
-        auto issue = [&](int c, const int* page) {   // lane 0
-            uint64_t* bar = &packed[c % PS];
-            uint32_t bytes = 0;
-#pragma unroll
-            for (int y = 0; y < YT; ++y) bytes += page[y] >= 0 ? L::TB : 0;
-            if (bytes == 0) {
-                mbar_arrive(bar);
-                return;
-            }
-            mbar_arrive_expect_tx(bar, bytes);
-#pragma unroll
-            for (int y = 0; y < YT; ++y)
-                if (page[y] >= 0)
-                    tma_load_1d(ring + ((c % PS) * YT + y) * L::TB,
-                                a.pages + ((int64_t)page[y] * a.hkv + h) * a.page_bytes +
-                                    (int64_t)(((step0 + c) * 8 + 4 * (y0 + y) + w) & ((1 << (a.page_shift - 4)) - 1)) * L::TB,
-                                L::TB, bar);
-        };
-        pages_of(0, pg);
-#pragma unroll
-        for (int y = 0; y < YT; ++y) nextpg[y] = pg[y];
-        for (int c = 0; c < min(PS, steps); ++c) {
-            int page[YT];
-#pragma unroll
-            for (int y = 0; y < YT; ++y) page[y] = __shfl_sync(0xffffffffu, pg[y], c);
-            if (lane == 0) issue(c, page);
-        }
+        const int r = lane >> 2, t = lane & 3;
+        if (HD != 64) begin();
         bool good = true;   // no wait of this warp has run out; the warps leave together
         int c = 0;
         for (; c < steps; ++c) {
