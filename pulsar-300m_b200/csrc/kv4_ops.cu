@@ -362,23 +362,26 @@ __device__ __forceinline__ Item item_of(uint32_t w, uint32_t n, int hq, int hkv,
     return it;
 }
 
-// 16384 tokens of 16 query and 4 kv heads of 64 take 31 us: 89 MB, 2.8 TB/s. One token: 2.5 us. What
-// bounds it is the arithmetic (some 290 instructions for a lane's 16 dims, 14 M in all, two a clock and
-// SM) behind the chain slot, position, table, vector; 24 warps an SM (80 registers, a few spilled) hide
-// that better than the 16 that fit without a bound: 32 us against 40. Tokens run along the warp so
-// that neighbouring slots share sectors of a tile: a token's value codes are 2-byte pieces 64 bytes
-// apart. Gathering whole tiles in shared memory to write them in 16-byte pieces gained nothing.
-template <int HD, int TURN>
+// ONE: a head an item, no loop. 16384 tokens of 16 query and 4 kv heads of 64 take 26 us: 89 MB, 3.4 TB/s.
+// One token: 2.3 us. What bounds it is the arithmetic (some 290 instructions for a lane's 16 dims, two a
+// clock and SM) behind the chain slot, position, table, vector; 24 warps an SM (80 registers, a few spilled)
+// hide that better than the 16 that fit without a bound: 32 us against 40. Two heads' work unrolled into one
+// another: 29 -> 26 us. Inputs and queries pass the caches as used once: the stores' mark alone is worth 3 us
+// here and a fifth of k_kv4_read's time. Tokens run along the warp so that neighbouring slots share sectors
+// of a tile: a token's value codes are 2-byte pieces 64 bytes apart. Gathering whole tiles in shared memory
+// to write them in 16-byte pieces gained nothing.
+template <int HD, int TURN, bool ONE>
 __global__ void __launch_bounds__(128, 6) k_kv4_append(const AppendArgs a) {
     constexpr int L = HD / 16, NG = Kv4Tile<HD>::NG;
     const int lane = threadIdx.x & 31, l = lane % L;
     const uint32_t w = blockIdx.x * 4 + (threadIdx.x >> 5);
     if (w >= a.warps) return;
-    const Item it = item_of<HD>(w, a.n, a.hq, a.hkv, a.heads, lane);
+    Item it = item_of<HD>(w, a.n, a.hq, a.hkv, ONE ? 1 : a.heads, lane);
+    if (ONE) it.h1 = it.h0 + 1;
     const __nv_bfloat16* src = it.kind == 0 ? a.q + it.tok * a.qs + it.h0 * a.qh
                              : it.kind == 1 ? a.k + it.tok * a.ks + it.h0 * a.kh : a.v + it.tok * a.vs + it.h0 * a.vh;
     const int64_t next = it.kind == 0 ? a.qh : it.kind == 1 ? a.kh : a.vh;
-    uint4 raw0 = __ldg(reinterpret_cast<const uint4*>(src) + l), raw1 = __ldg(reinterpret_cast<const uint4*>(src) + L + l);
+    uint4 raw0 = __ldcs(reinterpret_cast<const uint4*>(src) + l), raw1 = __ldcs(reinterpret_cast<const uint4*>(src) + L + l);
     int pos = a.pos ? a.pos[it.tok] : 0;
     const bool ok = !a.pos || (pos >= 0 && pos < a.max_pos);
     if (!ok) pos = 0;
@@ -390,7 +393,7 @@ __global__ void __launch_bounds__(128, 6) k_kv4_append(const AppendArgs a) {
     const bool put = it.live && ok && slot >= 0 && slot < a.num_slots;
     uint8_t* tile = a.pages + (put && it.kind ? tile_at<HD>(slot, it.h0, a.hkv, a.page_shift, a.page_bytes) : 0);
     __nv_bfloat16* dst = a.qo + (it.tok * a.hq + it.h0) * HD;
-#pragma unroll 1
+#pragma unroll 2
     for (int h = it.h0; h < it.h1; ++h) {
         f32x2 weight[8];
         if (wn) {
@@ -402,8 +405,8 @@ __global__ void __launch_bounds__(128, 6) k_kv4_append(const AppendArgs a) {
         hi.take(raw1);
         src += next;
         if (h + 1 < it.h1) {
-            raw0 = __ldg(reinterpret_cast<const uint4*>(src) + l);
-            raw1 = __ldg(reinterpret_cast<const uint4*>(src) + L + l);
+            raw0 = __ldcs(reinterpret_cast<const uint4*>(src) + l);
+            raw1 = __ldcs(reinterpret_cast<const uint4*>(src) + L + l);
         }
         if (wn) norm<HD>(lo, hi, weight, a.eps, lane);
         if (it.kind != 2) turn<HD, TURN>(a, lo, hi, t, pos, lane);
@@ -416,8 +419,8 @@ __global__ void __launch_bounds__(128, 6) k_kv4_append(const AppendArgs a) {
                 }
             }
             if (it.live) {
-                reinterpret_cast<uint4*>(dst)[l] = ok ? lo.bf16() : make_uint4(0, 0, 0, 0);
-                reinterpret_cast<uint4*>(dst)[L + l] = ok ? hi.bf16() : make_uint4(0, 0, 0, 0);
+                __stcs(reinterpret_cast<uint4*>(dst) + l, ok ? lo.bf16() : make_uint4(0, 0, 0, 0));
+                __stcs(reinterpret_cast<uint4*>(dst) + L + l, ok ? hi.bf16() : make_uint4(0, 0, 0, 0));
             }
             dst += HD;
         } else {
@@ -469,10 +472,10 @@ struct ReadArgs {
     int hkv, page_shift, heads;
 };
 
-// 32768 positions of 4 kv heads of 64: 44 MB in 11.4 us, 3.9 TB/s (8 heads of 128: 176 MB in 34 us,
-// 5.2 TB/s); 777 positions 2.3 us. Bound by instructions (80 for a lane's 16 dims) and, past that, by the
-// writes. Through shared memory in whole tiles it took 14.2 us; two heads' bytes asked for at a time cost
-// more registers than waiting: 12.
+// 32768 positions of 4 kv heads of 64: 44 MB in 9.2 us, 4.8 TB/s (16384 of 8 heads of 128: 88 MB in 18.4);
+// 777 positions 2.3 us. Bound by instructions (80 for a lane's 16 dims) and, past that, by the writes.
+// Through shared memory in whole tiles it was a fifth slower; two heads' bytes asked for at a time cost
+// more registers than waiting.
 template <int HD>
 __global__ void __launch_bounds__(128) k_kv4_read(const ReadArgs a) {
     constexpr int L = HD / 16, NG = Kv4Tile<HD>::NG;
@@ -501,27 +504,28 @@ __global__ void __launch_bounds__(128) k_kv4_read(const ReadArgs a) {
         }
         const uint4 x0 = values_of(from_word(w.x, lane), par.x), x1 = values_of(from_word(w.y, lane), par.y);
         if (it.live) {
-            dst[l] = x0;
-            dst[L + l] = x1;
+            __stcs(dst + l, x0);
+            __stcs(dst + L + l, x1);
         }
         dst += HD / 8;
         tile += a.page_bytes;
     }
 }
 
-template <int HD>
+template <int HD, bool ONE>
 auto append_kernel(int turn) {
-    return turn == TURN_NONE ? k_kv4_append<HD, TURN_NONE> : turn == TURN_WHOLE ? k_kv4_append<HD, TURN_WHOLE>
-         : turn == TURN_NEIGHBOURS ? k_kv4_append<HD, TURN_NEIGHBOURS> : k_kv4_append<HD, TURN_PART>;
+    return turn == TURN_NONE ? k_kv4_append<HD, TURN_NONE, ONE> : turn == TURN_WHOLE ? k_kv4_append<HD, TURN_WHOLE, ONE>
+         : turn == TURN_NEIGHBOURS ? k_kv4_append<HD, TURN_NEIGHBOURS, ONE> : k_kv4_append<HD, TURN_PART, ONE>;
 }
 
-// Heads of a warp's work, from the warps that one head each would take: one until those fill the SMs
-// (24 warps each), then more, which share the look-ups. Measured with 1 / 2 / 4 heads, 16 query and 4 kv
-// heads of 64: 1024 tokens 4.1 / 4.1 / 6.6 us, 2048 6.6 / 5.6 / 6.6, 6144 16.9 / 13.9 /
-// 14.7, 8192 (24576 warps) 24 / 20 / 18, 16384 46 / 36 / 32, with 8 heads 35; reading 16384 positions
-// 7.3 / 6.2 / 5.7.
-constexpr int64_t HEADS_2 = 3552, HEADS_4 = 21312;
-int heads_of(int64_t warps) { return warps < HEADS_2 ? 1 : warps < HEADS_4 ? 2 : 4; }
+// Heads of a warp's work, from the warps that one head each would take: four, which share the look-ups,
+// once one each would fill the SMs (24 warps each) four times. Measured with 1 / 2 / 4 / 8 heads, append to
+// 16 query and 4 kv heads of 64: 1024 tokens 3.2 / 5.1 / 6.6 / 7.2 us, 4096 (12288 warps) 8.8 / 9.1 / 8.5 / 9.6,
+// 8192 16.9 / 16.4 / 14.4 / 18.6, 16384 31.7 / 28.7 / 25.8 / 27.8; 32 and 8 heads of 128, 1536 tokens (18432
+// warps) 14.5 / 12.8 / 13.4 / 13.4, 8192 65 / 54 / 46 / 45; reading 8192 positions of 4 heads of 64 4.7 / 4.2 /
+// 4.6 / 4.1, 16384 7.2 / 6.1 / 5.7 / 5.8.
+constexpr int64_t HEADS_4 = 14208;
+int heads_of(int64_t warps) { return warps < HEADS_4 ? 1 : 4; }
 
 int page_geometry(const char* what, int64_t head_dim, int64_t page_size, int64_t num_pages, int64_t hkv,
                   const void* pages, int* shift, int64_t* page_bytes) {
@@ -575,7 +579,8 @@ extern "C" int pulsar_op_kv4_append(const void* q, const void* k, const void* v,
                        (int)max_pos, heads, eps};
     cudaStream_t st = (cudaStream_t)stream;
     const int grid = (int)((warps + 3) / 4);
-    auto* kernel = head_dim == 64 ? append_kernel<64>(turn) : append_kernel<128>(turn);
+    auto* kernel = heads == 1 ? (head_dim == 64 ? append_kernel<64, true>(turn) : append_kernel<128, true>(turn))
+                              : (head_dim == 64 ? append_kernel<64, false>(turn) : append_kernel<128, false>(turn));
     kernel<<<grid, 128, 0, st>>>(a);
     PULSAR_LAUNCH_CHECK("k_kv4_append");
     return PULSAR_OK;

@@ -285,21 +285,24 @@ def test_partial_rotation_matches_plain_32_bits(paged, n, d, rot):
     assert torch.equal(out, y.bfloat16())
 
 
-@pytest.mark.parametrize("n,d", [(2501, 64), (4001, 64), (2003, 128)])
-def test_several_heads_a_warp(paged, n, d):
+@pytest.mark.parametrize("n,d,rot,interleaved", [(2501, 64, 64, False), (6501, 64, 0, False), (2003, 128, 128, False),
+                                                 (2100, 128, 64, False), (2100, 64, 48, False), (2100, 64, 64, True),
+                                                 (2100, 128, 30, True)])
+def test_several_heads_a_warp(paged, n, d, rot, interleaved):
     """Head counts that fill a warp's share of heads or leave a part of one: the same bits as in calls of
     few tokens."""
     hq, hkv, page = 41, 9, 64
     q, k, v = (_randn(i, n, h, d).bfloat16().cuda() for i, h in ((1, hq), (2, hkv), (3, hkv)))
     pages = paged.kv4_pages(n // page + 1, hkv, d, page)
     slots, pos = torch.arange(n).flip(0).cuda(), torch.arange(n).int().cuda()
-    cos, sin = paged.rope_tables(n, d)
+    cos, sin = paged.rope_tables(n, rot) if rot else (None, None)
     qw, kw = 1 + 0.1 * _randn(4, hq, d).cuda(), 1 + 0.1 * _randn(5, hkv, d).cuda()
     few, parts = pages.clone(), []
-    out = paged.kv4_append(q, k, v, pages, slots, pos, cos, sin, q_norm=qw, k_norm=kw)
+    out = paged.kv4_append(q, k, v, pages, slots, pos, cos, sin, q_norm=qw, k_norm=kw, interleaved=interleaved)
     for a in range(0, n, 300):
         b = slice(a, a + 300)
-        parts.append(paged.kv4_append(q[b], k[b], v[b], few, slots[b], pos[b], cos, sin, q_norm=qw, k_norm=kw))
+        parts.append(paged.kv4_append(q[b], k[b], v[b], few, slots[b], pos[b], cos, sin, q_norm=qw, k_norm=kw,
+                                       interleaved=interleaved))
     assert torch.equal(out, torch.cat(parts)) and torch.equal(pages, few)
     many = paged.kv4_read(pages, slots, d)
     few = [paged.kv4_read(pages, slots[a:a + 300], d) for a in range(0, n, 300)]
