@@ -116,12 +116,11 @@ __device__ __forceinline__ float2 ld_cluster(const float* p, int rank) {
 template <int HD>
 constexpr int stages() { return HD == 64 ? 4 : 2; }
 
-// CTAs that an SM should hold: 16 warps where the registers allow it.
-template <int HD, int NT, int WARPS>
-constexpr int resident() { return NT == 1 ? 16 / WARPS : 1; }
+// CTAs of four warps that an SM holds: 16 warps where the registers allow it.
+constexpr int resident(int head_dim, int nt) { return nt == 1 ? 4 : nt == 2 && head_dim == 64 ? 3 : 2; }
 
 template <int HD, int NT, bool DUP, int WARPS>
-__global__ void __launch_bounds__(WARPS * 32, resident<HD, NT, WARPS>()) k_kv4_attn(const Kv4AttnArgs a) {
+__global__ void __launch_bounds__(WARPS * 32, resident(HD, NT) * 4 / WARPS) k_kv4_attn(const Kv4AttnArgs a) {
     using T = Kv4Tile<HD>;
     constexpr int NG = T::NG, NB = HD / 64, S = stages<HD>(), MT = HD / 16, TB = T::BYTES;
     constexpr int UT = DUP ? 4 : 8 * NT;
@@ -807,20 +806,22 @@ struct Plan {
 // units 87 / 109, 48 128 / 110.
 // Others: the fewest columns that hold max_q rows of a group (four: both halves of the weights in
 // one operand), at most 32 (heads of 128: 16, for the registers).
-// Splits of the keys: until the SMs are full (four CTAs each; two above 8 units), of at least 8 pairs of
-// tiles (two a warp); where there are many keys, of 32 to 64 pairs, so that sequences shorter than
-// max_kv even out (the splits that they lack end at once). Measured: 4 x 32768, 18 to 37 splits 19 to 19.6
-// us, 8 31, 74 23; 256 x 640, one 21.8, two 27; 48 x 1..8191 of heads of 128, 2 / 4 / 8 / 12 / 16 splits 93 /
-// 81 / 77 / 81 / 83; 64 x 5 rows on 1024 keys, 1 / 2 / 3 splits 24 / 38 / 45. k_kv4_prefill: the number
+// Splits of the keys: as many as the SMs hold at once, of at least 8 pairs of tiles (two a warp); where
+// there are many keys, of 32 to 64 pairs, so that sequences shorter than max_kv even out (the splits that
+// they lack end at once). One that starts a second wave costs more than it evens out: 33 x 2000 keys with 2
+// rows in 5 / 4 splits 18.4 / 12.0 us, with 5 rows in 3 / 2 34.9 / 22.6, 7 x 9000 in 22 / 21 14.6 / 11.8.
+// Measured around it: 4 x 32768, 18 to 37 splits 19 to 19.6 us, 8 31, 74 23; 256 x 640, one 21.8, two 27;
+// 48 x 1..8191 of heads of 128, 2 / 4 / 8 / 12 / 16 splits 93 / 81 / 77 / 81 / 83. k_kv4_prefill: the number
 // that the cost below finds best: 2048 rows on 16384 keys in 1 / 2 / 3 / 4 splits 441 / 241 / 321 / 254 us, on
-// 2048 keys 69 / 53 / 51 / 61, 4096 rows with a window of 1024 52 / 85 / 104 / 102, 1500 with one of 1000 on 16384
-// keys 55 / 48 / 46 / 63, 33 rows on 16000 keys in 1 / 8 / 32 splits 350 / 57 / 28.
+// 2048 keys 69 / 53 / 51 / 61, 4096 rows with a window of 1024 52 / 85 / 104 / 102, 1500 with one of 1000 on
+// 16384 keys 55 / 48 / 46 / 63, 33 rows on 16000 keys in 1 / 8 / 32 splits 350 / 57 / 28.
 // Two warps instead of four where there is a CTA for every unit tile and each has few keys: what a CTA
 // costs besides its keys is paid per warp (256 x 640: 21.8 us, with four 22.6).
-// A cluster joins its splits through shared memory where there are at most eight and all fit at once.
-// Measured against partials in memory and k_kv4_merge: 1 x 2048 6.2 / 6.5 us (on the host 12 / 22 a
-// call: one launch and no workspace), 16 x 1024 6.7 / 7.7, 4 x 1024 with 5 rows 13.4 / 14.9, heads of
-// 128, 16 x 2048 12.4 / 13.4, 1 x 512 8.4 / 7.8.
+// A cluster joins its splits through shared memory where there are at most eight and all clusters fit at
+// once; each stays inside one of the GPU's eight parts, which hold 17 SMs or more. Measured against
+// partials in memory and k_kv4_merge: 1 x 2048 6.2 / 6.5 us (on the host 12 / 22 a call: one launch and no
+// workspace), 16 x 1024 6.7 / 7.7, 33 x 2000 with 2 rows 12.0 / 13.4, with 5 rows 22.9 / 25.3, heads of 128,
+// 1 x 512 8.4 / 7.8; filling the SMs further: 96 clusters of 6 18.5 / 15.0, 80 of 7 27.5 / 22.3.
 constexpr int64_t MANY = 32;
 Plan make_plan(int64_t B, int64_t Hkv, int64_t group, int64_t head_dim, int64_t max_q, int64_t max_kv,
                int64_t window) {
@@ -857,8 +858,8 @@ Plan make_plan(int64_t B, int64_t Hkv, int64_t group, int64_t head_dim, int64_t 
             }
         }
     } else {
-        const int64_t fill = 148 * (p.nt == 1 ? 4 : 2);   // CTAs that the GPU holds at once
-        ns = ctas * 4 > fill * 3 ? 1 : (fill + ctas - 1) / ctas;
+        const int64_t fill = 148 * resident((int)head_dim, p.nt);   // CTAs that the GPU holds at once
+        ns = fill / ctas;
         if (ns > steps / 8) ns = steps / 8;
         if (ctas * ((steps + 63) / 64) > fill && ns < (steps + 63) / 64) ns = (steps + 31) / 32;
         if (ns > 128) ns = 128;
@@ -869,7 +870,7 @@ Plan make_plan(int64_t B, int64_t Hkv, int64_t group, int64_t head_dim, int64_t 
     if (p.split_len < 1) p.split_len = 1;
     p.nsplit = (int)((steps + p.split_len - 1) / p.split_len);
     if (p.nsplit < 1) p.nsplit = 1;
-    p.cluster = !p.many && p.nsplit > 1 && p.nsplit <= 8 && ctas * p.nsplit <= 148 * (p.nt == 1 ? 4 : 2);
+    p.cluster = !p.many && p.nsplit > 1 && p.nsplit <= 8 && ctas <= 8 * (17 * resident((int)head_dim, p.nt) / p.nsplit);
     return p;
 }
 
