@@ -1,5 +1,5 @@
 // Attention over the paged 4-bit KV cache (layout: kv4.cuh): pulsar_op_kv4_attention, and its kernel for
-// up to 32 units a sequence and kv head (decoding, verify blocks); more: kv4_prefill.cu.
+// few units a sequence and kv head (decoding, verify blocks, short prompts); more: kv4_prefill.cu.
 //
 // Row j of the n_b query rows of sequence b has position pos = len_b - n_b + j and sees the keys
 // max(0, pos - window + 1) .. pos (window 0: all of 0 .. pos):
@@ -799,22 +799,32 @@ struct Plan {
     int nt, dup, warps, unit_tile, utiles, step, nsplit, split_len, cluster;
 };
 
-// How a call is cut. More than MANY units of a sequence's rows go to k_kv4_prefill, 512 or 256 a CTA.
-// Measured (this kernel / that one, us), heads of 64: 8 x 4096 keys, 16 units 24 / 29, 32 36 / 30, 48 43 /
-// 31, 128 60 / 33; 1 x 16384, 32 units 20 / 22, 64 25 / 23, 128 44 / 25; 64 x 2048, 32 units 38 / 87, 64 75
-// / 88, 96 113 / 88; heads of 128: 8 x 4096, 16 units 34 / 35, 32 45 / 38, 64 60 / 39; 64 x 2048, 32
-// units 87 / 109, 48 128 / 110.
-// Others: the fewest columns that hold max_q rows of a group (four: both halves of the weights in
-// one operand), at most 32 (heads of 128: 16, for the registers).
+// Splits of `steps` steps of the keys.
+void split(Plan& p, int64_t steps, int64_t ns) {
+    p.split_len = (int)((steps + ns - 1) / ns);
+    if (p.split_len < 1) p.split_len = 1;
+    p.nsplit = (int)((steps + p.split_len - 1) / p.split_len);
+    if (p.nsplit < 1) p.nsplit = 1;
+}
+// The steps that a tile of ut units can need.
+int64_t steps_of(int64_t ut, int64_t step, int64_t group, int64_t max_q, int64_t max_kv, int64_t window) {
+    int64_t span = max_kv;
+    if (window > 0) {
+        const int64_t rows = (ut + group - 1) / group + 1;   // rows that a unit tile can touch
+        const int64_t w = window + (rows < max_q ? rows : max_q) + step;
+        if (w < span) span = w;
+    }
+    return (span + step - 1) / step;
+}
+
+// k_kv4_attn: the fewest columns that hold max_q rows of a group (four: both halves of the weights in one
+// operand), at most 32 (heads of 128: 16, for the registers).
 // Splits of the keys: as many as the SMs hold at once, of at least 8 pairs of tiles (two a warp); where
 // there are many keys, of 32 to 64 pairs, so that sequences shorter than max_kv even out (the splits that
 // they lack end at once). One that starts a second wave costs more than it evens out: 33 x 2000 keys with 2
 // rows in 5 / 4 splits 18.4 / 12.0 us, with 5 rows in 3 / 2 34.9 / 22.6, 7 x 9000 in 22 / 21 14.6 / 11.8.
 // Measured around it: 4 x 32768, 18 to 37 splits 19 to 19.6 us, 8 31, 74 23; 256 x 640, one 21.8, two 27;
-// 48 x 1..8191 of heads of 128, 2 / 4 / 8 / 12 / 16 splits 93 / 81 / 77 / 81 / 83. k_kv4_prefill: the number
-// that the cost below finds best: 2048 rows on 16384 keys in 1 / 2 / 3 / 4 splits 441 / 241 / 321 / 254 us, on
-// 2048 keys 69 / 53 / 51 / 61, 4096 rows with a window of 1024 52 / 85 / 104 / 102, 1500 with one of 1000 on
-// 16384 keys 55 / 48 / 46 / 63, 33 rows on 16000 keys in 1 / 8 / 32 splits 350 / 57 / 28.
+// 48 x 1..8191 of heads of 128, 2 / 4 / 8 / 12 / 16 splits 93 / 81 / 77 / 81 / 83.
 // Two warps instead of four where there is a CTA for every unit tile and each has few keys: what a CTA
 // costs besides its keys is paid per warp (256 x 640: 21.8 us, with four 22.6).
 // A cluster joins its splits through shared memory where there are at most eight and all clusters fit at
@@ -822,56 +832,78 @@ struct Plan {
 // partials in memory and k_kv4_merge: 1 x 2048 6.2 / 6.5 us (on the host 12 / 22 a call: one launch and no
 // workspace), 16 x 1024 6.7 / 7.7, 33 x 2000 with 2 rows 12.0 / 13.4, with 5 rows 22.9 / 25.3, heads of 128,
 // 1 x 512 8.4 / 7.8; filling the SMs further: 96 clusters of 6 18.5 / 15.0, 80 of 7 27.5 / 22.3.
-constexpr int64_t MANY = 32;
-Plan make_plan(int64_t B, int64_t Hkv, int64_t group, int64_t head_dim, int64_t max_q, int64_t max_kv,
-               int64_t window) {
+// cost: its time in us, for more than 32 units.
+Plan plan_attn(int64_t B, int64_t Hkv, int64_t group, int head_dim, int64_t max_q, int64_t max_kv, int64_t window,
+               double& cost) {
     Plan p{};
     const int64_t units = max_q * group, cap = head_dim == 64 ? 4 : 2;
-    p.many = units > MANY;
     p.dup = units <= 4;
     p.nt = (int)(units > 8 * cap ? cap : (units + 7) / 8);
-    const int64_t ut = p.many ? kv4_pf_units((int)head_dim) : p.dup ? 4 : 8 * p.nt;
-    const int64_t step = p.many ? KV4_PF_STEP : 32;
-    p.unit_tile = (int)ut;
-    p.step = (int)step;
-    p.utiles = (int)((units + ut - 1) / ut);
-    int64_t span = max_kv;
-    if (window > 0) {
-        const int64_t rows = (ut + group - 1) / group + 1;   // rows that a unit tile can touch
-        const int64_t w = window + (rows < max_q ? rows : max_q) + step;
-        if (w < span) span = w;
-    }
-    const int64_t steps = (span + step - 1) / step;
-    const int64_t ctas = B * Hkv * p.utiles;
-    int64_t ns = 1;
-    if (p.many) {
-        // in units of a step (3.45 us): waves of CTAs, each with 4 for its start and end, then the partials'
-        // way through memory and the merge
-        const int64_t most = steps / 2 < 64 ? steps / 2 : 64;
-        double best = 1e30;
-        for (int64_t s = 1; s <= most || s == 1; ++s) {
-            const double waves = (double)((ctas * s + 147) / 148), len = (double)((steps + s - 1) / s);
-            const double merge = s > 1 ? 0.6 + (double)(B * Hkv * units) * s * (head_dim + 2) * 8 / 13.8e6 : 0;
-            if (waves * (len + 4) + merge < best) {
-                best = waves * (len + 4) + merge;
-                ns = s;
-            }
-        }
-    } else {
-        const int64_t fill = 148 * resident((int)head_dim, p.nt);   // CTAs that the GPU holds at once
-        ns = fill / ctas;
-        if (ns > steps / 8) ns = steps / 8;
-        if (ctas * ((steps + 63) / 64) > fill && ns < (steps + 63) / 64) ns = (steps + 31) / 32;
-        if (ns > 128) ns = 128;
-        if (ns < 1) ns = 1;
-    }
-    p.warps = !p.many && p.nt == 1 && ns == 1 && ctas > 148 * 4 && steps <= 64 ? 2 : 4;
-    p.split_len = (int)((steps + ns - 1) / ns);
-    if (p.split_len < 1) p.split_len = 1;
-    p.nsplit = (int)((steps + p.split_len - 1) / p.split_len);
-    if (p.nsplit < 1) p.nsplit = 1;
-    p.cluster = !p.many && p.nsplit > 1 && p.nsplit <= 8 && ctas <= 8 * (17 * resident((int)head_dim, p.nt) / p.nsplit);
+    p.unit_tile = p.dup ? 4 : 8 * p.nt;
+    p.step = 32;
+    p.utiles = (int)((units + p.unit_tile - 1) / p.unit_tile);
+    const int64_t steps = steps_of(p.unit_tile, p.step, group, max_q, max_kv, window), ctas = B * Hkv * p.utiles;
+    const int64_t fill = 148 * resident(head_dim, p.nt);   // CTAs that the GPU holds at once
+    int64_t ns = fill / ctas;
+    if (ns > steps / 8) ns = steps / 8;
+    if (ctas * ((steps + 63) / 64) > fill && ns < (steps + 63) / 64) ns = (steps + 31) / 32;
+    if (ns > 128) ns = 128;
+    if (ns < 1) ns = 1;
+    p.warps = p.nt == 1 && ns == 1 && ctas > 148 * 4 && steps <= 64 ? 2 : 4;
+    split(p, steps, ns);
+    p.cluster = p.nsplit > 1 && p.nsplit <= 8 && ctas <= 8 * (17 * resident(head_dim, p.nt) / p.nsplit);
+    const double waves = (double)((ctas * p.nsplit + fill - 1) / fill), pairs = (p.split_len + 3) / 4;
+    cost = 5 + waves * (head_dim == 64 ? 8 + pairs * (waves > 1 ? 2.0 : 1.45) : 6 + pairs * (waves > 1 ? 2.5 : 2.0)) +
+           (p.nsplit > 1 && !p.cluster ? 3 : 0);
     return p;
+}
+
+// k_kv4_prefill: the splits that make the cost (us) least: the launch; for every wave of CTAs their start
+// and end and their steps, by the tiles of 128 units that a CTA has; the partials' way through memory.
+// 2048 rows on 16384 keys in 1 / 2 / 3 / 4 splits 441 / 241 / 321 / 254 us, on 2048 keys 69 / 53 / 51 / 61, 4096 rows
+// with a window of 1024 52 / 85 / 104 / 102, 1500 with one of 1000 on 16384 keys 55 / 48 / 46 / 63, 33 rows on
+// 16000 keys in 1 / 8 / 32 splits 350 / 57 / 28.
+Plan plan_prefill(int64_t B, int64_t Hkv, int64_t group, int head_dim, int64_t max_q, int64_t max_kv, int64_t window,
+                  double& cost) {
+    Plan p{};
+    const int64_t units = max_q * group;
+    p.many = true;
+    p.warps = 4;
+    p.unit_tile = kv4_pf_units(head_dim);
+    p.step = KV4_PF_STEP;
+    p.utiles = (int)((units + p.unit_tile - 1) / p.unit_tile);
+    const int64_t steps = steps_of(p.unit_tile, p.step, group, max_q, max_kv, window), ctas = B * Hkv * p.utiles;
+    const double tiles = (double)(p.utiles > 1 ? p.unit_tile / 128 : (units + 127) / 128);
+    const double ends = head_dim == 64 ? 1.5 + 3.5 * tiles : 10 * tiles, step = head_dim == 64 ? 1.2 + 0.55 * tiles : 1.4 + 0.8 * tiles;
+    const int64_t most = steps / 2 < 64 ? steps / 2 : 64;
+    int64_t ns = 1;
+    cost = 1e30;
+    for (int64_t s = 1; s <= most || s == 1; ++s) {
+        const double waves = (double)((ctas * s + 147) / 148), len = (double)((steps + s - 1) / s);
+        const double c = 6 + waves * (ends + len * step) +
+                         (s > 1 ? 1 + (double)(B * Hkv * units) * s * (head_dim + 2) * 8 / 4e6 : 0);
+        if (c < cost) {
+            cost = c;
+            ns = s;
+        }
+    }
+    split(p, steps, ns);
+    return p;
+}
+
+// How a call is cut. Up to 32 units a sequence k_kv4_attn; above, the kernel that costs less, which with
+// few keys is k_kv4_attn up to some hundred units. Measured (k_kv4_attn / k_kv4_prefill, us), 4 kv heads of 64:
+// 512 keys, 40 units 15.9 / 14.4, 256 16.4 / 18.6, 800 18 / 26; 4096 keys, 64 units 17.2 / 15.4, 512 25.9 / 30.8,
+// 800 38.6 / 32.8; 16384 keys, 32 units 19.0 / 21.1, 128 28 / 24, 512 91 / 39; 8 x 4096, 64 units 25.7 / 30.8, 128
+// 39 / 32; 64 x 2048, 32 units 38 / 86, 40 92 / 85; heads of 128: 512 keys, 256 units 16 / 29; 4096 keys, 256
+// units 27 / 33, 512 44 / 34; 64 x 2048, 32 units 104 / 109, 40 144 / 110.
+Plan make_plan(int64_t B, int64_t Hkv, int64_t group, int64_t head_dim, int64_t max_q, int64_t max_kv,
+               int64_t window) {
+    double cost, other;
+    const Plan p = plan_attn(B, Hkv, group, (int)head_dim, max_q, max_kv, window, cost);
+    if (max_q * group <= 32) return p;
+    const Plan q = plan_prefill(B, Hkv, group, (int)head_dim, max_q, max_kv, window, other);
+    return other < cost ? q : p;
 }
 
 template <int HD, int NT, bool DUP, int WARPS>
