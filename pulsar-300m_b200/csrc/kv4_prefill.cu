@@ -67,6 +67,7 @@ struct Misc {   // in shared memory after the operands
     float kscale[4], ev[4];  // per unpacked stage
     uint32_t bad[4][4];      // and tile of 16 tokens: some group of V is NaN
     uint8_t bad_groups[4][64];
+    uint32_t gone[4];        // a byte for each tile of 16 tokens: its page is none of the cache's
     uint32_t tmem;
     int abort;
 };
@@ -462,6 +463,7 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
                 }
                 if (lane == 0) {
                     ms.bad[sk][w] = any_bad[y];
+                    reinterpret_cast<uint8_t*>(&ms.gone[sk])[w] = !there[y];
                     if (w == 0) {
                         ms.kscale[sk] = kv4_exp2i(ek);
                         ms.ev[sk] = (float)ev;
@@ -498,13 +500,14 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
         uint32_t bad = 0;
         // the chunk's scale of scores, exponent of values and NaN marks, taken while its scores are computed
         float kq = 0.f, ev = 0.f;
-        uint32_t odd = 0;
+        uint32_t odd = 0, gone = 0;
         auto chunk = [&](int c) {
             const int sk = c % KS;
             const bool there = __all_sync(0xffffffffu, wait(&ms.kv_full[sk], (c / KS) & 1, abort));
             kq = ms.kscale[sk] * qscale;
             ev = ms.ev[sk];
             odd = ms.bad[sk][0] | ms.bad[sk][1] | ms.bad[sk][2] | ms.bad[sk][3];
+            gone = ms.gone[sk];
             return there;
         };
         bool ok = tile < tiles && n > 0;
@@ -514,7 +517,7 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
             ok = __all_sync(0xffffffffu, wait(&ms.s_full[tile], c & 1, abort));
             if (!ok) break;
             fence_after();
-            const bool edge = k0 < all_lo || k0 + CK > all_hi;
+            const bool edge = k0 < all_lo || k0 + CK > all_hi || gone != 0;
             const int lo_c = lo - k0, hi_c = hi - k0;
             // scores of keys 32 q .. of the chunk; those that the unit does not see: -inf
             auto scores = [&](int q, uint32_t* v) {
@@ -523,7 +526,7 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
                 if (edge) {
 #pragma unroll
                     for (int k = 0; k < 32; ++k)
-                        if (32 * q + k < lo_c || 32 * q + k >= hi_c) v[k] = 0xff800000u;
+                        if (32 * q + k < lo_c || 32 * q + k >= hi_c || (gone >> (8 * (2 * q + (k >> 4))) & 1)) v[k] = 0xff800000u;
                 }
             };
             // weights with the reference m; their sum

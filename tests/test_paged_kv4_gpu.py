@@ -339,7 +339,7 @@ def _filled(paged, lens, hkv, d, page, seed=0, spare=1, fill=0xFF):
     return pages, table
 
 
-def _attend(paged, lens, counts, hq, hkv, d, page, window=0, scale=None, seed=0, one=False, **kw):
+def _attend(paged, lens, counts, hq, hkv, d, page, window=0, scale=None, seed=0, one=False, max_q=None, **kw):
     pages, table = _filled(paged, lens, hkv, d, page, seed)
     cu = [0]
     for c in counts:
@@ -348,10 +348,10 @@ def _attend(paged, lens, counts, hq, hkv, d, page, window=0, scale=None, seed=0,
     t = torch.tensor(table, dtype=torch.int32).cuda()
     got = paged.kv4_attention(q, pages, t, torch.tensor(lens, dtype=torch.int32).cuda(),
                               None if one else torch.tensor(cu, dtype=torch.int32).cuda(),
-                              max_q=max(1, max(counts)), window=window, scale=scale, **kw)
+                              max_q=max_q or max(1, max(counts)), window=window, scale=scale, **kw)
     k, v = held(pages, d)
     ref, top, amp = plain_attention(q, k, v, table, lens, cu, d ** -0.5 if scale is None else scale, window)
-    assert_attention(got, ref, top, amp, max(counts) * (hq // hkv) > 8)
+    assert_attention(got, ref, top, amp, (max_q or max(counts)) * (hq // hkv) > 8)
     return got
 
 
@@ -414,6 +414,81 @@ def test_prompt_values_of_any_size(paged):
                                   torch.tensor([0, 60], dtype=torch.int32).cuda(), max_q=60, scale=0.2 / kx)
         hk, hv = held(pages, d)
         assert_attention(got, *plain_attention(q, hk, hv, table, lens, [0, 60], 0.2 / kx, 0), many=True)
+
+
+# The kernel for many rows is chosen where it costs less, so small calls reach it through a bound of rows
+# that they do not fill.
+@pytest.mark.parametrize("hq,hkv,d,page,window", [(16, 4, 64, 64, 0), (4, 1, 64, 16, 50), (3, 3, 64, 32, 0), (7, 1, 64, 128, 0),
+                                                  (8, 2, 128, 16, 0), (6, 1, 128, 64, 40)])
+def test_rows_below_a_large_bound(paged, hq, hkv, d, page, window):
+    _attend(paged, [100, 75, 150, 33, 20], [100, 40, 65, 1, 0], hq, hkv, d, page, window=window, max_q=8192)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_rows_below_a_large_bound_longer_than_their_keys(paged, d):
+    got = _attend(paged, [50, 0, 129], [90, 33, 140], 4, 2, d, 16, max_q=8192)
+    assert (got[:40] == 0).all() and (got[90:123] == 0).all() and (got[123:134] == 0).all()
+
+
+@pytest.mark.parametrize("d,window", [(64, 0), (128, 0), (64, 300)])
+def test_rows_below_a_large_bound_behind_many_keys(paged, d, window):
+    _attend(paged, [1500, 700], [20, 9], 4, 2, d, 64, window=window, max_q=4096)
+    _attend(paged, [2600], [40], 2, 2, d, 16, window=window, max_q=4096)
+
+
+@pytest.mark.parametrize("window", [0, 3000])
+def test_chunk_behind_several_thousand_keys(paged, window):
+    """Enough keys that the kernel for many rows takes few of them, in many splits."""
+    _attend(paged, [4300], [17], 8, 2, 64, 64, window=window)
+
+
+def test_values_of_any_size_below_a_large_bound(paged):
+    lens, page, d = [300], 64, 128
+    for kx, vx in ((2.0 ** -20, 2.0 ** 25), (2.0 ** 12, 2.0 ** -30)):
+        pages, table = _filled(paged, lens, 1, d, page)
+        k, v = _randn(1, 300, 1, d) * kx, _randn(2, 300, 1, d) * vx * torch.linspace(-3, 3, 300).exp2()[:, None, None]
+        slots = torch.tensor([table[0][i // page] * page + i % page for i in range(300)])
+        paged.kv4_append(None, k.cuda().bfloat16(), v.cuda().bfloat16(), pages, slots.cuda())
+        q = _randn(3, 60, 2, d).bfloat16().cuda()
+        got = paged.kv4_attention(q, pages, torch.tensor(table, dtype=torch.int32).cuda(),
+                                  torch.tensor(lens, dtype=torch.int32).cuda(),
+                                  torch.tensor([0, 60], dtype=torch.int32).cuda(), max_q=8192, scale=0.2 / kx)
+        hk, hv = held(pages, d)
+        assert_attention(got, *plain_attention(q, hk, hv, table, lens, [0, 60], 0.2 / kx, 0), many=True)
+
+
+def test_nan_stays_where_it_is_seen_below_a_large_bound(paged):
+    lens, page, rows = [40], 16, 20
+    pages, table = _filled(paged, lens, 1, 64, page)
+    at = torch.tensor([table[0][2] * page + 5]).cuda()          # key 37
+    bad = torch.full((1, 1, 64), float("nan"), dtype=torch.bfloat16, device="cuda")
+    paged.kv4_append(None, bad, bad, pages, at)
+    t, n = torch.tensor(table, dtype=torch.int32).cuda(), torch.tensor(lens, dtype=torch.int32).cuda()
+    q, cu = _randn(5, rows, 4, 64).bfloat16().cuda(), torch.tensor([0, rows], dtype=torch.int32).cuda()
+    got = paged.kv4_attention(q, pages, t, n, cu, max_q=8192)   # rows at positions 20 .. 39
+    assert torch.isfinite(got[:17].float()).all() and torch.isnan(got[17:].float()).all()
+    good, half = torch.ones_like(bad), torch.ones_like(bad)
+    half[..., 40] = float("inf")
+    paged.kv4_append(None, good, half, pages, at)
+    for window in (0, 2):
+        got = paged.kv4_attention(q, pages, t, n, cu, max_q=8192, window=window).float()
+        sees = torch.zeros(rows, dtype=torch.bool)
+        sees[rows - 3:rows - 1 if window else rows] = True
+        assert torch.isfinite(got[..., :32]).all() and torch.isfinite(got[~sees]).all()
+        assert torch.isnan(got[sees][..., 32:]).all()
+
+
+def test_peaked_scores_and_missing_pages_below_a_large_bound(paged):
+    _attend(paged, [200, 90], [70, 20], 4, 1, 64, 64, scale=4.0, max_q=8192)
+    lens, page = [200, 90], 32
+    pages, table = _filled(paged, lens, 2, 64, page)
+    table[0][1], table[0][4], table[1][0] = -1, 1 << 20, pages.shape[0]
+    q = _randn(4, 2, 8, 64).bfloat16().cuda()
+    got = paged.kv4_attention(q, pages, torch.tensor(table, dtype=torch.int32).cuda(),
+                              torch.tensor(lens, dtype=torch.int32).cuda(),
+                              torch.tensor([0, 1, 2], dtype=torch.int32).cuda(), max_q=8192)
+    k, v = held(pages, 64)
+    assert_attention(got, *plain_attention(q, k, v, table, lens, [0, 1, 2], 0.125, 0), many=True)
 
 
 @pytest.mark.parametrize("hq,d", [(4, 64), (7, 128)])
