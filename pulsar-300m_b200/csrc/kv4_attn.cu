@@ -457,8 +457,8 @@ __global__ void __launch_bounds__(WARPS * 32, resident(HD, NT) * 4 / WARPS) k_kv
         float sc[2][NT][4], kq[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            kq[nt][0] = q_scale[nt][0] * kv4_exp2i(ek);
-            kq[nt][1] = q_scale[nt][1] * kv4_exp2i(ek);
+            kq[nt][0] = kv4_score_factor(q_scale[nt][0], kv4_exp2i(ek));
+            kq[nt][1] = kv4_score_factor(q_scale[nt][1], kv4_exp2i(ek));
         }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {

@@ -108,6 +108,10 @@ __device__ __forceinline__ int kv4_exponent_out(uint32_t bits) {
 }
 __device__ __forceinline__ float kv4_exp2i(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
+// Factor from sums of operand products to scores, from its query's and its keys' part. It stays above zero
+// where both are tiny (queries and keys of zero, pages that are none): masked sums of -inf pass through it.
+__device__ __forceinline__ float kv4_score_factor(float q, float k) { return fmaxf(q * k, 1.17549435e-38f); }
+
 // The largest |value| that a parameter pair allows, as float bits (0 for NaN).
 __device__ __forceinline__ uint32_t kv4_top(uint32_t param) {
     const float x = fmaxf(fabsf(kv4_z(param)), fabsf(fmaf(15.f, kv4_s(param), kv4_z(param))));

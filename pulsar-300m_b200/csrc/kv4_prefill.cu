@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
         auto chunk = [&](int c) {
             const int sk = c % KS;
             const bool there = __all_sync(0xffffffffu, wait(&ms.kv_full[sk], (c / KS) & 1, abort));
-            kq = ms.kscale[sk] * qscale;
+            kq = kv4_score_factor(qscale, ms.kscale[sk]);
             ev = ms.ev[sk];
             odd = ms.bad[sk][0] | ms.bad[sk][1] | ms.bad[sk][2] | ms.bad[sk][3];
             gone = ms.gone[sk];

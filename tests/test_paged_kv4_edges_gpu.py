@@ -1,0 +1,120 @@
+"""Attention over the paged 4-bit KV cache at its edges, against the definition in 64 bits.
+
+Tolerance: a row's distance (2-norm over a head's dims) is at most 2^-8 of the row's own norm. Rounding
+the result to bf16 moves it by 2^-9 at most. Above 8 units keys, values and weights are rounded at 2^-12:
+with scale sum |q k| of a few units, random signs and Gaussian data that is some 2^-11.5 in the weights of a
+row and 2^-12.5 each in values and weights, together 2^-11 of the row, a quarter of the other 2^-9. Up to 8 units
+operands are good to 2^-16. A row that sees no key is exactly zero."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from test_paged_kv4_gpu import held
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def paged():
+    if not torch.cuda.is_available():
+        pytest.skip("CUDA not available")
+    from pulsar_b200 import paged
+    return paged
+
+
+def _randn(seed, *shape):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed))
+
+
+def _int(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def _cache(paged, lens, k, v, page, seed=0):
+    """The sequences' keys and values (bf16 [all keys, heads, D], one after the other) on shuffled pages;
+    unused places hold NaN."""
+    used = [-(-n // page) for n in lens]
+    perm = torch.randperm(sum(used) + 1, generator=torch.Generator().manual_seed(seed)).tolist()
+    width, table, slots = max(1, *used), [], []
+    for n, u in zip(lens, used):
+        mine = torch.tensor([perm.pop() for _ in range(u)] + [-1] * (width - u))
+        at = torch.arange(n)
+        table.append(mine.tolist())
+        slots.append(mine[at // page] * page + at % page)
+    pages = paged.kv4_pages(sum(used) + 1, k.shape[1], k.shape[2], page).fill_(0xFF)
+    paged.kv4_append(None, k.bfloat16().cuda(), v.bfloat16().cuda(), pages, torch.cat(slots).cuda())
+    return pages, table
+
+
+def _exact(q, pages, table, lens, counts, scale, window):
+    k, v = (x.cuda() for x in held(pages, q.shape[2]))
+    page, out, row = k.shape[1], torch.zeros(q.shape, dtype=torch.double, device="cuda"), 0
+    group = q.shape[1] // k.shape[2]
+    for pages_b, n, c in zip(table, lens, counts):
+        at = torch.arange(n, device="cuda")
+        where = torch.tensor(pages_b, device="cuda")[at // page]
+        at, where = (x[(where >= 0) & (where < len(k))] for x in (at, where))
+        kk, vv = (x[where, at % page].repeat_interleave(group, 1) for x in (k, v))
+        pos = n - c + torch.arange(c, device="cuda")[:, None]
+        see = (at <= pos) & (at > pos - window if window else at >= 0)
+        s = torch.einsum("qhd,khd->hqk", q[row:row + c].double(), kk) * scale
+        s = s.masked_fill(~see, -math.inf)
+        p = torch.exp(s - s.amax(-1, keepdim=True).clamp(min=-1e300) if len(at) else s)
+        p = p / p.sum(-1, keepdim=True).clamp(min=1e-300)
+        # a value that no row sees may be anything
+        out[row:row + c] = torch.einsum("hqk,khd->qhd", p, torch.where(see.any(0)[:, None, None], vv, 0.0))
+        row += c
+    return out
+
+
+def _attend(paged, q, pages, table, lens, counts, scale=None, window=0, **kw):
+    """The kernel's answer, held against the definition."""
+    cu = [sum(counts[:i]) for i in range(len(counts) + 1)]
+    kw.setdefault("max_q", max(1, *counts))
+    got = paged.kv4_attention(q, pages, _int(table), _int(lens), _int(cu), scale=scale, window=window, **kw)
+    ref = _exact(q, pages, table, lens, counts, q.shape[2] ** -0.5 if scale is None else scale, window)
+    assert torch.isfinite(got).all()
+    err, size = (got.double() - ref).norm(dim=-1), ref.norm(dim=-1)
+    assert (err[size == 0] == 0).all()
+    worst = (err / size.clamp(min=1e-300)).max().item()
+    assert worst <= 2.0 ** -8, f"a row is off by {worst:.3e} of its norm"
+    return got
+
+
+# Rows of a sequence, query heads, head dim, the bound of rows given: up to 8 units (query rows x heads of
+# a group), above, and the kernel for many rows (chosen by a bound of rows that small calls do not fill).
+KERNELS = [pytest.param(2, 4, 64, 2, id="few"), pytest.param(1, 7, 128, 1, id="few-128"),
+           pytest.param(5, 4, 64, 5, id="wide"), pytest.param(3, 5, 128, 3, id="wide-128"),
+           pytest.param(20, 4, 64, 8192, id="many"), pytest.param(20, 2, 128, 8192, id="many-128")]
+ABOVE_8 = KERNELS[2:]
+
+
+@pytest.mark.parametrize("rows,hq,d,max_q", KERNELS)
+@pytest.mark.parametrize("qx,kx", [(0.0, 0.0), (0.0, 1.0), (2.0 ** -110, 2.0 ** -110)])
+def test_queries_and_keys_of_zero(paged, rows, hq, d, max_q, qx, kx):
+    """Scores of zero: the mean of the visible values, whatever is masked beside them. A query of zero is
+    what an append gives for a position outside its tables, keys of zero what an empty cache holds."""
+    lens, counts = [0, 1, 40, 300, 129], [rows, rows, rows, rows, 0]
+    q = (_randn(1, sum(counts), hq, d) * qx).bfloat16().cuda()
+    k, v = _randn(2, sum(lens), 1, d) * kx, _randn(3, sum(lens), 1, d)
+    pages, table = _cache(paged, lens, k, v, 32)
+    for window in (0, 3, 100):
+        _attend(paged, q, pages, table, lens, counts, window=window, max_q=max_q)
+    table[3][4:8] = [-1] * 4          # a whole step of 128 keys without a page
+    table[2][0] = 1 << 20
+    _attend(paged, q, pages, table, lens, counts, max_q=max_q)
+    table[3] = [-1] * len(table[3])   # no page at all
+    assert (_attend(paged, q, pages, table, lens, counts, max_q=max_q)[3 * rows:] == 0).all()
+
+
+@pytest.mark.parametrize("rows,hq,d,max_q", KERNELS)
+def test_queries_of_zero_on_an_empty_cache(paged, rows, hq, d, max_q):
+    pages = paged.kv4_pages(8, 1, d, 32)
+    q = torch.zeros(2 * rows, hq, d, dtype=torch.bfloat16, device="cuda")
+    got = paged.kv4_attention(q, pages, _int([[0, 1, 2, 3], [4, 5, 6, 7]]), _int([100, 0]), _int([0, rows, 2 * rows]),
+                              max_q=max_q)
+    assert (got == 0).all()
