@@ -529,7 +529,7 @@ __global__ void __launch_bounds__(WARPS * 32, resident(HD, NT) * 4 / WARPS) k_kv
         weigh();
         bool up = false;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) up |= ls[nt][0] > pow2(14) || ls[nt][1] > pow2(14);
+        for (int nt = 0; nt < NT; ++nt) up |= ls[nt][0] > KV4_FULL || ls[nt][1] > KV4_FULL;
         if (__any_sync(0xffffffffu, up)) {   // fp16 would soon be left: move the references, weigh again
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
@@ -539,7 +539,7 @@ __global__ void __launch_bounds__(WARPS * 32, resident(HD, NT) * 4 / WARPS) k_kv
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                    x = fmaxf(fmaf(x, kq[nt][c], ev), m[nt][c]);
+                    x = fmaxf(fmaf(x, kq[nt][c], ev) - KV4_ROOM, m[nt][c]);
                     const float f = kv4_ex2(m[nt][c] - x);
                     m[nt][c] = x;
                     l[nt][c] *= f;

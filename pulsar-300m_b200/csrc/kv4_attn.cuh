@@ -79,6 +79,13 @@ __device__ __forceinline__ float kv4_ex2(float x) {
 __device__ __forceinline__ float kv4_s(uint32_t param) { return __uint_as_float(param << 16); }
 __device__ __forceinline__ float kv4_z(uint32_t param) { return __uint_as_float(param & 0xffff0000u); }
 
+// Weights in fp16, 2^(x - m) for a score x and a reference m of the unit: m moves when a sum of a few weights
+// passes FULL (so each stays below 65504), and then lies ROOM below the largest score so far, so that weights
+// down to 2^-21 of the largest keep their significand and what is lost below it is 2^-32 of the largest.
+// (64 equal scores sum to 2^13, so scores may grow fourfold before m moves again.) m at the largest score itself
+// gave 240 us instead of 243 for 2048 rows on 16384 keys, and lost a flat tail under one large weight.
+constexpr float KV4_FULL = 32768.f, KV4_ROOM = 7.f;
+
 // Operands in fp16 (values s c + z of 8-bit s, z and 4-bit c, rounded twice at 2^-12): fp16 has the
 // significand but not the range, so powers of two are taken out of keys and values.
 __device__ __forceinline__ uint32_t kv4_half2(float a, float b) {

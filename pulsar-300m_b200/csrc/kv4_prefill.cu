@@ -21,7 +21,7 @@
 // at 2^-12, weights too) but not the range, so powers of two move out: queries by their row, keys and
 // values by their step of 128 (2^eK, 2^eV from the largest |value| that s and z allow, over the keys that
 // some unit sees). Score and weight: x = 2^eK 2^eq scale log2(e) S + eV - m, P = 2^x; P V^ = 2^(s - m) V
-// and l = sum 2^-eV P. The reference m of a unit moves when a chunk's sum of weights passes 2^14
+// and l = sum 2^-eV P. The reference m of a unit moves when a chunk's sum of weights passes 2^15
 // (then the row of O is rescaled and the chunk's weights taken again), so P stays inside fp16 and no
 // maximum is looked for in other chunks.
 //
@@ -40,8 +40,6 @@
 using namespace pulsar;
 
 namespace {
-
-constexpr float FULL = 16384.f;   // a chunk's weights are taken again when their sum passes this
 
 template <int HD>
 struct Lay {
@@ -552,10 +550,10 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
                 parts(sum, x, y);
                 return x + y;
             };
-            // m to the largest score so far, the row of O with it (the scores say that P V of the chunk
-            // before has completed)
+            // m to the largest score so far less ROOM, the row of O with it (the scores say that P V of the
+            // chunk before has completed)
             auto raise = [&]() {
-                float top = m;
+                float top = -INFINITY;
 #pragma unroll
                 for (int q = 0; q < CK / 32; ++q) {
                     uint32_t v[32];
@@ -563,6 +561,7 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
 #pragma unroll
                     for (int k = 0; k < 32; ++k) top = fmaxf(top, fmaf(__uint_as_float(v[k]), kq, ev));
                 }
+                top = fmaxf(m, top - KV4_ROOM);
                 const float f = kv4_ex2(m - top);
                 m = top;
                 l *= f;
@@ -579,7 +578,7 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
             };
             if (c == 0) raise();
             float sum = weigh();
-            if (__any_sync(0xffffffffu, sum > FULL)) {
+            if (__any_sync(0xffffffffu, sum > KV4_FULL)) {
                 raise();
                 sum = weigh();
             }

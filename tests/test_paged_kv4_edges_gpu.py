@@ -118,3 +118,16 @@ def test_queries_of_zero_on_an_empty_cache(paged, rows, hq, d, max_q):
     got = paged.kv4_attention(q, pages, _int([[0, 1, 2, 3], [4, 5, 6, 7]]), _int([100, 0]), _int([0, rows, 2 * rows]),
                               max_q=max_q)
     assert (got == 0).all()
+
+
+@pytest.mark.parametrize("rows,hq,d,max_q", KERNELS)
+@pytest.mark.parametrize("max_kv", [None, 64])
+def test_one_key_above_a_flat_tail(paged, rows, hq, d, max_q, max_kv):
+    """Every key of a long tail weighs half a millionth of the first one, whose value is zero: the tail's
+    weights keep their precision (all of them are the same number, so roundings would not average out)."""
+    n = 16384
+    k, v = torch.zeros(n, 1, d), 1 + 0.5 * _randn(1, n, 1, d)
+    k[0], v[0] = 1.0, 0.0
+    pages, table = _cache(paged, [n], k, v, 64)
+    q = torch.ones(rows, hq, d, dtype=torch.bfloat16, device="cuda")
+    _attend(paged, q, pages, table, [n], [rows], scale=math.log(2.0 ** 24 / 8.45) / d, max_q=max_q, max_kv=max_kv)
