@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(WARPS * 32, resident(HD, NT) * 4 / WARPS) k_kv
     // Scores come in units of 2^(LIFT - CODE_EXP); m: their running maximum, nm = LIFT - scale m, so
     // that weights are 2^LIFT exp2(scale (s - m)). WIDE: m is the reference of the weights 2^(x - m), base 2
     float o[MT][NT][4], zacc[NT][NG][2], m[NT][2], nm[NT][2], l[NT][2];
-    const float scale = WIDE ? 1.f : a.scale_log2 * pow2(CODE_EXP - LIFT);
+    const float scale = a.scale_log2 * pow2(CODE_EXP - LIFT);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -271,6 +271,7 @@ __global__ void __launch_bounds__(WARPS * 32, resident(HD, NT) * 4 / WARPS) k_kv
     }
     const float minus_hi = t < 2 ? 0.f : -1.f;   // columns 4..7 of the doubled units (t >= 2) carry the lo halves
     uint32_t bad[NT][2] = {};   // WIDE: groups of V stored as NaN that the column sees
+    Kv4Unit unit;   // WIDE: powers of two of the step's values and of O
     int failed = -1;   // the pair whose copy did not land within the bound
 
     // one pair of tiles; EDGE: some of its keys are not seen by some unit, or a page is missing
@@ -428,7 +429,7 @@ __global__ void __launch_bounds__(WARPS * 32, resident(HD, NT) * 4 / WARPS) k_kv
 
     // The same with keys and values unpacked to fp16 numbers, s and z applied: more work a tile and less
     // a unit (no s and z on scores, one operand of weights instead of two a group). 2^ek, 2^ev come
-    // out of the pair's keys and values: x = 2^ek q.k scale + ev, weights 2^(x - m), l = sum 2^-ev weight
+    // out of the pair's keys and values: x = 2^ek q.k scale, weights 2^(x + ev - er - m), l = sum 2^(er - ev) weight
     auto wide_step = [&](auto edge_tag, const unsigned char* tp, int k0, bool ok0, bool ok1) {
         constexpr bool EDGE = decltype(edge_tag)::value;
         auto known = [&](int x, int token) {   // some unit sees the token
@@ -452,8 +453,9 @@ __global__ void __launch_bounds__(WARPS * 32, resident(HD, NT) * 4 / WARPS) k_kv
         topk = __reduce_max_sync(0xffffffffu, topk);
         topv = __reduce_max_sync(0xffffffffu, topv);
         if (EDGE) nan_v = __any_sync(0xffffffffu, nan_v);
-        const int ek = kv4_exponent_out(topk), evi = kv4_exponent_out(topv);
-        const float fk = kv4_exp2i(-ek), fv = kv4_exp2i(-evi), ev = (float)evi;
+        const int ek = kv4_exponent_out(topk);
+        unit.ev = kv4_exponent_out(topv);
+        const float fk = kv4_exp2i(-ek);
         float sc[2][NT][4], kq[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
@@ -513,7 +515,7 @@ __global__ void __launch_bounds__(WARPS * 32, resident(HD, NT) * 4 / WARPS) k_kv
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 ls[nt][0] = ls[nt][1] = 0.f;
-                const float b0 = ev - m[nt][0], b1 = ev - m[nt][1];
+                const float b0 = (float)(unit.ev - unit.er) - m[nt][0], b1 = (float)(unit.ev - unit.er) - m[nt][1];
 #pragma unroll
                 for (int x = 0; x < 2; ++x)
 #pragma unroll
@@ -527,10 +529,11 @@ __global__ void __launch_bounds__(WARPS * 32, resident(HD, NT) * 4 / WARPS) k_kv
             }
         };
         weigh();
-        bool up = false;
+        bool up = !unit.holds(unit.ev);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) up |= ls[nt][0] > KV4_FULL || ls[nt][1] > KV4_FULL;
         if (__any_sync(0xffffffffu, up)) {   // fp16 would soon be left: move the references, weigh again
+            const float moved = unit.next(topv), shift = (float)(unit.ev - unit.er);   // O into a new unit
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -539,23 +542,24 @@ __global__ void __launch_bounds__(WARPS * 32, resident(HD, NT) * 4 / WARPS) k_kv
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
                     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                    x = fmaxf(fmaf(x, kq[nt][c], ev) - KV4_ROOM, m[nt][c]);
+                    x = fmaxf(fmaf(x, kq[nt][c], shift) - KV4_ROOM, m[nt][c]);
                     const float f = kv4_ex2(m[nt][c] - x);
                     m[nt][c] = x;
                     l[nt][c] *= f;
 #pragma unroll
                     for (int y = 0; y < MT; ++y) {
-                        o[y][nt][c] *= f;
-                        o[y][nt][c + 2] *= f;
+                        o[y][nt][c] *= f * moved;
+                        o[y][nt][c + 2] *= f * moved;
                     }
                 }
             weigh();
         }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            l[nt][0] = fmaf(ls[nt][0], kv4_exp2i(-evi), l[nt][0]);
-            l[nt][1] = fmaf(ls[nt][1], kv4_exp2i(-evi), l[nt][1]);
+            l[nt][0] = fmaf(ls[nt][0], kv4_exp2i(unit.er - unit.ev), l[nt][0]);
+            l[nt][1] = fmaf(ls[nt][1], kv4_exp2i(unit.er - unit.ev), l[nt][1]);
         }
+        const float fv = kv4_exp2i(-unit.ev);
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
             const unsigned char* vt = tp + x * TB;
@@ -641,8 +645,8 @@ __global__ void __launch_bounds__(WARPS * 32, resident(HD, NT) * 4 / WARPS) k_kv
             for (int x = 4; x < 32; x <<= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
             if (failed >= 0) s = __int_as_float(0x7fffffff);
             if (r == 0 && (!DUP || t < 2)) {
-                wo[u * (HD + 2) + HD] = m[nt][c] * scale;
-                wo[u * (HD + 2) + HD + 1] = WIDE ? s : s * pow2(-LIFT);
+                wo[u * (HD + 2) + HD] = WIDE ? m[nt][c] + (float)unit.er : m[nt][c] * scale;
+                wo[u * (HD + 2) + HD + 1] = s * (WIDE ? kv4_exp2i(-unit.er) : pow2(-LIFT));
             }
             uint32_t none = bad[nt][c];
             if (WIDE) none = __reduce_or_sync(0x11111111u << t, none);

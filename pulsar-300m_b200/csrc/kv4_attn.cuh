@@ -115,6 +115,30 @@ __device__ __forceinline__ int kv4_exponent_out(uint32_t bits) {
 }
 __device__ __forceinline__ float kv4_exp2i(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
+// Values of a step are operands 2^-ev V, O is kept in units of 2^er, and weights carry 2^(ev - er): er follows ev
+// (O is rescaled) when it rises, or falls by more than SLACK, so that weights stay where fp16 is precise
+// whatever sizes the values of other steps have. ev falls at most SPAN below the largest so far: O then stays in
+// range, and values that far below lose precision. Where all are zero ev is er.
+constexpr int KV4_SLACK = 6, KV4_SPAN = 80;
+struct Kv4Unit {
+    int ev = 0, er = 0, largest = -1000;
+    __device__ __forceinline__ bool holds(int e) const { return (uint32_t)(e - er + KV4_SLACK) <= KV4_SLACK + 1; }
+    // A step whose largest |value| is top (float bits). The factor for O, 1 where er stays.
+    __device__ __forceinline__ float next(uint32_t top) {
+        ev = kv4_exponent_out(top);
+        if (holds(ev)) return 1.f;
+        if (top == 0) {
+            ev = er;
+            return 1.f;
+        }
+        largest = max(largest, ev);
+        ev = max(ev, largest - KV4_SPAN);
+        const int old = er;
+        if (!holds(ev)) er = ev;
+        return kv4_ex2((float)(old - er));
+    }
+};
+
 // Factor from sums of operand products to scores, from its query's and its keys' part. It stays above zero
 // where both are tiny (queries and keys of zero, pages that are none): masked sums of -inf pass through it.
 __device__ __forceinline__ float kv4_score_factor(float q, float k) { return fmaxf(q * k, 1.17549435e-38f); }

@@ -20,10 +20,10 @@
 // Exactness. fp16 has the significand for it (values s c + z of 8-bit s, z and 4-bit c are rounded
 // at 2^-12, weights too) but not the range, so powers of two move out: queries by their row, keys and
 // values by their step of 128 (2^eK, 2^eV from the largest |value| that s and z allow, over the keys that
-// some unit sees). Score and weight: x = 2^eK 2^eq scale log2(e) S + eV - m, P = 2^x; P V^ = 2^(s - m) V
-// and l = sum 2^-eV P. The reference m of a unit moves when a chunk's sum of weights passes 2^15
-// (then the row of O is rescaled and the chunk's weights taken again), so P stays inside fp16 and no
-// maximum is looked for in other chunks.
+// some unit sees). Score and weight: x = 2^eK 2^eq scale log2(e) S, P = 2^(x + eV - er - m); P V^ = 2^(x - er - m) V
+// and l = sum 2^(er - eV) P, with 2^er the unit of O (Kv4Unit). The reference m of a unit moves when a chunk's
+// sum of weights passes 2^15 (then the row of O is rescaled and the chunk's weights taken again), so P stays
+// inside fp16 and no maximum is looked for in other chunks.
 //
 // Keys that a unit does not see get weight 0 by selection. V^ is 0 for keys that no unit sees (pages
 // past the end may hold anything) and for groups stored as NaN; which (key, group) those were goes to
@@ -62,14 +62,17 @@ struct Misc {   // in shared memory after the operands
     uint64_t packed[8][3], kv_full[4], kv_empty[4], s_full[4], p_full[4], pv_done[4], drain[4];
     uint32_t stop[2][8];     // per step parity and unpacking warp: a wait has run out
     uint32_t top[2][8][2];   // largest |K|, |V| as float bits
-    float kscale[4], ev[4];  // per unpacked stage
-    uint32_t bad[4][4];      // and tile of 16 tokens: some group of V is NaN
+    float kscale[4], shift[4], factor[4];   // per unpacked stage: 2^eK, eV - er, what O is rescaled by
+    int er[4];
+    uint32_t mark[4];        // a byte for each tile of 16 tokens: GONE, BAD, MOVED
     uint8_t bad_groups[4][64];
-    uint32_t gone[4];        // a byte for each tile of 16 tokens: its page is none of the cache's
     uint32_t tmem;
     int abort;
 };
 static_assert(sizeof(Misc) <= 2048, "Misc fits its space");
+
+// A tile's page is none of the cache's; some group of V is NaN; the step's values have moved the unit of O.
+constexpr uint32_t GONE = 0x01010101u, BAD = 0x02020202u, MOVED = 0x04040404u;
 
 __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, volatile int* abort) {
     if (mbar_try(bar, parity)) return true;
@@ -349,6 +352,7 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
         const int r = lane >> 2, t = lane & 3;
         if (HD != 64) begin();
         bool good = true;   // no wait of this warp has run out; the warps leave together
+        Kv4Unit unit;       // (the same in all unpacking warps)
         int c = 0;
         for (; c < steps; ++c) {
             const int st = c % PS, sg = c & 1, k0 = base + c * SK;
@@ -392,8 +396,9 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
             topk = __reduce_max_sync(0xffffffffu, ms.top[sg][lane % L::UNPACK][0]);
             topv = __reduce_max_sync(0xffffffffu, ms.top[sg][lane % L::UNPACK][1]);
             if (__any_sync(0xffffffffu, ms.stop[sg][lane % L::UNPACK] != 0)) break;
-            const int ek = kv4_exponent_out(topk), ev = kv4_exponent_out(topv);
-            const float fk = kv4_exp2i(-ek), fv = kv4_exp2i(-ev);
+            const int ek = kv4_exponent_out(topk);
+            const float factor = unit.next(topv);
+            const float fk = kv4_exp2i(-ek), fv = kv4_exp2i(-unit.ev);
 #pragma unroll
             for (int y = 0; y < YT; ++y) {
                 const int ch = 2 * c + y0 + y, sk = ch % KS, tl = 4 * (y0 + y) + w;
@@ -460,11 +465,14 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
                     }
                 }
                 if (lane == 0) {
-                    ms.bad[sk][w] = any_bad[y];
-                    reinterpret_cast<uint8_t*>(&ms.gone[sk])[w] = !there[y];
+                    const bool moved = factor != 1.f && !(ch & 1);   // with the step's first chunk
+                    reinterpret_cast<uint8_t*>(&ms.mark[sk])[w] =
+                        (uint8_t)((there[y] ? 0u : GONE) | (any_bad[y] ? BAD : 0u) | (moved ? MOVED : 0u));
                     if (w == 0) {
                         ms.kscale[sk] = kv4_exp2i(ek);
-                        ms.ev[sk] = (float)ev;
+                        ms.shift[sk] = (float)(unit.ev - unit.er);
+                        ms.factor[sk] = factor;
+                        ms.er[sk] = unit.er;
                     }
                 }
                 fence_async();
@@ -496,16 +504,15 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
         const int all_lo = low(len - nq + ub / a.group), all_hi = len - nq + ua / a.group + 1;
         float m = KV4_NEG, l = 0.f;
         uint32_t bad = 0;
-        // the chunk's scale of scores, exponent of values and NaN marks, taken while its scores are computed
-        float kq = 0.f, ev = 0.f;
-        uint32_t odd = 0, gone = 0;
+        // the chunk's scale of scores, eV - er and marks, taken while its scores are computed
+        float kq = 0.f, shift = 0.f;
+        uint32_t mark = 0;
         auto chunk = [&](int c) {
             const int sk = c % KS;
             const bool there = __all_sync(0xffffffffu, wait(&ms.kv_full[sk], (c / KS) & 1, abort));
             kq = kv4_score_factor(qscale, ms.kscale[sk]);
-            ev = ms.ev[sk];
-            odd = ms.bad[sk][0] | ms.bad[sk][1] | ms.bad[sk][2] | ms.bad[sk][3];
-            gone = ms.gone[sk];
+            shift = ms.shift[sk];
+            mark = ms.mark[sk];
             return there;
         };
         bool ok = tile < tiles && n > 0;
@@ -515,7 +522,7 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
             ok = __all_sync(0xffffffffu, wait(&ms.s_full[tile], c & 1, abort));
             if (!ok) break;
             fence_after();
-            const bool edge = k0 < all_lo || k0 + CK > all_hi || gone != 0;
+            const bool edge = k0 < all_lo || k0 + CK > all_hi || (mark & GONE);
             const int lo_c = lo - k0, hi_c = hi - k0;
             // scores of keys 32 q .. of the chunk; those that the unit does not see: -inf
             auto scores = [&](int q, uint32_t* v) {
@@ -524,13 +531,13 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
                 if (edge) {
 #pragma unroll
                     for (int k = 0; k < 32; ++k)
-                        if (32 * q + k < lo_c || 32 * q + k >= hi_c || (gone >> (8 * (2 * q + (k >> 4))) & 1)) v[k] = 0xff800000u;
+                        if (32 * q + k < lo_c || 32 * q + k >= hi_c || (mark >> (8 * (2 * q + (k >> 4))) & 1)) v[k] = 0xff800000u;
                 }
             };
             // weights with the reference m; their sum
             uint32_t p[CK / 2];
             auto weigh = [&]() {
-                const f32x2 f2 = two(kq, kq), b2 = two(ev - m, ev - m);
+                const f32x2 f2 = two(kq, kq), b2 = two(shift - m, shift - m);
                 f32x2 sum = two(0.f, 0.f);
 #pragma unroll
                 for (int q = 0; q < CK / 32; ++q) {
@@ -550,8 +557,8 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
                 parts(sum, x, y);
                 return x + y;
             };
-            // m to the largest score so far less ROOM, the row of O with it (the scores say that P V of the
-            // chunk before has completed)
+            // m to the largest score so far less ROOM, the row of O with it and to its new unit (the scores say
+            // that P V of the chunk before has completed)
             auto raise = [&]() {
                 float top = -INFINITY;
 #pragma unroll
@@ -559,12 +566,13 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
                     uint32_t v[32];
                     scores(q, v);
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) top = fmaxf(top, fmaf(__uint_as_float(v[k]), kq, ev));
+                    for (int k = 0; k < 32; ++k) top = fmaxf(top, fmaf(__uint_as_float(v[k]), kq, shift));
                 }
                 top = fmaxf(m, top - KV4_ROOM);
-                const float f = kv4_ex2(m - top);
+                float f = kv4_ex2(m - top);
                 m = top;
                 l *= f;
+                if (mark & MOVED) f *= ms.factor[sk];
                 if (c > 0) {
 #pragma unroll
                     for (int q = 0; q < HD / 16; ++q) {
@@ -576,18 +584,22 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
                     }
                 }
             };
-            if (c == 0) raise();
-            float sum = weigh();
-            if (__any_sync(0xffffffffu, sum > KV4_FULL)) {
+            float sum = 0.f;
+            bool moved = c == 0 || (mark & MOVED);   // (the same for the warp)
+            if (!moved) {
+                sum = weigh();
+                moved = __any_sync(0xffffffffu, sum > KV4_FULL);
+            }
+            if (moved) {
                 raise();
                 sum = weigh();
             }
             st16(s_at, p);
             st16(s_at + 16, p + 16);
-            l = fmaf(sum, kv4_ex2(-ev), l);
-            if (odd) {
+            l = fmaf(sum, kv4_ex2(-shift), l);
+            if (mark & BAD) {
                 for (int k = max(lo_c, 0); k < min(hi_c, CK); ++k)
-                    if (ms.bad[sk][k >> 4]) bad |= ms.bad_groups[sk][k];
+                    if (mark >> (8 * (k >> 4)) & 2) bad |= ms.bad_groups[sk][k];
             }
             st_wait();
             fence_before();
@@ -601,6 +613,8 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
             ok = __all_sync(0xffffffffu, ok);
             fence_after();
             if (!ok) bad = 0xffu;
+            const int er = n > 0 ? ms.er[(n - 1) % KS] : 0;
+            l *= kv4_exp2i(-er);
             const bool row_ok = u < units;
             const int j = row_ok ? u / a.group : 0, g = row_ok ? u - j * a.group : 0;
             const int64_t at = (int64_t)(row0 + j) * a.hq + h * a.group + g;
@@ -632,7 +646,7 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
                 }
             }
             if (row_ok && rg.used > 1) {
-                a.part_ml[(at * a.nsplit + split) * 2] = m;
+                a.part_ml[(at * a.nsplit + split) * 2] = m + (float)er;
                 a.part_ml[(at * a.nsplit + split) * 2 + 1] = l;
             }
         }

@@ -131,3 +131,33 @@ def test_one_key_above_a_flat_tail(paged, rows, hq, d, max_q, max_kv):
     pages, table = _cache(paged, [n], k, v, 64)
     q = torch.ones(rows, hq, d, dtype=torch.bfloat16, device="cuda")
     _attend(paged, q, pages, table, [n], [rows], scale=math.log(2.0 ** 24 / 8.45) / d, max_q=max_q, max_kv=max_kv)
+
+
+@pytest.mark.parametrize("rows,hq,d,max_q", ABOVE_8)
+@pytest.mark.parametrize("size,first", [(2.0 ** 20, 1), (2.0 ** 40, 128), (2.0 ** 70, 256)])
+def test_large_values_of_no_weight(paged, rows, hq, d, max_q, size, first):
+    """Values of a sequence's first keys, of hardly any weight, are many times larger than those that
+    make the result: one key among others up to 2^20, whole steps of keys by any factor."""
+    n = 1100
+    base = _randn(1, 1, 1, d)
+    q = (base + 0.1 * _randn(2, rows, hq, d)).bfloat16().cuda()
+    k, v = _randn(3, n, 1, d), _randn(4, n, 1, d)
+    k[:first] = -12 * base[0] - 0.1 * _randn(5, first, 1, d)
+    v[:first] *= size
+    pages, table = _cache(paged, [n], k, v, 64)
+    for max_kv in (None, 64):
+        _attend(paged, q, pages, table, [n], [rows], max_q=max_q, max_kv=max_kv)
+    _attend(paged, q, pages, table, [n], [rows], max_q=max_q, window=900)
+
+
+@pytest.mark.parametrize("rows,hq,d,max_q", ABOVE_8)
+def test_values_that_grow_and_shrink(paged, rows, hq, d, max_q):
+    """Steps of values of sizes between 2^-30 and 2^30, in turn: the largest ones make the result."""
+    n = 1500
+    k, v = _randn(3, n, 1, d), _randn(4, n, 1, d) * (2.0 ** (_randn(5, 12).clamp(-3, 3) * 10).round())[
+        torch.arange(n) // 128][:, None, None]
+    v[1200:1300] = 0.0
+    pages, table = _cache(paged, [n], k, v, 16)
+    q = _randn(1, rows, hq, d).bfloat16().cuda()
+    for max_kv in (None, 64):
+        _attend(paged, q, pages, table, [n], [rows], max_q=max_q, max_kv=max_kv)
