@@ -47,7 +47,9 @@ using namespace pulsar;
 
 namespace {
 
-constexpr int LAZY = 30;   // more than log2 of the keys of a row, and weights of 2^(LIFT + LAZY) times values stay in fp32 up to 2^37
+// More than log2 of the keys of a row. Weights of 2^(LIFT + LAZY) times values stay in fp32 up to 2^37, and times
+// codes 2^-133 down to values of 2^-50.
+constexpr int LAZY = 30;
 constexpr float NEG = KV4_NEG;
 
 // d = a b + c (d and c may be the same registers)
@@ -215,8 +217,8 @@ __global__ void __launch_bounds__(WARPS * 32, resident(HD, NT) * 4 / WARPS) k_kv
                 top = max(top, max(qf[nt][i] << 16 & 0x7fffffffu, qf[nt][i] & 0x7fff0000u));
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const int eq = min(max((int)(top >> 23) - 127 - 3, -100), 100);
-            const float f = kv4_exp2i(-eq), s = a.scale_log2 * kv4_exp2i(eq);
+            const int eq = kv4_query_exponent(top);
+            const float f = kv4_exp2i(-eq), s = fminf(a.scale_log2 * kv4_exp2i(eq), 3.4e38f);
             q_scale[nt][0] = __shfl_sync(0xffffffffu, s, 8 * t);
             q_scale[nt][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
 #pragma unroll

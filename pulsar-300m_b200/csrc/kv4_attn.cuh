@@ -86,8 +86,9 @@ __device__ __forceinline__ float kv4_z(uint32_t param) { return __uint_as_float(
 // gave 240 us instead of 243 for 2048 rows on 16384 keys, and lost a flat tail under one large weight.
 constexpr float KV4_FULL = 32768.f, KV4_ROOM = 7.f;
 
-// Operands in fp16 (values s c + z of 8-bit s, z and 4-bit c, rounded twice at 2^-12): fp16 has the
-// significand but not the range, so powers of two are taken out of keys and values.
+// Operands in fp16 (values s c + z of 8-bit s, z and 4-bit c, rounded at 2^-12): fp16 has the significand but
+// not the range, so powers of two are taken out of keys and values. What is far below the largest of its step
+// falls under fp16's smallest numbers: the error is 2^-12 of a value or 2^-34 of that largest one.
 __device__ __forceinline__ uint32_t kv4_half2(float a, float b) {
     const __half2 v = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&v);
@@ -109,10 +110,17 @@ __device__ __forceinline__ void kv4_unpack4(uint32_t w, uint32_t s, uint32_t z, 
     for (int i = 0; i < 4; ++i) r[i] = *reinterpret_cast<const uint32_t*>(&x[i]);
 }
 
-// Power of two that brings a largest magnitude (float bits) to [2^9, 2^10): the exponent taken out.
+// Power of two that brings a largest magnitude (float bits) to [2^9, 2^10): the exponent taken out of a step's
+// keys or values. It reaches the largest numbers; at the lower end 2^-90 keeps sums of weights in range, and
+// numbers down to 2^-100 their significand.
 __device__ __forceinline__ int kv4_exponent_out(uint32_t bits) {
-    return min(max((int)(bits >> 23) - 127 - 9, -100), 100);
+    return min(max((int)(bits >> 23) - 127 - 9, -90), 119);
 }
+// The same for a query row, to [2^3, 2^4).
+__device__ __forceinline__ int kv4_query_exponent(uint32_t bits) {
+    return min(max((int)(bits >> 23) - 127 - 3, -120), 124);
+}
+// 2^e, e from -126 to 127.
 __device__ __forceinline__ float kv4_exp2i(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
 
 // Values of a step are operands 2^-ev V, O is kept in units of 2^er, and weights carry 2^(ev - er): er follows ev

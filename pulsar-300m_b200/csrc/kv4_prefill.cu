@@ -291,9 +291,9 @@ __global__ void __launch_bounds__(Lay<HD>::THREADS, 1) k_kv4_prefill(const Kv4At
 #pragma unroll
             for (int e = 0; e < 4; ++e) top = max(top, max(w[e] << 16 & 0x7fffffffu, w[e] & 0x7fff0000u));
         }
-        const int eq = min(max((int)(top >> 23) - 127 - 3, -100), 100);
+        const int eq = kv4_query_exponent(top);
         const float f = kv4_exp2i(-eq);
-        qscale = a.scale_log2 * kv4_exp2i(eq);
+        qscale = fminf(a.scale_log2 * kv4_exp2i(eq), 3.4e38f);
         const int row = tid & 127;
         const uint32_t qt = sb + L::Q + (uint32_t)(tid >> 7) * L::QB + (row >> 3) * 1024 + (row & 7) * 128;
 #pragma unroll 4

@@ -161,3 +161,13 @@ def test_values_that_grow_and_shrink(paged, rows, hq, d, max_q):
     q = _randn(1, rows, hq, d).bfloat16().cuda()
     for max_kv in (None, 64):
         _attend(paged, q, pages, table, [n], [rows], max_q=max_q, max_kv=max_kv)
+
+
+@pytest.mark.parametrize("rows,hq,d,max_q", ABOVE_8)
+@pytest.mark.parametrize("qx,kx,vx", [(1.0, 2.0 ** 120, 2.0 ** 120), (2.0 ** 115, 2.0 ** -90, 2.0 ** -90),
+                                      (2.0 ** -90, 2.0 ** 100, 2.0 ** 118)])
+def test_sizes_at_the_ends_of_the_type(paged, rows, hq, d, max_q, qx, kx, vx):
+    lens, counts = [300, 40], [rows, rows]
+    pages, table = _cache(paged, lens, _randn(1, 340, 1, d) * kx, _randn(2, 340, 1, d) * vx, 64)
+    q = (_randn(3, 2 * rows, hq, d) * qx).bfloat16().cuda()
+    _attend(paged, q, pages, table, lens, counts, scale=0.12 / qx / kx, max_q=max_q)
