@@ -159,8 +159,12 @@ int pulsar_op_kv4_attention_workspace(int64_t N, int64_t Hq, int64_t Hkv, int64_
  * kv_lens and only decides how the work is split. out [N, Hq, head_dim] bf16: softmax(scale q k^T) v,
  * 0 for a row that sees no key; rows of no sequence are not written. Page numbers outside the cache
  * count as masked; scale is positive and finite. q 4-byte, out and the workspace 16-byte aligned.
- * Up to 8 units (max_q times heads of a group) the operands are good to 2^-16 and values may reach
- * 2^37, above that to 2^-12 (fp16 with powers of two taken out); sums are 32-bit. workspace_dev:
+ * Sums are 32-bit. Up to 8 units (max_q times heads of a group) operands are good to 2^-16, for values
+ * between 2^-50 and 2^37 and queries below 2^67. Above, queries, keys, values and weights are fp16 with
+ * powers of two taken out of a row's query and of the keys and the values of each step of 32 or 128
+ * positions: good to 2^-12 of themselves or to 2^-34 of the step's largest (queries of a row: 2^-28,
+ * weights: 2^-32), whichever is more, from 2^-100 up; the step's largest may be one that only later rows
+ * see. Steps of values 2^80 below an earlier one lose more. workspace_dev:
  * scratch of at least pulsar_op_kv4_attention_workspace bytes, which calls on different streams must
  * not share. */
 int pulsar_op_kv4_attention(const void* q_dev, int64_t q_row_stride, int64_t q_head_stride, int64_t N, int64_t Hq,

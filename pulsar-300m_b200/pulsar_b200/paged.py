@@ -237,8 +237,12 @@ def kv4_attention(q, pages, block_table, kv_lens, cu_q=None, *, max_q: int = 1, 
     there is one row for each sequence. ``max_kv`` bounds kv_lens (default: the table's width); it only
     decides how the work is split. ``scale`` defaults to D ** -0.5.
 
-    Sums are in 32 bits; up to 8 units (max_q times the heads of a group) operands are good to 2^-16 and
-    values may reach 2^37, above that they are good to 2^-12 at any size.
+    Sums are in 32 bits. Up to 8 units (max_q times the heads of a group) operands are good to 2^-16, for
+    values between 2^-50 and 2^37 and queries below 2^67. Above, queries, keys, values and weights are fp16
+    numbers with powers of two taken out of a row's query, and of the keys and of the values of each step
+    of 32 or 128 positions. They are good to 2^-12 of themselves or to 2^-34 of the largest of the step
+    (queries of a row: 2^-28, weights: 2^-32), whichever is more, from 2^-100 up; the step's largest may be
+    one that only later rows of the call see. Steps of values 2^80 below an earlier one lose more.
 
     A row that sees no key is zero. Lengths past the table end there; pages numbered outside the cache
     are left out as if masked; rows that no sequence claims are not written.

@@ -171,3 +171,23 @@ def test_sizes_at_the_ends_of_the_type(paged, rows, hq, d, max_q, qx, kx, vx):
     pages, table = _cache(paged, lens, _randn(1, 340, 1, d) * kx, _randn(2, 340, 1, d) * vx, 64)
     q = (_randn(3, 2 * rows, hq, d) * qx).bfloat16().cuda()
     _attend(paged, q, pages, table, lens, counts, scale=0.12 / qx / kx, max_q=max_q)
+
+
+@pytest.mark.parametrize("rows,hq,d,max_q", ABOVE_8)
+def test_a_large_value_that_only_the_last_row_sees(paged, rows, hq, d, max_q):
+    """Above 8 units the values of a step of keys share a power of two, keys of later rows among them: values
+    2^20 below the largest still have their precision."""
+    n = 290
+    v = _randn(2, n, 1, d)
+    v[n - 1] *= 2.0 ** 20
+    pages, table = _cache(paged, [n], _randn(1, n, 1, d), v, 64)
+    _attend(paged, _randn(3, rows, hq, d).bfloat16().cuda(), pages, table, [n], [rows], max_q=max_q)
+
+
+@pytest.mark.parametrize("rows,hq,d,max_q", KERNELS[:2])
+@pytest.mark.parametrize("vx", [2.0 ** -47, 2.0 ** 34])
+def test_sizes_up_to_8_units(paged, rows, hq, d, max_q, vx):
+    """Up to 8 units values between 2^-50 and 2^37 keep their precision."""
+    lens, counts = [300, 40], [rows, rows]
+    pages, table = _cache(paged, lens, _randn(1, 340, 1, d), _randn(2, 340, 1, d) * vx, 64)
+    _attend(paged, _randn(3, 2 * rows, hq, d).bfloat16().cuda(), pages, table, lens, counts, max_q=max_q)
