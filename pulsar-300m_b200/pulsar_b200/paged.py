@@ -177,9 +177,9 @@ def kv4_append(q, k, v, pages, slots, positions=None, cos=None, sin=None, *, q_n
         out = torch.empty(n, hq, hd, dtype=_BF16, device=dev)
     _vector(slots, "slots", _I64, n, dev)
     rot = max_pos = 0
-    if cos is not None:
-        if sin is None or cos.dim() != 2 or cos.shape != sin.shape:
-            _refuse("cos and sin must be [max_pos, rot / 2]")
+    if cos is not None or sin is not None:
+        if cos is None or sin is None or cos.dim() != 2 or cos.shape != sin.shape:
+            _refuse("cos and sin must both be given, as [max_pos, rot / 2]")
         if cos.dtype != _F32 or sin.dtype != _F32 or cos.device != dev or sin.device != dev or not (
                 cos.is_contiguous() and sin.is_contiguous()):
             _refuse(f"cos and sin must be contiguous float32 tensors on {dev}")

@@ -191,3 +191,12 @@ def test_sizes_up_to_8_units(paged, rows, hq, d, max_q, vx):
     lens, counts = [300, 40], [rows, rows]
     pages, table = _cache(paged, lens, _randn(1, 340, 1, d), _randn(2, 340, 1, d) * vx, 64)
     _attend(paged, _randn(3, 2 * rows, hq, d).bfloat16().cuda(), pages, table, lens, counts, max_q=max_q)
+
+
+def test_half_a_rotation_table_is_refused(paged):
+    pages = paged.kv4_pages(4, 2, 64, 16)
+    x = torch.zeros(3, 2, 64, dtype=torch.bfloat16, device="cuda")
+    cos, sin = paged.rope_tables(8)
+    for c, s in ((cos, None), (None, sin)):
+        with pytest.raises(RuntimeError, match="cos and sin"):
+            paged.kv4_append(x, x, x, pages, torch.arange(3, device="cuda"), _int([0, 1, 2]), c, s)
