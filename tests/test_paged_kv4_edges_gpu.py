@@ -200,3 +200,43 @@ def test_half_a_rotation_table_is_refused(paged):
     for c, s in ((cos, None), (None, sin)):
         with pytest.raises(RuntimeError, match="cos and sin"):
             paged.kv4_append(x, x, x, pages, torch.arange(3, device="cuda"), _int([0, 1, 2]), c, s)
+
+
+@pytest.mark.parametrize("hq,hkv,d,page,window", [(16, 4, 64, 64, 0), (28, 4, 64, 16, 50), (16, 4, 128, 32, 70),
+                                                  (28, 4, 128, 64, 0), (4, 4, 64, 32, 1)])
+def test_many_short_sequences(paged, hq, hkv, d, page, window):
+    """More sequences and kv heads (640) than the GPU holds CTAs of four warps: blocks of two warps."""
+    edges = [0, 1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129]
+    lens = (edges + torch.randint(301, (145,), generator=torch.Generator().manual_seed(1)).tolist())
+    k, v = _randn(2, sum(lens), hkv, d), _randn(3, sum(lens), hkv, d)
+    pages, table = _cache(paged, lens, k, v, page)
+    for b in (40, 77, 120):
+        table[b][0] = -1
+    table[150] = [1 << 20] * len(table[150])
+    q = (1.5 * _randn(4, 160, hq, d)).bfloat16().cuda()
+    got = _attend(paged, q, pages, table, lens, [1] * 160, window=window, max_kv=300)
+    one = paged.kv4_attention(q, pages, _int(table), _int(lens), window=window, max_kv=300)
+    assert torch.equal(one, got)
+
+
+@pytest.mark.parametrize("rows,hq,d,max_q", KERNELS)
+@pytest.mark.parametrize("page,window", [(16, 0), (64, 0), (64, 4500)])
+def test_long_walks(paged, rows, hq, d, max_q, page, window):
+    """One CTA walks a whole sequence (max_kv far below the truth), so that pages are looked up again and
+    again on the way; some are missing, late ones too."""
+    lens, counts = [9000, 4200, 4097], [rows, rows, max(1, rows - 1)]
+    pages, table = _cache(paged, lens, _randn(1, sum(lens), 1, d), _randn(2, sum(lens), 1, d), page)
+    table[0][4500 // page], table[0][8500 // page], table[1][4150 // page], table[2][0] = -1, 1 << 20, -1, -1
+    q = (1.2 * _randn(3, sum(counts), hq, d)).bfloat16().cuda()
+    _attend(paged, q, pages, table, lens, counts, window=window, max_q=max_q, max_kv=64)
+
+
+@pytest.mark.parametrize("rows,hq,hkv,d,page,window,max_q", [
+    (65, 4, 1, 64, 64, 0, 65), (65, 4, 1, 64, 16, 70, 8192), (65, 8, 4, 128, 32, 0, 65), (65, 8, 4, 128, 32, 90, 8192),
+    (8, 3, 3, 64, 128, 50, 8), (5, 7, 1, 128, 16, 33, 5), (6, 8, 2, 64, 32, 0, 6)])
+def test_rows_by_their_norms(paged, rows, hq, hkv, d, page, window, max_q):
+    """Prompts, chunks and verify blocks: a key too many or too few moves a row by more than the bound."""
+    lens, counts = [150, 129, rows, 40, 0, 70], [rows, min(rows, 17), rows, 1, 2, 0]
+    pages, table = _cache(paged, lens, 1.3 * _randn(1, sum(lens), hkv, d), _randn(2, sum(lens), hkv, d), page)
+    q = (1.5 * _randn(3, sum(counts), hq, d)).bfloat16().cuda()
+    _attend(paged, q, pages, table, lens, counts, window=window, max_q=max_q)
