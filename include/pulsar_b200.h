@@ -160,7 +160,8 @@ int pulsar_op_kv4_attention_workspace(int64_t N, int64_t Hq, int64_t Hkv, int64_
  * 0 for a row that sees no key; rows of no sequence are not written. Page numbers outside the cache
  * count as masked; scale is positive and finite. q 4-byte, out and the workspace 16-byte aligned.
  * Sums are 32-bit. Up to 8 units (max_q times heads of a group) operands are good to 2^-16, for values
- * between 2^-50 and 2^37 and queries below 2^67. Above, queries, keys, values and weights are fp16 with
+ * between 2^-50 and 2^37, queries below 2^67, products of a query and a key from 2^-50 up and a scale of
+ * at most 2^50 (checked). Above, queries, keys, values and weights are fp16 with
  * powers of two taken out of a row's query and of the keys and the values of each step of 32 or 128
  * positions: good to 2^-12 of themselves or to 2^-34 of the step's largest (queries of a row: 2^-28,
  * weights: 2^-32), whichever is more, from 2^-100 up; the step's largest may be one that only later rows

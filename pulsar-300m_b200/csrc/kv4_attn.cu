@@ -261,14 +261,15 @@ __global__ void __launch_bounds__(WARPS * 32, resident(HD, NT) * 4 / WARPS) k_kv
     // that weights are 2^LIFT exp2(scale (s - m)). WIDE: m is the reference of the weights 2^(x - m), base 2
     float o[MT][NT][4], zacc[NT][NG][2], m[NT][2], nm[NT][2], l[NT][2];
     const float scale = a.scale_log2 * pow2(CODE_EXP - LIFT);
+    const float unseen = WIDE ? NEG : fmaxf(NEG / scale, -1e38f);   // scale times it is finite, at any scale
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int i = 0; i < MT; ++i) o[i][nt][0] = o[i][nt][1] = o[i][nt][2] = o[i][nt][3] = 0.f;
 #pragma unroll
         for (int g = 0; g < NG; ++g) zacc[nt][g][0] = zacc[nt][g][1] = 0.f;
-        m[nt][0] = m[nt][1] = WIDE ? NEG : NEG * pow2(LIFT - CODE_EXP);
-        nm[nt][0] = nm[nt][1] = -NEG * a.scale_log2;
+        m[nt][0] = m[nt][1] = unseen;
+        nm[nt][0] = nm[nt][1] = -unseen * scale;
         l[nt][0] = l[nt][1] = 0.f;
     }
     const float minus_hi = t < 2 ? 0.f : -1.f;   // columns 4..7 of the doubled units (t >= 2) carry the lo halves
@@ -995,6 +996,8 @@ extern "C" int pulsar_op_kv4_attention(const void* q, int64_t q_row_stride, int6
     PULSAR_CHECK_ARG(num_pages >= 0 && num_pages < (int64_t)1 << 31 && width >= 0 && width * page_size < (int64_t)1 << 30,
                      "kv4_attention: invalid page table");
     PULSAR_CHECK_ARG(scale > 0.f && scale < INFINITY, "kv4_attention: scale must be positive and finite");
+    // k_kv4_attn's scores up to 8 units are in units of 2^(LIFT - CODE_EXP)
+    PULSAR_CHECK_ARG(scale <= pow2(50) || max_q * (Hq / Hkv) > 8, "kv4_attention: a scale past 2^50 needs more than 8 units");
     PULSAR_CHECK_ARG(cu_q || (N == B && max_q == 1), "kv4_attention: without cu_q every sequence has one row");
     if (N == 0 || B == 0) return PULSAR_OK;
     PULSAR_CHECK_ARG(q && pages && kv_lens && out && (block_table || width == 0), "kv4_attention: null pointer");

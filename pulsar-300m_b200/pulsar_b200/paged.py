@@ -238,7 +238,8 @@ def kv4_attention(q, pages, block_table, kv_lens, cu_q=None, *, max_q: int = 1, 
     decides how the work is split. ``scale`` defaults to D ** -0.5.
 
     Sums are in 32 bits. Up to 8 units (max_q times the heads of a group) operands are good to 2^-16, for
-    values between 2^-50 and 2^37 and queries below 2^67. Above, queries, keys, values and weights are fp16
+    values between 2^-50 and 2^37, queries below 2^67, products of a query and a key from 2^-50 up and a
+    scale of at most 2^50 (checked). Above, queries, keys, values and weights are fp16
     numbers with powers of two taken out of a row's query, and of the keys and of the values of each step
     of 32 or 128 positions. They are good to 2^-12 of themselves or to 2^-34 of the largest of the step
     (queries of a row: 2^-28, weights: 2^-32), whichever is more, from 2^-100 up; the step's largest may be

@@ -240,3 +240,26 @@ def test_rows_by_their_norms(paged, rows, hq, hkv, d, page, window, max_q):
     pages, table = _cache(paged, lens, 1.3 * _randn(1, sum(lens), hkv, d), _randn(2, sum(lens), hkv, d), page)
     q = (1.5 * _randn(3, sum(counts), hq, d)).bfloat16().cuda()
     _attend(paged, q, pages, table, lens, counts, window=window, max_q=max_q)
+
+
+@pytest.mark.parametrize("rows,hq,d,max_q", KERNELS)
+@pytest.mark.parametrize("window", [0, 5])
+def test_large_scales(paged, rows, hq, d, max_q, window):
+    """Keys of 2^-40 whose scale makes up for it; short sequences, rows that see no key."""
+    lens, counts = [0, 1, 2, 40, 300], [rows] * 5
+    k, v = _randn(1, sum(lens), 1, d) * 2.0 ** -40, _randn(2, sum(lens), 1, d)
+    pages, table = _cache(paged, lens, k, v, 32)
+    q = _randn(3, sum(counts), hq, d).bfloat16().cuda()
+    _attend(paged, q, pages, table, lens, counts, scale=0.12 * 2.0 ** 40, window=window, max_q=max_q)
+
+
+def test_scale_past_its_range_is_refused(paged):
+    """Up to 8 units a scale past 2^50 would leave the range of the scores."""
+    pages = paged.kv4_pages(4, 1, 64, 16)
+    table, lens = _int([[0]] * 3), _int([1, 1, 1])
+    q = torch.zeros(3, 4, 64, dtype=torch.bfloat16, device="cuda")
+    for scale in (2.0 ** 51, 1e30):
+        with pytest.raises(RuntimeError, match="scale"):
+            paged.kv4_attention(q, pages, table, lens, scale=scale)
+    assert (paged.kv4_attention(q, pages, table, lens, scale=2.0 ** 50) == 0).all()
+    assert (paged.kv4_attention(q, pages, table, lens, _int([0, 1, 2, 3]), max_q=3, scale=1e30) == 0).all()
