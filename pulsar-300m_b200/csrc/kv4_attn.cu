@@ -28,11 +28,10 @@
 // Splits of the keys end in (m, l, O) partials, joined in split order: up to eight splits that fit the
 // GPU at once are a cluster and read each other's shared memory, else k_kv4_merge follows.
 //
-// Time and what bounds it (4 kv heads of 64, 16 query heads): 4 x 32768 keys 18.0 us, 2.3 TB/s of cache;
-// 256 x 513..767 20.2 us; 48 x 1..8191, 8 kv heads of 128, 71.5 us, 3.5 TB/s; 1 x 2048 6.5 us. The
-// copies alone took 13.7, 13.3, 50 and 5.8 us. The rest is issue slots: about 380 instructions for a pair of
-// tiles (heads of 128: 680) and 1000 a warp for its start and end, at 2 to 2.6 a clock and SM with 16
-// warps there.
+// Time and what bounds it (4 kv heads of 64, 16 query heads): 4 x 32768 keys 18.2 us, 2.3 TB/s of cache;
+// 256 x 513..767 20.2 us; 48 x 1..8191, 8 kv heads of 128, 71.6 us, 3.5 TB/s; 1 x 2048 6.5 us. The
+// copies alone took 13.7, 13.3, 50 and 5.8 us. The rest are instructions, about 380 for a pair of tiles (heads
+// of 128: 680) and 1000 a warp for its start and end, at 2 to 2.6 of 4 a clock and SM with 16 warps there.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 

@@ -472,8 +472,9 @@ struct ReadArgs {
     int hkv, page_shift, heads;
 };
 
-// 32768 positions of 4 kv heads of 64: 44 MB in 9.2 us, 4.8 TB/s (16384 of 8 heads of 128: 88 MB in 18.4);
-// 777 positions 2.3 us. Bound by instructions (80 for a lane's 16 dims) and, past that, by the writes.
+// 32768 positions of 4 kv heads of 64: 44 MB in 9.6 us, 4.6 TB/s (16384 of 8 heads of 128: 88 MB in 19.2);
+// 777 positions 2.4 us. Bound by the latency of the slot and then of its tile (long scoreboard 7.7 an issue at
+// 1.8 instructions a clock and SM, 80 for a lane's 16 dims).
 // Through shared memory in whole tiles it was a fifth slower; two heads' bytes asked for at a time cost
 // more registers than waiting.
 template <int HD>

@@ -9,10 +9,10 @@
 //   S = Q K^  tcgen05.mma kind::f16, M 128, N 64, fp32 in TMEM (a warp for each tile of units)
 //   softmax   a thread per unit (four warps a tile): weights in fp16 back to TMEM, over the scores
 //   O += P V^ with P read from TMEM as the A operand, O in TMEM
-// What bounds the kernel are the exponentials (16 a clock and SM). A tile's chain of MMA, scores,
-// weights and MMA is longer than its exponentials take, so four tiles are in flight at different
-// places of it, each with a softmax warp on every scheduler (heads of 128: the two that TMEM holds).
-// 2048 rows of 16 heads of 64 on 16384 keys (4 kv heads) take 238 us: 0.54 PFLOP/s of products, and
+// The exponentials (16 a clock and SM) take half of the time; what bounds the kernel is a tile's chain of MMA,
+// scores, weights and MMA, which is longer, so four tiles are in flight at different places of it, each with a
+// softmax warp on every scheduler (heads of 128: the two that TMEM holds; 2048 rows on 8192 keys 217 us).
+// 2048 rows of 16 heads of 64 on 16384 keys (4 kv heads) take 239 us: 0.54 PFLOP/s of products, and
 // 5 10^8 exponentials, which take 128 SMs (64 unit tiles x 2 splits) 130 us. Measured instead: three
 // tiles with weights beside the scores 277, two threads a unit 322, chunks of 32 keys 300, a quarter
 // of the exponentials as cubic polynomials 281.
